@@ -146,6 +146,61 @@ reef_status reef_gemm_w8a8(const int8_t *xq, const float *x_scales, int64_t rows
                            const float *bias, int64_t out_features, float *y,
                            int64_t y_row_stride, uint32_t *status_word, hipStream_t stream);
 
+/* The same two with an epilogue, y = activation(float(sum) * (row_scale * w_scale) + bias)
+ * + residual, every float step rounded on its own (with REEF_ACT_NONE and no residual, the
+ * outputs of the calls above bit for bit). GELU_TANH is the engine's form
+ * x / (1 + exp(-2 sqrt(2 / pi) (x + 0.044715 x^3))), GELU_ERF x erfc(-x / sqrt(2)) / 2, SILU
+ * x / (1 + exp(-x)). residual: fp32 [rows, out], row r at residual + r *
+ * residual_row_stride; it may be y itself (same pointer and stride), not overlap it
+ * otherwise. An infinite or NaN value before the activation or after the residual sets
+ * OVERFLOW. epilogue NULL: none. */
+typedef enum reef_activation {
+    REEF_ACT_NONE = 0,
+    REEF_ACT_RELU = 1,
+    REEF_ACT_GELU_TANH = 2,
+    REEF_ACT_GELU_ERF = 3,
+    REEF_ACT_SILU = 4
+} reef_activation;
+
+typedef struct reef_epilogue {
+    const float *residual; /* NULL: none */
+    int64_t residual_row_stride;
+    int64_t activation; /* reef_activation */
+} reef_epilogue;
+
+reef_status reef_linear_w8a8_epilogue(const float *x, int64_t rows, int64_t in_features,
+                                      int64_t x_row_stride, const int8_t *weight,
+                                      const float *w_scales, const float *bias,
+                                      const reef_epilogue *epilogue, int64_t out_features,
+                                      float *y, int64_t y_row_stride, void *workspace,
+                                      size_t workspace_bytes, uint32_t *status_word,
+                                      hipStream_t stream);
+
+reef_status reef_gemm_w8a8_epilogue(const int8_t *xq, const float *x_scales, int64_t rows,
+                                    int64_t in_features, const int8_t *weight,
+                                    const float *w_scales, const float *bias,
+                                    const reef_epilogue *epilogue, int64_t out_features, float *y,
+                                    int64_t y_row_stride, uint32_t *status_word,
+                                    hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Root-mean-square norm of a residual sum, as the int8 rows that reef_gemm_w8a8 reads:
+ * h = x + residual (fp32, one rounding; residual NULL: h = x), y = h * weight /
+ * sqrt(mean(h^2) + eps) over each row of `width` values (weight NULL: ones), scale =
+ * float(max|y| / 127) (1 where that is 0), code = rint(y / scale), ties to even, y unrounded
+ * (64-bit steps). q: packed [rows, width]; scales: [rows]. sum (NULL allowed, with a
+ * residual only) receives h; it may be x or residual itself (same pointer and stride), not
+ * overlap them otherwise. Any width and any stride of at least width; eps >= 0. A
+ * non-finite value of a row sets NON_FINITE, a scale beyond fp32 OVERFLOW; that row's codes
+ * are unspecified.
+ */
+reef_status reef_rmsnorm_quantize_int8(const float *x, int64_t rows, int64_t width,
+                                       int64_t x_row_stride, const float *residual,
+                                       int64_t residual_row_stride, const float *weight,
+                                       double eps, int8_t *q, float *scales, float *sum,
+                                       int64_t sum_row_stride, uint32_t *status_word,
+                                       hipStream_t stream);
+
 /* ---------------------------------------------------------------------------
  * Attention over int8 Q/K/V with an fp32 softmax and fp32 output.
  */

@@ -29,6 +29,8 @@ ATTN_PRECISE_PV = 0x1
 SCHED_AUTO, SCHED_ONE_ITEM, SCHED_SPLIT, SCHED_BALANCED, SCHED_PACKED = (0x00, 0x10, 0x20,
                                                                          0x30, 0x40)
 PAGE = 16
+# epilogues of the W8A8 product (reef_activation)
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu_tanh": 2, "gelu_erf": 3, "silu": 4}
 
 EXPORTS = [
     "reef_quantize_int8_per_tensor", "reef_quantize_int8_per_head",
@@ -40,7 +42,8 @@ EXPORTS = [
     "reef_attention_decode_int8_paged", "reef_attention_decode_int8_paged_noalloc",
     "reef_kv_pack_v_pages", "reef_kv_append_int8",
     "reef_kv_append_int8_paged", "reef_attention_int8_integer", "reef_linear_w8a8_workspace_bytes",
-    "reef_linear_w8a8", "reef_gemm_w8a8", "reef_attention_prefill_cache_workspace_bytes",
+    "reef_linear_w8a8", "reef_gemm_w8a8", "reef_linear_w8a8_epilogue", "reef_gemm_w8a8_epilogue",
+    "reef_rmsnorm_quantize_int8", "reef_attention_prefill_cache_workspace_bytes",
     "reef_attention_prefill_int8_cache",
 ]
 
@@ -102,10 +105,16 @@ class KvAppendParams(C.Structure):
                 ("new_tokens", C.c_int64), ("max_context", C.c_int64)]
 
 
+class Epilogue(C.Structure):
+    _fields_ = [("residual", C.c_void_p), ("residual_row_stride", C.c_int64),
+                ("activation", C.c_int64)]
+
+
 _P = C.c_void_p
 _I64 = C.c_int64
 _ST, _AP = C.POINTER(Strides), C.POINTER(AttentionParams)
 _DP, _KP = C.POINTER(DecodeParams), C.POINTER(KvAppendParams)
+_EP = C.POINTER(Epilogue)
 _SIGS = {
     "reef_quantize_int8_per_tensor": [_P, _I64, _P, _P, _P, _P],
     "reef_quantize_int8_per_head": [_P, _I64, _I64, _I64, _I64, _ST, _P, _P, _P, _P],
@@ -131,6 +140,11 @@ _SIGS = {
     "reef_linear_w8a8": [_P, _I64, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _P, C.c_size_t, _P,
                          _P],
     "reef_gemm_w8a8": [_P, _P, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _P, _P],
+    "reef_linear_w8a8_epilogue": [_P, _I64, _I64, _I64, _P, _P, _P, _EP, _I64, _P, _I64, _P,
+                                  C.c_size_t, _P, _P],
+    "reef_gemm_w8a8_epilogue": [_P, _P, _I64, _I64, _P, _P, _P, _EP, _I64, _P, _I64, _P, _P],
+    "reef_rmsnorm_quantize_int8": [_P, _I64, _I64, _I64, _P, _I64, _P, C.c_double, _P, _P, _P,
+                                   _I64, _P, _P],
     "reef_attention_int8_integer": [_AP, _P, _ST, _P, _ST, _P, _ST, C.c_uint32, _P, C.c_uint32,
                                     _P, _ST, _P],
     "reef_kv_append_int8": [_KP, _P, _ST, _P, _ST, _P, _P, _P, _P, _P, _P, _P, _P],
@@ -220,6 +234,7 @@ _STRIDES = struct.Struct("=3q")
 _ATTENTION = struct.Struct("=8qf2iI")
 _DECODE = struct.Struct("=6qf2iI")
 _APPEND = struct.Struct("=5q")
+_EPILOGUE = struct.Struct("=3q")
 
 
 def _require(t, dtype, name):
@@ -229,6 +244,14 @@ def _require(t, dtype, name):
             return
         raise InvalidArgument(f"{name} must be {dtype}, got {t.dtype}")
     raise InvalidArgument(f"{name} must be a GPU tensor")
+
+
+def _on_device(what, *tensors):
+    """Every tensor (None: absent) lies on the current device, whose stream the call takes."""
+    device = _torch()._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise InvalidArgument(f"{what}: every tensor must be on the current GPU")
 
 
 def _strides4(t):
@@ -681,10 +704,43 @@ def attention_int8_integer(q, k, v, table, *, score_shift, out_shift=8, query_st
 
 # --- W8A8 projection (operator/linear.hpp:106-132) ---------------------------------------
 
-def linear_w8a8(x, weight, w_scales, bias=None, status: StatusWord | None = None):
+def _epilogue(activation, residual, rows, fout, what):
+    """The packed reef_epilogue of an activation's name and a [rows, fout] residual."""
+    if activation not in ACTIVATIONS:
+        raise InvalidArgument(f"{what}: activation must be one of {', '.join(ACTIVATIONS)}")
+    if residual is None:
+        return None if activation == "none" else _EPILOGUE.pack(0, 0, ACTIVATIONS[activation])
+    _require(residual, _torch().float32, "residual")
+    if tuple(residual.shape) != (rows, fout) or _row_stride(residual) is None:
+        raise InvalidArgument(f"{what}: residual must be [rows, out] with contiguous rows")
+    return _EPILOGUE.pack(residual.data_ptr(), _row_stride(residual), ACTIVATIONS[activation])
+
+
+def _row_stride(t):
+    """Elements from row to row of a matrix with contiguous rows; None for any other."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        return None
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _product_out(out, rows, fout, device, what):
+    torch = _torch()
+    if out is None:
+        return torch.empty((rows, fout), dtype=torch.float32, device=device), fout
+    _require(out, torch.float32, "out")
+    stride = _row_stride(out)
+    if tuple(out.shape) != (rows, fout) or stride is None or stride < fout:
+        raise InvalidArgument(f"{what}: out must be [rows, out] with contiguous rows")
+    return out, stride
+
+
+def linear_w8a8(x, weight, w_scales, bias=None, status: StatusWord | None = None, *,
+                activation="none", residual=None):
     """y = linear(x, QuantizedWeight{weight, w_scales}, bias): x [rows, in] fp32,
     weight [out, in] int8, w_scales [out] fp32, bias [out] fp32 or None. Rows are
-    quantized per row on the device; outputs are bit-identical to the engine's."""
+    quantized per row on the device; outputs are bit-identical to the engine's.
+    activation (a key of ACTIVATIONS) is applied after the bias, then residual
+    [rows, out] fp32 is added."""
     torch = _torch()
     _require(x, torch.float32, "x")
     _require(weight, torch.int8, "weight")
@@ -693,15 +749,112 @@ def linear_w8a8(x, weight, w_scales, bias=None, status: StatusWord | None = None
         raise InvalidArgument("linear_w8a8 shapes: x [rows, in], weight [out, in]")
     rows, fin = x.shape
     fout = weight.shape[0]
+    epilogue = _epilogue(activation, residual, rows, fout, "linear_w8a8")
     n = _lib().reef_linear_w8a8_workspace_bytes(rows, fin)
     ws = torch.empty(n // 4 + 4, dtype=torch.float32, device=x.device)
     y = torch.empty((rows, fout), dtype=torch.float32, device=x.device)
     own = status or StatusWord(x.device)
     weight, w_scales = weight.contiguous(), w_scales.contiguous()
     bias = bias.contiguous() if bias is not None else None
-    check(_lib().reef_linear_w8a8(
-        _ptr(x), rows, fin, x.stride(0), _ptr(weight), _ptr(w_scales), _ptr(bias), fout, _ptr(y),
-        fout, _ptr(ws), ws.numel() * 4, _ptr(own.tensor), _stream()), "linear_w8a8")
+    check(_lib().reef_linear_w8a8_epilogue(
+        _ptr(x), rows, fin, x.stride(0), _ptr(weight), _ptr(w_scales), _ptr(bias), epilogue, fout,
+        _ptr(y), fout, _ptr(ws), ws.numel() * 4, _ptr(own.tensor), _stream()), "linear_w8a8")
     if status is None:
         own.check("linear_w8a8")
     return y
+
+
+def gemm_w8a8(xq, x_scales, weight, w_scales, bias=None, status: StatusWord | None = None, *,
+              activation="none", residual=None, out=None):
+    """The product of linear_w8a8 on rows that are int8 already: xq [rows, in] int8 with
+    x_scales [rows] (quantize_rows, rmsnorm_quantize). y = activation(float(sum) *
+    (x_scale * w_scale) + bias) + residual, fp32 [rows, out]; out (contiguous rows) may be
+    the residual itself, which then becomes the new residual stream."""
+    torch = _torch()
+    for t, dtype, name in ((xq, torch.int8, "xq"), (weight, torch.int8, "weight"),
+                           (x_scales, torch.float32, "x_scales"),
+                           (w_scales, torch.float32, "w_scales")):
+        _require(t, dtype, name)
+    if xq.dim() != 2 or weight.dim() != 2 or weight.shape[1] != xq.shape[1]:
+        raise InvalidArgument("gemm_w8a8 shapes: xq [rows, in], weight [out, in]")
+    (rows, fin), fout = xq.shape, weight.shape[0]
+    if x_scales.numel() != rows or w_scales.numel() != fout:
+        raise InvalidArgument("gemm_w8a8 shapes: x_scales [rows], w_scales [out]")
+    if bias is not None:
+        _require(bias, torch.float32, "bias")
+        if bias.numel() != fout:
+            raise InvalidArgument("gemm_w8a8 shapes: bias [out]")
+        bias = bias.contiguous()
+    _on_device("gemm_w8a8", xq, x_scales, weight, w_scales, bias, residual, out)
+    epilogue = _epilogue(activation, residual, rows, fout, "gemm_w8a8")
+    y, y_stride = _product_out(out, rows, fout, xq.device, "gemm_w8a8")
+    own = status or StatusWord(xq.device)
+    xq, x_scales, weight, w_scales = (xq.contiguous(), x_scales.contiguous(), weight.contiguous(),
+                                      w_scales.contiguous())
+    check(_lib().reef_gemm_w8a8_epilogue(
+        _ptr(xq), _ptr(x_scales), rows, fin, _ptr(weight), _ptr(w_scales), _ptr(bias), epilogue,
+        fout, _ptr(y), y_stride, _ptr(own.tensor), _stream()), "gemm_w8a8")
+    if status is None:
+        own.check("gemm_w8a8")
+    return y
+
+
+# --- norm ---------------------------------------------------------------------------------
+
+def rmsnorm_quantize(x, weight=None, *, residual=None, eps=1e-6, residual_out=None,
+                     status: StatusWord | None = None):
+    """The root-mean-square norm of x (+ residual) over the last dimension, as int8 rows
+    with scales: h = x + residual, y = h * weight / sqrt(mean(h^2) + eps), one scale
+    max|y| / 127 per row. x and residual [..., width] fp32, weight [width] fp32 or None.
+    Returns (int8 of x's shape, scales of x.shape[:-1]), and h as a third where there is a
+    residual: the new residual stream, in residual_out if that is given (contiguous, and x
+    or residual itself or apart from both)."""
+    torch = _torch()
+    _require(x, torch.float32, "x")
+    shape = x.shape
+    if len(shape) == 0 or x.numel() == 0:
+        raise InvalidArgument("rmsnorm_quantize: x must be [..., width] and not empty")
+    width = shape[-1]
+    if weight is not None:
+        _require(weight, torch.float32, "weight")
+        if tuple(weight.shape) != (width,):
+            raise InvalidArgument("rmsnorm_quantize: weight must be [width]")
+        weight = weight.contiguous()
+    if residual is not None:
+        _require(residual, torch.float32, "residual")
+        if residual.shape != shape:
+            raise InvalidArgument("rmsnorm_quantize: residual must have x's shape")
+    elif residual_out is not None:
+        raise InvalidArgument("rmsnorm_quantize: residual_out needs a residual")
+    _on_device("rmsnorm_quantize", x, weight, residual, residual_out)
+
+    def rows_of(t):
+        """A matrix of t's rows, copied only where they do not lie in one."""
+        m = t if t.dim() == 2 else t.reshape(-1, width)
+        return m if _row_stride(m) is not None and _row_stride(m) >= width else m.contiguous()
+
+    x2 = rows_of(x)
+    rows = x2.shape[0]
+    r2 = h = None
+    r_stride = h_stride = 0
+    if residual is not None:
+        r2 = rows_of(residual)
+        r_stride = _row_stride(r2)
+        h = residual_out
+        if h is None:
+            h = torch.empty(shape, dtype=torch.float32, device=x.device)
+        else:
+            _require(h, torch.float32, "residual_out")
+            if h.shape != shape or not h.is_contiguous():
+                raise InvalidArgument("rmsnorm_quantize: residual_out must be contiguous and have "
+                                      "x's shape")
+        h_stride = width
+    q = torch.empty(shape, dtype=torch.int8, device=x.device)
+    s = torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+    own = status or StatusWord(x.device)
+    check(_lib().reef_rmsnorm_quantize_int8(
+        _ptr(x2), rows, width, _row_stride(x2), _ptr(r2), r_stride, _ptr(weight), eps, _ptr(q),
+        _ptr(s), _ptr(h), h_stride, _ptr(own.tensor), _stream()), "rmsnorm_quantize")
+    if status is None:
+        own.check("rmsnorm_quantize requires finite values")
+    return (q, s) if residual is None else (q, s, h)

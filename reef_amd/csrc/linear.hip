@@ -35,15 +35,54 @@ struct GemmArgs {
     int32_t m_tiles, n_tiles;
     int32_t y_vec;  // rows of y start on 16 bytes
     uint32_t *status;
+    // the kernels with an epilogue only
+    const float *residual;  // [rows, out] or null; may be y
+    int64_t r_stride;
+    int32_t r_vec;  // rows of the residual start on 16 bytes
+    int32_t activation;
 };
+
+// The activations, each within a few units in the last place of fp32 (expf, erfcf): the
+// GELUs and SiLU as quotients and complements without a cancellation, so that their small
+// values left of 0 keep their digits.
+__device__ __forceinline__ float activate(float x, int activation) {
+    switch (activation) {  // uniform over the launch
+    case REEF_ACT_RELU:
+        return x < 0.0f ? 0.0f : x;  // (a NaN stays one)
+    case REEF_ACT_GELU_TANH: {
+        const float u = 1.5957691216057308f * __builtin_fmaf(0.044715f * x * x, x, x);
+        return x / (1.0f + expf(-u));
+    }
+    case REEF_ACT_GELU_ERF:
+        return 0.5f * x * erfcf(-0.70710678118654752f * x);
+    case REEF_ACT_SILU:
+        return x / (1.0f + expf(-x));
+    default:
+        return x;
+    }
+}
+
+// The residual's four values of one lane's block (zeros past the ends).
+__device__ __forceinline__ f32x4 load_residual(const GemmArgs &a, int m, int n) {
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (!a.residual || m >= a.rows) return v;
+    const float *r = a.residual + (int64_t)m * a.r_stride + n;
+    if (a.r_vec && n + 3 < a.out) return *reinterpret_cast<const f32x4 *>(r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (n + i < a.out) v[i] = r[i];
+    return v;
+}
 
 // The epilogue of one 16 x 16 block: lane l holds, in register i, feature
 // n0 + 4 (l / 16) + i of row m0 + l % 16, so a lane's four values are consecutive.
 // The engine's float steps, each rounded on its own: safe_multiply(row scale, column
-// scale), safe_multiply(sum, scale), add_bias. True when a result is not finite.
+// scale), safe_multiply(sum, scale), add_bias; with EPI the activation and the residual
+// after them. True when a result is not finite.
+template <bool EPI>
 __device__ __forceinline__ bool store_block(const GemmArgs &a, int m, int n, float xs,
                                             const float (&ws)[4], const float (&bias)[4],
-                                            const i32x4 &acc) {
+                                            const i32x4 &acc, const f32x4 &residual) {
     bool bad = false;
     f32x4 v;
 #pragma unroll
@@ -52,6 +91,11 @@ __device__ __forceinline__ bool store_block(const GemmArgs &a, int m, int n, flo
         const float scale = xs * ws[i];
         float r = (float)acc[i] * scale;
         if (a.bias) r = r + bias[i];
+        if constexpr (EPI) {
+            bad |= n + i < a.out && !__builtin_isfinite(r);
+            r = activate(r, a.activation);
+            if (a.residual) r = r + residual[i];
+        }
         v[i] = r;
         bad |= n + i < a.out && !__builtin_isfinite(r);
     }
@@ -95,7 +139,7 @@ __device__ __forceinline__ void load_columns(const GemmArgs &a, int n, float (&w
 // lanes that read one chunk of 16 consecutive rows hit 16 distinct bank groups.
 __device__ __forceinline__ int chunk_pos(int r, int c) { return c ^ ((r >> 1) & 7); }
 
-template <int BM, int BN, int WM, int WN, int ST>
+template <int BM, int BN, int WM, int WN, int ST, bool EPI>
 __device__ __forceinline__ void gemm_tile(const GemmArgs &a, int8_t *smem) {
     constexpr int W = WM * WN;                          // waves, WM x WN over the tile
     constexpr int MI = BM / WM / 16, NJ = BN / WN / 16;  // 16 x 16 blocks per wave
@@ -250,23 +294,41 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs &a, int8_t *smem) {
         const int m = m0 + (BM / WM) * wm + 16 * i + col;
         xs[i] = m < a.rows ? a.xs[m] : 0.0f;
     }
+    auto row_of = [&](int i) { return m0 + (BM / WM) * wm + 16 * i + col; };
+    auto feature_of = [&](int j) { return n0 + (BN / WN) * wn + 16 * j + 4 * grp; };
+    // The residual is loaded a column of blocks ahead: the stores between may not be
+    // overtaken by a later load (y may be the residual), so each block would wait for its
+    // own round trip.
+    f32x4 res[2][EPI ? MI : 1];
+    if constexpr (EPI) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) res[0][i] = load_residual(a, row_of(i), feature_of(0));
+    }
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-        const int n = n0 + (BN / WN) * wn + 16 * j + 4 * grp;
+        const int n = feature_of(j);
         float ws[4], bias[4];
         load_columns(a, n, ws, bias);
+        if constexpr (EPI) {
+            if (j + 1 < NJ) {
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+                    res[(j + 1) & 1][i] = load_residual(a, row_of(i), feature_of(j + 1));
+            }
+        }
 #pragma unroll
         for (int i = 0; i < MI; ++i)
-            bad |= store_block(a, m0 + (BM / WM) * wm + 16 * i + col, n, xs[i], ws, bias, acc[i][j]);
+            bad |= store_block<EPI>(a, row_of(i), n, xs[i], ws, bias, acc[i][j],
+                                    res[j & 1][EPI ? i : 0]);
     }
     if (bad) flag_status(a.status, REEF_STATUS_BIT_OVERFLOW);
 }
 
-template <int BM, int BN, int WM, int WN, int ST>
+template <int BM, int BN, int WM, int WN, int ST, bool EPI>
 __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_tile_kernel(GemmArgs a) {
     static_assert(ST * (BM + BN) * kBK <= 160 * 1024, "LDS fits");
     __shared__ __attribute__((aligned(1024))) int8_t smem[ST * (BM + BN) * kBK];
-    gemm_tile<BM, BN, WM, WN, ST>(a, smem);
+    gemm_tile<BM, BN, WM, WN, ST, EPI>(a, smem);
 }
 
 // ---- few rows: the weight streamed once -----------------------------------------------
@@ -277,7 +339,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_tile_kernel(GemmArgs a) 
 // fragments go from memory into operand registers (x from L2: it is small), the next
 // unit's loads in flight while one is multiplied; the waves' int32 sums are added
 // through LDS, exactly, in any order.
-template <int MT, int NT, int W>
+template <int MT, int NT, int W, bool EPI>
 __global__ __launch_bounds__(64 * W, 1) void gemm_rows_kernel(GemmArgs a) {
     __shared__ i32x4 part[W][MT * NT][64];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -361,22 +423,23 @@ __global__ __launch_bounds__(64 * W, 1) void gemm_rows_kernel(GemmArgs a) {
         const int m = m0 + 16 * (b / NT) + col, n = n0 + 16 * (b % NT) + 4 * grp;
         float ws[4], bias[4];
         load_columns(a, n, ws, bias);
-        bad |= store_block(a, m, n, m < a.rows ? a.xs[m] : 0.0f, ws, bias, sum);
+        const f32x4 residual = EPI ? load_residual(a, m, n) : f32x4{};
+        bad |= store_block<EPI>(a, m, n, m < a.rows ? a.xs[m] : 0.0f, ws, bias, sum, residual);
     }
     if (bad) flag_status(a.status, REEF_STATUS_BIT_OVERFLOW);
 }
 
-template <int BM, int BN, int WM, int WN, int ST>
+template <int BM, int BN, int WM, int WN, int ST, bool EPI>
 void launch_tiles(GemmArgs &a, hipStream_t stream) {
     a.m_tiles = (int32_t)ceil_div(a.rows, BM);
     a.n_tiles = (int32_t)ceil_div(a.out, BN);
-    hipLaunchKernelGGL((gemm_tile_kernel<BM, BN, WM, WN, ST>),
+    hipLaunchKernelGGL((gemm_tile_kernel<BM, BN, WM, WN, ST, EPI>),
                        dim3((unsigned)(a.m_tiles * a.n_tiles)), dim3(64 * WM * WN), 0, stream, a);
 }
 
-template <int MT, int NT, int W>
+template <int MT, int NT, int W, bool EPI>
 void launch_rows_kernel(const GemmArgs &a, hipStream_t stream) {
-    hipLaunchKernelGGL((gemm_rows_kernel<MT, NT, W>),
+    hipLaunchKernelGGL((gemm_rows_kernel<MT, NT, W, EPI>),
                        dim3((unsigned)ceil_div(a.out, 16 * NT), (unsigned)ceil_div(a.rows, 16 * MT)),
                        dim3(64 * W), 0, stream, a);
 }
@@ -391,16 +454,25 @@ struct TileChoice {
     int32_t bm, bn, step_ns;
     void (*launch)(GemmArgs &, hipStream_t);
 };
+template <bool EPI>
 const TileChoice kTiles[] = {
-    {256, 256, 1880, launch_tiles<256, 256, 2, 4, 2>}, {256, 192, 1600, launch_tiles<256, 192, 4, 2, 2>},
-    {256, 128, 970, launch_tiles<256, 128, 4, 2, 3>},  {128, 160, 690, launch_tiles<128, 160, 4, 2, 4>},
-    {128, 128, 610, launch_tiles<128, 128, 2, 4, 5>},  {128, 64, 410, launch_tiles<128, 64, 2, 2, 6>},
-    {64, 64, 300, launch_tiles<64, 64, 2, 2, 8>},      {64, 32, 240, launch_tiles<64, 32, 2, 2, 10>},
+    {256, 256, 1880, launch_tiles<256, 256, 2, 4, 2, EPI>},
+    {256, 192, 1600, launch_tiles<256, 192, 4, 2, 2, EPI>},
+    {256, 128, 970, launch_tiles<256, 128, 4, 2, 3, EPI>},
+    {128, 160, 690, launch_tiles<128, 160, 4, 2, 4, EPI>},
+    {128, 128, 610, launch_tiles<128, 128, 2, 4, 5, EPI>},
+    {128, 64, 410, launch_tiles<128, 64, 2, 2, 6, EPI>},
+    {64, 64, 300, launch_tiles<64, 64, 2, 2, 8, EPI>},
+    {64, 32, 240, launch_tiles<64, 32, 2, 2, 10, EPI>},
 };
 
+template <bool EPI>
+void launch_shape(GemmArgs &a, int64_t rows, int64_t out, hipStream_t stream);
+
 reef_status launch_gemm(const int8_t *xq, const float *xs, int64_t rows, int64_t in,
-                        const int8_t *w, const float *ws, const float *bias, int64_t out,
-                        float *y, int64_t y_stride, uint32_t *status, hipStream_t stream) {
+                        const int8_t *w, const float *ws, const float *bias,
+                        const reef_epilogue *epi, int64_t out, float *y, int64_t y_stride,
+                        uint32_t *status, hipStream_t stream) {
     GemmArgs a;
     a.x = xq;
     a.xs = xs;
@@ -415,6 +487,17 @@ reef_status launch_gemm(const int8_t *xq, const float *xs, int64_t rows, int64_t
     a.m_tiles = a.n_tiles = 0;
     a.y_vec = aligned(y, 16) && y_stride % 4 == 0;
     a.status = status;
+    a.residual = epi ? epi->residual : nullptr;
+    a.r_stride = epi ? epi->residual_row_stride : 0;
+    a.r_vec = aligned(a.residual, 16) && a.r_stride % 4 == 0;
+    a.activation = epi ? (int32_t)epi->activation : REEF_ACT_NONE;
+    if (a.residual || a.activation != REEF_ACT_NONE) launch_shape<true>(a, rows, out, stream);
+    else launch_shape<false>(a, rows, out, stream);
+    return launch_status();
+}
+
+template <bool EPI>
+void launch_shape(GemmArgs &a, int64_t rows, int64_t out, hipStream_t stream) {
     const int64_t cus = compute_units();
     // Few rows and features: while 16-feature workgroups with 16 or 32 rows each fit the
     // units at once, every wave's share of K is short and a tile's serial K loop is not
@@ -426,15 +509,15 @@ reef_status launch_gemm(const int8_t *xq, const float *xs, int64_t rows, int64_t
     // against 16.0), and past one workgroup a unit slower (4096 -> 11008: 15.2 against 11.3).
     const int64_t nb = ceil_div(out, 16);
     if (ceil_div(rows, 16) * nb <= cus) {
-        launch_rows_kernel<1, 1, 8>(a, stream);
+        launch_rows_kernel<1, 1, 8, EPI>(a, stream);
     } else if (ceil_div(rows, 32) * nb <= cus) {
-        launch_rows_kernel<2, 1, 8>(a, stream);
+        launch_rows_kernel<2, 1, 8, EPI>(a, stream);
     } else if (rows <= 16 && 4 * ceil_div(out, 32) <= 3 * cus) {
-        launch_rows_kernel<1, 2, 8>(a, stream);
+        launch_rows_kernel<1, 2, 8, EPI>(a, stream);
     } else {
         const TileChoice *best = nullptr;
         int64_t least = 0;
-        for (const TileChoice &t : kTiles) {
+        for (const TileChoice &t : kTiles<EPI>) {
             const int64_t cost = ceil_div(ceil_div(rows, t.bm) * ceil_div(out, t.bn), cus) * t.step_ns;
             if (!best || cost < least) {
                 best = &t;
@@ -443,7 +526,6 @@ reef_status launch_gemm(const int8_t *xq, const float *xs, int64_t rows, int64_t
         }
         best->launch(a, stream);
     }
-    return launch_status();
 }
 
 reef_status validate_gemm(const void *x, const float *xs, int64_t rows, int64_t in,
@@ -458,6 +540,14 @@ reef_status validate_gemm(const void *x, const float *xs, int64_t rows, int64_t 
     return REEF_OK;
 }
 
+reef_status validate_epilogue(const reef_epilogue *e, int64_t out) {
+    if (!e) return REEF_OK;
+    if (e->activation < REEF_ACT_NONE || e->activation > REEF_ACT_SILU ||
+        (e->residual && (e->residual_row_stride < out || !aligned(e->residual, 4))))
+        return REEF_INVALID_ARGUMENT;
+    return REEF_OK;
+}
+
 }  // namespace
 }  // namespace reef
 
@@ -469,27 +559,42 @@ extern "C" size_t reef_linear_w8a8_workspace_bytes(int64_t rows, int64_t in_feat
     return (size_t)(ceil_div(rows * in_features, 16) * 16 + rows * 4);
 }
 
+extern "C" reef_status reef_gemm_w8a8_epilogue(const int8_t *xq, const float *x_scales,
+                                               int64_t rows, int64_t in_features,
+                                               const int8_t *weight, const float *w_scales,
+                                               const float *bias, const reef_epilogue *epilogue,
+                                               int64_t out_features, float *y,
+                                               int64_t y_row_stride, uint32_t *status_word,
+                                               hipStream_t stream) {
+    reef_status s = validate_gemm(xq, x_scales, rows, in_features, weight, w_scales, out_features,
+                                  y, y_row_stride);
+    if (s == REEF_OK) s = validate_epilogue(epilogue, out_features);
+    if (s != REEF_OK) return s;
+    if (!aligned(xq, 16)) return REEF_UNSUPPORTED;
+    return launch_gemm(xq, x_scales, rows, in_features, weight, w_scales, bias, epilogue,
+                       out_features, y, y_row_stride, status_word, stream);
+}
+
 extern "C" reef_status reef_gemm_w8a8(const int8_t *xq, const float *x_scales, int64_t rows,
                                       int64_t in_features, const int8_t *weight,
                                       const float *w_scales, const float *bias,
                                       int64_t out_features, float *y, int64_t y_row_stride,
                                       uint32_t *status_word, hipStream_t stream) {
-    const reef_status s = validate_gemm(xq, x_scales, rows, in_features, weight, w_scales,
-                                        out_features, y, y_row_stride);
-    if (s != REEF_OK) return s;
-    if (!aligned(xq, 16)) return REEF_UNSUPPORTED;
-    return launch_gemm(xq, x_scales, rows, in_features, weight, w_scales, bias, out_features, y,
-                       y_row_stride, status_word, stream);
+    return reef_gemm_w8a8_epilogue(xq, x_scales, rows, in_features, weight, w_scales, bias, nullptr,
+                                   out_features, y, y_row_stride, status_word, stream);
 }
 
-extern "C" reef_status reef_linear_w8a8(const float *x, int64_t rows, int64_t in_features,
-                                        int64_t x_row_stride, const int8_t *weight,
-                                        const float *w_scales, const float *bias,
-                                        int64_t out_features, float *y, int64_t y_row_stride,
-                                        void *workspace, size_t workspace_bytes,
-                                        uint32_t *status_word, hipStream_t stream) {
+extern "C" reef_status reef_linear_w8a8_epilogue(const float *x, int64_t rows, int64_t in_features,
+                                                 int64_t x_row_stride, const int8_t *weight,
+                                                 const float *w_scales, const float *bias,
+                                                 const reef_epilogue *epilogue,
+                                                 int64_t out_features, float *y,
+                                                 int64_t y_row_stride, void *workspace,
+                                                 size_t workspace_bytes, uint32_t *status_word,
+                                                 hipStream_t stream) {
     reef_status s = validate_gemm(x, w_scales, rows, in_features, weight, w_scales, out_features,
                                   y, y_row_stride);
+    if (s == REEF_OK) s = validate_epilogue(epilogue, out_features);
     if (s != REEF_OK) return s;
     if (!workspace || !aligned(workspace, 16) ||
         workspace_bytes < reef_linear_w8a8_workspace_bytes(rows, in_features))
@@ -499,6 +604,17 @@ extern "C" reef_status reef_linear_w8a8(const float *x, int64_t rows, int64_t in
     s = reef_quantize_int8_per_token(x, rows, in_features, x_row_stride, xq, xs, status_word,
                                      stream);
     if (s != REEF_OK) return s;
-    return launch_gemm(xq, xs, rows, in_features, weight, w_scales, bias, out_features, y,
-                       y_row_stride, status_word, stream);
+    return launch_gemm(xq, xs, rows, in_features, weight, w_scales, bias, epilogue, out_features,
+                       y, y_row_stride, status_word, stream);
+}
+
+extern "C" reef_status reef_linear_w8a8(const float *x, int64_t rows, int64_t in_features,
+                                        int64_t x_row_stride, const int8_t *weight,
+                                        const float *w_scales, const float *bias,
+                                        int64_t out_features, float *y, int64_t y_row_stride,
+                                        void *workspace, size_t workspace_bytes,
+                                        uint32_t *status_word, hipStream_t stream) {
+    return reef_linear_w8a8_epilogue(x, rows, in_features, x_row_stride, weight, w_scales, bias,
+                                     nullptr, out_features, y, y_row_stride, workspace,
+                                     workspace_bytes, status_word, stream);
 }
