@@ -450,6 +450,96 @@ reef_status reef_kv_append_int8_paged(const reef_kv_append_params *p, const floa
                                       uint32_t *status_word, hipStream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Pages of the paged cache. block_table [batch, max_blocks_per_seq] int32 names the page of
+ * every 16-token block of a sequence, -1 where it has none; context_lens [batch] int32 its
+ * tokens; page_refs [num_pages] int32 how many table entries name a page: 0 is a free page,
+ * more than 1 a page that sequences share. All lie on the device, and the caller starts with
+ * every entry -1 and every count 0. One table may serve the caches of many layers: these
+ * calls keep the table and the counts and leave lists of (source, destination) pages, -1 in
+ * both where there is nothing to copy, for reef_kv_copy_pages on each layer's pool. Free
+ * pages are given out lowest first, in the order of the sequences and of their blocks.
+ *   - A sequence or pair with a negative index is padding; one past the end sets BAD_LENGTH,
+ *     as does a length below 0 or (fork) beyond the table; a page number at or past
+ *     num_pages, or one that page_refs does not count, sets BAD_PAGE. Neither is followed.
+ *   - batch, n <= 65535.
+ */
+
+/* The listed sequences give their pages back: their entries become -1, their lengths 0. */
+reef_status reef_kv_free(const int32_t *sequences, int64_t n, int32_t *block_table,
+                         int64_t max_blocks_per_seq, int32_t *context_lens, int64_t batch,
+                         int32_t *page_refs, int64_t num_pages, uint32_t *status_word,
+                         hipStream_t stream);
+
+/* children[i] becomes a copy of parents[i] that shares its pages (those that hold tokens;
+ * the pages the child had are given back). A sequence may be the parent of many, a child at
+ * most once and then no parent in the same call (the table is unspecified otherwise, the
+ * counts still agree with it). */
+reef_status reef_kv_fork(const int32_t *parents, const int32_t *children, int64_t n,
+                         int32_t *block_table, int64_t max_blocks_per_seq, int32_t *context_lens,
+                         int64_t batch, int32_t *page_refs, int64_t num_pages,
+                         uint32_t *status_word, hipStream_t stream);
+
+/* Room for new_tokens more tokens of every sequence, in pages of its own: blocks that the
+ * tokens at context_lens[b] .. context_lens[b] + new_tokens - 1 fall in and that have no
+ * page get one, and those whose page is shared get one instead of it; where that page holds
+ * tokens already (the last, partial one), copy_src[b] and copy_dst[b] (both [batch]) name
+ * the two. A sequence that would pass max_blocks_per_seq * 16 tokens keeps its blocks and
+ * sets CAPACITY, as do the blocks for which no free page is left (the others are served;
+ * the call may be repeated once there are). Lengths are not changed. The workspace needs
+ * reef_kv_reserve_workspace_bytes bytes, of any contents. */
+size_t reef_kv_reserve_workspace_bytes(int64_t batch, int64_t new_tokens);
+
+reef_status reef_kv_reserve(int32_t *block_table, int64_t max_blocks_per_seq,
+                            const int32_t *context_lens, int64_t batch, int64_t new_tokens,
+                            int32_t *page_refs, int64_t num_pages, int32_t *copy_src,
+                            int32_t *copy_dst, void *workspace, size_t workspace_bytes,
+                            uint32_t *status_word, hipStream_t stream);
+
+/* The pool's live pages move to its front: with L of them, the k-th live page from the
+ * pool's end that lies at or past L takes the k-th free place before L. The table and the
+ * counts are rewritten; copy_src and copy_dst (num_pages / 2 entries each) list the moves,
+ * all from pages at or past L to pages before it; num_live (NULL allowed) receives L. The
+ * workspace needs reef_kv_compact_workspace_bytes bytes, of any contents. */
+size_t reef_kv_compact_workspace_bytes(int64_t num_pages);
+
+reef_status reef_kv_compact(int32_t *block_table, int64_t max_blocks_per_seq, int64_t batch,
+                            int32_t *page_refs, int64_t num_pages, int32_t *copy_src,
+                            int32_t *copy_dst, int32_t *num_live, void *workspace,
+                            size_t workspace_bytes, uint32_t *status_word, hipStream_t stream);
+
+/* Page src[i] of one layer's pool (keys, values and their scales, the paged layout above)
+ * is copied to page dst[i], for n pairs. A pair with a negative page, or with both the same,
+ * is left out; one past num_pages sets BAD_PAGE and is left out. No page may be a
+ * destination twice, or a destination and a source (its contents are unspecified then). */
+reef_status reef_kv_copy_pages(const int32_t *src, const int32_t *dst, int64_t n,
+                               int64_t kv_heads, int64_t head_dim, int8_t *k_pages,
+                               int8_t *v_pages, float *k_scale_pages, float *v_scale_pages,
+                               int64_t num_pages, uint32_t *status_word, hipStream_t stream);
+
+/* Of a sequence's last p->new_tokens tokens (drafted ones, appended before), the accepted
+ * ones stay: rows kept[b][0 .. kept_lens[b] - 1] of them, ascending, move to the first
+ * kept_lens[b] of their places, keys, values and scales. kept: [batch, new_tokens] int32
+ * (entries past kept_lens[b] are not read); context_lens: [batch] int32, the drafted tokens
+ * counted in; new_lens (optional, apart from context_lens: REEF_INVALID_ARGUMENT where they
+ * overlap) receives context_lens[b] - new_tokens + kept_lens[b]. new_tokens <= 64. The rows
+ * behind the kept ones are left as they were. A length outside [new_tokens, max_context], a
+ * kept_lens outside [0, new_tokens], or rows that are not ascending in [0, new_tokens) set
+ * BAD_LENGTH, a page number outside [0, num_pages) BAD_PAGE; that sequence stays as it is
+ * and new_lens[b] is its length. In the paged cache the drafted tokens' pages must be the
+ * sequence's own (reef_kv_reserve). */
+reef_status reef_kv_keep_int8(const reef_kv_append_params *p, const int32_t *kept,
+                              const int32_t *kept_lens, const int32_t *context_lens,
+                              int8_t *k_cache, int8_t *v_cache, float *k_scales, float *v_scales,
+                              int32_t *new_lens, uint32_t *status_word, hipStream_t stream);
+
+reef_status reef_kv_keep_int8_paged(const reef_kv_append_params *p, const int32_t *kept,
+                                    const int32_t *kept_lens, const int32_t *context_lens,
+                                    const int32_t *block_table, int64_t max_blocks_per_seq,
+                                    int64_t num_pages, int8_t *k_pages, int8_t *v_pages,
+                                    float *k_scale_pages, float *v_scale_pages,
+                                    int32_t *new_lens, uint32_t *status_word, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Prefill over the int8 cache (chunked and multi-turn prompts): Attention::forward
  * with query_len > 1 on a cache that already holds the chunk's keys and values
  * (the engine appends first, then runs context() over every cached key with

@@ -43,7 +43,10 @@ EXPORTS = [
     "reef_kv_pack_v_pages", "reef_kv_append_int8",
     "reef_kv_append_int8_paged", "reef_attention_int8_integer", "reef_linear_w8a8_workspace_bytes",
     "reef_linear_w8a8", "reef_gemm_w8a8", "reef_linear_w8a8_epilogue", "reef_gemm_w8a8_epilogue",
-    "reef_rmsnorm_quantize_int8", "reef_attention_prefill_cache_workspace_bytes",
+    "reef_rmsnorm_quantize_int8", "reef_kv_free", "reef_kv_fork",
+    "reef_kv_reserve_workspace_bytes", "reef_kv_reserve", "reef_kv_compact_workspace_bytes",
+    "reef_kv_compact", "reef_kv_copy_pages", "reef_kv_keep_int8", "reef_kv_keep_int8_paged",
+    "reef_attention_prefill_cache_workspace_bytes",
     "reef_attention_prefill_int8_cache",
 ]
 
@@ -150,6 +153,15 @@ _SIGS = {
     "reef_kv_append_int8": [_KP, _P, _ST, _P, _ST, _P, _P, _P, _P, _P, _P, _P, _P],
     "reef_kv_append_int8_paged": [_KP, _P, _ST, _P, _ST, _P, _P, _I64, _I64, _P, _P, _P, _P, _P,
                                   _P, _P],
+    "reef_kv_free": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P],
+    "reef_kv_fork": [_P, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P],
+    "reef_kv_reserve_workspace_bytes": [_I64, _I64],
+    "reef_kv_reserve": [_P, _I64, _P, _I64, _I64, _P, _I64, _P, _P, _P, C.c_size_t, _P, _P],
+    "reef_kv_compact_workspace_bytes": [_I64],
+    "reef_kv_compact": [_P, _I64, _I64, _P, _I64, _P, _P, _P, _P, C.c_size_t, _P, _P],
+    "reef_kv_copy_pages": [_P, _P, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P, _P],
+    "reef_kv_keep_int8": [_KP, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
+    "reef_kv_keep_int8_paged": [_KP, _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P],
     "reef_attention_prefill_cache_workspace_bytes": [_AP],
     "reef_attention_prefill_int8_cache": [_AP, _P, _ST, _P, _P, _P, _P, _P, _I64, _P, _I64, _I64,
                                           _P, _ST, _P, C.c_size_t, _P, _P],
@@ -674,6 +686,209 @@ def kv_append_paged(k_new, v_new, start_positions, block_table, k_pages, v_pages
         "kv_append_paged")
     if status is None:
         own.check("kv_append_paged")
+
+
+# --- pages of the paged cache ---------------------------------------------------------------
+#
+# block_table [B, max_blocks], context_lens [B] and page_refs [P] are int32 on the GPU and
+# changed in place: a table starts filled with -1, page_refs with 0. See the C header.
+
+def _ints(what, **tensors):
+    """Contiguous int32 tensors on the current GPU."""
+    torch = _torch()
+    for name, t in tensors.items():
+        _require(t, torch.int32, name)
+        if not t.is_contiguous():
+            raise InvalidArgument(f"{what}: {name} must be contiguous")
+    _on_device(what, *tensors.values())
+
+
+def _table(what, block_table, context_lens, page_refs):
+    if block_table.dim() != 2 or page_refs.dim() != 1 or (
+            context_lens is not None and tuple(context_lens.shape) != block_table.shape[:1]):
+        raise InvalidArgument(f"{what} shapes: block_table [B, max_blocks], context_lens [B], "
+                              "page_refs [pages]")
+    return block_table.shape
+
+
+def kv_free(sequences, block_table, context_lens, page_refs, status: StatusWord | None = None):
+    """The listed sequences ([n] int32 rows of the table, negative: padding) give their pages
+    back; their table rows become -1 and their lengths 0."""
+    _ints("kv_free", sequences=sequences, block_table=block_table, context_lens=context_lens,
+          page_refs=page_refs)
+    B, blocks = _table("kv_free", block_table, context_lens, page_refs)
+    own = status or StatusWord(block_table.device)
+    check(_lib().reef_kv_free(_ptr(sequences), sequences.numel(), _ptr(block_table), blocks,
+                              _ptr(context_lens), B, _ptr(page_refs), page_refs.numel(),
+                              _ptr(own.tensor), _stream()), "kv_free")
+    if status is None:
+        own.check("kv_free")
+
+
+def kv_fork(parents, children, block_table, context_lens, page_refs,
+            status: StatusWord | None = None):
+    """Sequence children[i] becomes a copy of parents[i] (both [n] int32, negative: padding)
+    that shares its pages. A parent may have many children; a child is listed once and is no
+    parent in the same call."""
+    _ints("kv_fork", parents=parents, children=children, block_table=block_table,
+          context_lens=context_lens, page_refs=page_refs)
+    B, blocks = _table("kv_fork", block_table, context_lens, page_refs)
+    if parents.numel() != children.numel():
+        raise InvalidArgument("kv_fork: as many parents as children")
+    own = status or StatusWord(block_table.device)
+    check(_lib().reef_kv_fork(_ptr(parents), _ptr(children), parents.numel(), _ptr(block_table),
+                              blocks, _ptr(context_lens), B, _ptr(page_refs), page_refs.numel(),
+                              _ptr(own.tensor), _stream()), "kv_fork")
+    if status is None:
+        own.check("kv_fork")
+
+
+def kv_reserve(block_table, context_lens, page_refs, new_tokens: int,
+               status: StatusWord | None = None):
+    """Pages of its own for every sequence's next new_tokens tokens: absent ones from the free
+    pages, and instead of shared ones. Returns (source, destination) pages [B] int32 for
+    kv_copy_pages on each layer's pool: a shared page that holds tokens is copied, -1 where
+    there is nothing to copy. Lengths are left; kv_append_paged writes the tokens."""
+    torch = _torch()
+    _ints("kv_reserve", block_table=block_table, context_lens=context_lens, page_refs=page_refs)
+    B, blocks = _table("kv_reserve", block_table, context_lens, page_refs)
+    device = block_table.device
+    n = _lib().reef_kv_reserve_workspace_bytes(B, new_tokens)
+    ints = torch.empty(n // 4 + 2 * B, dtype=torch.int32, device=device)
+    source, place = ints[:B], ints[B:2 * B]
+    own = status or StatusWord(device)
+    check(_lib().reef_kv_reserve(
+        _ptr(block_table), blocks, _ptr(context_lens), B, new_tokens, _ptr(page_refs),
+        page_refs.numel(), _ptr(source), _ptr(place), ints.data_ptr() + 8 * B, n,
+        _ptr(own.tensor), _stream()), "kv_reserve")
+    if status is None:
+        own.check("kv_reserve")
+    return source, place
+
+
+def kv_compact(block_table, page_refs, status: StatusWord | None = None):
+    """The pool's L live pages become its first L: table and counts are rewritten. Returns
+    (source, destination) pages [pages // 2] int32 for kv_copy_pages on each layer's pool, -1
+    behind the last move, and L as a [1] int32 tensor."""
+    torch = _torch()
+    _ints("kv_compact", block_table=block_table, page_refs=page_refs)
+    B, blocks = _table("kv_compact", block_table, None, page_refs)
+    pages, device = page_refs.numel(), block_table.device
+    n, half = _lib().reef_kv_compact_workspace_bytes(pages), pages // 2
+    ints = torch.empty(n // 4 + 2 * max(half, 1) + 1, dtype=torch.int32, device=device)
+    live, source, place = ints[:1], ints[1:1 + half], ints[1 + half:1 + 2 * half]
+    own = status or StatusWord(device)
+    base = ints.data_ptr()
+    check(_lib().reef_kv_compact(
+        _ptr(block_table), blocks, B, _ptr(page_refs), pages, base + 4, base + 4 * (1 + half),
+        base, base + 4 * (1 + 2 * half), n, _ptr(own.tensor), _stream()), "kv_compact")
+    if status is None:
+        own.check("kv_compact")
+    return source, place, live
+
+
+def _pool_shapes(what, k_pages, v_pages, k_scale_pages, v_scale_pages):
+    torch = _torch()
+    for t, dtype, name in ((k_pages, torch.int8, "k_pages"), (v_pages, torch.int8, "v_pages"),
+                           (k_scale_pages, torch.float32, "k_scale_pages"),
+                           (v_scale_pages, torch.float32, "v_scale_pages")):
+        _require(t, dtype, name)
+        if not t.is_contiguous():
+            raise InvalidArgument(f"{what}: {name} must be contiguous")
+    _on_device(what, k_pages, v_pages, k_scale_pages, v_scale_pages)
+    if k_pages.dim() != 4 or k_pages.shape[2] != PAGE:
+        raise InvalidArgument(f"{what}: k_pages must be [pages, heads, 16, head_dim]")
+    P, H, _, D = k_pages.shape
+    if (v_pages.numel() != k_pages.numel() or k_scale_pages.numel() != P * H * PAGE
+            or v_scale_pages.numel() != P * H * PAGE):
+        raise InvalidArgument(f"{what}: pages and scale pages do not match")
+    return P, H, D
+
+
+def kv_copy_pages(source, place, k_pages, v_pages, k_scale_pages, v_scale_pages,
+                  status: StatusWord | None = None):
+    """Page source[i] of one layer's pool (keys, values, scales) is copied to page place[i]
+    (both [n] int32; pairs with a negative page are left out). No page may be a destination
+    twice, or a source and a destination."""
+    _ints("kv_copy_pages", source=source, place=place)
+    P, H, D = _pool_shapes("kv_copy_pages", k_pages, v_pages, k_scale_pages, v_scale_pages)
+    if source.numel() != place.numel():
+        raise InvalidArgument("kv_copy_pages: as many sources as destinations")
+    if source.numel() == 0:
+        return
+    own = status or StatusWord(k_pages.device)
+    check(_lib().reef_kv_copy_pages(
+        _ptr(source), _ptr(place), source.numel(), H, D, _ptr(k_pages), _ptr(v_pages),
+        _ptr(k_scale_pages), _ptr(v_scale_pages), P, _ptr(own.tensor), _stream()),
+        "kv_copy_pages")
+    if status is None:
+        own.check("kv_copy_pages")
+
+
+def _kept(what, kept, kept_lens, context_lens):
+    _ints(what, kept=kept, kept_lens=kept_lens, context_lens=context_lens)
+    if kept.dim() != 2 or tuple(kept_lens.shape) != kept.shape[:1] or (
+            context_lens.shape != kept_lens.shape):
+        raise InvalidArgument(f"{what} shapes: kept [B, drafts], kept_lens [B], context_lens [B]")
+    return kept.shape
+
+
+def kv_keep(kept, kept_lens, context_lens, k_cache, v_pages, k_scales, v_scales,
+            status: StatusWord | None = None):
+    """Of every sequence's last T tokens (drafted ones, appended before) rows kept[b][:n] with
+    n = kept_lens[b] stay and move to the first n of their places (kept [B, T] int32,
+    ascending; context_lens [B] counts the drafted tokens in). Contiguous cache as in
+    kv_append. Returns the new lengths, context_lens - T + kept_lens."""
+    torch = _torch()
+    B, T = _kept("kv_keep", kept, kept_lens, context_lens)
+    H, L, D = k_cache.shape[1:]
+    _contiguous_cache("kv_keep", B, k_cache, v_pages, k_scales, v_scales)
+    lens = torch.empty_like(context_lens)
+    own = status or StatusWord(k_cache.device)
+    check(_lib().reef_kv_keep_int8(
+        _packed(_APPEND, KvAppendParams, B, H, D, T, L), _ptr(kept), _ptr(kept_lens),
+        _ptr(context_lens), _ptr(k_cache), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales),
+        _ptr(lens), _ptr(own.tensor), _stream()), "kv_keep")
+    if status is None:
+        own.check("kv_keep")
+    return lens
+
+
+def _contiguous_cache(what, B, k_cache, v_pages, k_scales, v_scales):
+    torch = _torch()
+    for t, dtype, name in ((k_cache, torch.int8, "k_cache"), (v_pages, torch.int8, "v_pages"),
+                           (k_scales, torch.float32, "k_scales"),
+                           (v_scales, torch.float32, "v_scales")):
+        _require(t, dtype, name)
+        if not t.is_contiguous():
+            raise InvalidArgument(f"{what}: {name} must be contiguous")
+    _on_device(what, k_cache, v_pages, k_scales, v_scales)
+    if k_cache.dim() != 4 or k_cache.shape[0] != B or v_pages.numel() != k_cache.numel() or (
+            k_scales.numel() * k_cache.shape[3] != k_cache.numel()
+            or v_scales.numel() != k_scales.numel()):
+        raise InvalidArgument(f"{what}: cache shape mismatch")
+
+
+def kv_keep_paged(kept, kept_lens, context_lens, block_table, k_pages, v_pages, k_scale_pages,
+                  v_scale_pages, status: StatusWord | None = None):
+    """kv_keep in the paged cache; the drafted tokens' pages must be the sequence's own."""
+    torch = _torch()
+    B, T = _kept("kv_keep_paged", kept, kept_lens, context_lens)
+    _ints("kv_keep_paged", block_table=block_table)
+    P, H, D = _pool_shapes("kv_keep_paged", k_pages, v_pages, k_scale_pages, v_scale_pages)
+    if block_table.dim() != 2 or block_table.shape[0] != B:
+        raise InvalidArgument("kv_keep_paged: block_table must be [B, max_blocks]")
+    blocks = block_table.shape[1]
+    lens = torch.empty_like(context_lens)
+    own = status or StatusWord(k_pages.device)
+    check(_lib().reef_kv_keep_int8_paged(
+        _packed(_APPEND, KvAppendParams, B, H, D, T, blocks * PAGE), _ptr(kept), _ptr(kept_lens),
+        _ptr(context_lens), _ptr(block_table), blocks, P, _ptr(k_pages), _ptr(v_pages),
+        _ptr(k_scale_pages), _ptr(v_scale_pages), _ptr(lens), _ptr(own.tensor), _stream()),
+        "kv_keep_paged")
+    if status is None:
+        own.check("kv_keep_paged")
+    return lens
 
 
 # --- integer-only attention (int8.hpp:156-279) -----------------------------------------

@@ -14,7 +14,8 @@ from concurrent.futures import ThreadPoolExecutor
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 SOURCES = ["quant.hip", "prefill.hip", "prefill_packed.hip", "prefill_cache.hip", "decode.hip",
-           "kv_append.hip", "int_head.hip", "linear.hip", "norm.hip"]
+           "kv_append.hip", "int_head.hip", "linear.hip", "norm.hip",
+           "kv_pages.hip"]
 LIB = os.path.join(PKG, "libreef_hip.so")
 
 FLAGS = [
