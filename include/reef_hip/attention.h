@@ -403,6 +403,59 @@ reef_status reef_attention_decode_int8_paged_noalloc(
     const int32_t *block_table, int64_t max_blocks_per_seq, int64_t num_pages,
     const int32_t *context_lens, float *out, uint32_t *status_word, hipStream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Attention of a tree of drafted tokens over the int8 cache (speculative decoding; also a
+ * chain of a few new tokens per sequence, of lengths that differ): the T = draft_len tokens
+ * of every sequence, whose keys and values the cache already holds in its last T places
+ * (reef_kv_append_int8), each see the tokens before them and their own ancestors.
+ *
+ * q: [B, Hq, T, D] int8 with optional strides (multiples of 16; a projection [B, T, Hq * D]
+ * is {T*Hq*D, D, Hq*D}), q_scales by q_granularity (PER_TOKEN: [B, Hq, T]); out: [B, Hq, T,
+ * D] fp32 with optional strides (multiples of 4, 16-byte aligned). The cache, block table
+ * and scales as for decode. context_lens: [B] int32 on the device, the drafted tokens
+ * counted in (NULL, contiguous cache only: max_context). tree_mask: [B, T] uint64 on the
+ * device; bit j of tree_mask[b][i] is set where row i sees drafted token j, itself among
+ * them (bits from T on are ignored); NULL: a chain, row i sees drafted tokens 0 .. i. A row
+ * whose mask is 0 is padding: zeros. With a window, row i sits at position P + (set bits of
+ * its mask) - 1, P = context_lens[b] - T, as do the drafted tokens, and sees the last
+ * `window` positions up to its own. Pages that hold only tokens before every row's window
+ * are not looked up.
+ * A sequence whose length is outside [T, max_context] sets BAD_LENGTH and yields zeros; a
+ * page number outside [0, P) sets BAD_PAGE and its tokens take no part.
+ *
+ * Workspace as for decode: reef_attention_decode_tree_workspace_bytes(p) bytes (0: invalid
+ * or unsupported sizes), 16-byte aligned, zero-filled before its first use; every call
+ * leaves it ready for the next of any shape it is large enough for. Calls that may run at
+ * the same time need separate workspaces.
+ */
+typedef struct reef_tree_params {
+    int64_t batch, q_heads, kv_heads, head_dim; /* head_dim 64 or 128 */
+    int64_t draft_len;   /* tokens per sequence, 1 .. 64 */
+    int64_t max_context; /* tokens per sequence the cache can hold, a multiple of 16 */
+    int64_t window;      /* 0: global */
+    float softmax_scale; /* > 0 */
+    int32_t q_granularity;
+    uint32_t flags; /* 0 */
+    uint32_t reserved;
+} reef_tree_params;
+
+size_t reef_attention_decode_tree_workspace_bytes(const reef_tree_params *p);
+
+reef_status reef_attention_decode_tree_int8(
+    const reef_tree_params *p, const int8_t *q, const reef_strides *q_strides,
+    const float *q_scales, const int8_t *k_cache, const int8_t *v_cache, const float *k_scales,
+    const float *v_scales, const int32_t *context_lens, const uint64_t *tree_mask, float *out,
+    const reef_strides *out_strides, void *workspace, size_t workspace_bytes,
+    uint32_t *status_word, hipStream_t stream);
+
+reef_status reef_attention_decode_tree_int8_paged(
+    const reef_tree_params *p, const int8_t *q, const reef_strides *q_strides,
+    const float *q_scales, const int8_t *k_pages, const int8_t *v_pages,
+    const float *k_scale_pages, const float *v_scale_pages, const int32_t *block_table,
+    int64_t max_blocks_per_seq, int64_t num_pages, const int32_t *context_lens,
+    const uint64_t *tree_mask, float *out, const reef_strides *out_strides, void *workspace,
+    size_t workspace_bytes, uint32_t *status_word, hipStream_t stream);
+
 /* Token-major values [pages * 16, D] (page-contiguous) -> transposed pages
  * [pages, D, 16]. */
 reef_status reef_kv_pack_v_pages(const int8_t *v_tokens, int64_t pages, int64_t head_dim,

@@ -45,6 +45,8 @@ EXPORTS = [
     "reef_linear_w8a8", "reef_gemm_w8a8", "reef_linear_w8a8_epilogue", "reef_gemm_w8a8_epilogue",
     "reef_rmsnorm_quantize_int8", "reef_kv_free", "reef_kv_fork",
     "reef_kv_reserve_workspace_bytes", "reef_kv_reserve", "reef_kv_compact_workspace_bytes",
+    "reef_attention_decode_tree_workspace_bytes", "reef_attention_decode_tree_int8",
+    "reef_attention_decode_tree_int8_paged",
     "reef_kv_compact", "reef_kv_copy_pages", "reef_kv_keep_int8", "reef_kv_keep_int8_paged",
     "reef_attention_prefill_cache_workspace_bytes",
     "reef_attention_prefill_int8_cache",
@@ -108,6 +110,13 @@ class KvAppendParams(C.Structure):
                 ("new_tokens", C.c_int64), ("max_context", C.c_int64)]
 
 
+class TreeParams(C.Structure):
+    _fields_ = [("batch", C.c_int64), ("q_heads", C.c_int64), ("kv_heads", C.c_int64),
+                ("head_dim", C.c_int64), ("draft_len", C.c_int64), ("max_context", C.c_int64),
+                ("window", C.c_int64), ("softmax_scale", C.c_float), ("q_granularity", C.c_int32),
+                ("flags", C.c_uint32), ("reserved", C.c_uint32)]
+
+
 class Epilogue(C.Structure):
     _fields_ = [("residual", C.c_void_p), ("residual_row_stride", C.c_int64),
                 ("activation", C.c_int64)]
@@ -117,7 +126,7 @@ _P = C.c_void_p
 _I64 = C.c_int64
 _ST, _AP = C.POINTER(Strides), C.POINTER(AttentionParams)
 _DP, _KP = C.POINTER(DecodeParams), C.POINTER(KvAppendParams)
-_EP = C.POINTER(Epilogue)
+_EP, _TP = C.POINTER(Epilogue), C.POINTER(TreeParams)
 _SIGS = {
     "reef_quantize_int8_per_tensor": [_P, _I64, _P, _P, _P, _P],
     "reef_quantize_int8_per_head": [_P, _I64, _I64, _I64, _I64, _ST, _P, _P, _P, _P],
@@ -153,6 +162,11 @@ _SIGS = {
     "reef_kv_append_int8": [_KP, _P, _ST, _P, _ST, _P, _P, _P, _P, _P, _P, _P, _P],
     "reef_kv_append_int8_paged": [_KP, _P, _ST, _P, _ST, _P, _P, _I64, _I64, _P, _P, _P, _P, _P,
                                   _P, _P],
+    "reef_attention_decode_tree_workspace_bytes": [_TP],
+    "reef_attention_decode_tree_int8": [_TP, _P, _ST, _P, _P, _P, _P, _P, _P, _P, _P, _ST, _P,
+                                        C.c_size_t, _P, _P],
+    "reef_attention_decode_tree_int8_paged": [_TP, _P, _ST, _P, _P, _P, _P, _P, _P, _I64, _I64,
+                                              _P, _P, _P, _ST, _P, C.c_size_t, _P, _P],
     "reef_kv_free": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P],
     "reef_kv_fork": [_P, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P],
     "reef_kv_reserve_workspace_bytes": [_I64, _I64],
@@ -247,6 +261,7 @@ _ATTENTION = struct.Struct("=8qf2iI")
 _DECODE = struct.Struct("=6qf2iI")
 _APPEND = struct.Struct("=5q")
 _EPILOGUE = struct.Struct("=3q")
+_TREE = struct.Struct("=7qfi2I")
 
 
 def _require(t, dtype, name):
@@ -614,6 +629,131 @@ def attention_decode_paged(q, q_scales, k_pages, v_pages, k_scale_pages, v_scale
         _ptr(ws), ws.numel() * 4, _ptr(own.tensor), _stream()), "attention_decode_paged")
     if status is None:
         own.check("attention_decode_paged")
+    return out
+
+
+# --- attention of drafted tokens ------------------------------------------------------------
+
+_TREE_WS = {}
+
+
+def tree_workspace(params: TreeParams, device):
+    """A zero-filled workspace of the tree attention: every launch leaves it ready for the
+    next, of any shape it is large enough for."""
+    n = lib().reef_attention_decode_tree_workspace_bytes(C.byref(params))
+    torch = _torch()
+    return torch.zeros(max(n, 256), dtype=torch.uint8, device=device)
+
+
+def _tree_workspace(n, device, stream):
+    """This stream's workspace. A call under graph capture takes one of its own, which lives
+    in the graph's memory: graphs that replay at the same time share nothing."""
+    torch = _torch()
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(max(n, 256), dtype=torch.uint8, device=device)
+    key = (device.index, stream)
+    ws = _TREE_WS.get(key)
+    if ws is None or ws.numel() < n:
+        ws = _TREE_WS[key] = torch.zeros(max(n, 256), dtype=torch.uint8, device=device)
+    return ws
+
+
+def _tree_inputs(what, q, q_scales, tree_mask, window, softmax_scale, q_granularity, kv_heads,
+                 max_context, context_lens, out):
+    torch = _torch()
+    _require(q, torch.int8, "q")
+    _require(q_scales, torch.float32, "q_scales")
+    if q.dim() != 4:
+        raise InvalidArgument(f"{what}: q must be [B, heads, drafts, head_dim]")
+    B, Hq, T, D = q.shape
+    scales = {PER_TENSOR: 1, PER_HEAD: Hq, PER_TOKEN: B * Hq * T}.get(q_granularity)
+    if q_scales.numel() != scales:
+        raise InvalidArgument(f"{what}: q_scales do not match q_granularity")
+    if tree_mask is not None:
+        _require(tree_mask, torch.int64, "tree_mask")
+        if tuple(tree_mask.shape) != (B, T):
+            raise InvalidArgument(f"{what}: tree_mask must be [B, drafts] int64")
+        tree_mask = tree_mask.contiguous()
+    if context_lens is not None:
+        _require(context_lens, torch.int32, "context_lens")
+        if tuple(context_lens.shape) != (B,):
+            raise InvalidArgument(f"{what}: context_lens must be [B]")
+        context_lens = context_lens.contiguous()
+    if out is None:
+        out = torch.empty((B, Hq, T, D), dtype=torch.float32, device=q.device)
+    else:
+        _require(out, torch.float32, "out")
+        if out.shape != q.shape:
+            raise InvalidArgument(f"{what}: out must have q's shape")
+    _on_device(what, q, q_scales, tree_mask, context_lens, out)
+    if softmax_scale is None:
+        softmax_scale = 1.0 / math.sqrt(D)
+    p = _packed(_TREE, TreeParams, B, Hq, kv_heads, D, T, max_context, window, softmax_scale,
+                q_granularity, 0, 0)
+    return p, q_scales.contiguous(), tree_mask, context_lens, out
+
+
+def attention_decode_tree(q, q_scales, k_cache, v_pages, k_scales, v_scales, context_lens=None, *,
+                          tree_mask=None, window=0, softmax_scale=None, q_granularity=PER_TOKEN,
+                          workspace=None, status: StatusWord | None = None, out=None):
+    """Attention of T drafted tokens per sequence over a contiguous int8 cache that holds them
+    in its last T places (kv_append).
+
+    q [B, Hq, T, D] int8 (any strides with contiguous head_dim), T <= 64; q_scales [B, Hq, T]
+    by default; the cache as for attention_decode; context_lens [B] int32 (the drafted
+    tokens counted in) or None; tree_mask [B, T] int64, bit j of row i set where token i sees
+    drafted token j (itself among them; 0: padding, zeros), None for a chain. Returns fp32
+    [B, Hq, T, D].
+    """
+    _contiguous_cache("attention_decode_tree", q.shape[0], k_cache, v_pages, k_scales, v_scales)
+    H, L, D = k_cache.shape[1:]
+    if q.dim() == 4 and q.shape[3] != D:
+        raise InvalidArgument("attention_decode_tree: q and the cache differ in head_dim")
+    p, q_scales, tree_mask, context_lens, out = _tree_inputs(
+        "attention_decode_tree", q, q_scales, tree_mask, window, softmax_scale, q_granularity, H, L,
+        context_lens, out)
+    stream = _stream()
+    n = _lib().reef_attention_decode_tree_workspace_bytes(p)
+    ws = _tree_workspace(n, q.device, stream) if workspace is None else workspace
+    own = status or StatusWord(q.device)
+    check(_lib().reef_attention_decode_tree_int8(
+        p, _ptr(q), _strides4(q), _ptr(q_scales), _ptr(k_cache), _ptr(v_pages), _ptr(k_scales),
+        _ptr(v_scales), _ptr(context_lens), _ptr(tree_mask), _ptr(out), _strides4(out), _ptr(ws),
+        ws.numel() * ws.element_size(), _ptr(own.tensor), stream), "attention_decode_tree")
+    if status is None:
+        own.check("attention_decode_tree")
+    return out
+
+
+def attention_decode_tree_paged(q, q_scales, k_pages, v_pages, k_scale_pages, v_scale_pages,
+                                block_table, context_lens, *, tree_mask=None, window=0,
+                                softmax_scale=None, q_granularity=PER_TOKEN, workspace=None,
+                                status: StatusWord | None = None, out=None):
+    """attention_decode_tree over a paged int8 cache: k_pages [P, Hkv, 16, D], v_pages [P,
+    Hkv, D, 16], scale pages [P, Hkv, 16], block_table [B, max_blocks] int32, context_lens
+    [B] int32."""
+    what = "attention_decode_tree_paged"
+    P, H, D = _pool_shapes(what, k_pages, v_pages, k_scale_pages, v_scale_pages)
+    _ints(what, block_table=block_table, context_lens=context_lens)
+    if q.dim() == 4 and q.shape[3] != D:
+        raise InvalidArgument(f"{what}: q and the cache differ in head_dim")
+    if block_table.dim() != 2 or block_table.shape[0] != q.shape[0]:
+        raise InvalidArgument(f"{what}: block_table must be [B, max_blocks]")
+    blocks = block_table.shape[1]
+    p, q_scales, tree_mask, context_lens, out = _tree_inputs(
+        what, q, q_scales, tree_mask, window, softmax_scale, q_granularity, H, blocks * PAGE,
+        context_lens, out)
+    stream = _stream()
+    n = _lib().reef_attention_decode_tree_workspace_bytes(p)
+    ws = _tree_workspace(n, q.device, stream) if workspace is None else workspace
+    own = status or StatusWord(q.device)
+    check(_lib().reef_attention_decode_tree_int8_paged(
+        p, _ptr(q), _strides4(q), _ptr(q_scales), _ptr(k_pages), _ptr(v_pages),
+        _ptr(k_scale_pages), _ptr(v_scale_pages), _ptr(block_table), blocks, P,
+        _ptr(context_lens), _ptr(tree_mask), _ptr(out), _strides4(out), _ptr(ws),
+        ws.numel() * ws.element_size(), _ptr(own.tensor), stream), what)
+    if status is None:
+        own.check(what)
     return out
 
 

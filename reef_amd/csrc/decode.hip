@@ -25,14 +25,12 @@
 #include <cmath>
 #include <mutex>
 
-#include "reef_common.hpp"
+#include "decode_common.hpp"
 
 namespace reef {
 namespace {
 
 constexpr int kDecodeWaves = 4;          // waves per workgroup
-constexpr int kBlockKeys = 64;           // keys per inner step (4 pages)
-constexpr int kPage = 16;                // tokens per page
 constexpr int kPlanItems = 2048;         // items whose block offsets a workgroup plans in LDS
 constexpr int kWgPerCu = 2;              // resident workgroups per compute unit (at most)
 
@@ -103,34 +101,6 @@ __device__ __forceinline__ PageRef page_ref(const DecodeArgs &a, int b, int kvh,
         r.vs = a.vs + tok;
     }
     return r;
-}
-
-// int8 x 16 (one 16-byte word) -> two fp16 x 8 operands, exactly. After the XOR a
-// byte holds u = b + 128; a byte permute puts each u under the exponent byte 0x64,
-// which reads as the fp16 1024 + u, and subtracting 1152 leaves b. Five
-// instructions per 4 values.
-__device__ __forceinline__ void int8x16_to_f16(i32x4 w, f16x8 &lo, f16x8 &hi) {
-    const f16x2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const uint32_t u = (uint32_t)w[j] ^ 0x80808080u;
-        const f16x2 a = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias;
-        const f16x2 c = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias;
-        f16x8 &dst = j < 2 ? lo : hi;
-        const int e = 4 * (j & 1);
-        dst[e] = a[0];
-        dst[e + 1] = a[1];
-        dst[e + 2] = c[0];
-        dst[e + 3] = c[1];
-    }
-}
-
-// A 16-byte load of the streamed cache; NT marks it non-temporal (read once: a
-// contiguous cache is not re-read within a step, and keeping it out of the caches
-// measured faster there).
-template <bool NT>
-__device__ __forceinline__ i32x4 load_stream(const i32x4 *p) {
-    return NT ? __builtin_nontemporal_load(p) : *p;
 }
 
 // One 64-key block in registers: the operands of both matrix products and,
@@ -205,16 +175,6 @@ __device__ __forceinline__ void load_block(const DecodeArgs &a, int b, int kvh, 
         x.v[d] = load_stream<!PAGED>(reinterpret_cast<const i32x4 *>(gp.vt + (16 * d + col) * kPage));
     x.ks = gp.ks[col];
     x.vs = gp.vs[col];
-}
-
-// The values of a row's 16 lanes, on every lane of the row (DPP row_newbcast). As shuffles
-// through LDS the 16 index registers made the paged kernel spill inside its key loop (ragged
-// paged decode of 128 sequences: 44.1 us, 41.0 this way).
-template <int R = 0>
-__device__ __forceinline__ void row_lanes(float x, float (&out)[16]) {
-    out[R] = __int_as_float(
-        __builtin_amdgcn_mov_dpp(__float_as_int(x), 0x150 + R, 0xf, 0xf, true));
-    if constexpr (R < 15) row_lanes<R + 1>(x, out);
 }
 
 // Scores, online softmax and P.V of one block for keys [lo, k_end).
@@ -416,14 +376,6 @@ __device__ void plan_blocks(const DecodeArgs &a, int32_t *sOff, int32_t *sWave) 
         if (i < a.items) sOff[i + 1] = before + x;
         __syncthreads();
     }
-}
-
-// Workgroup g of G owns units [start(g), start(g + 1)) of the T units (64-key
-// blocks of all items, or items), start(g) = g T / G; unit u lies in workgroup
-// ((u + 1) G - 1) / T.
-__device__ __forceinline__ int64_t wg_start(int64_t g, int64_t T, int64_t G) { return g * T / G; }
-__device__ __forceinline__ int wg_of(int64_t u, int64_t T, int64_t G) {
-    return (int)(((u + 1) * G - 1) / T);
 }
 
 // Log-sum-exp merge of the waves' (max, sum, output in absolute value units)

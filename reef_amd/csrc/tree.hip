@@ -1,0 +1,801 @@
+// Attention of a tree of drafted tokens over an int8 KV cache for gfx950 (speculative
+// decoding): T query tokens per sequence, whose keys and values the cache already holds in
+// its last T places. Row i sees every token before them and, of the drafted ones, those whose
+// bit its mask sets (its ancestors and itself).
+//
+//   s_j = float(int32 q_i . k_j) * (s_q * s_k[j]) * softmax_scale
+//   out_i = sum_j softmax(s)_j * float(v_j) * s_v[j]
+//
+// The products are those of the decode kernel (decode.hip): 64-key blocks straight from
+// memory into operand registers, S^T = K . q^T on v_mfma_i32_16x16x64_i8, out^T = V^T . P^T on
+// v_mfma_f32_16x16x32_f16 with P split into fp16 hi + lo. The instruction's 16 columns hold
+// (token, query head) pairs of one KV head, column t * group + g, so T tokens of a group of G
+// heads are T G columns in tiles of 16. A wave keeps NC tiles: what it reads and converts of a
+// block serves them all.
+#include <algorithm>
+#include <cmath>
+
+#include "decode_common.hpp"
+
+namespace reef {
+namespace {
+
+constexpr int kWaves = 8;      // waves of a workgroup: two per SIMD
+constexpr int kPlan = 2048;    // sequences of a launch (more are launched in slices)
+constexpr int kMaxDrafts = 64; // bits of a mask word
+constexpr int kXcds = 8;       // workgroup i of a launch runs on XCD i % 8
+constexpr int kCounters = 2048;
+
+struct TreeArgs {
+    const int8_t *q;
+    const float *qs;
+    const int8_t *k, *v;  // contiguous cache or page pool
+    const float *ks, *vs;
+    const int32_t *block_table;   // paged only
+    const int32_t *context_lens;  // may be null
+    const uint64_t *mask;         // [batch, drafts]; null: row i sees drafted tokens 0 .. i
+    float *out;
+    uint32_t *counters;  // one per workgroup; zero between launches
+    uint64_t *slots;
+    uint32_t *status;
+    int64_t q_sb, q_sh, q_st, o_sb, o_sh, o_st;
+    int32_t batch, q_heads, kv_heads, group, drafts;
+    int32_t max_context, window;
+    int32_t cw;      // the workgroup's waves split the columns cw ways (and the keys 8 / cw)
+    int32_t chunks;  // column ranges of 16 NC cw columns; an item is (sequence, kv head, range)
+    int32_t max_blocks, num_pages;  // paged only
+    int32_t q_gran;
+    float score_scale;  // softmax_scale * log2(e)
+};
+
+// A sequence's keys: its length (0 if out of range), the tokens before the drafts, the first
+// key any row sees, and its 64-key blocks from the one with that key on. A sequence with no
+// keys counts one block, so that some workgroup stores its zeros.
+struct SeqKeys {
+    int len, prefix, lo, first_block, blocks;
+    bool bad;
+};
+
+__device__ __forceinline__ SeqKeys seq_keys(const TreeArgs &a, int b) {
+    SeqKeys r;
+    int len = a.context_lens ? a.context_lens[b] : a.max_context;
+    r.bad = len < a.drafts || len > a.max_context;
+    if (r.bad) len = 0;
+    r.len = len;
+    r.prefix = max(0, len - a.drafts);
+    r.lo = a.window > 0 ? max(0, r.prefix + 1 - a.window) : 0;  // (the shallowest row's)
+    r.first_block = r.lo / kBlockKeys;
+    r.blocks = len > 0 ? (len + kBlockKeys - 1) / kBlockKeys - r.first_block : 1;
+    return r;
+}
+
+// sOff[i] = blocks of sequences 0 .. i - 1, for i <= batch (a workgroup-wide scan).
+__device__ void plan_blocks(const TreeArgs &a, int32_t *sOff, int32_t *sWave) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (tid == 0) sOff[0] = 0;
+    int32_t run = 0;
+    for (int base = 0; base < a.batch; base += 64 * kWaves) {
+        const int i = base + tid;
+        int32_t x = i < a.batch ? seq_keys(a, i).blocks : 0;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int32_t y = __shfl_up(x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 63) sWave[wave] = x;
+        __syncthreads();
+        int32_t before = run;
+        for (int w = 0; w < kWaves; ++w) {
+            if (w < wave) before += sWave[w];
+            run += sWave[w];
+        }
+        if (i < a.batch) sOff[i + 1] = before + x;
+        __syncthreads();
+    }
+}
+
+// Where a lane's K row and its lane group's page lie, for one 64-key block.
+struct BlockAt {
+    const int8_t *k, *vt;
+    const float *ks, *vs;
+    bool live;  // the lane group's page holds keys of this sequence
+};
+
+template <int D, bool PAGED>
+__device__ __forceinline__ BlockAt block_at(const TreeArgs &a, int b, int kvh, int kb,
+                                            const SeqKeys &sk, int pages, int col, int grp,
+                                            bool &bad_page) {
+    BlockAt r;
+    const int kp = kb / kPage + (col >> 2), gp = kb / kPage + grp;
+    // Pages past the sequence's last, or wholly before the first key that any row sees (they
+    // may have been given back), are not read: their lanes read a safe page.
+    const int n_pages = (sk.len + kPage - 1) / kPage, first = sk.lo / kPage;
+    const bool k_in = kp >= first && kp < n_pages, g_in = gp >= first && gp < n_pages;
+    int64_t kt, gt;  // the pages' first tokens
+    if (PAGED) {
+        const int ke = __shfl(pages, col >> 2), ge = __shfl(pages, grp);
+        const bool k_ok = k_in && ke >= 0 && ke < a.num_pages;
+        const bool g_ok = g_in && ge >= 0 && ge < a.num_pages;
+        bad_page |= g_in && !g_ok;
+        r.live = g_ok;
+        kt = ((int64_t)(k_ok ? ke : 0) * a.kv_heads + kvh) * kPage;
+        gt = ((int64_t)(g_ok ? ge : 0) * a.kv_heads + kvh) * kPage;
+    } else {
+        const int64_t seq = ((int64_t)b * a.kv_heads + kvh) * a.max_context;
+        r.live = g_in;
+        kt = seq + (k_in ? kp : 0) * kPage;
+        gt = seq + (g_in ? gp : 0) * kPage;
+    }
+    r.k = a.k + (kt + (col & 3)) * D + 16 * grp;
+    r.vt = a.v + gt * D + col * kPage;
+    r.ks = a.ks + gt + col;
+    r.vs = a.vs + gt + col;
+    return r;
+}
+
+// Table entries of the block at key kb: lane l holds that of page l % 4.
+template <bool PAGED>
+__device__ __forceinline__ int block_pages(const TreeArgs &a, int b, int kb, const SeqKeys &sk,
+                                           int lane) {
+    const int p = kb / kPage + (lane & 3);
+    if (!PAGED || p >= (sk.len + kPage - 1) / kPage || p < sk.lo / kPage) return 0;
+    return a.block_table[(int64_t)b * a.max_blocks + p];
+}
+
+// Largest x over the 16 lanes of a row, in every lane of it.
+template <int CTRL>
+__device__ __forceinline__ float dpp_fmax(float x) {
+    return fmaxf(x, __int_as_float(
+                        __builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xF, 0xF, false)));
+}
+__device__ __forceinline__ float row_fmax(float x) {
+    x = dpp_fmax<0xB1>(x);   // quad_perm [1, 0, 3, 2]
+    x = dpp_fmax<0x4E>(x);   // quad_perm [2, 3, 0, 1]
+    x = dpp_fmax<0x141>(x);  // row_half_mirror
+    return dpp_fmax<0x140>(x);  // row_mirror
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_or(uint32_t x) {
+    return x | (uint32_t)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xF, 0xF, false);
+}
+__device__ __forceinline__ uint32_t row_or(uint32_t x) {
+    x = dpp_or<0xB1>(x);
+    x = dpp_or<0x4E>(x);
+    x = dpp_or<0x141>(x);
+    return dpp_or<0x140>(x);
+}
+
+// Bits lo .. hi - 1 of 16, for any lo and hi.
+__device__ __forceinline__ uint32_t bits16(int lo, int hi) {
+    lo = min(max(lo, 0), 16);
+    hi = min(max(hi, 0), 16);
+    return (0xffffu >> (16 - hi)) & ~((1u << lo) - 1u);
+}
+
+// What a lane's column of one tile is: a row of the tree for one query head, or nothing.
+struct Column {
+    bool live;       // a column of this launch
+    bool shown;      // its row sees something
+    int head, token;
+    float c;         // log2-domain score per unit of the int32 sum and the key's scale
+    int lo;          // the first token before the drafts that it sees
+    uint64_t drafts; // the drafted tokens that it sees
+};
+
+__device__ __forceinline__ Column column_of(const TreeArgs &a, int b, int kvh, int index,
+                                            const SeqKeys &sk) {
+    Column r;
+    r.live = index < a.drafts * a.group;
+    const int i = r.live ? index : 0;
+    r.token = i / a.group;
+    r.head = kvh * a.group + i % a.group;
+    const uint64_t all = a.drafts == 64 ? ~0ull : (1ull << a.drafts) - 1;
+    const uint64_t *row = a.mask ? a.mask + (int64_t)b * a.drafts : nullptr;
+    uint64_t m = row ? row[r.token] & all : (2ull << r.token) - 1;
+    r.lo = 0;
+    if (a.window > 0) {
+        // Row i sits at prefix + |mask_i| - 1 (its ancestors before it); a drafted token as
+        // far back as the window is hidden.
+        const int depth = __popcll(m) - 1;
+        r.lo = max(0, sk.prefix + depth + 1 - a.window);
+        if (a.window < a.drafts) {
+            for (int j = 0; j < a.drafts; ++j) {
+                const int dj = __popcll(row ? row[j] & all : (2ull << j) - 1) - 1;
+                if (dj <= depth - a.window) m &= ~(1ull << j);
+            }
+        }
+    }
+    r.drafts = m;
+    r.shown = r.live && (row ? (row[r.token] & all) != 0 : true) && sk.len > 0;
+    if (!r.shown) {
+        r.lo = INT32_MAX;
+        r.drafts = 0;
+    }
+    float cq = 1.0f;
+    if (r.live)
+        cq = a.q_gran == REEF_SCALE_PER_TENSOR ? a.qs[0]
+             : a.q_gran == REEF_SCALE_PER_HEAD
+                 ? a.qs[r.head]
+                 : a.qs[((int64_t)b * a.q_heads + r.head) * a.drafts + r.token];
+    r.c = cq * a.score_scale;
+    return r;
+}
+
+// One part of one tile in the workspace: the output in [d][half][lane] order, then (max, sum).
+template <int D>
+struct TreeSlot {
+    static constexpr int O = 2 * (D / 16);
+    static constexpr int ELEMS = (O + 1) * kWave;
+};
+
+__device__ __forceinline__ uint64_t pack(float x, float y) {
+    return (uint64_t)__float_as_uint(x) | ((uint64_t)__float_as_uint(y) << 32);
+}
+__device__ __forceinline__ float lo32(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi32(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+
+// The launch's work is the 64-key blocks of all items (sequence, kv head, column range),
+// dealt out to the workgroups in equal runs. Within a run each item's part is one segment:
+// the workgroup's eight waves split the range's columns cw ways and the segment's blocks
+// 8 / cw ways, keep a running softmax and merge in LDS. An item inside one run is stored
+// directly; the parts of an item cut by a run's end go to the workspace, and the one that
+// counts in last merges them in order (reef_common.hpp, cross-workgroup parts). Waves that
+// split the columns read the same blocks at about the same time: one reads memory, the
+// others the caches.
+template <int D, bool PAGED, int NC>
+__global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(TreeArgs a) {
+    constexpr int DB = D / 16, KS = D / 64;
+    __shared__ int32_t sOff[kPlan + 1];
+    __shared__ int32_t sWave[kWaves];
+    __shared__ f32x4 sO[kWaves][DB][kWave];
+    __shared__ float2 sML[kWaves][kWave];
+    __shared__ uint32_t sLast;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, grp = lane >> 4;
+    const int CW = a.cw, KW = kWaves / CW;
+    const int cwi = wave % CW, kwi = wave / CW;
+
+    const bool same = a.context_lens == nullptr;
+    const int nb = same ? seq_keys(a, 0).blocks : 0;
+    if (!same) plan_blocks(a, sOff, sWave);
+    auto blocks_before = [&](int b) -> int {  // of the sequences before b
+        return same ? b * nb : __builtin_amdgcn_readfirstlane(sOff[b]);
+    };
+    const int per_seq = a.kv_heads * a.chunks;  // items of a sequence
+    const int64_t T = (int64_t)blocks_before(a.batch) * per_seq;
+    // No more workgroups than there are items, or parts with a block for every wave.
+    const int64_t G = min((int64_t)gridDim.x,
+                          max((int64_t)a.batch * per_seq, (T + KW - 1) / KW));
+    // The workgroups of one XCD hold consecutive runs: the column ranges of one (sequence,
+    // kv head) meet in its L2.
+    const int x = blockIdx.x % kXcds, place = blockIdx.x / kXcds;
+    const int64_t per = G / kXcds, rem = G % kXcds;
+    if (place >= per + (x < rem ? 1 : 0)) return;
+    const int64_t g = x * per + min((int64_t)x, rem) + place;
+    int64_t u = wg_start(g, T, G);
+    const int64_t u0 = u, u1 = wg_start(g + 1, T, G);
+    int b = 0;
+    {
+        int hi = a.batch - 1;
+        while (b < hi) {
+            const int mid = (b + hi + 1) >> 1;
+            if ((int64_t)blocks_before(mid) * per_seq <= u0) b = mid;
+            else hi = mid - 1;
+        }
+    }
+
+    while (u < u1) {
+        SeqKeys sk = seq_keys(a, b);
+        sk.len = __builtin_amdgcn_readfirstlane(sk.len);
+        sk.prefix = __builtin_amdgcn_readfirstlane(sk.prefix);
+        sk.lo = __builtin_amdgcn_readfirstlane(sk.lo);
+        sk.first_block = __builtin_amdgcn_readfirstlane(sk.first_block);
+        sk.blocks = __builtin_amdgcn_readfirstlane(sk.blocks);
+        const int64_t seq_u0 = (int64_t)blocks_before(b) * per_seq;
+        const int in_seq = (int)(u - seq_u0);
+        const int hc = in_seq / sk.blocks, s_blk = in_seq - hc * sk.blocks;
+        const int e_blk = (int)min((int64_t)sk.blocks, s_blk + (u1 - u));
+        const int kvh = hc / a.chunks, chunk = hc % a.chunks;
+        const int64_t item_u0 = u - s_blk;
+        if (sk.bad && s_blk == 0 && hc == 0 && threadIdx.x == 0)
+            flag_status(a.status, REEF_STATUS_BIT_BAD_LENGTH);
+
+        const int tile0 = (chunk * CW + cwi) * NC;  // this wave's first tile
+        Column cn[NC];
+        i32x4 qop[NC][KS];
+#pragma unroll
+        for (int t = 0; t < NC; ++t) {
+            cn[t] = column_of(a, b, kvh, 16 * (tile0 + t) + col, sk);
+            const int8_t *qrow = a.q + b * a.q_sb + cn[t].head * a.q_sh + cn[t].token * a.q_st;
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+                qop[t][s] = cn[t].live ? *reinterpret_cast<const i32x4 *>(qrow + 64 * s + 16 * grp)
+                                       : i32x4{0, 0, 0, 0};
+        }
+        const bool wave_live = 16 * tile0 < a.drafts * a.group;  // wave-uniform
+
+        float m_run[NC], l_run[NC], s_run = 0.0f, inv_s = 0.0f;
+        f32x4 acc[NC][DB];
+#pragma unroll
+        for (int t = 0; t < NC; ++t) {
+            m_run[t] = -INFINITY;
+            l_run[t] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) acc[t][d] = f32x4{};
+        }
+        bool bad_page = false;
+        const int k_begin = (sk.first_block + s_blk + kwi) * kBlockKeys;
+        const int k_end = min(sk.len, (sk.first_block + e_blk) * kBlockKeys);
+        const int k_step = KW * kBlockKeys;
+        // Keys that every row sees: [full_lo, prefix).
+        const int full_lo = a.window > 0 ? max(0, sk.prefix + a.drafts - a.window) : 0;
+        if (wave_live && k_begin < k_end) {
+            i32x4 kop[4][KS], vop[DB];
+            float ks, vs;
+            BlockAt at = block_at<D, PAGED>(a, b, kvh, k_begin, sk,
+                                            block_pages<PAGED>(a, b, k_begin, sk, lane), col, grp,
+                                            bad_page);
+            auto load_k = [&](const BlockAt &p) {
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int s = 0; s < KS; ++s)
+                        kop[t][s] = *reinterpret_cast<const i32x4 *>(p.k + 4 * t * D + 64 * s);
+                ks = *p.ks;
+            };
+            auto load_v = [&](const BlockAt &p) {
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+                    vop[d] = *reinterpret_cast<const i32x4 *>(p.vt + 16 * d * kPage);
+                vs = *p.vs;
+            };
+            load_k(at);
+            load_v(at);
+            int pg_next = block_pages<PAGED>(a, b, k_begin + k_step, sk, lane);
+            for (int kb = k_begin; kb < k_end; kb += k_step) {
+                const bool more = kb + k_step < k_end;
+                const bool live = at.live;
+                const int pg_after = block_pages<PAGED>(a, b, kb + 2 * k_step, sk, lane);
+                // Scores of every tile, times the key's scale.
+                float xs[NC][16];
+                {
+                    float ksc[16];
+                    row_lanes(ks, ksc);
+#pragma unroll
+                    for (int t = 0; t < NC; ++t)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            i32x4 s = {0, 0, 0, 0};
+#pragma unroll
+                            for (int e = 0; e < KS; ++e) s = mfma_16x16x64_i8(kop[j][e], qop[t][e], s);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                xs[t][4 * j + i] = (float)s[i] * ksc[4 * j + i];
+                        }
+                }
+                // The key registers are free: the next block's keys fly from here on, its
+                // values from the end of the products on.
+                if (more) {
+                    at = block_at<D, PAGED>(a, b, kvh, kb + k_step, sk, pg_next, col, grp, bad_page);
+                    load_k(at);
+                }
+                pg_next = pg_after;
+                // Blocks that every row sees whole skip the masks. In the others a hidden key's
+                // score is -inf, and the value scale of a key that no row of the wave sees
+                // is 0 (the cache there may hold anything).
+                const int kk = kb + 16 * grp;
+                float vsc = vs;
+                if (kb < full_lo || kb + kBlockKeys > sk.prefix || !__all(live)) {
+                    uint32_t any = 0;
+#pragma unroll
+                    for (int t = 0; t < NC; ++t) {
+                        uint32_t vis = bits16(cn[t].lo - kk, sk.prefix - kk);
+                        const int j = kk - sk.prefix;  // drafted token of this group's first key
+                        vis |= (j >= 0 ? (j < 64 ? (uint32_t)(cn[t].drafts >> j) : 0u)
+                                       : (j > -16 ? (uint32_t)(cn[t].drafts << -j) : 0u)) & 0xffffu;
+                        if (!live) vis = 0;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (!(vis >> r & 1u)) xs[t][r] = -INFINITY;
+                        any |= vis;
+                    }
+                    any = row_or(any);
+                    if (!(any >> col & 1u)) vsc = 0.0f;
+                }
+                float mt[NC];
+                bool grow = false;
+#pragma unroll
+                for (int t = 0; t < NC; ++t) {
+                    float m = fmaxf(fmaxf(xs[t][0], xs[t][1]), xs[t][2]);
+#pragma unroll
+                    for (int r = 3; r < 15; r += 2) m = fmaxf(fmaxf(m, xs[t][r]), xs[t][r + 1]);
+                    m = fmaxf(m, xs[t][15]);
+                    m = fmaxf(m, __shfl_xor(m, 16));
+                    mt[t] = xor32_max(m) * cn[t].c;
+                    grow |= mt[t] > m_run[t] + 6.0f;
+                }
+                float vmax = row_fmax(vsc);
+                vmax = fmaxf(vmax, __shfl_xor(vmax, 16));
+                vmax = xor32_max(vmax);
+                // Lazy rescale: a row's maximum moves only when it grows by more than 2^6, and
+                // the unit of the accumulator (s_run / 2^8, s_run the largest value scale so
+                // far) only when a value scale passes it 2-fold, so a weight
+                // p * v_scale * 2^8 / s_run stays below 2^15 in fp16, and above its subnormals
+                // (hi and lo keep 11 bits each) where its share of the row counts.
+                if (__any(grow || vmax > s_run * 2.0f)) {
+                    const float s_new = fmaxf(s_run, vmax);
+                    const float units = s_new > 0.0f ? s_run / s_new : 1.0f;
+                    inv_s = s_new > 0.0f ? 256.0f / s_new : 0.0f;
+                    s_run = s_new;
+#pragma unroll
+                    for (int t = 0; t < NC; ++t) {
+                        const float m_new = fmaxf(m_run[t], mt[t]);
+                        const float alpha =
+                            m_run[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[t] - m_new);
+                        m_run[t] = m_new;
+                        l_run[t] *= alpha;
+                        const float alpha_o = alpha * units;
+#pragma unroll
+                        for (int d = 0; d < DB; ++d) acc[t][d] *= alpha_o;
+                    }
+                }
+                // P operands: lane group g's keys 16 g + 8 h + e for the two halves h.
+                f16x8 hi[NC][2], lo[NC][2];
+                {
+                    float vv[16];
+                    row_lanes(vsc * inv_s, vv);
+#pragma unroll
+                    for (int t = 0; t < NC; ++t) {
+                        const float m_use = m_run[t] == -INFINITY ? 0.0f : m_run[t];
+                        float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float w[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const float p = __builtin_amdgcn_exp2f(
+                                    __builtin_fmaf(xs[t][8 * h + e], cn[t].c, -m_use));
+                                sum[e & 1] += p;
+                                w[e] = p * vv[8 * h + e];
+                            }
+                            split_weights(w, hi[t][h], lo[t][h]);
+                        }
+                        l_run[t] += sum[0] + sum[1];
+                    }
+                }
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    f16x8 v0, v1;
+                    int8x16_to_f16(vop[d], v0, v1);
+#pragma unroll
+                    for (int t = 0; t < NC; ++t) {
+                        acc[t][d] = mfma_16x16x32_f16(v0, hi[t][0], acc[t][d]);
+                        acc[t][d] = mfma_16x16x32_f16(v0, lo[t][0], acc[t][d]);
+                        acc[t][d] = mfma_16x16x32_f16(v1, hi[t][1], acc[t][d]);
+                        acc[t][d] = mfma_16x16x32_f16(v1, lo[t][1], acc[t][d]);
+                    }
+                }
+                if (more) load_v(at);
+            }
+        }
+        if (bad_page) flag_status(a.status, REEF_STATUS_BIT_BAD_PAGE);
+
+        // The workgroups that hold a part of this item: gf .. gl, each with at least one block.
+        const int gf = wg_of(item_u0, T, G), gl = wg_of(item_u0 + sk.blocks - 1, T, G);
+        const int parts = gl - gf + 1;
+        const int64_t slot_elems = (int64_t)CW * NC * TreeSlot<D>::ELEMS;
+        // A part's slot is its workgroup's first, unless its item begins inside the run.
+        uint64_t *mine = a.slots + (2 * g + (item_u0 <= u0 ? 0 : 1)) * slot_elems;
+        auto tile_slot = [&](uint64_t *s, int t) {
+            return s + (cwi * NC + t) * TreeSlot<D>::ELEMS;
+        };
+        auto store_out = [&](const Column &c, int d, f32x4 o, float l) {
+            if (!c.live) return;
+            const float inv = c.shown && l > 0.0f ? 1.0f / l : 0.0f;
+            float *row = a.out + b * a.o_sb + c.head * a.o_sh + c.token * a.o_st;
+            f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (inv > 0.0f) y = o * inv;
+            *reinterpret_cast<f32x4 *>(row + 16 * d + 4 * grp) = y;
+        };
+        // The key-split waves of a column range merge tile by tile through LDS, each the
+        // channel blocks d = kwi, kwi + KW, ...
+#pragma unroll
+        for (int t = 0; t < NC; ++t) {
+            float l = l_run[t];
+            l += __shfl_xor(l, 16);
+            l = xor32_sum(l);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) sO[wave][d][lane] = acc[t][d] * (s_run * (1.0f / 256.0f));
+            sML[wave][lane] = float2{m_run[t], l};
+            __syncthreads();
+            float m = -INFINITY;
+            for (int w = cwi; w < kWaves; w += CW) m = fmaxf(m, sML[w][lane].x);
+            l = 0.0f;
+            float scale[kWaves];
+#pragma unroll
+            for (int i = 0; i < kWaves; ++i) {
+                scale[i] = 0.0f;
+                if (i < KW) {
+                    const float2 ml = sML[i * CW + cwi][lane];
+                    scale[i] = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - m);
+                    l = __builtin_fmaf(scale[i], ml.y, l);
+                }
+            }
+            for (int d = kwi; d < DB; d += KW) {
+                f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < kWaves; ++i)
+                    if (i < KW) {
+                        const f32x4 p = sO[i * CW + cwi][d][lane];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(scale[i], p[e], o[e]);
+                    }
+                if (parts == 1) {
+                    store_out(cn[t], d, o, l);
+                } else if (cn[t].live) {
+                    uint64_t *s = tile_slot(mine, t);
+                    part_store(s + (2 * d) * kWave + lane, pack(o[0], o[1]));
+                    part_store(s + (2 * d + 1) * kWave + lane, pack(o[2], o[3]));
+                }
+            }
+            if (parts > 1 && kwi == 0 && cn[t].live)
+                part_store(tile_slot(mine, t) + TreeSlot<D>::O * kWave + lane, pack(m, l));
+            __syncthreads();  // frees sO / sML
+        }
+        if (parts > 1) {
+            part_stores_done();
+            __syncthreads();
+            if (threadIdx.x == 0)
+                sLast = part_count(a.counters + gf) == (uint32_t)(parts - 1) ? 1u : 0u;
+            __syncthreads();
+            if (__builtin_amdgcn_readfirstlane(sLast)) {
+                part_claimed();
+                if (threadIdx.x == 0) part_reset(a.counters + gf);
+                const bool first_second = wg_start(gf, T, G) < item_u0;
+                constexpr int kAhead = 4;  // parts whose loads are in flight together
+#pragma unroll
+                for (int t = 0; t < NC; ++t) {
+                    if (!cn[t].live) continue;
+                    for (int d = kwi; d < DB; d += KW) {
+                        float m = -INFINITY, l = 0.0f;
+                        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+                        for (int p0 = 0; p0 < parts; p0 += kAhead) {
+                            uint64_t ml[kAhead], v0[kAhead], v1[kAhead];
+#pragma unroll
+                            for (int i = 0; i < kAhead; ++i) {
+                                const int p = min(p0 + i, parts - 1);
+                                uint64_t *s = tile_slot(
+                                    a.slots + (2 * (int64_t)(gf + p) + (p == 0 && first_second)) *
+                                                  slot_elems, t);
+                                ml[i] = part_load(s + TreeSlot<D>::O * kWave + lane);
+                                v0[i] = part_load(s + (2 * d) * kWave + lane);
+                                v1[i] = part_load(s + (2 * d + 1) * kWave + lane);
+                            }
+#pragma unroll
+                            for (int i = 0; i < kAhead; ++i) {
+                                if (p0 + i >= parts) break;
+                                const float mp = lo32(ml[i]), mn = fmaxf(m, mp);
+                                const float er = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+                                const float ep = mp == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mp - mn);
+                                l = __builtin_fmaf(ep, hi32(ml[i]), l * er);
+                                o[0] = __builtin_fmaf(ep, lo32(v0[i]), o[0] * er);
+                                o[1] = __builtin_fmaf(ep, hi32(v0[i]), o[1] * er);
+                                o[2] = __builtin_fmaf(ep, lo32(v1[i]), o[2] * er);
+                                o[3] = __builtin_fmaf(ep, hi32(v1[i]), o[3] * er);
+                                m = mn;
+                            }
+                        }
+                        store_out(cn[t], d, o, l);
+                    }
+                }
+            }
+            __syncthreads();  // sLast is read before the next segment writes it
+        }
+        u += e_blk - s_blk;
+        if (u == seq_u0 + (int64_t)sk.blocks * per_seq) ++b;
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------
+
+// How a launch of `batch` sequences is laid out: tiles per wave, the ways the waves split the
+// columns, the column ranges, and the workgroups.
+struct TreeShape {
+    int64_t nc, cw, chunks, wgs;
+};
+
+TreeShape tree_shape(const reef_tree_params *p, int64_t batch) {
+    TreeShape s;
+    const int64_t cus = compute_units();
+    const int64_t tiles = ceil_div(p->draft_len * (p->q_heads / p->kv_heads), 16);
+    s.nc = tiles > 1 ? 2 : 1;
+    s.cw = 1;
+    while (s.cw < kWaves && s.cw * s.nc < tiles) s.cw *= 2;
+    s.chunks = ceil_div(tiles, s.nc * s.cw);
+    // Columns are rather split over workgroups than keys while that gives no more items than
+    // compute units: column ranges have nothing to merge.
+    while (s.cw > 1 && 2 * batch * p->kv_heads * s.chunks <= cus) {
+        s.cw /= 2;
+        s.chunks = ceil_div(tiles, s.nc * s.cw);
+    }
+    const int64_t units =
+        batch * p->kv_heads * s.chunks * ceil_div(p->max_context, kBlockKeys);
+    s.wgs = std::max<int64_t>(1, std::min(std::min(cus, units), (int64_t)kCounters));
+    return s;
+}
+
+constexpr int64_t kCounterBytes = kCounters * 4;
+
+int64_t tree_workspace(const reef_tree_params *p) {
+    const int64_t elems = p->head_dim == 128 ? TreeSlot<128>::ELEMS : TreeSlot<64>::ELEMS;
+    // the slices of a large batch: full ones and the last
+    int64_t most = 0;
+    for (const int64_t batch : {std::min<int64_t>(p->batch, kPlan), p->batch % kPlan}) {
+        if (batch == 0) continue;
+        const TreeShape s = tree_shape(p, batch);
+        most = std::max(most, s.wgs * 2 * s.cw * s.nc * elems * 8);
+    }
+    return kCounterBytes + most;
+}
+
+bool params_ok(const reef_tree_params *p) {
+    return p && p->batch > 0 && p->q_heads > 0 && p->kv_heads > 0 && p->head_dim > 0 &&
+           p->draft_len > 0 && p->max_context > 0 && p->q_heads % p->kv_heads == 0;
+}
+
+bool params_supported(const reef_tree_params *p) {
+    return (p->head_dim == 64 || p->head_dim == 128) && p->draft_len <= kMaxDrafts &&
+           p->q_heads <= 65535 && p->batch <= 65535 && p->max_context < (int64_t(1) << 30);
+}
+
+bool strides_ok(const reef_strides *s, int64_t unit) {
+    return !s || (s->batch >= 0 && s->head >= 0 && s->token >= 0 && s->batch % unit == 0 &&
+                  s->head % unit == 0 && s->token % unit == 0);
+}
+
+reef_status validate(const reef_tree_params *p, const int8_t *q, const reef_strides *q_strides,
+                     const float *q_scales, const int8_t *k, const int8_t *v, const float *ks,
+                     const float *vs, const uint64_t *mask, const float *out,
+                     const reef_strides *out_strides, const void *workspace,
+                     size_t workspace_bytes) {
+    if (!params_ok(p) || !q || !q_scales || !k || !v || !ks || !vs || !out ||
+        p->max_context % kPage != 0 || p->window < 0 || !std::isfinite(p->softmax_scale) ||
+        !(p->softmax_scale > 0.0f) || p->flags != 0 ||
+        (p->q_granularity != REEF_SCALE_PER_TENSOR && p->q_granularity != REEF_SCALE_PER_HEAD &&
+         p->q_granularity != REEF_SCALE_PER_TOKEN))
+        return REEF_INVALID_ARGUMENT;
+    if (!params_supported(p)) return REEF_UNSUPPORTED;
+    if (p->draft_len > p->max_context) return REEF_CAPACITY;
+    if (!aligned(q, 16) || !strides_ok(q_strides, 16) || !aligned(out, 16) ||
+        !strides_ok(out_strides, 4) || !aligned(k, 16) || !aligned(v, 16) || !aligned(ks, 4) ||
+        !aligned(vs, 4) || !aligned(mask, 8))
+        return REEF_INVALID_ARGUMENT;
+    if (!workspace || !aligned(workspace, 16) ||
+        workspace_bytes < (size_t)tree_workspace(p))
+        return REEF_INVALID_ARGUMENT;
+    const TreeShape s = tree_shape(p, std::min<int64_t>(p->batch, kPlan));
+    if (std::min<int64_t>(p->batch, kPlan) * p->kv_heads * s.chunks *
+            ceil_div(p->max_context, kBlockKeys) >= (int64_t(1) << 31))
+        return REEF_UNSUPPORTED;
+    return REEF_OK;
+}
+
+template <bool PAGED>
+reef_status launch_tree(const reef_tree_params *p, TreeArgs &a, const reef_strides *qs,
+                        const reef_strides *os, void *workspace, hipStream_t stream) {
+    const int64_t D = p->head_dim, T = p->draft_len, Hq = p->q_heads;
+    a.q_sb = qs ? qs->batch : Hq * T * D;
+    a.q_sh = qs ? qs->head : T * D;
+    a.q_st = qs ? qs->token : D;
+    a.o_sb = os ? os->batch : Hq * T * D;
+    a.o_sh = os ? os->head : T * D;
+    a.o_st = os ? os->token : D;
+    a.q_heads = (int32_t)Hq;
+    a.kv_heads = (int32_t)p->kv_heads;
+    a.group = (int32_t)(Hq / p->kv_heads);
+    a.drafts = (int32_t)T;
+    a.max_context = (int32_t)p->max_context;
+    a.window = (int32_t)std::min<int64_t>(p->window, int64_t(1) << 30);
+    a.q_gran = p->q_granularity;
+    a.score_scale = p->softmax_scale * kLog2e;
+    a.counters = static_cast<uint32_t *>(workspace);
+    a.slots = reinterpret_cast<uint64_t *>(static_cast<char *>(workspace) + kCounterBytes);
+    for (int64_t b0 = 0; b0 < p->batch; b0 += kPlan) {  // (the slices follow one another)
+        const int64_t batch = std::min<int64_t>(kPlan, p->batch - b0);
+        const TreeShape s = tree_shape(p, batch);
+        TreeArgs c = a;
+        c.batch = (int32_t)batch;
+        c.cw = (int32_t)s.cw;
+        c.chunks = (int32_t)s.chunks;
+        c.q += b0 * a.q_sb;
+        c.out += b0 * a.o_sb;
+        if (a.q_gran == REEF_SCALE_PER_TOKEN) c.qs += b0 * Hq * T;
+        if (a.mask) c.mask += b0 * T;
+        if (a.context_lens) c.context_lens += b0;
+        if (PAGED) {
+            c.block_table += b0 * a.max_blocks;
+        } else {
+            const int64_t tokens = b0 * p->kv_heads * p->max_context;
+            c.k += tokens * D;
+            c.v += tokens * D;
+            c.ks += tokens;
+            c.vs += tokens;
+        }
+        const dim3 grid((unsigned)s.wgs), block(64 * kWaves);
+        if (D == 128 && s.nc == 1)
+            hipLaunchKernelGGL((tree_kernel<128, PAGED, 1>), grid, block, 0, stream, c);
+        else if (D == 128)
+            hipLaunchKernelGGL((tree_kernel<128, PAGED, 2>), grid, block, 0, stream, c);
+        else if (s.nc == 1)
+            hipLaunchKernelGGL((tree_kernel<64, PAGED, 1>), grid, block, 0, stream, c);
+        else
+            hipLaunchKernelGGL((tree_kernel<64, PAGED, 2>), grid, block, 0, stream, c);
+        if (hipGetLastError() != hipSuccess) return REEF_HIP_ERROR;
+    }
+    return REEF_OK;
+}
+
+}  // namespace
+}  // namespace reef
+
+using namespace reef;
+
+extern "C" size_t reef_attention_decode_tree_workspace_bytes(const reef_tree_params *p) {
+    if (!params_ok(p) || !params_supported(p)) return 0;
+    return (size_t)tree_workspace(p);
+}
+
+extern "C" reef_status reef_attention_decode_tree_int8(
+    const reef_tree_params *p, const int8_t *q, const reef_strides *q_strides,
+    const float *q_scales, const int8_t *k_cache, const int8_t *v_cache, const float *k_scales,
+    const float *v_scales, const int32_t *context_lens, const uint64_t *tree_mask, float *out,
+    const reef_strides *out_strides, void *workspace, size_t workspace_bytes,
+    uint32_t *status_word, hipStream_t stream) {
+    const reef_status s = validate(p, q, q_strides, q_scales, k_cache, v_cache, k_scales, v_scales,
+                                   tree_mask, out, out_strides, workspace, workspace_bytes);
+    if (s != REEF_OK) return s;
+    TreeArgs a = {};
+    a.q = q;
+    a.qs = q_scales;
+    a.k = k_cache;
+    a.v = v_cache;
+    a.ks = k_scales;
+    a.vs = v_scales;
+    a.context_lens = context_lens;
+    a.mask = tree_mask;
+    a.out = out;
+    a.status = status_word;
+    return launch_tree<false>(p, a, q_strides, out_strides, workspace, stream);
+}
+
+extern "C" reef_status reef_attention_decode_tree_int8_paged(
+    const reef_tree_params *p, const int8_t *q, const reef_strides *q_strides,
+    const float *q_scales, const int8_t *k_pages, const int8_t *v_pages,
+    const float *k_scale_pages, const float *v_scale_pages, const int32_t *block_table,
+    int64_t max_blocks_per_seq, int64_t num_pages, const int32_t *context_lens,
+    const uint64_t *tree_mask, float *out, const reef_strides *out_strides, void *workspace,
+    size_t workspace_bytes, uint32_t *status_word, hipStream_t stream) {
+    const reef_status s =
+        validate(p, q, q_strides, q_scales, k_pages, v_pages, k_scale_pages, v_scale_pages,
+                 tree_mask, out, out_strides, workspace, workspace_bytes);
+    if (s != REEF_OK) return s;
+    if (!block_table || !context_lens || num_pages <= 0 || num_pages >= (int64_t(1) << 31) ||
+        max_blocks_per_seq * kPage < p->max_context || max_blocks_per_seq >= (int64_t(1) << 30))
+        return REEF_INVALID_ARGUMENT;
+    TreeArgs a = {};
+    a.q = q;
+    a.qs = q_scales;
+    a.k = k_pages;
+    a.v = v_pages;
+    a.ks = k_scale_pages;
+    a.vs = v_scale_pages;
+    a.block_table = block_table;
+    a.max_blocks = (int32_t)max_blocks_per_seq;
+    a.num_pages = (int32_t)num_pages;
+    a.context_lens = context_lens;
+    a.mask = tree_mask;
+    a.out = out;
+    a.status = status_word;
+    return launch_tree<true>(p, a, q_strides, out_strides, workspace, stream);
+}
