@@ -20,9 +20,12 @@
 namespace reef {
 namespace {
 
-constexpr int kWaves = 8;      // waves of a workgroup: two per SIMD
+constexpr int kWaves = 4;      // waves of a workgroup, one per SIMD
+constexpr int kWgPerCu = 2;    // workgroups of a compute unit
+constexpr int kMaxSplit = 2;   // ways a workgroup's waves split the columns, at most
 constexpr int kPlan = 2048;    // sequences of a launch (more are launched in slices)
 constexpr int kMaxDrafts = 64; // bits of a mask word
+constexpr int kMaxGroup = 1024;  // query heads of a kv head
 constexpr int kXcds = 8;       // workgroup i of a launch runs on XCD i % 8
 constexpr int kCounters = 2048;
 
@@ -40,9 +43,11 @@ struct TreeArgs {
     uint32_t *status;
     int64_t q_sb, q_sh, q_st, o_sb, o_sh, o_st;
     int32_t batch, q_heads, kv_heads, group, drafts;
+    uint32_t group_inverse;  // floor(2^32 / group) + 1: i / group for i * group < 2^32
     int32_t max_context, window;
-    int32_t cw;      // the workgroup's waves split the columns cw ways (and the keys 8 / cw)
+    int32_t cw;      // the workgroup's waves split the columns cw ways (and the keys 4 / cw)
     int32_t chunks;  // column ranges of 16 NC cw columns; an item is (sequence, kv head, range)
+    int32_t extra;   // units that an item counts beside its blocks
     int32_t max_blocks, num_pages;  // paged only
     int32_t q_gran;
     float score_scale;  // softmax_scale * log2(e)
@@ -69,14 +74,15 @@ __device__ __forceinline__ SeqKeys seq_keys(const TreeArgs &a, int b) {
     return r;
 }
 
-// sOff[i] = blocks of sequences 0 .. i - 1, for i <= batch (a workgroup-wide scan).
+// sOff[i] = units of an item of each of sequences 0 .. i - 1, added, for i <= batch (a
+// workgroup-wide scan).
 __device__ void plan_blocks(const TreeArgs &a, int32_t *sOff, int32_t *sWave) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (tid == 0) sOff[0] = 0;
     int32_t run = 0;
     for (int base = 0; base < a.batch; base += 64 * kWaves) {
         const int i = base + tid;
-        int32_t x = i < a.batch ? seq_keys(a, i).blocks : 0;
+        int32_t x = i < a.batch ? seq_keys(a, i).blocks + a.extra : 0;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const int32_t y = __shfl_up(x, o);
@@ -94,14 +100,14 @@ __device__ void plan_blocks(const TreeArgs &a, int32_t *sOff, int32_t *sWave) {
     }
 }
 
-// Where a lane's K row and its lane group's page lie, for one 64-key block.
+// Where a 64-key block lies, in units of one kv head's 16-token page: the page of this lane's
+// K row, and that of its lane group.
 struct BlockAt {
-    const int8_t *k, *vt;
-    const float *ks, *vs;
+    uint32_t k_slot, g_slot;
     bool live;  // the lane group's page holds keys of this sequence
 };
 
-template <int D, bool PAGED>
+template <bool PAGED>
 __device__ __forceinline__ BlockAt block_at(const TreeArgs &a, int b, int kvh, int kb,
                                             const SeqKeys &sk, int pages, int col, int grp,
                                             bool &bad_page) {
@@ -111,25 +117,20 @@ __device__ __forceinline__ BlockAt block_at(const TreeArgs &a, int b, int kvh, i
     // may have been given back), are not read: their lanes read a safe page.
     const int n_pages = (sk.len + kPage - 1) / kPage, first = sk.lo / kPage;
     const bool k_in = kp >= first && kp < n_pages, g_in = gp >= first && gp < n_pages;
-    int64_t kt, gt;  // the pages' first tokens
     if (PAGED) {
         const int ke = __shfl(pages, col >> 2), ge = __shfl(pages, grp);
         const bool k_ok = k_in && ke >= 0 && ke < a.num_pages;
         const bool g_ok = g_in && ge >= 0 && ge < a.num_pages;
         bad_page |= g_in && !g_ok;
         r.live = g_ok;
-        kt = ((int64_t)(k_ok ? ke : 0) * a.kv_heads + kvh) * kPage;
-        gt = ((int64_t)(g_ok ? ge : 0) * a.kv_heads + kvh) * kPage;
+        r.k_slot = (uint32_t)((k_ok ? ke : 0) * a.kv_heads + kvh);
+        r.g_slot = (uint32_t)((g_ok ? ge : 0) * a.kv_heads + kvh);
     } else {
-        const int64_t seq = ((int64_t)b * a.kv_heads + kvh) * a.max_context;
+        const uint32_t seq = (uint32_t)((b * a.kv_heads + kvh) * (a.max_context / kPage));
         r.live = g_in;
-        kt = seq + (k_in ? kp : 0) * kPage;
-        gt = seq + (g_in ? gp : 0) * kPage;
+        r.k_slot = seq + (k_in ? kp : 0);
+        r.g_slot = seq + (g_in ? gp : 0);
     }
-    r.k = a.k + (kt + (col & 3)) * D + 16 * grp;
-    r.vt = a.v + gt * D + col * kPage;
-    r.ks = a.ks + gt + col;
-    r.vs = a.vs + gt + col;
     return r;
 }
 
@@ -172,52 +173,46 @@ __device__ __forceinline__ uint32_t bits16(int lo, int hi) {
     return (0xffffu >> (16 - hi)) & ~((1u << lo) - 1u);
 }
 
-// What a lane's column of one tile is: a row of the tree for one query head, or nothing.
+// A column of one tile: a row of the tree for one query head, or nothing.
 struct Column {
-    bool live;       // a column of this launch
-    bool shown;      // its row sees something
+    bool live;  // a column of this launch
     int head, token;
-    float c;         // log2-domain score per unit of the int32 sum and the key's scale
-    int lo;          // the first token before the drafts that it sees
-    uint64_t drafts; // the drafted tokens that it sees
 };
 
-__device__ __forceinline__ Column column_of(const TreeArgs &a, int b, int kvh, int index,
-                                            const SeqKeys &sk) {
-    Column r;
-    r.live = index < a.drafts * a.group;
-    const int i = r.live ? index : 0;
-    r.token = i / a.group;
-    r.head = kvh * a.group + i % a.group;
+__device__ __forceinline__ Column column_of(const TreeArgs &a, int kvh, int index) {
+    const bool live = index < a.drafts * a.group;
+    const int i = live ? index : 0;
+    const int token = a.group == 1 ? i : (int)__umulhi((uint32_t)i, a.group_inverse);
+    return {live, kvh * a.group + i - token * a.group, token};
+}
+
+// What the column's row sees: the first token before the drafts, and the drafted ones.
+struct Sight {
+    int lo;
+    uint64_t drafts;
+};
+
+__device__ __forceinline__ uint64_t mask_word(const TreeArgs &a, int b, int token) {
+    if (!a.mask) return (2ull << token) - 1;
     const uint64_t all = a.drafts == 64 ? ~0ull : (1ull << a.drafts) - 1;
-    const uint64_t *row = a.mask ? a.mask + (int64_t)b * a.drafts : nullptr;
-    uint64_t m = row ? row[r.token] & all : (2ull << r.token) - 1;
-    r.lo = 0;
+    return a.mask[(int64_t)b * a.drafts + token] & all;
+}
+
+__device__ __forceinline__ Sight sight_of(const TreeArgs &a, int b, const SeqKeys &sk, uint64_t m) {
+    Sight r = {0, m};
     if (a.window > 0) {
         // Row i sits at prefix + |mask_i| - 1 (its ancestors before it); a drafted token as
         // far back as the window is hidden.
-        const int depth = __popcll(m) - 1;
+        const int depth = (int)__popcll(m) - 1;
         r.lo = max(0, sk.prefix + depth + 1 - a.window);
         if (a.window < a.drafts) {
             for (int j = 0; j < a.drafts; ++j) {
-                const int dj = __popcll(row ? row[j] & all : (2ull << j) - 1) - 1;
-                if (dj <= depth - a.window) m &= ~(1ull << j);
+                const int dj = (int)__popcll(mask_word(a, b, j)) - 1;
+                if (dj <= depth - a.window) r.drafts &= ~(1ull << j);
             }
         }
     }
-    r.drafts = m;
-    r.shown = r.live && (row ? (row[r.token] & all) != 0 : true) && sk.len > 0;
-    if (!r.shown) {
-        r.lo = INT32_MAX;
-        r.drafts = 0;
-    }
-    float cq = 1.0f;
-    if (r.live)
-        cq = a.q_gran == REEF_SCALE_PER_TENSOR ? a.qs[0]
-             : a.q_gran == REEF_SCALE_PER_HEAD
-                 ? a.qs[r.head]
-                 : a.qs[((int64_t)b * a.q_heads + r.head) * a.drafts + r.token];
-    r.c = cq * a.score_scale;
+    if (m == 0 || sk.len == 0) r = {INT32_MAX, 0};  // padding, or no keys
     return r;
 }
 
@@ -234,86 +229,214 @@ __device__ __forceinline__ uint64_t pack(float x, float y) {
 __device__ __forceinline__ float lo32(uint64_t v) { return __uint_as_float((uint32_t)v); }
 __device__ __forceinline__ float hi32(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
 
-// The launch's work is the 64-key blocks of all items (sequence, kv head, column range),
-// dealt out to the workgroups in equal runs. Within a run each item's part is one segment:
-// the workgroup's eight waves split the range's columns cw ways and the segment's blocks
-// 8 / cw ways, keep a running softmax and merge in LDS. An item inside one run is stored
-// directly; the parts of an item cut by a run's end go to the workspace, and the one that
-// counts in last merges them in order (reef_common.hpp, cross-workgroup parts). Waves that
-// split the columns read the same blocks at about the same time: one reads memory, the
-// others the caches.
+// A workgroup's part of one item (sequence, kv head, column range): its blocks [s_blk, e_blk).
+struct Segment {
+    SeqKeys sk;
+    int b, kvh, chunk, s_blk, e_blk;
+    int first_u;  // the item's first block in the launch's numbering
+    int units;    // of the run, the item's extra ones included
+};
+
+// Waits for this wave's LDS accesses, then for the workgroup; loads in flight stay so
+// (__syncthreads() would wait for them).
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// The kernel's argument, read again: each phase of a segment loads what it needs (from the
+// scalar cache) instead of holding every pointer and stride through the key loop, which
+// spilled a hundred scalar registers into vector lanes.
+__device__ __forceinline__ TreeArgs reread_args() {
+    auto p = __builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const TreeArgs *)p;
+}
+
+// The launch's work is the 64-key blocks of all items, dealt out to the workgroups in equal
+// runs. An item counts some units before its blocks, for the time that its rows, its merge
+// and its stores take: workgroups with many short items get fewer blocks. Within a run each item's part is one segment: the workgroup's four waves split the
+// range's columns cw ways and the segment's blocks 4 / cw ways, keep a running softmax and
+// merge in LDS. An item inside one run is stored directly; the parts of an item cut by a
+// run's end go to the workspace, and the one that counts in last merges them in order
+// (reef_common.hpp, cross-workgroup parts). Waves that split the columns read the same
+// blocks at about the same time: one reads memory, the others the caches.
 template <int D, bool PAGED, int NC>
-__global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(TreeArgs a) {
+__global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs arg) {
     constexpr int DB = D / 16, KS = D / 64;
+    // One tile of columns has one reader of the cache: kept out of the caches.
+    constexpr bool NT = !PAGED && NC == 1;
     __shared__ int32_t sOff[kPlan + 1];
     __shared__ int32_t sWave[kWaves];
     __shared__ f32x4 sO[kWaves][DB][kWave];
     __shared__ float2 sML[kWaves][kWave];
+    __shared__ i32x4 sQ[kWaves][NC * KS][kWave];  // query operands, each wave its own
+    __shared__ Sight sSight[kWaves][NC][16];
     __shared__ uint32_t sLast;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
-    const int CW = a.cw, KW = kWaves / CW;
+    const int CW = arg.cw, KW = kWaves / CW;
     const int cwi = wave % CW, kwi = wave / CW;
 
-    const bool same = a.context_lens == nullptr;
-    const int nb = same ? seq_keys(a, 0).blocks : 0;
-    if (!same) plan_blocks(a, sOff, sWave);
-    auto blocks_before = [&](int b) -> int {  // of the sequences before b
+    const bool same = arg.context_lens == nullptr;
+    const int nb = same ? seq_keys(arg, 0).blocks + arg.extra : 0;
+    if (!same) plan_blocks(arg, sOff, sWave);
+    auto units_before = [&](int b) -> int {  // of an item of each sequence before b
         return same ? b * nb : __builtin_amdgcn_readfirstlane(sOff[b]);
     };
-    const int per_seq = a.kv_heads * a.chunks;  // items of a sequence
-    const int64_t T = (int64_t)blocks_before(a.batch) * per_seq;
+    const int per_seq = arg.kv_heads * arg.chunks;  // items of a sequence
+    const int T = units_before(arg.batch) * per_seq;  // (fits: checked for full caches)
     // No more workgroups than there are items, or parts with a block for every wave.
-    const int64_t G = min((int64_t)gridDim.x,
-                          max((int64_t)a.batch * per_seq, (T + KW - 1) / KW));
+    const int items = arg.batch * per_seq;
+    const int G = min((int)gridDim.x, max(items, (T - items * arg.extra + KW - 1) / KW));
+    // Workgroup w's run: T / G units, one more for each of the first T % G.
+    const int quota = T / G, longer = T - quota * G;
+    auto run_start = [&](int w) { return w * quota + min(w, longer); };
+    auto run_of = [&](int u) {
+        const int mid = longer * (quota + 1);
+        return u < mid ? u / (quota + 1) : longer + (u - mid) / quota;
+    };
     // The workgroups of one XCD hold consecutive runs: the column ranges of one (sequence,
     // kv head) meet in its L2.
     const int x = blockIdx.x % kXcds, place = blockIdx.x / kXcds;
-    const int64_t per = G / kXcds, rem = G % kXcds;
+    const int per = G / kXcds, rem = G % kXcds;
     if (place >= per + (x < rem ? 1 : 0)) return;
-    const int64_t g = x * per + min((int64_t)x, rem) + place;
-    int64_t u = wg_start(g, T, G);
-    const int64_t u0 = u, u1 = wg_start(g + 1, T, G);
-    int b = 0;
-    {
-        int hi = a.batch - 1;
-        while (b < hi) {
-            const int mid = (b + hi + 1) >> 1;
-            if ((int64_t)blocks_before(mid) * per_seq <= u0) b = mid;
-            else hi = mid - 1;
-        }
-    }
+    const int g = x * per + min(x, rem) + place;
+    const int u0 = run_start(g), u1 = run_start(g + 1);
 
-    while (u < u1) {
-        SeqKeys sk = seq_keys(a, b);
-        sk.len = __builtin_amdgcn_readfirstlane(sk.len);
-        sk.prefix = __builtin_amdgcn_readfirstlane(sk.prefix);
-        sk.lo = __builtin_amdgcn_readfirstlane(sk.lo);
-        sk.first_block = __builtin_amdgcn_readfirstlane(sk.first_block);
-        sk.blocks = __builtin_amdgcn_readfirstlane(sk.blocks);
-        const int64_t seq_u0 = (int64_t)blocks_before(b) * per_seq;
-        const int in_seq = (int)(u - seq_u0);
-        const int hc = in_seq / sk.blocks, s_blk = in_seq - hc * sk.blocks;
-        const int e_blk = (int)min((int64_t)sk.blocks, s_blk + (u1 - u));
-        const int kvh = hc / a.chunks, chunk = hc % a.chunks;
-        const int64_t item_u0 = u - s_blk;
-        if (sk.bad && s_blk == 0 && hc == 0 && threadIdx.x == 0)
-            flag_status(a.status, REEF_STATUS_BIT_BAD_LENGTH);
+    auto segment_at = [&](const TreeArgs &a, int u, int b) {
+        Segment s;
+        s.b = b;
+        s.sk = seq_keys(a, b);
+        s.sk.len = __builtin_amdgcn_readfirstlane(s.sk.len);
+        s.sk.prefix = __builtin_amdgcn_readfirstlane(s.sk.prefix);
+        s.sk.lo = __builtin_amdgcn_readfirstlane(s.sk.lo);
+        s.sk.first_block = __builtin_amdgcn_readfirstlane(s.sk.first_block);
+        s.sk.blocks = __builtin_amdgcn_readfirstlane(s.sk.blocks);
+        const int in_seq = u - units_before(b) * per_seq;
+        const int per_item = s.sk.blocks + a.extra, hc = in_seq / per_item;
+        const int at = in_seq - hc * per_item, end = min(per_item, at + (u1 - u));
+        s.s_blk = max(0, at - a.extra);
+        s.e_blk = max(0, end - a.extra);  // (none where the run ends before the item's blocks)
+        s.units = end - at;
+        s.kvh = hc / a.chunks;
+        s.chunk = hc - s.kvh * a.chunks;
+        s.first_u = u - at + a.extra;
+        return s;
+    };
+    auto first_key = [&](const Segment &s) {
+        return (s.sk.first_block + s.s_blk + kwi) * kBlockKeys;
+    };
+    auto end_key = [&](const Segment &s) {
+        return min(s.sk.len, (s.sk.first_block + s.e_blk) * kBlockKeys);
+    };
+    auto first_tile = [&](const Segment &s) { return (s.chunk * CW + cwi) * NC; };
+    auto column = [&](const TreeArgs &a, const Segment &s, int t) {
+        return column_of(a, s.kvh, 16 * (first_tile(s) + t) + col);
+    };
+    const int k_step = KW * kBlockKeys;
 
-        const int tile0 = (chunk * CW + cwi) * NC;  // this wave's first tile
-        Column cn[NC];
-        i32x4 qop[NC][KS];
+    // A block's operands, and what a segment's rows need, in registers.
+    i32x4 kop[4][KS], vop[DB], qreg[NC][KS];
+    float ks = 0.0f, vs = 0.0f, c[NC];
+    uint64_t mreg[NC];
+    BlockAt at;
+    bool bad_page = false;
+    int pg_next;
+    auto load_k = [&](const TreeArgs &a) {
+        const int8_t *p = a.k + (int64_t)at.k_slot * (kPage * D) + (col & 3) * D + 16 * grp;
 #pragma unroll
-        for (int t = 0; t < NC; ++t) {
-            cn[t] = column_of(a, b, kvh, 16 * (tile0 + t) + col, sk);
-            const int8_t *qrow = a.q + b * a.q_sb + cn[t].head * a.q_sh + cn[t].token * a.q_st;
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int s = 0; s < KS; ++s)
-                qop[t][s] = cn[t].live ? *reinterpret_cast<const i32x4 *>(qrow + 64 * s + 16 * grp)
-                                       : i32x4{0, 0, 0, 0};
+                kop[t][s] = load_stream<NT>(reinterpret_cast<const i32x4 *>(p + 4 * t * D + 64 * s));
+        ks = a.ks[(int64_t)at.g_slot * kPage + col];
+    };
+    auto load_v = [&](const TreeArgs &a) {
+        const int8_t *p = a.v + (int64_t)at.g_slot * (kPage * D) + col * kPage;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+            vop[d] = load_stream<NT>(reinterpret_cast<const i32x4 *>(p + 16 * d * kPage));
+        vs = a.vs[(int64_t)at.g_slot * kPage + col];
+    };
+    // Whether this wave has anything to do in a segment.
+    auto busy = [&](const TreeArgs &a, const Segment &s) {
+        return 16 * first_tile(s) < a.drafts * a.group && first_key(s) < end_key(s);
+    };
+    // The loads of a segment's rows, and of its first block where `block` (pages: its table
+    // entries).
+    auto issue = [&](const TreeArgs &a, const Segment &s, int pages, bool block) {
+        if (!busy(a, s)) return;
+#pragma unroll
+        for (int t = 0; t < NC; ++t) {
+            const Column cn = column(a, s, t);
+            mreg[t] = mask_word(a, s.b, cn.token);
+            c[t] = a.q_gran == REEF_SCALE_PER_TENSOR ? a.qs[0]
+                   : a.q_gran == REEF_SCALE_PER_HEAD
+                       ? a.qs[cn.head]
+                       : a.qs[((int64_t)s.b * a.q_heads + cn.head) * a.drafts + cn.token];
+            const int8_t *qrow = a.q + s.b * a.q_sb + cn.head * a.q_sh + cn.token * a.q_st;
+#pragma unroll
+            for (int e = 0; e < KS; ++e)
+                qreg[t][e] = *reinterpret_cast<const i32x4 *>(qrow + 64 * e + 16 * grp);
         }
-        const bool wave_live = 16 * tile0 < a.drafts * a.group;  // wave-uniform
+        if (!block) return;
+        at = block_at<PAGED>(a, s.b, s.kvh, first_key(s), s.sk, pages, col, grp, bad_page);
+        load_k(a);
+        load_v(a);
+    };
+
+    // The run's first sequence: the last one that begins at or before u0, among 64 evenly
+    // spaced ones, then among the kPlan / 64 of its stretch.
+    int b = 0;
+    if (same) {
+        b = u0 / (nb * per_seq);
+    } else {
+        constexpr int kStretch = kPlan / 64;
+        static_assert(kStretch <= 64, "two steps of a wave");
+        const int far = lane * kStretch;
+        b = kStretch * (__popcll(__ballot(far < arg.batch && sOff[far] * per_seq <= u0)) - 1);
+        const int near = b + lane;
+        b += __popcll(__ballot(lane < kStretch && near < arg.batch && sOff[near] * per_seq <= u0)) - 1;
+        b = __builtin_amdgcn_readfirstlane(b);
+    }
+    Segment seg = segment_at(arg, u0, b);
+    if (seg.e_blk <= seg.s_blk) return;  // (uniform)
+    pg_next = block_pages<PAGED>(arg, b, first_key(seg) + k_step, seg.sk, lane);
+    issue(arg, seg, block_pages<PAGED>(arg, b, first_key(seg), seg.sk, lane), true);
+    for (int u = u0;;) {
+        TreeArgs a = reread_args();
+        if (seg.sk.bad && seg.s_blk == 0 && seg.kvh == 0 && seg.chunk == 0 && threadIdx.x == 0)
+            flag_status(a.status, REEF_STATUS_BIT_BAD_LENGTH);
+        const bool mine = busy(a, seg);  // wave-uniform
+        // This segment's rows: operands and sights to LDS (this wave's own places).
+        float cs[NC];
+        uint32_t shown = 0;  // bit t: this lane's row of tile t sees something
+        if (mine) {
+#pragma unroll
+            for (int t = 0; t < NC; ++t) {
+                const bool live = column(a, seg, t).live;
+#pragma unroll
+                for (int e = 0; e < KS; ++e)
+                    sQ[wave][t * KS + e][lane] = live ? qreg[t][e] : i32x4{0, 0, 0, 0};
+                cs[t] = live ? c[t] * a.score_scale : 1.0f;
+                shown |= (mreg[t] != 0 ? 1u : 0u) << t;
+                const Sight sight = sight_of(a, seg.b, seg.sk, live ? mreg[t] : 0);
+                if (grp == 0) sSight[wave][t][col] = sight;
+            }
+        }
+        // The next segment, and the table entries of its first two blocks.
+        u += seg.units;
+        bool more_segs = u < u1;
+        Segment nxt = seg;
+        int pg_first = 0, pg_second = 0;
+        if (more_segs) {
+            const bool same_seq = u < units_before(seg.b + 1) * per_seq;
+            nxt = segment_at(a, u, same_seq ? seg.b : seg.b + 1);
+            more_segs = nxt.e_blk > nxt.s_blk;
+            pg_first = block_pages<PAGED>(a, nxt.b, first_key(nxt), nxt.sk, lane);
+            pg_second = block_pages<PAGED>(a, nxt.b, first_key(nxt) + k_step, nxt.sk, lane);
+        }
 
         float m_run[NC], l_run[NC], s_run = 0.0f, inv_s = 0.0f;
         f32x4 acc[NC][DB];
@@ -324,76 +447,62 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(TreeArgs a) {
 #pragma unroll
             for (int d = 0; d < DB; ++d) acc[t][d] = f32x4{};
         }
-        bool bad_page = false;
-        const int k_begin = (sk.first_block + s_blk + kwi) * kBlockKeys;
-        const int k_end = min(sk.len, (sk.first_block + e_blk) * kBlockKeys);
-        const int k_step = KW * kBlockKeys;
+        const int k_end = end_key(seg);
         // Keys that every row sees: [full_lo, prefix).
-        const int full_lo = a.window > 0 ? max(0, sk.prefix + a.drafts - a.window) : 0;
-        if (wave_live && k_begin < k_end) {
-            i32x4 kop[4][KS], vop[DB];
-            float ks, vs;
-            BlockAt at = block_at<D, PAGED>(a, b, kvh, k_begin, sk,
-                                            block_pages<PAGED>(a, b, k_begin, sk, lane), col, grp,
-                                            bad_page);
-            auto load_k = [&](const BlockAt &p) {
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int s = 0; s < KS; ++s)
-                        kop[t][s] = *reinterpret_cast<const i32x4 *>(p.k + 4 * t * D + 64 * s);
-                ks = *p.ks;
-            };
-            auto load_v = [&](const BlockAt &p) {
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-                    vop[d] = *reinterpret_cast<const i32x4 *>(p.vt + 16 * d * kPage);
-                vs = *p.vs;
-            };
-            load_k(at);
-            load_v(at);
-            int pg_next = block_pages<PAGED>(a, b, k_begin + k_step, sk, lane);
-            for (int kb = k_begin; kb < k_end; kb += k_step) {
+        const int full_lo = a.window > 0 ? max(0, seg.sk.prefix + a.drafts - a.window) : 0;
+        if (mine) {
+            for (int kb = first_key(seg); kb < k_end; kb += k_step) {
                 const bool more = kb + k_step < k_end;
                 const bool live = at.live;
-                const int pg_after = block_pages<PAGED>(a, b, kb + 2 * k_step, sk, lane);
+                const int pg_after = block_pages<PAGED>(a, seg.b, kb + 2 * k_step, seg.sk, lane);
                 // Scores of every tile, times the key's scale.
                 float xs[NC][16];
                 {
                     float ksc[16];
                     row_lanes(ks, ksc);
 #pragma unroll
-                    for (int t = 0; t < NC; ++t)
+                    for (int t = 0; t < NC; ++t) {
+                        i32x4 qop[KS];
+#pragma unroll
+                        for (int e = 0; e < KS; ++e) qop[e] = sQ[wave][t * KS + e][lane];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             i32x4 s = {0, 0, 0, 0};
 #pragma unroll
-                            for (int e = 0; e < KS; ++e) s = mfma_16x16x64_i8(kop[j][e], qop[t][e], s);
+                            for (int e = 0; e < KS; ++e) s = mfma_16x16x64_i8(kop[j][e], qop[e], s);
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
                                 xs[t][4 * j + i] = (float)s[i] * ksc[4 * j + i];
                         }
+                    }
                 }
-                // The key registers are free: the next block's keys fly from here on, its
-                // values from the end of the products on.
-                if (more) {
-                    at = block_at<D, PAGED>(a, b, kvh, kb + k_step, sk, pg_next, col, grp, bad_page);
-                    load_k(at);
+                __builtin_amdgcn_sched_barrier(0);
+                // The key registers are free: the next block's keys fly from here on (after a
+                // segment's last block the next segment's first), its values as the products
+                // below free theirs. With nothing to follow, this block's are read again.
+                if (more || more_segs) {
+                    at = block_at<PAGED>(a, more ? seg.b : nxt.b, more ? seg.kvh : nxt.kvh,
+                                         more ? kb + k_step : first_key(nxt), more ? seg.sk : nxt.sk,
+                                         more ? pg_next : pg_first, col, grp, bad_page);
                 }
+                load_k(a);
+                const int8_t *v_next = a.v + (int64_t)at.g_slot * (kPage * D) + col * kPage;
+                __builtin_amdgcn_sched_barrier(0);
                 pg_next = pg_after;
                 // Blocks that every row sees whole skip the masks. In the others a hidden key's
                 // score is -inf, and the value scale of a key that no row of the wave sees
                 // is 0 (the cache there may hold anything).
                 const int kk = kb + 16 * grp;
                 float vsc = vs;
-                if (kb < full_lo || kb + kBlockKeys > sk.prefix || !__all(live)) {
+                if (kb < full_lo || kb + kBlockKeys > seg.sk.prefix || !__all(live)) {
                     uint32_t any = 0;
 #pragma unroll
                     for (int t = 0; t < NC; ++t) {
-                        uint32_t vis = bits16(cn[t].lo - kk, sk.prefix - kk);
-                        const int j = kk - sk.prefix;  // drafted token of this group's first key
-                        vis |= (j >= 0 ? (j < 64 ? (uint32_t)(cn[t].drafts >> j) : 0u)
-                                       : (j > -16 ? (uint32_t)(cn[t].drafts << -j) : 0u)) & 0xffffu;
+                        const Sight sight = sSight[wave][t][col];
+                        uint32_t vis = bits16(sight.lo - kk, seg.sk.prefix - kk);
+                        const int j = kk - seg.sk.prefix;  // drafted token of the group's first key
+                        vis |= (j >= 0 ? (j < 64 ? (uint32_t)(sight.drafts >> j) : 0u)
+                                       : (j > -16 ? (uint32_t)(sight.drafts << -j) : 0u)) & 0xffffu;
                         if (!live) vis = 0;
 #pragma unroll
                         for (int r = 0; r < 16; ++r)
@@ -412,7 +521,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(TreeArgs a) {
                     for (int r = 3; r < 15; r += 2) m = fmaxf(fmaxf(m, xs[t][r]), xs[t][r + 1]);
                     m = fmaxf(m, xs[t][15]);
                     m = fmaxf(m, __shfl_xor(m, 16));
-                    mt[t] = xor32_max(m) * cn[t].c;
+                    mt[t] = xor32_max(m) * cs[t];
                     grow |= mt[t] > m_run[t] + 6.0f;
                 }
                 float vmax = row_fmax(vsc);
@@ -455,60 +564,88 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(TreeArgs a) {
 #pragma unroll
                             for (int e = 0; e < 8; ++e) {
                                 const float p = __builtin_amdgcn_exp2f(
-                                    __builtin_fmaf(xs[t][8 * h + e], cn[t].c, -m_use));
+                                    __builtin_fmaf(xs[t][8 * h + e], cs[t], -m_use));
                                 sum[e & 1] += p;
                                 w[e] = p * vv[8 * h + e];
                             }
                             split_weights(w, hi[t][h], lo[t][h]);
                         }
                         l_run[t] += sum[0] + sum[1];
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 }
+                if (NC > 1) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    f16x8 v0, v1;
-                    int8x16_to_f16(vop[d], v0, v1);
+                for (int d = 0; d < DB; d += 2) {
+                    f16x8 v[2][2];
 #pragma unroll
-                    for (int t = 0; t < NC; ++t) {
-                        acc[t][d] = mfma_16x16x32_f16(v0, hi[t][0], acc[t][d]);
-                        acc[t][d] = mfma_16x16x32_f16(v0, lo[t][0], acc[t][d]);
-                        acc[t][d] = mfma_16x16x32_f16(v1, hi[t][1], acc[t][d]);
-                        acc[t][d] = mfma_16x16x32_f16(v1, lo[t][1], acc[t][d]);
+                    for (int i = 0; i < 2; ++i) {
+                        int8x16_to_f16(vop[d + i], v[i][0], v[i][1]);
+                        vop[d + i] = load_stream<NT>(
+                            reinterpret_cast<const i32x4 *>(v_next + 16 * (d + i) * kPage));
+                    }
+                    // Products of one accumulator are NC * 2 apart.
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int t = 0; t < NC; ++t)
+                                acc[t][d + i] = mfma_16x16x32_f16(v[i][h], hi[t][h], acc[t][d + i]);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int t = 0; t < NC; ++t)
+                                acc[t][d + i] = mfma_16x16x32_f16(v[i][h], lo[t][h], acc[t][d + i]);
                     }
                 }
-                if (more) load_v(at);
+                if (NC > 1) __builtin_amdgcn_s_setprio(0);
+                vs = a.vs[(int64_t)at.g_slot * kPage + col];
             }
         }
+        a = reread_args();
         if (bad_page) flag_status(a.status, REEF_STATUS_BIT_BAD_PAGE);
+        bad_page = false;
+        // The next segment's rows and first block fly while this one is merged.
+        if (more_segs) {
+            issue(a, nxt, pg_first, !mine);
+            pg_next = pg_second;
+        }
+        a = reread_args();
 
         // The workgroups that hold a part of this item: gf .. gl, each with at least one block.
-        const int gf = wg_of(item_u0, T, G), gl = wg_of(item_u0 + sk.blocks - 1, T, G);
-        const int parts = gl - gf + 1;
+        const int gf = run_of(seg.first_u);
+        const int parts = run_of(seg.first_u + seg.sk.blocks - 1) - gf + 1;
         const int64_t slot_elems = (int64_t)CW * NC * TreeSlot<D>::ELEMS;
-        // A part's slot is its workgroup's first, unless its item begins inside the run.
-        uint64_t *mine = a.slots + (2 * g + (item_u0 <= u0 ? 0 : 1)) * slot_elems;
+        // A workgroup has two slots: for an item that begins in its run, and one that began
+        // before.
+        uint64_t *own = a.slots + (2 * (int64_t)g + (g == gf ? 1 : 0)) * slot_elems;
         auto tile_slot = [&](uint64_t *s, int t) {
             return s + (cwi * NC + t) * TreeSlot<D>::ELEMS;
         };
-        auto store_out = [&](const Column &c, int d, f32x4 o, float l) {
-            if (!c.live) return;
-            const float inv = c.shown && l > 0.0f ? 1.0f / l : 0.0f;
-            float *row = a.out + b * a.o_sb + c.head * a.o_sh + c.token * a.o_st;
+        auto store_out = [&](const Column &cn, int d, f32x4 o, float l) {
+            if (!cn.live) return;
+            float *row = a.out + seg.b * a.o_sb + cn.head * a.o_sh + cn.token * a.o_st;
             f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (inv > 0.0f) y = o * inv;
+            if (l > 0.0f) y = o * (1.0f / l);
             *reinterpret_cast<f32x4 *>(row + 16 * d + 4 * grp) = y;
         };
         // The key-split waves of a column range merge tile by tile through LDS, each the
-        // channel blocks d = kwi, kwi + KW, ...
+        // channel blocks d = kwi, kwi + KW, ... A row that sees nothing has the sum 0.
 #pragma unroll
         for (int t = 0; t < NC; ++t) {
+            const Column cn = column(a, seg, t);
             float l = l_run[t];
             l += __shfl_xor(l, 16);
             l = xor32_sum(l);
+            if (!(shown >> t & 1u)) {
+                l = 0.0f;
+                m_run[t] = -INFINITY;
+            }
 #pragma unroll
             for (int d = 0; d < DB; ++d) sO[wave][d][lane] = acc[t][d] * (s_run * (1.0f / 256.0f));
             sML[wave][lane] = float2{m_run[t], l};
-            __syncthreads();
+            lds_barrier();
             float m = -INFINITY;
             for (int w = cwi; w < kWaves; w += CW) m = fmaxf(m, sML[w][lane].x);
             l = 0.0f;
@@ -532,16 +669,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(TreeArgs a) {
                         for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(scale[i], p[e], o[e]);
                     }
                 if (parts == 1) {
-                    store_out(cn[t], d, o, l);
-                } else if (cn[t].live) {
-                    uint64_t *s = tile_slot(mine, t);
+                    store_out(cn, d, o, l);
+                } else if (cn.live) {
+                    uint64_t *s = tile_slot(own, t);
                     part_store(s + (2 * d) * kWave + lane, pack(o[0], o[1]));
                     part_store(s + (2 * d + 1) * kWave + lane, pack(o[2], o[3]));
                 }
             }
-            if (parts > 1 && kwi == 0 && cn[t].live)
-                part_store(tile_slot(mine, t) + TreeSlot<D>::O * kWave + lane, pack(m, l));
-            __syncthreads();  // frees sO / sML
+            if (parts > 1 && kwi == 0 && cn.live)
+                part_store(tile_slot(own, t) + TreeSlot<D>::O * kWave + lane, pack(m, l));
+            lds_barrier();  // frees sO / sML
         }
         if (parts > 1) {
             part_stores_done();
@@ -552,25 +689,28 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(TreeArgs a) {
             if (__builtin_amdgcn_readfirstlane(sLast)) {
                 part_claimed();
                 if (threadIdx.x == 0) part_reset(a.counters + gf);
-                const bool first_second = wg_start(gf, T, G) < item_u0;
                 constexpr int kAhead = 4;  // parts whose loads are in flight together
 #pragma unroll
                 for (int t = 0; t < NC; ++t) {
-                    if (!cn[t].live) continue;
-                    for (int d = kwi; d < DB; d += KW) {
+                    const Column cn = column(a, seg, t);
+                    if (!cn.live) continue;
+                    for (int d = kwi; d < DB; d += 2 * KW) {  // (DB / KW is 1 or even)
+                        const int d2 = min(d + KW, DB - 1);
                         float m = -INFINITY, l = 0.0f;
-                        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+                        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f}, o2 = o;
                         for (int p0 = 0; p0 < parts; p0 += kAhead) {
-                            uint64_t ml[kAhead], v0[kAhead], v1[kAhead];
+                            uint64_t ml[kAhead], v0[kAhead], v1[kAhead], w0[kAhead], w1[kAhead];
 #pragma unroll
                             for (int i = 0; i < kAhead; ++i) {
                                 const int p = min(p0 + i, parts - 1);
                                 uint64_t *s = tile_slot(
-                                    a.slots + (2 * (int64_t)(gf + p) + (p == 0 && first_second)) *
+                                    a.slots + (2 * (int64_t)(gf + p) + (p == 0 ? 1 : 0)) *
                                                   slot_elems, t);
                                 ml[i] = part_load(s + TreeSlot<D>::O * kWave + lane);
                                 v0[i] = part_load(s + (2 * d) * kWave + lane);
                                 v1[i] = part_load(s + (2 * d + 1) * kWave + lane);
+                                w0[i] = part_load(s + (2 * d2) * kWave + lane);
+                                w1[i] = part_load(s + (2 * d2 + 1) * kWave + lane);
                             }
 #pragma unroll
                             for (int i = 0; i < kAhead; ++i) {
@@ -583,17 +723,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(TreeArgs a) {
                                 o[1] = __builtin_fmaf(ep, hi32(v0[i]), o[1] * er);
                                 o[2] = __builtin_fmaf(ep, lo32(v1[i]), o[2] * er);
                                 o[3] = __builtin_fmaf(ep, hi32(v1[i]), o[3] * er);
+                                o2[0] = __builtin_fmaf(ep, lo32(w0[i]), o2[0] * er);
+                                o2[1] = __builtin_fmaf(ep, hi32(w0[i]), o2[1] * er);
+                                o2[2] = __builtin_fmaf(ep, lo32(w1[i]), o2[2] * er);
+                                o2[3] = __builtin_fmaf(ep, hi32(w1[i]), o2[3] * er);
                                 m = mn;
                             }
                         }
-                        store_out(cn[t], d, o, l);
+                        store_out(cn, d, o, l);
+                        if (d + KW < DB) store_out(cn, d2, o2, l);
                     }
                 }
             }
             __syncthreads();  // sLast is read before the next segment writes it
         }
-        u += e_blk - s_blk;
-        if (u == seq_u0 + (int64_t)sk.blocks * per_seq) ++b;
+        if (!more_segs) break;
+        seg = nxt;
     }
 }
 
@@ -602,7 +747,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_kernel(TreeArgs a) {
 // How a launch of `batch` sequences is laid out: tiles per wave, the ways the waves split the
 // columns, the column ranges, and the workgroups.
 struct TreeShape {
-    int64_t nc, cw, chunks, wgs;
+    int64_t nc, cw, chunks, wgs, extra;
 };
 
 TreeShape tree_shape(const reef_tree_params *p, int64_t batch) {
@@ -611,17 +756,12 @@ TreeShape tree_shape(const reef_tree_params *p, int64_t batch) {
     const int64_t tiles = ceil_div(p->draft_len * (p->q_heads / p->kv_heads), 16);
     s.nc = tiles > 1 ? 2 : 1;
     s.cw = 1;
-    while (s.cw < kWaves && s.cw * s.nc < tiles) s.cw *= 2;
+    while (s.cw < kMaxSplit && s.cw * s.nc < tiles) s.cw *= 2;
     s.chunks = ceil_div(tiles, s.nc * s.cw);
-    // Columns are rather split over workgroups than keys while that gives no more items than
-    // compute units: column ranges have nothing to merge.
-    while (s.cw > 1 && 2 * batch * p->kv_heads * s.chunks <= cus) {
-        s.cw /= 2;
-        s.chunks = ceil_div(tiles, s.nc * s.cw);
-    }
+    s.extra = (s.nc == 2 ? 5 : 2) * (kWaves / s.cw);
     const int64_t units =
         batch * p->kv_heads * s.chunks * ceil_div(p->max_context, kBlockKeys);
-    s.wgs = std::max<int64_t>(1, std::min(std::min(cus, units), (int64_t)kCounters));
+    s.wgs = std::max<int64_t>(1, std::min(std::min(kWgPerCu * cus, units), (int64_t)kCounters));
     return s;
 }
 
@@ -646,7 +786,7 @@ bool params_ok(const reef_tree_params *p) {
 
 bool params_supported(const reef_tree_params *p) {
     return (p->head_dim == 64 || p->head_dim == 128) && p->draft_len <= kMaxDrafts &&
-           p->q_heads <= 65535 && p->batch <= 65535 && p->max_context < (int64_t(1) << 30);
+           p->q_heads <= 65535 && p->q_heads / p->kv_heads <= kMaxGroup && p->batch <= 65535 && p->max_context < (int64_t(1) << 30);
 }
 
 bool strides_ok(const reef_strides *s, int64_t unit) {
@@ -674,9 +814,12 @@ reef_status validate(const reef_tree_params *p, const int8_t *q, const reef_stri
     if (!workspace || !aligned(workspace, 16) ||
         workspace_bytes < (size_t)tree_workspace(p))
         return REEF_INVALID_ARGUMENT;
+    // pages of one kv head are numbered in 31 bits (of 2 KB each, keys and values)
+    if (p->batch * p->kv_heads * (p->max_context / kPage) >= (int64_t(1) << 31))
+        return REEF_UNSUPPORTED;
     const TreeShape s = tree_shape(p, std::min<int64_t>(p->batch, kPlan));
     if (std::min<int64_t>(p->batch, kPlan) * p->kv_heads * s.chunks *
-            ceil_div(p->max_context, kBlockKeys) >= (int64_t(1) << 31))
+            (ceil_div(p->max_context, kBlockKeys) + s.extra) >= (int64_t(1) << 31))
         return REEF_UNSUPPORTED;
     return REEF_OK;
 }
@@ -694,6 +837,7 @@ reef_status launch_tree(const reef_tree_params *p, TreeArgs &a, const reef_strid
     a.q_heads = (int32_t)Hq;
     a.kv_heads = (int32_t)p->kv_heads;
     a.group = (int32_t)(Hq / p->kv_heads);
+    a.group_inverse = (uint32_t)((uint64_t(1) << 32) / (uint64_t)a.group + 1);
     a.drafts = (int32_t)T;
     a.max_context = (int32_t)p->max_context;
     a.window = (int32_t)std::min<int64_t>(p->window, int64_t(1) << 30);
@@ -708,6 +852,7 @@ reef_status launch_tree(const reef_tree_params *p, TreeArgs &a, const reef_strid
         c.batch = (int32_t)batch;
         c.cw = (int32_t)s.cw;
         c.chunks = (int32_t)s.chunks;
+        c.extra = (int32_t)s.extra;
         c.q += b0 * a.q_sb;
         c.out += b0 * a.o_sb;
         if (a.q_gran == REEF_SCALE_PER_TOKEN) c.qs += b0 * Hq * T;
@@ -783,6 +928,7 @@ extern "C" reef_status reef_attention_decode_tree_int8_paged(
     if (!block_table || !context_lens || num_pages <= 0 || num_pages >= (int64_t(1) << 31) ||
         max_blocks_per_seq * kPage < p->max_context || max_blocks_per_seq >= (int64_t(1) << 30))
         return REEF_INVALID_ARGUMENT;
+    if (num_pages * p->kv_heads >= (int64_t(1) << 31)) return REEF_UNSUPPORTED;
     TreeArgs a = {};
     a.q = q;
     a.qs = q_scales;
