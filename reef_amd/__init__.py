@@ -273,6 +273,20 @@ def _require(t, dtype, name):
     raise InvalidArgument(f"{name} must be a GPU tensor")
 
 
+def _expect(what, dtype, *tensors):
+    """(tensor, name) pairs: contiguous, of one type, on the current device, whose stream the
+    call takes."""
+    device = _torch()._C._cuda_getDevice()
+    for t, name in tensors:
+        try:
+            if t.dtype is dtype and t.get_device() == device and t.is_contiguous():
+                continue
+        except AttributeError:
+            pass
+        _require(t, dtype, name)
+        raise InvalidArgument(f"{what}: {name} must be contiguous and on the current GPU")
+
+
 def _on_device(what, *tensors):
     """Every tensor (None: absent) lies on the current device, whose stream the call takes."""
     device = _torch()._C._cuda_getDevice()
@@ -659,38 +673,41 @@ def _tree_workspace(n, device, stream):
 
 
 def _tree_inputs(what, q, q_scales, tree_mask, window, softmax_scale, q_granularity, kv_heads,
-                 max_context, context_lens, out):
+                 max_context, head_dim, context_lens, out):
     torch = _torch()
     _require(q, torch.int8, "q")
-    _require(q_scales, torch.float32, "q_scales")
-    if q.dim() != 4:
-        raise InvalidArgument(f"{what}: q must be [B, heads, drafts, head_dim]")
-    B, Hq, T, D = q.shape
-    scales = {PER_TENSOR: 1, PER_HEAD: Hq, PER_TOKEN: B * Hq * T}.get(q_granularity)
+    if q.dim() != 4 or q.shape[3] != head_dim:
+        raise InvalidArgument(f"{what}: q must be [B, heads, drafts, head_dim of the cache]")
+    B, Hq, T, D = shape = q.shape
+    if not q_scales.is_contiguous():
+        q_scales = q_scales.contiguous()
+    _expect(what, torch.float32, (q_scales, "q_scales"))
+    scales = B * Hq * T if q_granularity == PER_TOKEN else Hq if q_granularity == PER_HEAD else 1
     if q_scales.numel() != scales:
         raise InvalidArgument(f"{what}: q_scales do not match q_granularity")
     if tree_mask is not None:
-        _require(tree_mask, torch.int64, "tree_mask")
-        if tuple(tree_mask.shape) != (B, T):
+        if not tree_mask.is_contiguous():
+            tree_mask = tree_mask.contiguous()
+        _expect(what, torch.int64, (tree_mask, "tree_mask"))
+        if tree_mask.shape != (B, T):
             raise InvalidArgument(f"{what}: tree_mask must be [B, drafts] int64")
-        tree_mask = tree_mask.contiguous()
     if context_lens is not None:
-        _require(context_lens, torch.int32, "context_lens")
-        if tuple(context_lens.shape) != (B,):
+        _expect(what, torch.int32, (context_lens, "context_lens"))
+        if context_lens.shape != (B,):
             raise InvalidArgument(f"{what}: context_lens must be [B]")
-        context_lens = context_lens.contiguous()
     if out is None:
-        out = torch.empty((B, Hq, T, D), dtype=torch.float32, device=q.device)
+        out = torch.empty(shape, dtype=torch.float32, device=q.device)
+        _on_device(what, q)
     else:
         _require(out, torch.float32, "out")
-        if out.shape != q.shape:
+        if out.shape != shape:
             raise InvalidArgument(f"{what}: out must have q's shape")
-    _on_device(what, q, q_scales, tree_mask, context_lens, out)
+        _on_device(what, q, out)
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(D)
     p = _packed(_TREE, TreeParams, B, Hq, kv_heads, D, T, max_context, window, softmax_scale,
                 q_granularity, 0, 0)
-    return p, q_scales.contiguous(), tree_mask, context_lens, out
+    return p, q_scales, tree_mask, out
 
 
 def attention_decode_tree(q, q_scales, k_cache, v_pages, k_scales, v_scales, context_lens=None, *,
@@ -705,13 +722,11 @@ def attention_decode_tree(q, q_scales, k_cache, v_pages, k_scales, v_scales, con
     drafted token j (itself among them; 0: padding, zeros), None for a chain. Returns fp32
     [B, Hq, T, D].
     """
-    _contiguous_cache("attention_decode_tree", q.shape[0], k_cache, v_pages, k_scales, v_scales)
-    H, L, D = k_cache.shape[1:]
-    if q.dim() == 4 and q.shape[3] != D:
-        raise InvalidArgument("attention_decode_tree: q and the cache differ in head_dim")
-    p, q_scales, tree_mask, context_lens, out = _tree_inputs(
+    H, L, D = _contiguous_cache("attention_decode_tree", q.shape[0], k_cache, v_pages, k_scales,
+                                v_scales)
+    p, q_scales, tree_mask, out = _tree_inputs(
         "attention_decode_tree", q, q_scales, tree_mask, window, softmax_scale, q_granularity, H, L,
-        context_lens, out)
+        D, context_lens, out)
     stream = _stream()
     n = _lib().reef_attention_decode_tree_workspace_bytes(p)
     ws = _tree_workspace(n, q.device, stream) if workspace is None else workspace
@@ -734,14 +749,12 @@ def attention_decode_tree_paged(q, q_scales, k_pages, v_pages, k_scale_pages, v_
     [B] int32."""
     what = "attention_decode_tree_paged"
     P, H, D = _pool_shapes(what, k_pages, v_pages, k_scale_pages, v_scale_pages)
-    _ints(what, block_table=block_table, context_lens=context_lens)
-    if q.dim() == 4 and q.shape[3] != D:
-        raise InvalidArgument(f"{what}: q and the cache differ in head_dim")
+    _expect(what, _torch().int32, (block_table, "block_table"), (context_lens, "context_lens"))
     if block_table.dim() != 2 or block_table.shape[0] != q.shape[0]:
         raise InvalidArgument(f"{what}: block_table must be [B, max_blocks]")
     blocks = block_table.shape[1]
-    p, q_scales, tree_mask, context_lens, out = _tree_inputs(
-        what, q, q_scales, tree_mask, window, softmax_scale, q_granularity, H, blocks * PAGE,
+    p, q_scales, tree_mask, out = _tree_inputs(
+        what, q, q_scales, tree_mask, window, softmax_scale, q_granularity, H, blocks * PAGE, D,
         context_lens, out)
     stream = _stream()
     n = _lib().reef_attention_decode_tree_workspace_bytes(p)
@@ -833,19 +846,9 @@ def kv_append_paged(k_new, v_new, start_positions, block_table, k_pages, v_pages
 # block_table [B, max_blocks], context_lens [B] and page_refs [P] are int32 on the GPU and
 # changed in place: a table starts filled with -1, page_refs with 0. See the C header.
 
-def _ints(what, **tensors):
-    """Contiguous int32 tensors on the current GPU."""
-    torch = _torch()
-    for name, t in tensors.items():
-        _require(t, torch.int32, name)
-        if not t.is_contiguous():
-            raise InvalidArgument(f"{what}: {name} must be contiguous")
-    _on_device(what, *tensors.values())
-
-
 def _table(what, block_table, context_lens, page_refs):
     if block_table.dim() != 2 or page_refs.dim() != 1 or (
-            context_lens is not None and tuple(context_lens.shape) != block_table.shape[:1]):
+            context_lens is not None and context_lens.shape != block_table.shape[:1]):
         raise InvalidArgument(f"{what} shapes: block_table [B, max_blocks], context_lens [B], "
                               "page_refs [pages]")
     return block_table.shape
@@ -854,8 +857,8 @@ def _table(what, block_table, context_lens, page_refs):
 def kv_free(sequences, block_table, context_lens, page_refs, status: StatusWord | None = None):
     """The listed sequences ([n] int32 rows of the table, negative: padding) give their pages
     back; their table rows become -1 and their lengths 0."""
-    _ints("kv_free", sequences=sequences, block_table=block_table, context_lens=context_lens,
-          page_refs=page_refs)
+    _expect("kv_free", _torch().int32, (sequences, "sequences"), (block_table, "block_table"),
+            (context_lens, "context_lens"), (page_refs, "page_refs"))
     B, blocks = _table("kv_free", block_table, context_lens, page_refs)
     own = status or StatusWord(block_table.device)
     check(_lib().reef_kv_free(_ptr(sequences), sequences.numel(), _ptr(block_table), blocks,
@@ -870,8 +873,8 @@ def kv_fork(parents, children, block_table, context_lens, page_refs,
     """Sequence children[i] becomes a copy of parents[i] (both [n] int32, negative: padding)
     that shares its pages. A parent may have many children; a child is listed once and is no
     parent in the same call."""
-    _ints("kv_fork", parents=parents, children=children, block_table=block_table,
-          context_lens=context_lens, page_refs=page_refs)
+    _expect("kv_fork", _torch().int32, (parents, "parents"), (children, "children"),
+            (block_table, "block_table"), (context_lens, "context_lens"), (page_refs, "page_refs"))
     B, blocks = _table("kv_fork", block_table, context_lens, page_refs)
     if parents.numel() != children.numel():
         raise InvalidArgument("kv_fork: as many parents as children")
@@ -890,7 +893,8 @@ def kv_reserve(block_table, context_lens, page_refs, new_tokens: int,
     kv_copy_pages on each layer's pool: a shared page that holds tokens is copied, -1 where
     there is nothing to copy. Lengths are left; kv_append_paged writes the tokens."""
     torch = _torch()
-    _ints("kv_reserve", block_table=block_table, context_lens=context_lens, page_refs=page_refs)
+    _expect("kv_reserve", torch.int32, (block_table, "block_table"),
+            (context_lens, "context_lens"), (page_refs, "page_refs"))
     B, blocks = _table("kv_reserve", block_table, context_lens, page_refs)
     device = block_table.device
     n = _lib().reef_kv_reserve_workspace_bytes(B, new_tokens)
@@ -911,7 +915,7 @@ def kv_compact(block_table, page_refs, status: StatusWord | None = None):
     (source, destination) pages [pages // 2] int32 for kv_copy_pages on each layer's pool, -1
     behind the last move, and L as a [1] int32 tensor."""
     torch = _torch()
-    _ints("kv_compact", block_table=block_table, page_refs=page_refs)
+    _expect("kv_compact", torch.int32, (block_table, "block_table"), (page_refs, "page_refs"))
     B, blocks = _table("kv_compact", block_table, None, page_refs)
     pages, device = page_refs.numel(), block_table.device
     n, half = _lib().reef_kv_compact_workspace_bytes(pages), pages // 2
@@ -928,14 +932,11 @@ def kv_compact(block_table, page_refs, status: StatusWord | None = None):
 
 
 def _pool_shapes(what, k_pages, v_pages, k_scale_pages, v_scale_pages):
+    """(pages, heads, head_dim) of a paged cache."""
     torch = _torch()
-    for t, dtype, name in ((k_pages, torch.int8, "k_pages"), (v_pages, torch.int8, "v_pages"),
-                           (k_scale_pages, torch.float32, "k_scale_pages"),
-                           (v_scale_pages, torch.float32, "v_scale_pages")):
-        _require(t, dtype, name)
-        if not t.is_contiguous():
-            raise InvalidArgument(f"{what}: {name} must be contiguous")
-    _on_device(what, k_pages, v_pages, k_scale_pages, v_scale_pages)
+    _expect(what, torch.int8, (k_pages, "k_pages"), (v_pages, "v_pages"))
+    _expect(what, torch.float32, (k_scale_pages, "k_scale_pages"),
+            (v_scale_pages, "v_scale_pages"))
     if k_pages.dim() != 4 or k_pages.shape[2] != PAGE:
         raise InvalidArgument(f"{what}: k_pages must be [pages, heads, 16, head_dim]")
     P, H, _, D = k_pages.shape
@@ -950,7 +951,7 @@ def kv_copy_pages(source, place, k_pages, v_pages, k_scale_pages, v_scale_pages,
     """Page source[i] of one layer's pool (keys, values, scales) is copied to page place[i]
     (both [n] int32; pairs with a negative page are left out). No page may be a destination
     twice, or a source and a destination."""
-    _ints("kv_copy_pages", source=source, place=place)
+    _expect("kv_copy_pages", _torch().int32, (source, "source"), (place, "place"))
     P, H, D = _pool_shapes("kv_copy_pages", k_pages, v_pages, k_scale_pages, v_scale_pages)
     if source.numel() != place.numel():
         raise InvalidArgument("kv_copy_pages: as many sources as destinations")
@@ -966,8 +967,9 @@ def kv_copy_pages(source, place, k_pages, v_pages, k_scale_pages, v_scale_pages,
 
 
 def _kept(what, kept, kept_lens, context_lens):
-    _ints(what, kept=kept, kept_lens=kept_lens, context_lens=context_lens)
-    if kept.dim() != 2 or tuple(kept_lens.shape) != kept.shape[:1] or (
+    _expect(what, _torch().int32, (kept, "kept"), (kept_lens, "kept_lens"),
+            (context_lens, "context_lens"))
+    if kept.dim() != 2 or kept_lens.shape != kept.shape[:1] or (
             context_lens.shape != kept_lens.shape):
         raise InvalidArgument(f"{what} shapes: kept [B, drafts], kept_lens [B], context_lens [B]")
     return kept.shape
@@ -981,8 +983,7 @@ def kv_keep(kept, kept_lens, context_lens, k_cache, v_pages, k_scales, v_scales,
     kv_append. Returns the new lengths, context_lens - T + kept_lens."""
     torch = _torch()
     B, T = _kept("kv_keep", kept, kept_lens, context_lens)
-    H, L, D = k_cache.shape[1:]
-    _contiguous_cache("kv_keep", B, k_cache, v_pages, k_scales, v_scales)
+    H, L, D = _contiguous_cache("kv_keep", B, k_cache, v_pages, k_scales, v_scales)
     lens = torch.empty_like(context_lens)
     own = status or StatusWord(k_cache.device)
     check(_lib().reef_kv_keep_int8(
@@ -995,18 +996,15 @@ def kv_keep(kept, kept_lens, context_lens, k_cache, v_pages, k_scales, v_scales,
 
 
 def _contiguous_cache(what, B, k_cache, v_pages, k_scales, v_scales):
+    """(heads, tokens, head_dim) of a contiguous cache of B sequences."""
     torch = _torch()
-    for t, dtype, name in ((k_cache, torch.int8, "k_cache"), (v_pages, torch.int8, "v_pages"),
-                           (k_scales, torch.float32, "k_scales"),
-                           (v_scales, torch.float32, "v_scales")):
-        _require(t, dtype, name)
-        if not t.is_contiguous():
-            raise InvalidArgument(f"{what}: {name} must be contiguous")
-    _on_device(what, k_cache, v_pages, k_scales, v_scales)
-    if k_cache.dim() != 4 or k_cache.shape[0] != B or v_pages.numel() != k_cache.numel() or (
-            k_scales.numel() * k_cache.shape[3] != k_cache.numel()
-            or v_scales.numel() != k_scales.numel()):
+    _expect(what, torch.int8, (k_cache, "k_cache"), (v_pages, "v_pages"))
+    _expect(what, torch.float32, (k_scales, "k_scales"), (v_scales, "v_scales"))
+    shape, n = k_cache.shape, k_cache.numel()
+    if len(shape) != 4 or shape[0] != B or v_pages.numel() != n or (
+            k_scales.numel() * shape[3] != n or v_scales.numel() * shape[3] != n):
         raise InvalidArgument(f"{what}: cache shape mismatch")
+    return shape[1:]
 
 
 def kv_keep_paged(kept, kept_lens, context_lens, block_table, k_pages, v_pages, k_scale_pages,
@@ -1014,7 +1012,7 @@ def kv_keep_paged(kept, kept_lens, context_lens, block_table, k_pages, v_pages, 
     """kv_keep in the paged cache; the drafted tokens' pages must be the sequence's own."""
     torch = _torch()
     B, T = _kept("kv_keep_paged", kept, kept_lens, context_lens)
-    _ints("kv_keep_paged", block_table=block_table)
+    _expect("kv_keep_paged", torch.int32, (block_table, "block_table"))
     P, H, D = _pool_shapes("kv_keep_paged", k_pages, v_pages, k_scale_pages, v_scale_pages)
     if block_table.dim() != 2 or block_table.shape[0] != B:
         raise InvalidArgument("kv_keep_paged: block_table must be [B, max_blocks]")
@@ -1156,6 +1154,16 @@ def gemm_w8a8(xq, x_scales, weight, w_scales, bias=None, status: StatusWord | No
 
 # --- norm ---------------------------------------------------------------------------------
 
+def _rows_of(t, width):
+    """t's rows as a matrix, and the elements from row to row; copied only where they do not
+    lie evenly."""
+    if t.is_contiguous():
+        return t, width
+    m = t if t.dim() == 2 else t.reshape(-1, width)
+    stride = _row_stride(m)
+    return (m, stride) if stride is not None and stride >= width else (m.contiguous(), width)
+
+
 def rmsnorm_quantize(x, weight=None, *, residual=None, eps=1e-6, residual_out=None,
                      status: StatusWord | None = None):
     """The root-mean-square norm of x (+ residual) over the last dimension, as int8 rows
@@ -1172,9 +1180,10 @@ def rmsnorm_quantize(x, weight=None, *, residual=None, eps=1e-6, residual_out=No
     width = shape[-1]
     if weight is not None:
         _require(weight, torch.float32, "weight")
-        if tuple(weight.shape) != (width,):
+        if weight.shape != (width,):
             raise InvalidArgument("rmsnorm_quantize: weight must be [width]")
-        weight = weight.contiguous()
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
     if residual is not None:
         _require(residual, torch.float32, "residual")
         if residual.shape != shape:
@@ -1183,33 +1192,24 @@ def rmsnorm_quantize(x, weight=None, *, residual=None, eps=1e-6, residual_out=No
         raise InvalidArgument("rmsnorm_quantize: residual_out needs a residual")
     _on_device("rmsnorm_quantize", x, weight, residual, residual_out)
 
-    def rows_of(t):
-        """A matrix of t's rows, copied only where they do not lie in one."""
-        m = t if t.dim() == 2 else t.reshape(-1, width)
-        return m if _row_stride(m) is not None and _row_stride(m) >= width else m.contiguous()
-
-    x2 = rows_of(x)
-    rows = x2.shape[0]
+    x2, x_stride = _rows_of(x, width)
     r2 = h = None
-    r_stride = h_stride = 0
+    r_stride = 0
     if residual is not None:
-        r2 = rows_of(residual)
-        r_stride = _row_stride(r2)
+        r2, r_stride = _rows_of(residual, width)
         h = residual_out
         if h is None:
             h = torch.empty(shape, dtype=torch.float32, device=x.device)
         else:
-            _require(h, torch.float32, "residual_out")
-            if h.shape != shape or not h.is_contiguous():
-                raise InvalidArgument("rmsnorm_quantize: residual_out must be contiguous and have "
-                                      "x's shape")
-        h_stride = width
+            _expect("rmsnorm_quantize", torch.float32, (h, "residual_out"))
+            if h.shape != shape:
+                raise InvalidArgument("rmsnorm_quantize: residual_out must have x's shape")
     q = torch.empty(shape, dtype=torch.int8, device=x.device)
     s = torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
     own = status or StatusWord(x.device)
     check(_lib().reef_rmsnorm_quantize_int8(
-        _ptr(x2), rows, width, _row_stride(x2), _ptr(r2), r_stride, _ptr(weight), eps, _ptr(q),
-        _ptr(s), _ptr(h), h_stride, _ptr(own.tensor), _stream()), "rmsnorm_quantize")
+        _ptr(x2), s.numel(), width, x_stride, _ptr(r2), r_stride, _ptr(weight), eps, _ptr(q),
+        _ptr(s), _ptr(h), width, _ptr(own.tensor), _stream()), "rmsnorm_quantize")
     if status is None:
         own.check("rmsnorm_quantize requires finite values")
     return (q, s) if residual is None else (q, s, h)

@@ -296,12 +296,18 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
         const int mid = longer * (quota + 1);
         return u < mid ? u / (quota + 1) : longer + (u - mid) / quota;
     };
-    // The workgroups of one XCD hold consecutive runs: the column ranges of one (sequence,
-    // kv head) meet in its L2.
-    const int x = blockIdx.x % kXcds, place = blockIdx.x / kXcds;
-    const int per = G / kXcds, rem = G % kXcds;
-    if (place >= per + (x < rem ? 1 : 0)) return;
-    const int g = x * per + min(x, rem) + place;
+    // With several tiles the workgroups of one XCD hold consecutive runs: the column ranges of
+    // one (sequence, kv head) meet in its L2. With one tile nothing is shared, and plain order
+    // is faster (64 x 4096 x 8 heads of 128, 3 drafted: 98.5 us against 101.3).
+    int g = blockIdx.x;
+    if (NC == 1) {
+        if (g >= G) return;
+    } else {
+        const int x = blockIdx.x % kXcds, place = blockIdx.x / kXcds;
+        const int per = G / kXcds, rem = G % kXcds;
+        if (place >= per + (x < rem ? 1 : 0)) return;
+        g = x * per + min(x, rem) + place;
+    }
     const int u0 = run_start(g), u1 = run_start(g + 1);
 
     auto segment_at = [&](const TreeArgs &a, int u, int b) {

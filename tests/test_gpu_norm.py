@@ -63,6 +63,22 @@ def test_norm_matches_formula(reef, width, residual, weight):
     check(out[0], out[1], h, w, 1e-5)
 
 
+@pytest.mark.parametrize("rows,width", [(2050, 700), (2049, 2047), (3001, 1024), (9000, 8190)])
+def test_norm_of_many_rows(reef, rows, width):
+    """A wave per row, and streams beyond the last-level cache (9000 x 8190 with a residual)."""
+    print(f"\n[case] norm of many rows {rows}x{width}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x, r = (torch.randn((rows, width), generator=g, device="cuda") for _ in range(2))
+    w = torch.rand(width, generator=g, device="cuda") + 0.5
+    q, s, h = reef.rmsnorm_quantize(x, w, residual=r)
+    assert torch.equal(h, x + r)
+    some = torch.cat([torch.arange(40), torch.arange(rows - 40, rows)])
+    check(q[some], s[some], h[some].cpu().numpy(), w.cpu().numpy(), 1e-6)
+    d = h.double()  # the others on the GPU
+    y = d * w.double() / (d.square().mean(1, keepdim=True) + 1e-6).sqrt()
+    assert float((q.double() * s[:, None].double() - y).abs().max() / s.max()) < 0.5 + 1e-4
+
+
 @pytest.mark.parametrize("width", [100, 2048, 6001, 20000])
 @pytest.mark.parametrize("alias", ["x", "residual"])
 def test_norm_in_place_and_strided(reef, width, alias):
