@@ -183,10 +183,12 @@ __global__ __launch_bounds__(kScanThreads) void reserve_pages(ReserveArgs a) {
     for (int64_t base = 0; base < a.t.num_pages && found < wanted; base += 4 * kScanThreads) {
         const int64_t p = base + 4 * tid;
         bool is_free[4];
-        int mine = 0, all;
+        int refs[4], mine = 0, all;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) refs[j] = a.t.refs[min(p + j, (int64_t)a.t.num_pages - 1)];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            is_free[j] = p + j < a.t.num_pages && a.t.refs[p + j] == 0;
+            is_free[j] = p + j < a.t.num_pages && refs[j] == 0;
             mine += is_free[j];
         }
         int rank = found + block_scan(mine, all, sWave);
@@ -250,11 +252,16 @@ __global__ __launch_bounds__(kCompactThreads) void count_live(CompactArgs a) {
     __shared__ int sSum;
     if (threadIdx.x == 0) sSum = 0;
     __syncthreads();
-    int n = 0;
+    // (loads without a branch between them: one round trip, not sixteen)
+    int refs[kCompactEach], n = 0;
+#pragma unroll
     for (int j = 0; j < kCompactEach; ++j) {
         const int64_t p = (int64_t)blockIdx.x * kCompactChunk + j * kCompactThreads + threadIdx.x;
-        n += p < a.t.num_pages && a.t.refs[p] > 0;
+        refs[j] = a.t.refs[min(p, (int64_t)a.t.num_pages - 1)];
+        if (p >= a.t.num_pages) refs[j] = 0;
     }
+#pragma unroll
+    for (int j = 0; j < kCompactEach; ++j) n += refs[j] > 0;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
     if ((threadIdx.x & 63) == 0) atomicAdd(&sSum, n);
@@ -288,9 +295,13 @@ __global__ __launch_bounds__(kCompactThreads) void list_moves(CompactArgs a) {
     // this thread's pages are consecutive
     const int64_t p0 = (int64_t)blockIdx.x * kCompactChunk + tid * kCompactEach;
     uint32_t live = 0;
+    int refs[kCompactEach];
 #pragma unroll
     for (int j = 0; j < kCompactEach; ++j)
-        live |= (p0 + j < a.t.num_pages && a.t.refs[p0 + j] > 0 ? 1u : 0u) << j;
+        refs[j] = a.t.refs[min(p0 + j, (int64_t)a.t.num_pages - 1)];
+#pragma unroll
+    for (int j = 0; j < kCompactEach; ++j)
+        live |= (p0 + j < a.t.num_pages && refs[j] > 0 ? 1u : 0u) << j;
     int s = __popc(live);
 #pragma unroll
     for (int o = 1; o < kWave; o <<= 1) {
