@@ -270,13 +270,16 @@ __global__ __launch_bounds__(kCompactThreads) void count_live(CompactArgs a) {
 }
 
 __global__ __launch_bounds__(kCompactThreads) void list_moves(CompactArgs a) {
-    __shared__ int sBefore, sTotal, sWave[kCompactThreads / kWave];
+    constexpr int W = kCompactThreads / kWave;
+    static_assert(kCompactEach * W == kWave, "one count per lane");
+    __shared__ int sBefore[W], sTotal[W], sLive[kWave];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (tid == 0) {
-        sBefore = 0;
-        sTotal = 0;
-    }
-    __syncthreads();
+    // Page j of this thread is tid + 256 j of the chunk: in order, (j, wave, lane).
+    const int64_t base = (int64_t)blockIdx.x * kCompactChunk + tid;
+    int refs[kCompactEach];
+#pragma unroll
+    for (int j = 0; j < kCompactEach; ++j)
+        refs[j] = a.t.refs[min(base + j * kCompactThreads, (int64_t)a.t.num_pages - 1)];
     int before = 0, total = 0;
     for (int c = tid; c < a.chunks; c += kCompactThreads) {
         const int n = a.counts[c];
@@ -288,36 +291,37 @@ __global__ __launch_bounds__(kCompactThreads) void list_moves(CompactArgs a) {
         before += __shfl_xor(before, o);
         total += __shfl_xor(total, o);
     }
-    if (lane == 0) {
-        atomicAdd(&sBefore, before);
-        atomicAdd(&sTotal, total);
+    uint64_t live[kCompactEach];
+#pragma unroll
+    for (int j = 0; j < kCompactEach; ++j) {
+        live[j] = __ballot(base + j * kCompactThreads < a.t.num_pages && refs[j] > 0);
+        if (lane == j) sLive[W * j + wave] = __popcll(live[j]);
     }
-    // this thread's pages are consecutive
-    const int64_t p0 = (int64_t)blockIdx.x * kCompactChunk + tid * kCompactEach;
-    uint32_t live = 0;
-    int refs[kCompactEach];
+    if (lane == 0) {
+        sBefore[wave] = before;
+        sTotal[wave] = total;
+    }
+    __syncthreads();
+    before = total = 0;
 #pragma unroll
-    for (int j = 0; j < kCompactEach; ++j)
-        refs[j] = a.t.refs[min(p0 + j, (int64_t)a.t.num_pages - 1)];
-#pragma unroll
-    for (int j = 0; j < kCompactEach; ++j)
-        live |= (p0 + j < a.t.num_pages && refs[j] > 0 ? 1u : 0u) << j;
-    int s = __popc(live);
+    for (int w = 0; w < W; ++w) {
+        before += sBefore[w];
+        total += sTotal[w];
+    }
+    const int own = sLive[lane];
+    int s = own;
 #pragma unroll
     for (int o = 1; o < kWave; o <<= 1) {
         const int y = __shfl_up(s, o);
         if (lane >= o) s += y;
     }
-    if (lane == 63) sWave[wave] = s;
-    __syncthreads();
-    total = sTotal;
-    int n = sBefore + s - __popc(live);  // live pages before the next one
-    for (int w = 0; w < wave; ++w) n += sWave[w];
+    s += before - own;  // live pages before the 64 of (j, wave) = (lane / W, lane % W)
 #pragma unroll
     for (int j = 0; j < kCompactEach; ++j) {
-        const int64_t p = p0 + j;
-        if (p >= a.t.num_pages) break;
-        const bool is_live = live >> j & 1u;
+        const int64_t p = base + j * kCompactThreads;
+        const int n = __shfl(s, W * j + wave) + (int)__popcll(live[j] & ((1ull << lane) - 1));
+        if (p >= a.t.num_pages) continue;
+        const bool is_live = live[j] >> lane & 1u;
         if (p == total) a.counts[a.chunks] = total - n;  // moves: the live pages from here on
         int rank = -1;
         if (is_live && p >= total) {
@@ -327,7 +331,6 @@ __global__ __launch_bounds__(kCompactThreads) void list_moves(CompactArgs a) {
             a.dst[p - n] = (int)p;
         }
         a.rank[p] = rank;
-        n += is_live;
     }
     if (blockIdx.x == 0 && tid == 0) {
         if (total == a.t.num_pages) a.counts[a.chunks] = 0;
