@@ -22,7 +22,7 @@ namespace {
 
 constexpr int kWaves = 4;      // waves of a workgroup, one per SIMD
 constexpr int kWgPerCu = 2;    // workgroups of a compute unit
-constexpr int kMaxSplit = 2;   // ways a workgroup's waves split the columns, at most
+constexpr int kMinBlocks = 2;  // blocks of a wave in a run, at least, while items are whole
 constexpr int kPlan = 2048;    // sequences of a launch (more are launched in slices)
 constexpr int kMaxDrafts = 64; // bits of a mask word
 constexpr int kMaxGroup = 1024;  // query heads of a kv head
@@ -45,8 +45,7 @@ struct TreeArgs {
     int32_t batch, q_heads, kv_heads, group, drafts;
     uint32_t group_inverse;  // floor(2^32 / group) + 1: i / group for i * group < 2^32
     int32_t max_context, window;
-    int32_t cw;      // the workgroup's waves split the columns cw ways (and the keys 4 / cw)
-    int32_t chunks;  // column ranges of 16 NC cw columns; an item is (sequence, kv head, range)
+    int32_t chunks;  // column ranges of 16 NC columns; an item is (sequence, kv head, range)
     int32_t extra;   // units that an item counts beside its blocks
     int32_t max_blocks, num_pages;  // paged only
     int32_t q_gran;
@@ -155,6 +154,18 @@ __device__ __forceinline__ float row_fmax(float x) {
     x = dpp_fmax<0x141>(x);  // row_half_mirror
     return dpp_fmax<0x140>(x);  // row_mirror
 }
+// max / sum of x over lanes l and l ^ 16 (v_permlane16_swap: no trip through LDS).
+__device__ __forceinline__ float xor16_max(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                    false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float xor16_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                    false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_or(uint32_t x) {
     return x | (uint32_t)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xF, 0xF, false);
@@ -254,12 +265,10 @@ __device__ __forceinline__ TreeArgs reread_args() {
 
 // The launch's work is the 64-key blocks of all items, dealt out to the workgroups in equal
 // runs. An item counts some units before its blocks, for the time that its rows, its merge
-// and its stores take: workgroups with many short items get fewer blocks. Within a run each item's part is one segment: the workgroup's four waves split the
-// range's columns cw ways and the segment's blocks 4 / cw ways, keep a running softmax and
-// merge in LDS. An item inside one run is stored directly; the parts of an item cut by a
+// and its stores take: workgroups with many short items get fewer blocks. Within a run each item's part is one segment: the workgroup's four waves take the
+// segment's blocks in turn, keep a running softmax each and merge in LDS. An item inside one run is stored directly; the parts of an item cut by a
 // run's end go to the workspace, and the one that counts in last merges them in order
-// (reef_common.hpp, cross-workgroup parts). Waves that split the columns read the same
-// blocks at about the same time: one reads memory, the others the caches.
+// (reef_common.hpp, cross-workgroup parts).
 template <int D, bool PAGED, int NC>
 __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs arg) {
     constexpr int DB = D / 16, KS = D / 64;
@@ -275,8 +284,6 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
-    const int CW = arg.cw, KW = kWaves / CW;
-    const int cwi = wave % CW, kwi = wave / CW;
 
     const bool same = arg.context_lens == nullptr;
     const int nb = same ? seq_keys(arg, 0).blocks + arg.extra : 0;
@@ -286,9 +293,13 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
     };
     const int per_seq = arg.kv_heads * arg.chunks;  // items of a sequence
     const int T = units_before(arg.batch) * per_seq;  // (fits: checked for full caches)
-    // No more workgroups than there are items, or parts with a block for every wave.
+    // No more workgroups than there are items, or parts with kMinBlocks for every wave: more
+    // parts are a longer merge, fewer a longer run (with at least 1, 2, 4 and 8 blocks a wave:
+    // 1 x 8192 keys, 8/1 heads of 128, 16 drafted 31, 26, 26, 32 us; 1 x 8192, 8/8 heads, 1
+    // drafted 33, 25, 23, 26; 3 x 1000-3000, 8/1 heads, 64 drafted 34, 30, 31, 39).
     const int items = arg.batch * per_seq;
-    const int G = min((int)gridDim.x, max(items, (T - items * arg.extra + KW - 1) / KW));
+    const int G = min((int)gridDim.x, max(items, (T - items * arg.extra + kMinBlocks * kWaves - 1) /
+                                                     (kMinBlocks * kWaves)));
     // Workgroup w's run: T / G units, one more for each of the first T % G.
     const int quota = T / G, longer = T - quota * G;
     auto run_start = [&](int w) { return w * quota + min(w, longer); };
@@ -331,16 +342,16 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
         return s;
     };
     auto first_key = [&](const Segment &s) {
-        return (s.sk.first_block + s.s_blk + kwi) * kBlockKeys;
+        return (s.sk.first_block + s.s_blk + wave) * kBlockKeys;
     };
     auto end_key = [&](const Segment &s) {
         return min(s.sk.len, (s.sk.first_block + s.e_blk) * kBlockKeys);
     };
-    auto first_tile = [&](const Segment &s) { return (s.chunk * CW + cwi) * NC; };
+    auto first_tile = [&](const Segment &s) { return s.chunk * NC; };
     auto column = [&](const TreeArgs &a, const Segment &s, int t) {
         return column_of(a, s.kvh, 16 * (first_tile(s) + t) + col);
     };
-    const int k_step = KW * kBlockKeys;
+    constexpr int k_step = kWaves * kBlockKeys;
 
     // A block's operands, and what a segment's rows need, in registers.
     i32x4 kop[4][KS], vop[DB], qreg[NC][KS];
@@ -366,13 +377,11 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
         vs = a.vs[(int64_t)at.g_slot * kPage + col];
     };
     // Whether this wave has anything to do in a segment.
-    auto busy = [&](const TreeArgs &a, const Segment &s) {
-        return 16 * first_tile(s) < a.drafts * a.group && first_key(s) < end_key(s);
-    };
+    auto busy = [&](const Segment &s) { return first_key(s) < end_key(s); };
     // The loads of a segment's rows, and of its first block where `block` (pages: its table
     // entries).
     auto issue = [&](const TreeArgs &a, const Segment &s, int pages, bool block) {
-        if (!busy(a, s)) return;
+        if (!busy(s)) return;
 #pragma unroll
         for (int t = 0; t < NC; ++t) {
             const Column cn = column(a, s, t);
@@ -414,7 +423,7 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
         TreeArgs a = reread_args();
         if (seg.sk.bad && seg.s_blk == 0 && seg.kvh == 0 && seg.chunk == 0 && threadIdx.x == 0)
             flag_status(a.status, REEF_STATUS_BIT_BAD_LENGTH);
-        const bool mine = busy(a, seg);  // wave-uniform
+        const bool mine = busy(seg);  // wave-uniform
         // This segment's rows: operands and sights to LDS (this wave's own places).
         float cs[NC];
         uint32_t shown = 0;  // bit t: this lane's row of tile t sees something
@@ -526,13 +535,10 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
 #pragma unroll
                     for (int r = 3; r < 15; r += 2) m = fmaxf(fmaxf(m, xs[t][r]), xs[t][r + 1]);
                     m = fmaxf(m, xs[t][15]);
-                    m = fmaxf(m, __shfl_xor(m, 16));
-                    mt[t] = xor32_max(m) * cs[t];
+                    mt[t] = xor32_max(xor16_max(m)) * cs[t];
                     grow |= mt[t] > m_run[t] + 6.0f;
                 }
-                float vmax = row_fmax(vsc);
-                vmax = fmaxf(vmax, __shfl_xor(vmax, 16));
-                vmax = xor32_max(vmax);
+                const float vmax = xor32_max(xor16_max(row_fmax(vsc)));
                 // Lazy rescale: a row's maximum moves only when it grows by more than 2^6, and
                 // the unit of the accumulator (s_run / 2^8, s_run the largest value scale so
                 // far) only when a value scale passes it 2-fold, so a weight
@@ -622,13 +628,11 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
         // The workgroups that hold a part of this item: gf .. gl, each with at least one block.
         const int gf = run_of(seg.first_u);
         const int parts = run_of(seg.first_u + seg.sk.blocks - 1) - gf + 1;
-        const int64_t slot_elems = (int64_t)CW * NC * TreeSlot<D>::ELEMS;
+        constexpr int64_t slot_elems = NC * TreeSlot<D>::ELEMS;
         // A workgroup has two slots: for an item that begins in its run, and one that began
         // before.
         uint64_t *own = a.slots + (2 * (int64_t)g + (g == gf ? 1 : 0)) * slot_elems;
-        auto tile_slot = [&](uint64_t *s, int t) {
-            return s + (cwi * NC + t) * TreeSlot<D>::ELEMS;
-        };
+        auto tile_slot = [&](uint64_t *s, int t) { return s + t * TreeSlot<D>::ELEMS; };
         auto store_out = [&](const Column &cn, int d, f32x4 o, float l) {
             if (!cn.live) return;
             float *row = a.out + seg.b * a.o_sb + cn.head * a.o_sh + cn.token * a.o_st;
@@ -636,14 +640,12 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
             if (l > 0.0f) y = o * (1.0f / l);
             *reinterpret_cast<f32x4 *>(row + 16 * d + 4 * grp) = y;
         };
-        // The key-split waves of a column range merge tile by tile through LDS, each the
-        // channel blocks d = kwi, kwi + KW, ... A row that sees nothing has the sum 0.
+        // The waves merge tile by tile through LDS, each the channel blocks d = wave, wave + 4,
+        // ... A row that sees nothing has the sum 0.
 #pragma unroll
         for (int t = 0; t < NC; ++t) {
             const Column cn = column(a, seg, t);
-            float l = l_run[t];
-            l += __shfl_xor(l, 16);
-            l = xor32_sum(l);
+            float l = xor32_sum(xor16_sum(l_run[t]));
             if (!(shown >> t & 1u)) {
                 l = 0.0f;
                 m_run[t] = -INFINITY;
@@ -652,28 +654,29 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
             for (int d = 0; d < DB; ++d) sO[wave][d][lane] = acc[t][d] * (s_run * (1.0f / 256.0f));
             sML[wave][lane] = float2{m_run[t], l};
             lds_barrier();
+            float2 ml[kWaves];
             float m = -INFINITY;
-            for (int w = cwi; w < kWaves; w += CW) m = fmaxf(m, sML[w][lane].x);
-            l = 0.0f;
-            float scale[kWaves];
 #pragma unroll
-            for (int i = 0; i < kWaves; ++i) {
-                scale[i] = 0.0f;
-                if (i < KW) {
-                    const float2 ml = sML[i * CW + cwi][lane];
-                    scale[i] = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - m);
-                    l = __builtin_fmaf(scale[i], ml.y, l);
-                }
+            for (int w = 0; w < kWaves; ++w) {
+                ml[w] = sML[w][lane];
+                m = fmaxf(m, ml[w].x);
             }
-            for (int d = kwi; d < DB; d += KW) {
+            l = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                ml[w].x = ml[w].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[w].x - m);
+                l = __builtin_fmaf(ml[w].x, ml[w].y, l);
+            }
+#pragma unroll
+            for (int n = 0; n < DB / kWaves; ++n) {
+                const int d = wave + n * kWaves;
                 f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int i = 0; i < kWaves; ++i)
-                    if (i < KW) {
-                        const f32x4 p = sO[i * CW + cwi][d][lane];
+                for (int w = 0; w < kWaves; ++w) {
+                    const f32x4 p = sO[w][d][lane];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(scale[i], p[e], o[e]);
-                    }
+                    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(ml[w].x, p[e], o[e]);
+                }
                 if (parts == 1) {
                     store_out(cn, d, o, l);
                 } else if (cn.live) {
@@ -682,7 +685,7 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
                     part_store(s + (2 * d + 1) * kWave + lane, pack(o[2], o[3]));
                 }
             }
-            if (parts > 1 && kwi == 0 && cn.live)
+            if (parts > 1 && wave == 0 && cn.live)
                 part_store(tile_slot(own, t) + TreeSlot<D>::O * kWave + lane, pack(m, l));
             lds_barrier();  // frees sO / sML
         }
@@ -695,50 +698,51 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
             if (__builtin_amdgcn_readfirstlane(sLast)) {
                 part_claimed();
                 if (threadIdx.x == 0) part_reset(a.counters + gf);
-                constexpr int kAhead = 4;  // parts whose loads are in flight together
+                // A chain of round trips beneath the caches: kAhead parts' loads in flight at a
+                // time, all of a wave's channel blocks of a tile.
+                constexpr int kAhead = 4, ND = DB / kWaves;
 #pragma unroll
                 for (int t = 0; t < NC; ++t) {
                     const Column cn = column(a, seg, t);
                     if (!cn.live) continue;
-                    for (int d = kwi; d < DB; d += 2 * KW) {  // (DB / KW is 1 or even)
-                        const int d2 = min(d + KW, DB - 1);
-                        float m = -INFINITY, l = 0.0f;
-                        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f}, o2 = o;
-                        for (int p0 = 0; p0 < parts; p0 += kAhead) {
-                            uint64_t ml[kAhead], v0[kAhead], v1[kAhead], w0[kAhead], w1[kAhead];
+                    float m = -INFINITY, l = 0.0f;
+                    f32x4 o[ND];
 #pragma unroll
-                            for (int i = 0; i < kAhead; ++i) {
-                                const int p = min(p0 + i, parts - 1);
-                                uint64_t *s = tile_slot(
-                                    a.slots + (2 * (int64_t)(gf + p) + (p == 0 ? 1 : 0)) *
-                                                  slot_elems, t);
-                                ml[i] = part_load(s + TreeSlot<D>::O * kWave + lane);
-                                v0[i] = part_load(s + (2 * d) * kWave + lane);
-                                v1[i] = part_load(s + (2 * d + 1) * kWave + lane);
-                                w0[i] = part_load(s + (2 * d2) * kWave + lane);
-                                w1[i] = part_load(s + (2 * d2 + 1) * kWave + lane);
-                            }
+                    for (int n = 0; n < ND; ++n) o[n] = f32x4{};
+                    for (int p0 = 0; p0 < parts; p0 += kAhead) {
+                        uint64_t ml[kAhead], v[kAhead][ND][2];
 #pragma unroll
-                            for (int i = 0; i < kAhead; ++i) {
-                                if (p0 + i >= parts) break;
-                                const float mp = lo32(ml[i]), mn = fmaxf(m, mp);
-                                const float er = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-                                const float ep = mp == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mp - mn);
-                                l = __builtin_fmaf(ep, hi32(ml[i]), l * er);
-                                o[0] = __builtin_fmaf(ep, lo32(v0[i]), o[0] * er);
-                                o[1] = __builtin_fmaf(ep, hi32(v0[i]), o[1] * er);
-                                o[2] = __builtin_fmaf(ep, lo32(v1[i]), o[2] * er);
-                                o[3] = __builtin_fmaf(ep, hi32(v1[i]), o[3] * er);
-                                o2[0] = __builtin_fmaf(ep, lo32(w0[i]), o2[0] * er);
-                                o2[1] = __builtin_fmaf(ep, hi32(w0[i]), o2[1] * er);
-                                o2[2] = __builtin_fmaf(ep, lo32(w1[i]), o2[2] * er);
-                                o2[3] = __builtin_fmaf(ep, hi32(w1[i]), o2[3] * er);
-                                m = mn;
-                            }
+                        for (int i = 0; i < kAhead; ++i) {
+                            const int p = min(p0 + i, parts - 1);
+                            const uint64_t *s = tile_slot(
+                                a.slots + (2 * (int64_t)(gf + p) + (p == 0 ? 1 : 0)) * slot_elems, t) + lane;
+                            ml[i] = part_load(s + TreeSlot<D>::O * kWave);
+#pragma unroll
+                            for (int n = 0; n < ND; ++n)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h)
+                                    v[i][n][h] = part_load(s + (2 * (wave + n * kWaves) + h) * kWave);
                         }
-                        store_out(cn, d, o, l);
-                        if (d + KW < DB) store_out(cn, d2, o2, l);
+#pragma unroll
+                        for (int i = 0; i < kAhead; ++i) {
+                            if (p0 + i >= parts) break;
+                            const float mp = lo32(ml[i]), mn = fmaxf(m, mp);
+                            const float er = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+                            const float ep = mp == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mp - mn);
+                            l = __builtin_fmaf(ep, hi32(ml[i]), l * er);
+#pragma unroll
+                            for (int n = 0; n < ND; ++n)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    o[n][2 * h] = __builtin_fmaf(ep, lo32(v[i][n][h]), o[n][2 * h] * er);
+                                    o[n][2 * h + 1] =
+                                        __builtin_fmaf(ep, hi32(v[i][n][h]), o[n][2 * h + 1] * er);
+                                }
+                            m = mn;
+                        }
                     }
+#pragma unroll
+                    for (int n = 0; n < ND; ++n) store_out(cn, wave + n * kWaves, o[n], l);
                 }
             }
             __syncthreads();  // sLast is read before the next segment writes it
@@ -750,10 +754,10 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
 
 // ---- host ------------------------------------------------------------------------------
 
-// How a launch of `batch` sequences is laid out: tiles per wave, the ways the waves split the
-// columns, the column ranges, and the workgroups.
+// How a launch of `batch` sequences is laid out: tiles per wave, the column ranges, the
+// workgroups, and the units that an item counts beside its blocks.
 struct TreeShape {
-    int64_t nc, cw, chunks, wgs, extra;
+    int64_t nc, chunks, wgs, extra;
 };
 
 TreeShape tree_shape(const reef_tree_params *p, int64_t batch) {
@@ -761,10 +765,12 @@ TreeShape tree_shape(const reef_tree_params *p, int64_t batch) {
     const int64_t cus = compute_units();
     const int64_t tiles = ceil_div(p->draft_len * (p->q_heads / p->kv_heads), 16);
     s.nc = tiles > 1 ? 2 : 1;
-    s.cw = 1;
-    while (s.cw < kMaxSplit && s.cw * s.nc < tiles) s.cw *= 2;
-    s.chunks = ceil_div(tiles, s.nc * s.cw);
-    s.extra = (s.nc == 2 ? 5 : 2) * (kWaves / s.cw);
+    // More columns become further items that read the same keys, from L2 mostly: split over
+    // the waves of a workgroup instead, the keys were cut into more parts (32 x 8/1 heads, 64
+    // drafted, 512 columns: 102 us in ranges of 32, 103 of 64, 109 of 128; 1 x 8192 keys, 128
+    // columns: 27 in ranges of 32, 35 of 64).
+    s.chunks = ceil_div(tiles, s.nc);
+    s.extra = (s.nc == 2 ? 5 : 2) * kWaves;
     const int64_t units =
         batch * p->kv_heads * s.chunks * ceil_div(p->max_context, kBlockKeys);
     s.wgs = std::max<int64_t>(1, std::min(std::min(kWgPerCu * cus, units), (int64_t)kCounters));
@@ -780,7 +786,7 @@ int64_t tree_workspace(const reef_tree_params *p) {
     for (const int64_t batch : {std::min<int64_t>(p->batch, kPlan), p->batch % kPlan}) {
         if (batch == 0) continue;
         const TreeShape s = tree_shape(p, batch);
-        most = std::max(most, s.wgs * 2 * s.cw * s.nc * elems * 8);
+        most = std::max(most, s.wgs * 2 * s.nc * elems * 8);
     }
     return kCounterBytes + most;
 }
@@ -792,7 +798,8 @@ bool params_ok(const reef_tree_params *p) {
 
 bool params_supported(const reef_tree_params *p) {
     return (p->head_dim == 64 || p->head_dim == 128) && p->draft_len <= kMaxDrafts &&
-           p->q_heads <= 65535 && p->q_heads / p->kv_heads <= kMaxGroup && p->batch <= 65535 && p->max_context < (int64_t(1) << 30);
+           p->q_heads <= 65535 && p->q_heads / p->kv_heads <= kMaxGroup && p->batch <= 65535 &&
+           p->max_context < (int64_t(1) << 30);
 }
 
 bool strides_ok(const reef_strides *s, int64_t unit) {
@@ -856,7 +863,6 @@ reef_status launch_tree(const reef_tree_params *p, TreeArgs &a, const reef_strid
         const TreeShape s = tree_shape(p, batch);
         TreeArgs c = a;
         c.batch = (int32_t)batch;
-        c.cw = (int32_t)s.cw;
         c.chunks = (int32_t)s.chunks;
         c.extra = (int32_t)s.extra;
         c.q += b0 * a.q_sb;
