@@ -421,7 +421,8 @@ reef_status reef_attention_decode_int8_paged_noalloc(
  * `window` positions up to its own. Pages that hold only tokens before every row's window
  * are not looked up.
  * A sequence whose length is outside [T, max_context] sets BAD_LENGTH and yields zeros; a
- * page number outside [0, P) sets BAD_PAGE and its tokens take no part.
+ * page number outside [0, P) sets BAD_PAGE and its tokens take no part. A drafted token
+ * whose scales are not finite leaves the rows that see it not finite, and no others.
  *
  * Workspace as for decode: reef_attention_decode_tree_workspace_bytes(p) bytes (0: invalid
  * or unsupported sizes), 16-byte aligned, zero-filled before its first use; every call
@@ -513,7 +514,8 @@ reef_status reef_kv_append_int8_paged(const reef_kv_append_params *p, const floa
  * pages are given out lowest first, in the order of the sequences and of their blocks.
  *   - A sequence or pair with a negative index is padding; one past the end sets BAD_LENGTH,
  *     as does a length below 0 or (fork) beyond the table; a page number at or past
- *     num_pages, or one that page_refs does not count, sets BAD_PAGE. Neither is followed.
+ *     num_pages, or a page given back that page_refs does not count, sets BAD_PAGE. Neither
+ *     is followed.
  *   - batch, n <= 65535.
  */
 
@@ -532,14 +534,14 @@ reef_status reef_kv_fork(const int32_t *parents, const int32_t *children, int64_
                          int64_t batch, int32_t *page_refs, int64_t num_pages,
                          uint32_t *status_word, hipStream_t stream);
 
-/* Room for new_tokens more tokens of every sequence, in pages of its own: blocks that the
- * tokens at context_lens[b] .. context_lens[b] + new_tokens - 1 fall in and that have no
- * page get one, and those whose page is shared get one instead of it; where that page holds
- * tokens already (the last, partial one), copy_src[b] and copy_dst[b] (both [batch]) name
- * the two. A sequence that would pass max_blocks_per_seq * 16 tokens keeps its blocks and
- * sets CAPACITY, as do the blocks for which no free page is left (the others are served;
- * the call may be repeated once there are). Lengths are not changed. The workspace needs
- * reef_kv_reserve_workspace_bytes bytes, of any contents. */
+/* Room for new_tokens more tokens of every sequence (one of length 0 too), in pages of its
+ * own: blocks that the tokens at context_lens[b] .. context_lens[b] + new_tokens - 1 fall in
+ * and that have no page get one, and those whose page is shared get one instead of it; where
+ * that page holds tokens already (the last, partial one), copy_src[b] and copy_dst[b] (both
+ * [batch]) name the two. A sequence that would pass max_blocks_per_seq * 16 tokens keeps its
+ * blocks and sets CAPACITY, as do the blocks for which no free page is left (the others are
+ * served; with their copies made, the call may be repeated once there are). Lengths are not
+ * changed. The workspace needs reef_kv_reserve_workspace_bytes bytes, of any contents. */
 size_t reef_kv_reserve_workspace_bytes(int64_t batch, int64_t new_tokens);
 
 reef_status reef_kv_reserve(int32_t *block_table, int64_t max_blocks_per_seq,

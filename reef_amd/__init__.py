@@ -860,6 +860,8 @@ def kv_free(sequences, block_table, context_lens, page_refs, status: StatusWord 
     _expect("kv_free", _torch().int32, (sequences, "sequences"), (block_table, "block_table"),
             (context_lens, "context_lens"), (page_refs, "page_refs"))
     B, blocks = _table("kv_free", block_table, context_lens, page_refs)
+    if sequences.numel() == 0:
+        return
     own = status or StatusWord(block_table.device)
     check(_lib().reef_kv_free(_ptr(sequences), sequences.numel(), _ptr(block_table), blocks,
                               _ptr(context_lens), B, _ptr(page_refs), page_refs.numel(),
@@ -878,6 +880,8 @@ def kv_fork(parents, children, block_table, context_lens, page_refs,
     B, blocks = _table("kv_fork", block_table, context_lens, page_refs)
     if parents.numel() != children.numel():
         raise InvalidArgument("kv_fork: as many parents as children")
+    if parents.numel() == 0:
+        return
     own = status or StatusWord(block_table.device)
     check(_lib().reef_kv_fork(_ptr(parents), _ptr(children), parents.numel(), _ptr(block_table),
                               blocks, _ptr(context_lens), B, _ptr(page_refs), page_refs.numel(),
@@ -897,7 +901,8 @@ def kv_reserve(block_table, context_lens, page_refs, new_tokens: int,
             (context_lens, "context_lens"), (page_refs, "page_refs"))
     B, blocks = _table("kv_reserve", block_table, context_lens, page_refs)
     device = block_table.device
-    n = _lib().reef_kv_reserve_workspace_bytes(B, new_tokens)
+    fits = 0 < new_tokens <= blocks * PAGE  # (refused below otherwise)
+    n = _lib().reef_kv_reserve_workspace_bytes(B, new_tokens) if fits else 0
     ints = torch.empty(n // 4 + 2 * B, dtype=torch.int32, device=device)
     source, place = ints[:B], ints[B:2 * B]
     own = status or StatusWord(device)
@@ -1066,6 +1071,7 @@ def _epilogue(activation, residual, rows, fout, what):
     _require(residual, _torch().float32, "residual")
     if tuple(residual.shape) != (rows, fout) or _row_stride(residual) is None:
         raise InvalidArgument(f"{what}: residual must be [rows, out] with contiguous rows")
+    _on_device(what, residual)
     return _EPILOGUE.pack(residual.data_ptr(), _row_stride(residual), ACTIVATIONS[activation])
 
 
@@ -1081,6 +1087,7 @@ def _product_out(out, rows, fout, device, what):
     if out is None:
         return torch.empty((rows, fout), dtype=torch.float32, device=device), fout
     _require(out, torch.float32, "out")
+    _on_device(what, out)
     stride = _row_stride(out)
     if tuple(out.shape) != (rows, fout) or stride is None or stride < fout:
         raise InvalidArgument(f"{what}: out must be [rows, out] with contiguous rows")
@@ -1138,7 +1145,7 @@ def gemm_w8a8(xq, x_scales, weight, w_scales, bias=None, status: StatusWord | No
         if bias.numel() != fout:
             raise InvalidArgument("gemm_w8a8 shapes: bias [out]")
         bias = bias.contiguous()
-    _on_device("gemm_w8a8", xq, x_scales, weight, w_scales, bias, residual, out)
+    _on_device("gemm_w8a8", xq, x_scales, weight, w_scales, bias)
     epilogue = _epilogue(activation, residual, rows, fout, "gemm_w8a8")
     y, y_stride = _product_out(out, rows, fout, xq.device, "gemm_w8a8")
     own = status or StatusWord(xq.device)
@@ -1190,7 +1197,7 @@ def rmsnorm_quantize(x, weight=None, *, residual=None, eps=1e-6, residual_out=No
             raise InvalidArgument("rmsnorm_quantize: residual must have x's shape")
     elif residual_out is not None:
         raise InvalidArgument("rmsnorm_quantize: residual_out needs a residual")
-    _on_device("rmsnorm_quantize", x, weight, residual, residual_out)
+    _on_device("rmsnorm_quantize", x, weight, residual)
 
     x2, x_stride = _rows_of(x, width)
     r2 = h = None

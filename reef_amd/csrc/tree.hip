@@ -506,11 +506,15 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
                 pg_next = pg_after;
                 // Blocks that every row sees whole skip the masks. In the others a hidden key's
                 // score is -inf, and the value scale of a key that no row of the wave sees
-                // is 0 (the cache there may hold anything).
+                // is 0 (the cache there may hold anything). A drafted token whose value scale
+                // is not finite makes the rows that see it NaN through their sums, and no
+                // others: its scale is 0 too.
                 const int kk = kb + 16 * grp;
                 float vsc = vs;
                 if (kb < full_lo || kb + kBlockKeys > seg.sk.prefix || !__all(live)) {
                     uint32_t any = 0;
+                    const bool finite = __builtin_fabsf(vsc) < INFINITY;
+                    const uint32_t nan = row_or(finite ? 0u : 1u << col);
 #pragma unroll
                     for (int t = 0; t < NC; ++t) {
                         const Sight sight = sSight[wave][t][col];
@@ -522,10 +526,15 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
 #pragma unroll
                         for (int r = 0; r < 16; ++r)
                             if (!(vis >> r & 1u)) xs[t][r] = -INFINITY;
+                        if (vis & nan) {
+#pragma unroll
+                            for (int r = 0; r < 16; ++r)
+                                if (vis & nan & 1u << r) xs[t][r] = __builtin_nanf("");
+                        }
                         any |= vis;
                     }
                     any = row_or(any);
-                    if (!(any >> col & 1u)) vsc = 0.0f;
+                    if (!finite || !(any >> col & 1u)) vsc = 0.0f;
                 }
                 float mt[NC];
                 bool grow = false;
@@ -637,7 +646,7 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
             if (!cn.live) return;
             float *row = a.out + seg.b * a.o_sb + cn.head * a.o_sh + cn.token * a.o_st;
             f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (l > 0.0f) y = o * (1.0f / l);
+            if (l != 0.0f) y = o * (1.0f / l);  // (NaN where the row's sum is)
             *reinterpret_cast<f32x4 *>(row + 16 * d + 4 * grp) = y;
         };
         // The waves merge tile by tile through LDS, each the channel blocks d = wave, wave + 4,

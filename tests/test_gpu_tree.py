@@ -323,6 +323,29 @@ def test_bad_lengths_and_pages(reef):
         assert np.abs(out - ref)[[0, 1, 3]].max() <= tol
 
 
+@pytest.mark.parametrize("D,Hq,H,T", [(64, 2, 2, 7), (128, 8, 1, 20)])
+@pytest.mark.parametrize("what", ["nan key", "nan value", "inf value"])
+def test_a_drafted_token_that_is_not_finite(reef, D, Hq, H, T, what):
+    """Its scale reaches the rows that see it, which are not finite, and no other."""
+    print(f"\n[case] tree with a drafted token that is not finite: {what} {Hq}/{H}x{D} T {T}",
+          flush=True)
+    rng = np.random.default_rng(D)
+    B, L = 2, 720
+    lens = [700, T]
+    q, k, v, qs, ks, vs = problem(rng, B, Hq, H, D, T, lens, L)
+    m = tree_masks(rng, B, T, "tree")
+    ref, tol = reference(q, k, v, qs, ks, vs, lens, m, 0, 1 / math.sqrt(D))
+    bad = 1
+    for b in range(B):
+        (ks if what == "nan key" else vs)[b, :, lens[b] - T + bad] = float(what[:3])
+    out = reef.attention_decode_tree(gpu(q), gpu(qs), *contiguous(k, v, ks, vs),
+                                     gpu(np.array(lens, np.int32)), tree_mask=words(m)).cpu().numpy()
+    sees = np.broadcast_to(m[:, None, :, bad], out.shape[:3])
+    assert sees.any() and not sees.all()
+    assert not np.isfinite(out[sees]).any()
+    assert np.abs(out - ref)[~sees].max() <= tol
+
+
 def test_workspace_serves_every_shape(reef):
     """One explicit workspace, sized for the largest, through calls of several shapes."""
     print("\n[case] tree workspace over shapes", flush=True)
