@@ -206,6 +206,148 @@ inline void linear_w8a8(const float *x, int64_t rows, int64_t in_features, int64
           "linear");
 }
 
+// The same with an activation and a residual in the product's epilogue, and the product
+// alone on rows that are int8 already (quantize_rows, rmsnorm_quantize).
+inline void linear_w8a8(const float *x, int64_t rows, int64_t in_features, int64_t x_row_stride,
+                        const int8_t *weight, const float *w_scales, const float *bias,
+                        const reef_epilogue &epilogue, int64_t out_features, float *y,
+                        int64_t y_row_stride, void *workspace, size_t workspace_bytes,
+                        uint32_t *status_word, hipStream_t stream) {
+    check(reef_linear_w8a8_epilogue(x, rows, in_features, x_row_stride, weight, w_scales, bias,
+                                    &epilogue, out_features, y, y_row_stride, workspace,
+                                    workspace_bytes, status_word, stream),
+          "linear");
+}
+
+inline void gemm_w8a8(const int8_t *xq, const float *x_scales, int64_t rows, int64_t in_features,
+                      const int8_t *weight, const float *w_scales, const float *bias,
+                      const reef_epilogue &epilogue, int64_t out_features, float *y,
+                      int64_t y_row_stride, uint32_t *status_word, hipStream_t stream) {
+    check(reef_gemm_w8a8_epilogue(xq, x_scales, rows, in_features, weight, w_scales, bias,
+                                  &epilogue, out_features, y, y_row_stride, status_word, stream),
+          "gemm_w8a8");
+}
+
+// The root-mean-square norm of x (+ residual) as int8 rows with scales.
+inline void rmsnorm_quantize(const float *x, int64_t rows, int64_t width, int64_t x_row_stride,
+                             const float *residual, int64_t residual_row_stride,
+                             const float *weight, double eps, int8_t *q, float *scales,
+                             float *sum, int64_t sum_row_stride, uint32_t *status_word,
+                             hipStream_t stream) {
+    check(reef_rmsnorm_quantize_int8(x, rows, width, x_row_stride, residual, residual_row_stride,
+                                     weight, eps, q, scales, sum, sum_row_stride, status_word,
+                                     stream),
+          "rmsnorm_quantize");
+}
+
+// --- drafted tokens (speculative decoding) and pages of the cache ---------------------------
+
+// The tree_workspace_bytes(p) bytes are the caller's, zero-filled once before first use.
+inline size_t tree_workspace_bytes(const reef_tree_params &p) {
+    return reef_attention_decode_tree_workspace_bytes(&p);
+}
+
+// Drafted tokens, appended to the cache before, over a contiguous int8 cache. tree_mask
+// nullptr: a chain.
+inline void decode_tree(const reef_tree_params &p, const int8_t *q, const reef_strides *q_strides,
+                        const float *q_scales, const int8_t *k_cache, const int8_t *v_cache,
+                        const float *k_scales, const float *v_scales, const int32_t *context_lens,
+                        const uint64_t *tree_mask, float *out, const reef_strides *out_strides,
+                        void *workspace, size_t workspace_bytes, uint32_t *status_word,
+                        hipStream_t stream) {
+    check(reef_attention_decode_tree_int8(&p, q, q_strides, q_scales, k_cache, v_cache, k_scales,
+                                          v_scales, context_lens, tree_mask, out, out_strides,
+                                          workspace, workspace_bytes, status_word, stream),
+          "attention of drafted tokens");
+}
+
+inline void decode_tree_paged(const reef_tree_params &p, const int8_t *q,
+                              const reef_strides *q_strides, const float *q_scales,
+                              const int8_t *k_pages, const int8_t *v_pages,
+                              const float *k_scale_pages, const float *v_scale_pages,
+                              const int32_t *block_table, int64_t max_blocks_per_seq,
+                              int64_t num_pages, const int32_t *context_lens,
+                              const uint64_t *tree_mask, float *out,
+                              const reef_strides *out_strides, void *workspace,
+                              size_t workspace_bytes, uint32_t *status_word, hipStream_t stream) {
+    check(reef_attention_decode_tree_int8_paged(
+              &p, q, q_strides, q_scales, k_pages, v_pages, k_scale_pages, v_scale_pages,
+              block_table, max_blocks_per_seq, num_pages, context_lens, tree_mask, out,
+              out_strides, workspace, workspace_bytes, status_word, stream),
+          "attention of drafted tokens");
+}
+
+// The accepted ones of a sequence's drafted tokens move to the first of their places.
+inline void kv_keep(const reef_kv_append_params &p, const int32_t *kept, const int32_t *kept_lens,
+                    const int32_t *context_lens, int8_t *k_cache, int8_t *v_cache,
+                    float *k_scales, float *v_scales, int32_t *new_lens, uint32_t *status_word,
+                    hipStream_t stream) {
+    check(reef_kv_keep_int8(&p, kept, kept_lens, context_lens, k_cache, v_cache, k_scales,
+                            v_scales, new_lens, status_word, stream),
+          "kv_keep");
+}
+
+inline void kv_keep_paged(const reef_kv_append_params &p, const int32_t *kept,
+                          const int32_t *kept_lens, const int32_t *context_lens,
+                          const int32_t *block_table, int64_t max_blocks_per_seq,
+                          int64_t num_pages, int8_t *k_pages, int8_t *v_pages,
+                          float *k_scale_pages, float *v_scale_pages, int32_t *new_lens,
+                          uint32_t *status_word, hipStream_t stream) {
+    check(reef_kv_keep_int8_paged(&p, kept, kept_lens, context_lens, block_table,
+                                  max_blocks_per_seq, num_pages, k_pages, v_pages, k_scale_pages,
+                                  v_scale_pages, new_lens, status_word, stream),
+          "kv_keep");
+}
+
+inline void kv_copy_pages(const int32_t *src, const int32_t *dst, int64_t n, int64_t kv_heads,
+                          int64_t head_dim, int8_t *k_pages, int8_t *v_pages,
+                          float *k_scale_pages, float *v_scale_pages, int64_t num_pages,
+                          uint32_t *status_word, hipStream_t stream) {
+    check(reef_kv_copy_pages(src, dst, n, kv_heads, head_dim, k_pages, v_pages, k_scale_pages,
+                             v_scale_pages, num_pages, status_word, stream),
+          "kv_copy_pages");
+}
+
+// A block table with its lengths and page counts, all on the device, and the calls that
+// change it (attention.h, "Pages of the paged cache"). A full pool throws std::length_error
+// once the status word is checked.
+struct page_table {
+    int32_t *blocks;  // [batch, max_blocks]
+    int64_t batch, max_blocks;
+    int32_t *lens;  // [batch]
+    int32_t *refs;  // [pages]
+    int64_t pages;
+
+    void free(const int32_t *sequences, int64_t n, uint32_t *status_word,
+              hipStream_t stream) const {
+        check(reef_kv_free(sequences, n, blocks, max_blocks, lens, batch, refs, pages, status_word,
+                           stream),
+              "kv_free");
+    }
+    void fork(const int32_t *parents, const int32_t *children, int64_t n, uint32_t *status_word,
+              hipStream_t stream) const {
+        check(reef_kv_fork(parents, children, n, blocks, max_blocks, lens, batch, refs, pages,
+                           status_word, stream),
+              "kv_fork");
+    }
+    size_t reserve_workspace_bytes(int64_t new_tokens) const {
+        return reef_kv_reserve_workspace_bytes(batch, new_tokens);
+    }
+    void reserve(int64_t new_tokens, int32_t *copy_src, int32_t *copy_dst, void *workspace,
+                 size_t workspace_bytes, uint32_t *status_word, hipStream_t stream) const {
+        check(reef_kv_reserve(blocks, max_blocks, lens, batch, new_tokens, refs, pages, copy_src,
+                              copy_dst, workspace, workspace_bytes, status_word, stream),
+              "kv_reserve");
+    }
+    size_t compact_workspace_bytes() const { return reef_kv_compact_workspace_bytes(pages); }
+    void compact(int32_t *copy_src, int32_t *copy_dst, int32_t *num_live, void *workspace,
+                 size_t workspace_bytes, uint32_t *status_word, hipStream_t stream) const {
+        check(reef_kv_compact(blocks, max_blocks, batch, refs, pages, copy_src, copy_dst, num_live,
+                              workspace, workspace_bytes, status_word, stream),
+              "kv_compact");
+    }
+};
+
 }  // namespace reef_hip
 
 #endif  // REEF_HIP_ATTENTION_HPP

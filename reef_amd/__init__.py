@@ -276,11 +276,14 @@ def _require(t, dtype, name):
 def _expect(what, dtype, *tensors):
     """(tensor, name) pairs: contiguous, of one type, on the current device, whose stream the
     call takes."""
-    device = _torch()._C._cuda_getDevice()
+    device = None
     for t, name in tensors:
         try:
-            if t.dtype is dtype and t.get_device() == device and t.is_contiguous():
-                continue
+            if t.dtype is dtype and t.is_cuda and t.is_contiguous():
+                if device is None:
+                    device = _torch()._C._cuda_getDevice()
+                if t.get_device() == device:
+                    continue
         except AttributeError:
             pass
         _require(t, dtype, name)

@@ -595,11 +595,11 @@ extern "C" reef_status reef_kv_reserve(int32_t *block_table, int64_t max_blocks_
         !aligned(workspace, 4))
         return REEF_INVALID_ARGUMENT;
     if (new_tokens > max_blocks_per_seq * kPage) return REEF_CAPACITY;
-    if (workspace_bytes < reef_kv_reserve_workspace_bytes(batch, new_tokens))
-        return REEF_INVALID_ARGUMENT;
     a.nb = (int32_t)touched_blocks(new_tokens);
     a.items = batch * a.nb;
     if (new_tokens >= (int64_t(1) << 30) || a.items >= (int64_t(1) << 31)) return REEF_UNSUPPORTED;
+    if (workspace_bytes < reef_kv_reserve_workspace_bytes(batch, new_tokens))
+        return REEF_INVALID_ARGUMENT;
     a.new_tokens = (int32_t)new_tokens;
     a.copy_src = copy_src;
     a.copy_dst = copy_dst;
