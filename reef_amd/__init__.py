@@ -664,15 +664,25 @@ def tree_workspace(params: TreeParams, device):
 
 def _tree_workspace(n, device, stream):
     """This stream's workspace. A call under graph capture takes one of its own, which lives
-    in the graph's memory: graphs that replay at the same time share nothing."""
+    in the graph's memory: graphs that replay at the same time share nothing. Only its
+    counters have to be zero, the first 8 KB: not a megabyte of parts at every replay."""
     torch = _torch()
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(max(n, 256), dtype=torch.uint8, device=device)
+        ws = torch.empty(max(n, 8192), dtype=torch.uint8, device=device)
+        ws[:8192].zero_()
+        return ws
     key = (device.index, stream)
     ws = _TREE_WS.get(key)
     if ws is None or ws.numel() < n:
         ws = _TREE_WS[key] = torch.zeros(max(n, 256), dtype=torch.uint8, device=device)
     return ws
+
+
+def _given(workspace):
+    _on_device("workspace", workspace)
+    if not workspace.is_contiguous():
+        raise InvalidArgument("workspace must be contiguous")
+    return workspace
 
 
 def _tree_inputs(what, q, q_scales, tree_mask, window, softmax_scale, q_granularity, kv_heads,
@@ -732,7 +742,7 @@ def attention_decode_tree(q, q_scales, k_cache, v_pages, k_scales, v_scales, con
         D, context_lens, out)
     stream = _stream()
     n = _lib().reef_attention_decode_tree_workspace_bytes(p)
-    ws = _tree_workspace(n, q.device, stream) if workspace is None else workspace
+    ws = _tree_workspace(n, q.device, stream) if workspace is None else _given(workspace)
     own = status or StatusWord(q.device)
     check(_lib().reef_attention_decode_tree_int8(
         p, _ptr(q), _strides4(q), _ptr(q_scales), _ptr(k_cache), _ptr(v_pages), _ptr(k_scales),
@@ -761,7 +771,7 @@ def attention_decode_tree_paged(q, q_scales, k_pages, v_pages, k_scale_pages, v_
         context_lens, out)
     stream = _stream()
     n = _lib().reef_attention_decode_tree_workspace_bytes(p)
-    ws = _tree_workspace(n, q.device, stream) if workspace is None else workspace
+    ws = _tree_workspace(n, q.device, stream) if workspace is None else _given(workspace)
     own = status or StatusWord(q.device)
     check(_lib().reef_attention_decode_tree_int8_paged(
         p, _ptr(q), _strides4(q), _ptr(q_scales), _ptr(k_pages), _ptr(v_pages),

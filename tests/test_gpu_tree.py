@@ -361,6 +361,30 @@ def test_workspace_serves_every_shape(reef):
         assert np.abs(out.cpu().numpy() - ref).max() <= tol
 
 
+def test_refuses_what_lies_elsewhere(reef):
+    """A workspace in host memory, q and scales that do not match: refused before a launch."""
+    print("\n[case] tree refusals", flush=True)
+    rng = np.random.default_rng(17)
+    q, k, v, qs, ks, vs = problem(rng, 1, 2, 1, 64, 3, [40], 48)
+    cache = contiguous(k, v, ks, vs)
+    p = reef.TreeParams(1, 2, 1, 64, 3, 48, 0, 0.1, 2, 0, 0)
+    ws = reef.tree_workspace(p, "cuda")
+    for call in (lambda: reef.attention_decode_tree(gpu(q), gpu(qs), *cache, workspace=ws.cpu()),
+                 lambda: reef.attention_decode_tree(gpu(q), gpu(qs), *cache, workspace=ws[:100]),
+                 lambda: reef.attention_decode_tree(gpu(q), gpu(qs), *cache,
+                                                    workspace=torch.stack([ws, ws])[:, ::2]),
+                 lambda: reef.attention_decode_tree(gpu(q), gpu(qs[:, :1]), *cache),
+                 lambda: reef.attention_decode_tree(gpu(q)[..., :32], gpu(qs), *cache),
+                 lambda: reef.attention_decode_tree(gpu(q), gpu(qs), *cache, out=gpu(qs)),
+                 lambda: reef.attention_decode_tree(gpu(q), gpu(qs), *cache, window=-1),
+                 lambda: reef.attention_decode_tree(
+                     gpu(q), gpu(qs), *cache, tree_mask=torch.zeros((1, 2), dtype=torch.int64, device="cuda")),
+                 lambda: reef.attention_decode_tree(
+                     gpu(q), gpu(qs), *cache, torch.zeros(2, dtype=torch.int32, device="cuda"))):
+        with pytest.raises(reef.InvalidArgument):
+            call()
+
+
 def test_two_streams_and_a_large_batch(reef):
     """Calls on two streams at once have a workspace each; over 2048 sequences run in slices."""
     print("\n[case] tree on two streams, 2100 sequences", flush=True)
