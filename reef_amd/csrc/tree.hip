@@ -57,7 +57,10 @@ struct TreeArgs {
 // keys counts one block, so that some workgroup stores its zeros.
 struct SeqKeys {
     int len, prefix, lo, first_block, blocks;
-    bool bad;
+    // (an int: the padding behind a bool became an array in LDS when segments were copied, at
+    // places worked out from the dispatch packet, and reading that packet, which lies in host
+    // memory, held up every launch by 4 us and more)
+    int bad;
 };
 
 __device__ __forceinline__ SeqKeys seq_keys(const TreeArgs &a, int b) {
@@ -203,10 +206,10 @@ struct Sight {
     uint64_t drafts;
 };
 
-__device__ __forceinline__ uint64_t mask_word(const TreeArgs &a, int b, int token) {
-    if (!a.mask) return (2ull << token) - 1;
+// The drafted tokens that a row sees, of its mask word (without masks: the chain).
+__device__ __forceinline__ uint64_t seen_drafts(const TreeArgs &a, int token, uint64_t word) {
     const uint64_t all = a.drafts == 64 ? ~0ull : (1ull << a.drafts) - 1;
-    return a.mask[(int64_t)b * a.drafts + token] & all;
+    return a.mask ? word & all : (2ull << token) - 1;
 }
 
 __device__ __forceinline__ Sight sight_of(const TreeArgs &a, int b, const SeqKeys &sk, uint64_t m) {
@@ -218,7 +221,8 @@ __device__ __forceinline__ Sight sight_of(const TreeArgs &a, int b, const SeqKey
         r.lo = max(0, sk.prefix + depth + 1 - a.window);
         if (a.window < a.drafts) {
             for (int j = 0; j < a.drafts; ++j) {
-                const int dj = (int)__popcll(mask_word(a, b, j)) - 1;
+                const uint64_t word = a.mask ? a.mask[(int64_t)b * a.drafts + j] : 0;
+                const int dj = (int)__popcll(seen_drafts(a, j, word)) - 1;
                 if (dj <= depth - a.window) r.drafts &= ~(1ull << j);
             }
         }
@@ -359,9 +363,9 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
     constexpr int k_step = kWaves * kBlockKeys;
 
     // A block's operands, and what a segment's rows need, in registers.
-    i32x4 kop[4][KS], vop[DB], qreg[NC][KS];
-    float ks = 0.0f, vs = 0.0f, c[NC];
-    uint64_t mreg[NC];
+    i32x4 kop[4][KS], vop[DB];
+    float ks = 0.0f, vs = 0.0f, cs[NC];
+    uint32_t shown = 0;  // bit t: this lane's row of tile t sees something
     BlockAt at;
     bool bad_page = false;
     int pg_next;
@@ -383,24 +387,50 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
     };
     // Whether this wave has anything to do in a segment.
     auto busy = [&](const Segment &s) { return first_key(s) < end_key(s); };
-    // The loads of a segment's rows, and of its first block where `block` (pages: its table
-    // entries).
-    auto issue = [&](const TreeArgs &a, const Segment &s, int pages, bool block) {
-        if (!busy(s)) return;
+    // A segment's rows on their way to LDS (each wave its own places). All their loads leave
+    // together, from addresses without a branch: one round trip. (Kept in registers across the
+    // segment before, they were spilled as they came, one round trip after another: 16 x U[512,
+    // 8192] keys, 16 drafted 76 us, 71 this way.)
+    struct Rows {
+        i32x4 q[NC][KS];
+        float c[NC];
+        uint64_t m[NC];
+    };
+    auto load_rows = [&](const TreeArgs &a, const Segment &s) {
+        Rows r;
+        const uint64_t *masks = a.mask ? a.mask : reinterpret_cast<const uint64_t *>(a.q);
 #pragma unroll
         for (int t = 0; t < NC; ++t) {
             const Column cn = column(a, s, t);
-            mreg[t] = mask_word(a, s.b, cn.token);
-            c[t] = a.q_gran == REEF_SCALE_PER_TENSOR ? a.qs[0]
-                   : a.q_gran == REEF_SCALE_PER_HEAD
-                       ? a.qs[cn.head]
-                       : a.qs[((int64_t)s.b * a.q_heads + cn.head) * a.drafts + cn.token];
+            r.m[t] = masks[a.mask ? (int64_t)s.b * a.drafts + cn.token : 0];
+            const int64_t row = ((int64_t)s.b * a.q_heads + cn.head) * a.drafts + cn.token;
+            r.c[t] = a.qs[a.q_gran == REEF_SCALE_PER_TOKEN ? row
+                          : a.q_gran == REEF_SCALE_PER_HEAD ? cn.head
+                                                            : 0];
             const int8_t *qrow = a.q + s.b * a.q_sb + cn.head * a.q_sh + cn.token * a.q_st;
 #pragma unroll
             for (int e = 0; e < KS; ++e)
-                qreg[t][e] = *reinterpret_cast<const i32x4 *>(qrow + 64 * e + 16 * grp);
+                r.q[t][e] = *reinterpret_cast<const i32x4 *>(qrow + 64 * e + 16 * grp);
         }
-        if (!block) return;
+        return r;
+    };
+    auto put_rows = [&](const TreeArgs &a, const Segment &s, const Rows &r) {
+        shown = 0;
+#pragma unroll
+        for (int t = 0; t < NC; ++t) {
+            const Column cn = column(a, s, t);
+            const uint64_t m = cn.live ? seen_drafts(a, cn.token, r.m[t]) : 0;
+#pragma unroll
+            for (int e = 0; e < KS; ++e)
+                sQ[wave][t * KS + e][lane] = cn.live ? r.q[t][e] : i32x4{0, 0, 0, 0};
+            cs[t] = cn.live ? r.c[t] * a.score_scale : 1.0f;
+            shown |= (m != 0 ? 1u : 0u) << t;
+            const Sight sight = sight_of(a, s.b, s.sk, m);
+            if (grp == 0) sSight[wave][t][col] = sight;
+        }
+    };
+    // The loads of a segment's first block (pages: its table entries).
+    auto issue = [&](const TreeArgs &a, const Segment &s, int pages) {
         at = block_at<PAGED>(a, s.b, s.kvh, first_key(s), s.sk, pages, col, grp, bad_page);
         load_k(a);
         load_v(a);
@@ -423,28 +453,19 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
     Segment seg = segment_at(arg, u0, b);
     if (seg.e_blk <= seg.s_blk) return;  // (uniform)
     pg_next = block_pages<PAGED>(arg, b, first_key(seg) + k_step, seg.sk, lane);
-    issue(arg, seg, block_pages<PAGED>(arg, b, first_key(seg), seg.sk, lane), true);
+    {
+        const int pages = block_pages<PAGED>(arg, b, first_key(seg), seg.sk, lane);
+        if (busy(seg)) {
+            const Rows rows = load_rows(arg, seg);
+            issue(arg, seg, pages);
+            put_rows(arg, seg, rows);
+        }
+    }
     for (int u = u0;;) {
         TreeArgs a = reread_args();
         if (seg.sk.bad && seg.s_blk == 0 && seg.kvh == 0 && seg.chunk == 0 && threadIdx.x == 0)
             flag_status(a.status, REEF_STATUS_BIT_BAD_LENGTH);
         const bool mine = busy(seg);  // wave-uniform
-        // This segment's rows: operands and sights to LDS (this wave's own places).
-        float cs[NC];
-        uint32_t shown = 0;  // bit t: this lane's row of tile t sees something
-        if (mine) {
-#pragma unroll
-            for (int t = 0; t < NC; ++t) {
-                const bool live = column(a, seg, t).live;
-#pragma unroll
-                for (int e = 0; e < KS; ++e)
-                    sQ[wave][t * KS + e][lane] = live ? qreg[t][e] : i32x4{0, 0, 0, 0};
-                cs[t] = live ? c[t] * a.score_scale : 1.0f;
-                shown |= (mreg[t] != 0 ? 1u : 0u) << t;
-                const Sight sight = sight_of(a, seg.b, seg.sk, live ? mreg[t] : 0);
-                if (grp == 0) sSight[wave][t][col] = sight;
-            }
-        }
         // The next segment, and the table entries of its first two blocks.
         u += seg.units;
         bool more_segs = u < u1;
@@ -632,9 +653,10 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
         a = reread_args();
         if (bad_page) flag_status(a.status, REEF_STATUS_BIT_BAD_PAGE);
         bad_page = false;
-        // The next segment's rows and first block fly while this one is merged.
+        // The next segment's first block flies while this one is merged (a wave that had none of
+        // this segment asks for it now).
         if (more_segs) {
-            issue(a, nxt, pg_first, !mine);
+            if (!mine && busy(nxt)) issue(a, nxt, pg_first);
             pg_next = pg_second;
         }
         a = reread_args();
@@ -763,6 +785,10 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
         }
         if (!more_segs) break;
         seg = nxt;
+        if (busy(seg)) {
+            a = reread_args();
+            put_rows(a, seg, load_rows(a, seg));
+        }
     }
 }
 
