@@ -276,12 +276,13 @@ __device__ __forceinline__ TreeArgs reread_args() {
 // merges them in order (reef_common.hpp, cross-workgroup parts).
 //
 // Bound by memory with few columns (64 x 4096 keys x 8 heads of 128, 3 drafted, 12 columns:
-// 558 MB in 97 us, 5.8 TB/s), by the softmax's vector work and the items' fixed costs with many
-// (32 sequences of one head, 64 drafted, 512 columns: 71 M scores in 95-101 us).
+// 558 MB in 90 us, 6.2 TB/s), by the softmax's vector work and the items' fixed costs with many
+// (32 sequences of one head, 64 drafted, 512 columns: 71 M scores in 90 us).
 template <int D, bool PAGED, int NC>
 __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs arg) {
     constexpr int DB = D / 16, KS = D / 64;
-    // One tile of columns has one reader of the cache: kept out of the caches.
+    // One tile of columns has one reader of the cache: kept out of the caches (64 x 4096 keys, 3
+    // drafted: 90 us against 98).
     constexpr bool NT = !PAGED && NC == 1;
     __shared__ int32_t sOff[kPlan + 1];
     __shared__ int32_t sWave[kWaves];
@@ -303,9 +304,9 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
     const int per_seq = arg.kv_heads * arg.chunks;  // items of a sequence
     const int T = units_before(arg.batch) * per_seq;  // (fits: checked for full caches)
     // No more workgroups than there are items, or parts with kMinBlocks for every wave: more
-    // parts are a longer merge, fewer a longer run (with at least 1, 2, 4 and 8 blocks a wave:
-    // 1 x 8192 keys, 8/1 heads of 128, 16 drafted 31, 26, 26, 32 us; 1 x 8192, 8/8 heads, 1
-    // drafted 33, 25, 23, 26; 3 x 1000-3000, 8/1 heads, 64 drafted 34, 30, 31, 39).
+    // parts are a longer merge, fewer a longer run (with at least 1, 2 and 3 blocks a wave:
+    // 1 x 8192 keys, 8/1 heads of 128, 16 drafted 23.4, 21.7, 22.4 us; 1 x 8192, 8/8 heads, 1
+    // drafted 22.2, 19.2, 19.4; 3 x 1000-3000, 8/1 heads, 64 drafted 22.5, 20.8, 22.9).
     const int items = arg.batch * per_seq;
     const int G = min((int)gridDim.x, max(items, (T - items * arg.extra + kMinBlocks * kWaves - 1) /
                                                      (kMinBlocks * kWaves)));
@@ -317,8 +318,9 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
         return u < mid ? u / (quota + 1) : longer + (u - mid) / quota;
     };
     // With several tiles the workgroups of one XCD hold consecutive runs: the column ranges of
-    // one (sequence, kv head) meet in its L2. With one tile nothing is shared, and plain order
-    // is faster (64 x 4096 x 8 heads of 128, 3 drafted: 98.5 us against 101.3).
+    // one (sequence, kv head) meet in its L2 (32 sequences of one head, 64 drafted 90 us against
+    // 99). With one tile nothing is shared, and plain order is faster (64 x 4096 x 8 heads of
+    // 128, 3 drafted: 90 us against 100).
     int g = blockIdx.x;
     if (NC == 1) {
         if (g >= G) return;
@@ -806,11 +808,14 @@ TreeShape tree_shape(const reef_tree_params *p, int64_t batch) {
     const int64_t tiles = ceil_div(p->draft_len * (p->q_heads / p->kv_heads), 16);
     s.nc = tiles > 1 ? 2 : 1;
     // More columns become further items that read the same keys, from L2 mostly: split over
-    // the waves of a workgroup instead, the keys were cut into more parts (32 x 8/1 heads, 64
-    // drafted, 512 columns: 102 us in ranges of 32, 103 of 64, 109 of 128; 1 x 8192 keys, 128
-    // columns: 27 in ranges of 32, 35 of 64).
+    // the waves of a workgroup instead, the keys were cut into more parts (an earlier form: 32 x
+    // 8/1 heads, 64 drafted, 512 columns 102 us in ranges of 32, 103 of 64, 109 of 128; 1 x 8192
+    // keys, 128 columns 27 in ranges of 32, 35 of 64).
     s.chunks = ceil_div(tiles, s.nc);
-    s.extra = (s.nc == 2 ? 5 : 2) * kWaves;
+    // (with 2, 3 and 5 a wave for two tiles: 16 x U[512, 8192] keys, 8/32 heads, 16 drafted
+    // 62.7, 63.6, 65 us, 3 x 1000-3000 keys, 64 drafted 20.3, 19.6, 20.9; with 1 and 2 for
+    // one tile: 1 x 8192 keys, 8/8 heads, 1 drafted 20.3, 19.2)
+    s.extra = (s.nc == 2 ? 3 : 2) * kWaves;
     const int64_t units =
         batch * p->kv_heads * s.chunks * ceil_div(p->max_context, kBlockKeys);
     s.wgs = std::max<int64_t>(1, std::min(std::min(kWgPerCu * cus, units), (int64_t)kCounters));
