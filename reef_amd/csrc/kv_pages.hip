@@ -236,7 +236,9 @@ __global__ __launch_bounds__(kScanThreads) void reserve_pages(ReserveArgs a) {
 // live page from the pool's end into the k-th free place from its front, so the ranks come
 // from one prefix count of the live pages.
 
-constexpr int kCompactThreads = 256, kCompactEach = 16;
+// (8192 pages: 4 a thread are 2.3 us faster than 16, 1 a thread 0.5 more, but then a pool of a
+// million has each of its 4096 workgroups add up as many counts)
+constexpr int kCompactThreads = 256, kCompactEach = 4;
 constexpr int kCompactChunk = kCompactThreads * kCompactEach;
 
 struct CompactArgs {
@@ -252,7 +254,7 @@ __global__ __launch_bounds__(kCompactThreads) void count_live(CompactArgs a) {
     __shared__ int sSum;
     if (threadIdx.x == 0) sSum = 0;
     __syncthreads();
-    // (loads without a branch between them: one round trip, not sixteen)
+    // (loads without a branch between them: one round trip, not four)
     int refs[kCompactEach], n = 0;
 #pragma unroll
     for (int j = 0; j < kCompactEach; ++j) {
@@ -271,7 +273,8 @@ __global__ __launch_bounds__(kCompactThreads) void count_live(CompactArgs a) {
 
 __global__ __launch_bounds__(kCompactThreads) void list_moves(CompactArgs a) {
     constexpr int W = kCompactThreads / kWave;
-    static_assert(kCompactEach * W == kWave, "one count per lane");
+    constexpr int kCounts = kCompactEach * W;
+    static_assert(kCounts <= kWave, "one count per lane");
     __shared__ int sBefore[W], sTotal[W], sLive[kWave];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // Page j of this thread is tid + 256 j of the chunk: in order, (j, wave, lane).
@@ -308,7 +311,7 @@ __global__ __launch_bounds__(kCompactThreads) void list_moves(CompactArgs a) {
         before += sBefore[w];
         total += sTotal[w];
     }
-    const int own = sLive[lane];
+    const int own = lane < kCounts ? sLive[lane] : 0;
     int s = own;
 #pragma unroll
     for (int o = 1; o < kWave; o <<= 1) {

@@ -151,7 +151,7 @@ def test_reserve_and_compact():
         assert compact(**bad) == INVALID, bad
     assert compact(pages=1 << 31) == UNSUPPORTED
     size = lib.reef_kv_compact_workspace_bytes
-    assert size(100) == 4 * (100 + 1 + 1) and size(4097) == 4 * (4097 + 2 + 1) and size(0) == 0
+    assert size(100) == 4 * (100 + 1 + 1) and size(4097) == 4 * (4097 + 5 + 1) and size(0) == 0
     assert compact(ws_bytes=size(100) - 1) == INVALID
 
 
