@@ -398,3 +398,54 @@ def test_a_step_of_a_search_in_a_graph(reef):
         step()
         assert all(torch.equal(x, y) for x, y in zip(state + work, eager))
     status.check("graph")
+
+
+@pytest.mark.parametrize("pages,entries", [(300_001, 180_000), (1_048_576, 400_000), (262_144, 262_144)])
+def test_compact_of_a_large_pool(reef, pages, entries):
+    """More chunks of pages than a workgroup has threads; a tenth of the entries shared; the last
+    pool is full."""
+    print(f"\n[case] compact {pages} pages, {entries} entries", flush=True)
+    rng = np.random.default_rng(pages)
+    m = Model(64, -(-entries // 64), pages)
+    flat = m.table.reshape(-1)
+    flat[:entries] = rng.permutation(pages)[:entries]
+    if entries < pages:
+        flat[rng.permutation(entries)[:entries // 10]] = flat[0]
+    rng.shuffle(flat)
+    m.refs[:] = np.bincount(flat[flat >= 0], minlength=pages)
+    table, _, refs = m.device()
+    for _ in range(2):  # the second time there is nothing to move
+        src, dst, live = m.compact()
+        s, d, n = reef.kv_compact(table, refs)
+        assert int(n) == live
+        assert np.array_equal(host(s), src) and np.array_equal(host(d), dst)
+        m.check(table, None, refs)
+
+
+def test_page_calls_without_work_and_refusals(reef):
+    """Empty lists do nothing; what does not match is refused before a launch."""
+    print("\n[case] page refusals", flush=True)
+    m = Model(4, 3, 20)
+    m.reserve(5)
+    m.lens[:] = 5
+    table, lens, refs = m.device()
+    none, one = gpu(i32([])), gpu(i32([1]))
+    reef.kv_free(none, table, lens, refs)
+    reef.kv_fork(none, none, table, lens, refs)
+    m.check(table, lens, refs)
+    for n in (0, -1):
+        with pytest.raises(reef.InvalidArgument):
+            reef.kv_reserve(table, lens, refs, n)
+    for n in (49, 1 << 40):
+        with pytest.raises(reef.CapacityError):
+            reef.kv_reserve(table, lens, refs, n)
+    for call in (lambda: reef.kv_free(one.long(), table, lens, refs),
+                 lambda: reef.kv_free(one, table[:, ::2], lens, refs),
+                 lambda: reef.kv_free(one, table, lens[:3], refs),
+                 lambda: reef.kv_free(one, table.view(-1), lens, refs),
+                 lambda: reef.kv_fork(one, gpu(i32([2, 3])), table, lens, refs),
+                 lambda: reef.kv_reserve(table, lens, refs.view(4, 5), 1),
+                 lambda: reef.kv_compact(table, refs.cpu())):
+        with pytest.raises(reef.InvalidArgument):
+            call()
+    m.check(table, lens, refs)
