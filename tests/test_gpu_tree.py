@@ -447,3 +447,51 @@ def test_tree_in_graphs(reef):
         assert all(torch.equal(out, eager) for _, out in graphs)
         assert torch.equal(step(), eager)
     status.check("graphs")
+
+
+@pytest.mark.parametrize("layout", ["contiguous", "paged"])
+def test_offsets_past_32_bits(reef, layout):
+    """The last tokens of a cache of 2.2 GB of keys and as much of values: attention within a
+    window, and the kept rows."""
+    print(f"\n[case] tree and keep past 2^31 bytes, {layout}", flush=True)
+    rng = np.random.default_rng(18)
+    Hq, H, D, T, window, L = 4, 1, 128, 5, 100, 17_200_000
+    n, tail = L - 3, 192  # the last `tail` places hold something
+    q, k, v, qs, ks, vs = problem(rng, 1, Hq, H, D, T, [tail - 3], tail)
+    m = tree_masks(rng, 1, T, "tree")
+    ref, tol = reference(q, k, v, qs, ks, vs, [tail - 3], m, window, 1 / math.sqrt(D))
+    P = L // PAGE
+    small = contiguous(k, v, ks, vs)
+    if layout == "contiguous":
+        cache = [torch.zeros((1, H, L, D), dtype=torch.int8, device="cuda"),
+                 torch.zeros((1, H, P, D, PAGE), dtype=torch.int8, device="cuda"),
+                 *(torch.full((1, H, L), float("nan"), device="cuda") for _ in range(2))]
+        ends = [t[:, :, -s.shape[2]:] for t, s in zip(cache, small)]
+    else:
+        cache = [torch.zeros((P, H, PAGE, D), dtype=torch.int8, device="cuda"),
+                 torch.zeros((P, H, D, PAGE), dtype=torch.int8, device="cuda"),
+                 *(torch.full((P, H, PAGE), float("nan"), device="cuda") for _ in range(2))]
+        ends = [t[-(tail // PAGE):].view(s.shape) for t, s in zip(cache, small)]
+    for end, s in zip(ends, small):
+        end.copy_(s)
+    lens = gpu(np.array([n], np.int32))
+    args = [lens]
+    if layout == "paged":
+        args = [torch.arange(P, dtype=torch.int32, device="cuda")[None], lens]
+    call = reef.attention_decode_tree if layout == "contiguous" else reef.attention_decode_tree_paged
+    out = call(gpu(q), gpu(qs), *cache, *args, tree_mask=words(m), window=window)
+    assert np.abs(out.cpu().numpy() - ref).max() <= tol
+    kept, some = np.array([[1, 3, 4, 0, 0]], np.int32), gpu(np.array([3], np.int32))
+    if layout == "contiguous":
+        new = reef.kv_keep(gpu(kept), some, lens, *cache)
+    else:
+        new = reef.kv_keep_paged(gpu(kept), some, lens, args[0], *cache)
+    assert int(new) == n - T + 3
+    first = tail - 3 - T
+    for a, s, to in ((k, small[0], ends[0]), (ks, small[2], ends[2]), (vs, small[3], ends[3])):
+        want = a.copy()
+        want[:, :, first:first + 3] = a[:, :, first + kept[0, :3]]
+        assert np.array_equal(want, to.cpu().numpy(), equal_nan=False)
+    want = v.copy()
+    want[:, :, first:first + 3] = v[:, :, first + kept[0, :3]]
+    assert np.array_equal(contiguous(k, want, ks, vs)[1].cpu().numpy(), ends[1].cpu().numpy())
