@@ -497,6 +497,7 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
             for (int kb = first_key(seg); kb < k_end; kb += k_step) {
                 const bool more = kb + k_step < k_end;
                 const bool live = at.live;
+                const float ks_now = ks;
                 const int pg_after = block_pages<PAGED>(a, seg.b, kb + 2 * k_step, seg.sk, lane);
                 // Scores of every tile, times the key's scale.
                 float xs[NC][16];
@@ -534,14 +535,16 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
                 pg_next = pg_after;
                 // Blocks that every row sees whole skip the masks. In the others a hidden key's
                 // score is -inf, and the value scale of a key that no row of the wave sees
-                // is 0 (the cache there may hold anything). A drafted token whose value scale
-                // is not finite makes the rows that see it NaN through their sums, and no
-                // others: its scale is 0 too.
+                // is 0 (the cache there may hold anything). A token whose key or value scale is
+                // not finite makes the rows that see it NaN through their scores (an infinite key
+                // scale alone would be a weight of 0 where the product is negative), and no
+                // others: its value scale is 0 too.
                 const int kk = kb + 16 * grp;
                 float vsc = vs;
                 if (kb < full_lo || kb + kBlockKeys > seg.sk.prefix || !__all(live)) {
                     uint32_t any = 0;
-                    const bool finite = __builtin_fabsf(vsc) < INFINITY;
+                    const bool finite =
+                        __builtin_fabsf(vsc) < INFINITY && __builtin_fabsf(ks_now) < INFINITY;
                     const uint32_t nan = row_or(finite ? 0u : 1u << col);
 #pragma unroll
                     for (int t = 0; t < NC; ++t) {

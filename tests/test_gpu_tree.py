@@ -346,6 +346,33 @@ def test_a_drafted_token_that_is_not_finite(reef, D, Hq, H, T, what):
     assert np.abs(out - ref)[~sees].max() <= tol
 
 
+@pytest.mark.parametrize("D,Hq,H,T", [(64, 2, 2, 7), (128, 8, 1, 20)])
+@pytest.mark.parametrize("value", [np.inf, -np.inf])
+def test_a_drafted_token_with_an_infinite_key_scale(reef, D, Hq, H, T, value):
+    """Its score is an infinity of either sign: the rows that see it are not finite whichever,
+    and the others are right. The token lies in a sequence's last block, or in its only one."""
+    print(f"\n[case] tree with a key scale of {value} {Hq}/{H}x{D} T {T}", flush=True)
+    rng = np.random.default_rng(D + T)
+    B, L = 3, 720
+    lens = [700, T, 64]
+    q, k, v, qs, ks, vs = problem(rng, B, Hq, H, D, T, lens, L)
+    m = tree_masks(rng, B, T, "tree")
+    ref, tol = reference(q, k, v, qs, ks, vs, lens, m, 0, 1 / math.sqrt(D))
+    bad = 1
+    at = [n - T + bad for n in lens]
+    signs = [(q[b, h, t].astype(int) @ k[b, h // (Hq // H), at[b]].astype(int)) * value > 0
+             for b in range(B) for h in range(Hq) for t in range(T) if m[b, t, bad]]
+    assert any(signs) and not all(signs)
+    for b in range(B):
+        ks[b, :, at[b]] = value
+    out = reef.attention_decode_tree(gpu(q), gpu(qs), *contiguous(k, v, ks, vs),
+                                     gpu(np.array(lens, np.int32)), tree_mask=words(m)).cpu().numpy()
+    sees = np.broadcast_to(m[:, None, :, bad], out.shape[:3])
+    assert sees.any() and not sees.all()
+    assert not np.isfinite(out[sees]).any()
+    assert np.abs(out - ref)[~sees].max() <= tol
+
+
 def test_workspace_serves_every_shape(reef):
     """One explicit workspace, sized for the largest, through calls of several shapes."""
     print("\n[case] tree workspace over shapes", flush=True)
