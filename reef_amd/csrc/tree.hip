@@ -200,6 +200,29 @@ __device__ __forceinline__ Column column_of(const TreeArgs &a, int kvh, int inde
     return {live, kvh * a.group + i - token * a.group, token};
 }
 
+// Values accumulate in units of 2^-8 of a power of two, so that the unit's inverse is exact and
+// one subtraction. The least of them: its inverse times a weight's 2^6 is in fp32.
+constexpr float kLeastUnit = 0x1p-112f;
+
+// The power of two at or above x > 0 (2^127 for all above it).
+__device__ __forceinline__ float power_above(float x) {
+    return fminf(__uint_as_float((__float_as_uint(x) + 0x7fffffu) & 0x7f800000u), 0x1p127f);
+}
+__device__ __forceinline__ float inverse_unit(float power) {  // 2^8 / power
+    return __uint_as_float((262u << 23) - __float_as_uint(power));
+}
+
+// Largest |x| of a row's 16 lanes among those that bit r of `bits` names for lane r.
+template <int R = 0>
+__device__ __forceinline__ float row_top(float x, uint32_t bits, float top = 0.0f) {
+    if constexpr (R % 4 == 0) asm("" : "+v"(x), "+v"(top), "+v"(bits));
+    const float v = __int_as_float(
+        __builtin_amdgcn_mov_dpp(__float_as_int(x), 0x150 + R, 0xf, 0xf, true));
+    top = bits >> R & 1u ? fmaxf(top, __builtin_fabsf(v)) : top;
+    if constexpr (R < 15) return row_top<R + 1>(x, bits, top);
+    return top;
+}
+
 // What the column's row sees: the first token before the drafts, and the drafted ones.
 struct Sight {
     int lo;
@@ -251,6 +274,14 @@ struct Segment {
     int first_u;  // the item's first block in the launch's numbering
     int units;    // of the run, the item's extra ones included
 };
+
+// An offset added where it is used: as part of a base address that outlives the key loop it took
+// registers that then spilled, and the reload held up every segment's first block (16 x U[512,
+// 8192] keys, 16 drafted: 57 us against 59).
+__device__ __forceinline__ int held(int offset) {
+    asm volatile("" : "+v"(offset));
+    return offset;
+}
 
 // Waits for this wave's LDS accesses, then for the workgroup; loads in flight stay so
 // (__syncthreads() would wait for them).
@@ -372,7 +403,8 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
     bool bad_page = false;
     int pg_next;
     auto load_k = [&](const TreeArgs &a) {
-        const int8_t *p = a.k + (int64_t)at.k_slot * (kPage * D) + (col & 3) * D + 16 * grp;
+        const int in_page = held((col & 3) * D + 16 * grp);
+        const int8_t *p = a.k + (int64_t)at.k_slot * (kPage * D) + in_page;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -481,12 +513,13 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
             pg_second = block_pages<PAGED>(a, nxt.b, first_key(nxt) + k_step, nxt.sk, lane);
         }
 
-        float m_run[NC], l_run[NC], s_run = 0.0f, inv_s = 0.0f;
+        float m_run[NC], l_run[NC], s_run[NC], s_least = kLeastUnit;
         f32x4 acc[NC][DB];
 #pragma unroll
         for (int t = 0; t < NC; ++t) {
             m_run[t] = -INFINITY;
             l_run[t] = 0.0f;
+            s_run[t] = kLeastUnit;
 #pragma unroll
             for (int d = 0; d < DB; ++d) acc[t][d] = f32x4{};
         }
@@ -530,7 +563,8 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
                                          more ? pg_next : pg_first, col, grp, bad_page);
                 }
                 load_k(a);
-                const int8_t *v_next = a.v + (int64_t)at.g_slot * (kPage * D) + col * kPage;
+                const int8_t *v_next =
+                    a.v + (int64_t)at.g_slot * (kPage * D) + held(col * kPage);
                 __builtin_amdgcn_sched_barrier(0);
                 pg_next = pg_after;
                 // Blocks that every row sees whole skip the masks. In the others a hidden key's
@@ -541,8 +575,12 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
                 // others: its value scale is 0 too.
                 const int kk = kb + 16 * grp;
                 float vsc = vs;
-                if (kb < full_lo || kb + kBlockKeys > seg.sk.prefix || !__all(live)) {
-                    uint32_t any = 0;
+                uint32_t seen = ~0u;  // 16 bits a tile: which of its 16 keys this lane's row sees
+                static_assert(NC <= 2, "tiles in one word");
+                const bool whole =
+                    kb >= full_lo && kb + kBlockKeys <= seg.sk.prefix && __all(live);
+                if (!whole) {
+                    uint32_t any = seen = 0;
                     const bool finite =
                         __builtin_fabsf(vsc) < INFINITY && __builtin_fabsf(ks_now) < INFINITY;
                     const uint32_t nan = row_or(finite ? 0u : 1u << col);
@@ -563,35 +601,42 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
                                 if (vis & nan & 1u << r) xs[t][r] = __builtin_nanf("");
                         }
                         any |= vis;
+                        seen |= vis << (16 * t);
                     }
                     any = row_or(any);
                     if (!finite || !(any >> col & 1u)) vsc = 0.0f;
                 }
-                float mt[NC];
-                bool grow = false;
+                float mt[NC];  // over this lane's keys
+                bool grow = __builtin_fabsf(vsc) > s_least * 2.0f;
 #pragma unroll
                 for (int t = 0; t < NC; ++t) {
                     float m = fmaxf(fmaxf(xs[t][0], xs[t][1]), xs[t][2]);
 #pragma unroll
                     for (int r = 3; r < 15; r += 2) m = fmaxf(fmaxf(m, xs[t][r]), xs[t][r + 1]);
                     m = fmaxf(m, xs[t][15]);
-                    mt[t] = xor32_max(xor16_max(m)) * cs[t];
+                    mt[t] = m * cs[t];
                     grow |= mt[t] > m_run[t] + 6.0f;
                 }
-                const float vmax = xor32_max(xor16_max(row_fmax(vsc)));
                 // Lazy rescale: a row's maximum moves only when it grows by more than 2^6, and
-                // the unit of the accumulator (s_run / 2^8, s_run the largest value scale so
-                // far) only when a value scale passes it 2-fold, so a weight
-                // p * v_scale * 2^8 / s_run stays below 2^15 in fp16, and above its subnormals
-                // (hi and lo keep 11 bits each) where its share of the row counts.
-                if (__any(grow || vmax > s_run * 2.0f)) {
-                    const float s_new = fmaxf(s_run, vmax);
-                    const float units = s_new > 0.0f ? s_run / s_new : 1.0f;
-                    inv_s = s_new > 0.0f ? 256.0f / s_new : 0.0f;
-                    s_run = s_new;
+                // the unit of its accumulator (s_run / 2^8, s_run a power of two at or above the
+                // largest value scale that the row has seen) only when a value scale passes s_run
+                // 2-fold, so a weight p * v_scale * 2^8 / s_run stays below 2^15 in fp16, and is
+                // off by at most half a subnormal step, 2^-33 of s_run (hi and lo keep 11 bits
+                // each). Each row by what it sees itself: a drafted token of large values does not
+                // push the weights of the rows that do not see it into the subnormals. Whether any
+                // row may have to move is asked of each lane's keys and of s_least, the least
+                // s_run; the rows' own maxima are taken only then.
+                if (__any(grow)) {
+                    float least = INFINITY;
 #pragma unroll
                     for (int t = 0; t < NC; ++t) {
-                        const float m_new = fmaxf(m_run[t], mt[t]);
+                        const float ct = whole ? row_fmax(__builtin_fabsf(vsc))
+                                               : row_top(vsc, seen >> (16 * t));
+                        const float s_new = power_above(fmaxf(s_run[t], xor32_max(xor16_max(ct))));
+                        const float units = s_run[t] / s_new;
+                        s_run[t] = s_new;
+                        least = fminf(least, s_new);
+                        const float m_new = fmaxf(m_run[t], xor32_max(xor16_max(mt[t])));
                         const float alpha =
                             m_run[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[t] - m_new);
                         m_run[t] = m_new;
@@ -600,15 +645,18 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
 #pragma unroll
                         for (int d = 0; d < DB; ++d) acc[t][d] *= alpha_o;
                     }
+                    s_least = __int_as_float(
+                        __builtin_amdgcn_readfirstlane(__float_as_int(-row_fmax(-least))));
                 }
                 // P operands: lane group g's keys 16 g + 8 h + e for the two halves h.
                 f16x8 hi[NC][2], lo[NC][2];
                 {
                     float vv[16];
-                    row_lanes(vsc * inv_s, vv);
+                    row_lanes(vsc, vv);
 #pragma unroll
                     for (int t = 0; t < NC; ++t) {
                         const float m_use = m_run[t] == -INFINITY ? 0.0f : m_run[t];
+                        const float inv_s = inverse_unit(s_run[t]);
                         float sum[2] = {0.0f, 0.0f};
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
@@ -618,7 +666,8 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
                                 const float p = __builtin_amdgcn_exp2f(
                                     __builtin_fmaf(xs[t][8 * h + e], cs[t], -m_use));
                                 sum[e & 1] += p;
-                                w[e] = p * vv[8 * h + e];
+                                // (p first: what the row does not see has p = 0)
+                                w[e] = p * inv_s * vv[8 * h + e];
                             }
                             split_weights(w, hi[t][h], lo[t][h]);
                         }
@@ -692,7 +741,8 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
                 m_run[t] = -INFINITY;
             }
 #pragma unroll
-            for (int d = 0; d < DB; ++d) sO[wave][d][lane] = acc[t][d] * (s_run * (1.0f / 256.0f));
+            for (int d = 0; d < DB; ++d)
+                sO[wave][d][lane] = acc[t][d] * (s_run[t] * (1.0f / 256.0f));
             sML[wave][lane] = float2{m_run[t], l};
             lds_barrier();
             float2 ml[kWaves];

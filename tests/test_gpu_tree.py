@@ -373,6 +373,77 @@ def test_a_drafted_token_with_an_infinite_key_scale(reef, D, Hq, H, T, value):
     assert np.abs(out - ref)[~sees].max() <= tol
 
 
+def reference_by_row(q, k, v, qs, ks, vs, lens, m, window, scale):
+    """(out, tolerance [B, Hq, T, 1]): the tolerance of the file's head from what each row sees
+    alone, its exponents and 127 times its largest value scale. (A weight is off by 2^-33 of a
+    power of two that is less than twice that scale; the row sum does not share this.)"""
+    out, _ = reference(q, k, v, qs, ks, vs, lens, m, window, scale)
+    B, Hq, T, D = q.shape
+    tol = np.zeros((B, Hq, T, 1))
+    for b in range(B):
+        n = int(lens[b])
+        depth = m[b].sum(1) - 1
+        pos = np.concatenate([np.arange(n - T), n - T + depth])
+        seen = np.concatenate([np.ones((T, n - T), bool), m[b]], 1)
+        if window:
+            seen &= pos[None, :] > (n - T + depth)[:, None] - window
+        seen[m[b].sum(1) == 0] = False
+        for h in range(Hq):
+            kk = k[b, h * k.shape[1] // Hq, :n] * ks[b, h * k.shape[1] // Hq, :n, None].astype(np.float64)
+            s = np.abs((q[b, h] * qs[b, h][:, None].astype(np.float64)) @ kk.T) * scale / math.log(2)
+            for t in np.flatnonzero(seen.any(1)):
+                X = s[t, seen[t]].max()
+                most = 127.0 * vs[b, h * k.shape[1] // Hq, :n][seen[t]].max()
+                tol[b, h, t] = most * (2 * (2.8 * X * U + 6 * U + n * 2.0 ** -33) + 14 * U)
+    return out, tol
+
+
+@pytest.mark.parametrize("D,Hq,H,T", [(64, 2, 2, 7), (128, 8, 1, 20), (128, 3, 3, 64)])
+@pytest.mark.parametrize("large", [1e4, 1e8, 1e30, 1e36])
+def test_large_values_of_a_hidden_token(reef, D, Hq, H, T, large):
+    """A token whose values are finite and far above all others' changes nothing for the rows that
+    do not see it: a drafted one in a sequence's last block or its only one, and one that
+    only the shallow rows' windows reach."""
+    print(f"\n[case] tree with value scales of {large} {Hq}/{H}x{D} T {T}", flush=True)
+    rng = np.random.default_rng(D + T + 1)
+    B, L = 3, 720
+    lens = [700, 64, max(T, 33)]
+    q, k, v, qs, ks, vs = problem(rng, B, Hq, H, D, T, lens, L)
+    m = tree_masks(rng, B, T, "tree")
+    for window in (0, 25):
+        scales = vs.copy()
+        for b in range(B):
+            scales[b, :, lens[b] - T + 1] = large
+            if window and lens[b] - T >= window:
+                scales[b, :, lens[b] - T + 1 - window] = large
+        ref, tol = reference_by_row(q, k, v, qs, ks, scales, lens, m, window, 1 / math.sqrt(D))
+        sees = tol[..., 0] > large * 1e-7
+        assert sees.any() and (tol[~sees] < 1e-3).all() and not sees.all()
+        cache, ln = contiguous(k, v, ks, scales), gpu(np.array(lens, np.int32))
+        out = reef.attention_decode_tree(gpu(q), gpu(qs), *cache, ln, tree_mask=words(m), window=window)
+        assert (np.abs(out.cpu().numpy() - ref) <= tol).all()
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-36])
+def test_small_values(reef, size):
+    """Value scales whose inverse times 2^8 is beyond fp32; beside them drafted tokens of
+    ordinary ones, which some rows see."""
+    print(f"\n[case] tree with value scales of {size}", flush=True)
+    rng = np.random.default_rng(31)
+    B, Hq, H, D, T, lens = 2, 4, 1, 64, 12, [300, 30]
+    q, k, v, qs, ks, vs = problem(rng, B, Hq, H, D, T, lens, 304)
+    m = tree_masks(rng, B, T, "tree")
+    vs = (rng.uniform(0.5, 1.0, vs.shape) * size).astype(np.float32)
+    for mixed in (False, True):
+        if mixed:
+            for b in range(B):
+                vs[b, :, lens[b] - T + 1] = 0.01
+        ref, tol = reference_by_row(q, k, v, qs, ks, vs, lens, m, 0, 1 / math.sqrt(D))
+        out = reef.attention_decode_tree(gpu(q), gpu(qs), *contiguous(k, v, ks, vs),
+                                         gpu(np.array(lens, np.int32)), tree_mask=words(m))
+        assert (np.abs(out.cpu().numpy().astype(np.float64) - ref) <= tol).all()
+
+
 def test_workspace_serves_every_shape(reef):
     """One explicit workspace, sized for the largest, through calls of several shapes."""
     print("\n[case] tree workspace over shapes", flush=True)
