@@ -422,9 +422,10 @@ reef_status reef_attention_decode_int8_paged_noalloc(
  * are not looked up.
  * A sequence whose length is outside [T, max_context] sets BAD_LENGTH and yields zeros; a
  * page number outside [0, P) sets BAD_PAGE and its tokens take no part. A drafted token
- * whose scales are not finite leaves the rows that see it not finite, and no others. A row's
- * error is relative to the largest value scale among the tokens that it sees itself: finite
- * ones of any size elsewhere do not change it.
+ * whose scales are not finite leaves the rows that see it not finite, and no others. Scales
+ * are positive, as the quantizers make them; with a query scale of 0 all that the row sees
+ * has the same weight. A row's error is relative to the largest value scale among the tokens
+ * that it sees itself: finite ones of any size elsewhere do not change it.
  *
  * Workspace as for decode: reef_attention_decode_tree_workspace_bytes(p) bytes (0: invalid
  * or unsupported sizes), 16-byte aligned, zero-filled before its first use; every call

@@ -454,10 +454,13 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
         for (int t = 0; t < NC; ++t) {
             const Column cn = column(a, s, t);
             const uint64_t m = cn.live ? seen_drafts(a, cn.token, r.m[t]) : 0;
+            // (a factor of 0 would make a hidden key's -inf a NaN: scores of 0 times 1 instead)
+            const float c = r.c[t] * a.score_scale;
+            const bool scaled = cn.live && c != 0.0f;
 #pragma unroll
             for (int e = 0; e < KS; ++e)
-                sQ[wave][t * KS + e][lane] = cn.live ? r.q[t][e] : i32x4{0, 0, 0, 0};
-            cs[t] = cn.live ? r.c[t] * a.score_scale : 1.0f;
+                sQ[wave][t * KS + e][lane] = scaled ? r.q[t][e] : i32x4{0, 0, 0, 0};
+            cs[t] = scaled ? c : 1.0f;
             shown |= (m != 0 ? 1u : 0u) << t;
             const Sight sight = sight_of(a, s.b, s.sk, m);
             if (grp == 0) sSight[wave][t][col] = sight;

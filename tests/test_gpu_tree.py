@@ -444,6 +444,25 @@ def test_small_values(reef, size):
         assert (np.abs(out.cpu().numpy().astype(np.float64) - ref) <= tol).all()
 
 
+@pytest.mark.parametrize("D,Hq,H,T,window", [(64, 2, 2, 7, 0), (128, 8, 1, 20, 0), (64, 4, 2, 6, 30)])
+def test_query_scales_of_zero(reef, D, Hq, H, T, window):
+    """Rows whose scale is 0 (so are their scores): the mean of the values that they see. A row
+    whose mask is 0 too stays zeros."""
+    print(f"\n[case] tree with query scales of 0 {Hq}/{H}x{D} T {T}", flush=True)
+    rng = np.random.default_rng(D + T + 2)
+    lens = [300, T, 64]
+    q, k, v, qs, ks, vs = problem(rng, 3, Hq, H, D, T, lens, 304)
+    qs[:, :, ::2] = 0
+    m = tree_masks(rng, 3, T, "tree")
+    m[1, T - 1] = False
+    ref, tol = reference(q, k, v, qs, ks, vs, lens, m, window, 1 / math.sqrt(D))
+    cache = contiguous(*poison(k, v, ks, vs, lens))
+    out = reef.attention_decode_tree(gpu(q), gpu(qs), *cache, gpu(np.array(lens, np.int32)),
+                                     tree_mask=words(m), window=window).cpu().numpy()
+    assert np.abs(out - ref).max() <= tol
+    assert not out[1, :, T - 1].any()
+
+
 def test_workspace_serves_every_shape(reef):
     """One explicit workspace, sized for the largest, through calls of several shapes."""
     print("\n[case] tree workspace over shapes", flush=True)
