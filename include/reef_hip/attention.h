@@ -543,8 +543,9 @@ reef_status reef_kv_fork(const int32_t *parents, const int32_t *children, int64_
  * that page holds tokens already (the last, partial one), copy_src[b] and copy_dst[b] (both
  * [batch]) name the two. A sequence that would pass max_blocks_per_seq * 16 tokens keeps its
  * blocks and sets CAPACITY, as do the blocks for which no free page is left (the others are
- * served; with their copies made, the call may be repeated once there are). Lengths are not
- * changed. The workspace needs reef_kv_reserve_workspace_bytes bytes, of any contents. */
+ * served; with their copies made, the call may be repeated once there are), unless the others
+ * left such a block its page alone. Every sharer of a page gets one; the page that none keeps
+ * becomes free. Lengths are not changed. The workspace needs reef_kv_reserve_workspace_bytes bytes, of any contents. */
 size_t reef_kv_reserve_workspace_bytes(int64_t batch, int64_t new_tokens);
 
 reef_status reef_kv_reserve(int32_t *block_table, int64_t max_blocks_per_seq,

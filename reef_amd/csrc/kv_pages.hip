@@ -132,6 +132,8 @@ struct Need {
     uint32_t flags;
 };
 
+// AGAIN: the counts as this launch's own drops left them.
+template <bool AGAIN = false>
 __device__ __forceinline__ Need need_of(const ReserveArgs &a, int64_t item) {
     Need n = {false, false, -1, 0, 0};
     const int b = (int)(item / a.nb), i = (int)(item % a.nb);
@@ -150,7 +152,8 @@ __device__ __forceinline__ Need need_of(const ReserveArgs &a, int64_t item) {
         if (holds) n.flags = REEF_STATUS_BIT_BAD_PAGE;  // tokens without a page
     } else if (page >= a.t.num_pages) {
         n.flags = REEF_STATUS_BIT_BAD_PAGE;
-    } else if (a.t.refs[page] > 1) {
+    } else if ((AGAIN ? __hip_atomic_load(a.t.refs + page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+                      : a.t.refs[page]) > 1) {
         n.due = true;
         n.old = page;
         n.copy = holds;
@@ -211,10 +214,7 @@ __global__ __launch_bounds__(kScanThreads) void reserve_pages(ReserveArgs a) {
         const int rank = given + block_scan(n.due, all, sWave);
         given += all;
         if (!n.due) continue;
-        if (rank >= found) {  // no page left: the block stays as it is
-            flag_status(a.t.status, REEF_STATUS_BIT_CAPACITY);
-            continue;
-        }
+        if (rank >= found) continue;  // no page left: the block stays as it is
         const int page = a.free_pages[rank];
         a.t.table[n.entry] = page;
         a.t.refs[page] = 1;
@@ -228,6 +228,13 @@ __global__ __launch_bounds__(kScanThreads) void reserve_pages(ReserveArgs a) {
     __syncthreads();
     for (int r = tid; r < found; r += kScanThreads)
         if (a.old_pages[r] >= 0) drop_ref(a.t.refs, a.old_pages[r]);
+    if (found == wanted) return;
+    // Pages ran out. A block that got none may still have what it needs: the last sharer of a page
+    // that the others have left.
+    __syncthreads();
+    bool lacking = false;
+    for (int64_t i = tid; i < a.items; i += kScanThreads) lacking |= need_of<true>(a, i).due;
+    if (lacking) flag_status(a.t.status, REEF_STATUS_BIT_CAPACITY);
 }
 
 // ---- compact ---------------------------------------------------------------------------

@@ -220,6 +220,47 @@ def test_copy_on_write_keeps_the_parent(reef):
     assert one is not None
 
 
+@pytest.mark.parametrize("sharers,free,short", [(2, 1, False), (2, 0, True), (5, 4, False), (5, 3, True),
+                                                (2, 2, False), (1300, 1299, False), (1300, 1298, True)])
+def test_the_last_sharer_needs_no_page(reef, sharers, free, short):
+    """With one free page fewer than sharers of a page, the last of them is left with it alone:
+    every block has a page of its own, nothing is missing. With fewer still, some lack one."""
+    print(f"\n[case] reserve {sharers} sharers {free} free pages", flush=True)
+    m = Model(sharers, 2, 1 + free)
+    m.table[:, 0], m.lens[:], m.refs[0] = 0, 5, sharers
+    table, lens, refs = m.device()
+    src, dst, _ = m.reserve(1)
+    status = reef.StatusWord()
+    s, d = reef.kv_reserve(table, lens, refs, 1, status=status)
+    assert np.array_equal(host(s), src) and np.array_equal(host(d), dst)
+    m.check(table, lens, refs)
+    if short:
+        with pytest.raises(reef.CapacityError):
+            status.check("reserve")
+        assert m.refs.max() > 1
+    else:
+        status.check("reserve")
+        assert (m.refs[m.table[:, 0]] == 1).all()
+        if free < sharers:  # again: there is nothing left to do
+            reef.kv_reserve(table, lens, refs, 1)
+            m.check(table, lens, refs)
+
+
+def test_no_page_for_an_absent_block(reef):
+    """Beside a last sharer that needs none, a sequence without a page lacks one."""
+    print("\n[case] reserve a last sharer and an absent block", flush=True)
+    m = Model(3, 2, 2)
+    m.table[:2, 0], m.lens[:2], m.refs[0] = 0, 5, 2
+    table, lens, refs = m.device()
+    m.reserve(1)
+    status = reef.StatusWord()
+    reef.kv_reserve(table, lens, refs, 1, status=status)
+    m.check(table, lens, refs)
+    assert m.table[2, 0] == -1
+    with pytest.raises(reef.CapacityError):
+        status.check("reserve")
+
+
 @pytest.mark.parametrize("paged", [False, True])
 @pytest.mark.parametrize("B,H,D,T", [(1, 1, 64, 1), (5, 3, 128, 7), (9, 2, 64, 64), (3, 8, 128, 33),
                                      (66, 1, 128, 16)])
