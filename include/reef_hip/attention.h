@@ -579,9 +579,9 @@ reef_status reef_kv_copy_pages(const int32_t *src, const int32_t *dst, int64_t n
  * ones stay: rows kept[b][0 .. kept_lens[b] - 1] of them, ascending, move to the first
  * kept_lens[b] of their places, keys, values and scales. kept: [batch, new_tokens] int32
  * (entries past kept_lens[b] are not read); context_lens: [batch] int32, the drafted tokens
- * counted in; new_lens (optional, apart from context_lens: REEF_INVALID_ARGUMENT where they
- * overlap) receives context_lens[b] - new_tokens + kept_lens[b]. new_tokens <= 64. The rows
- * behind the kept ones are left as they were. A length outside [new_tokens, max_context], a
+ * counted in; new_lens (optional, apart from context_lens, kept and kept_lens:
+ * REEF_INVALID_ARGUMENT where it overlaps one) receives context_lens[b] - new_tokens +
+ * kept_lens[b]. new_tokens <= 64. The rows behind the kept ones are left as they were. A length outside [new_tokens, max_context], a
  * kept_lens outside [0, new_tokens], or rows that are not ascending in [0, new_tokens) set
  * BAD_LENGTH, a page number outside [0, num_pages) BAD_PAGE; that sequence stays as it is
  * and new_lens[b] is its length. In the paged cache the drafted tokens' pages must be the

@@ -531,9 +531,13 @@ reef_status keep(const reef_kv_append_params *p, const int32_t *kept, const int3
     if (p->new_tokens > kMaxDrafts || (p->head_dim != 64 && p->head_dim != 128) ||
         p->max_context >= (int64_t(1) << 30) || p->batch > 65535 || p->kv_heads > 65535)
         return REEF_UNSUPPORTED;
-    // every workgroup of a sequence reads its length
-    const uintptr_t l0 = reinterpret_cast<uintptr_t>(lens), n0 = reinterpret_cast<uintptr_t>(new_lens);
-    if (new_lens && l0 < n0 + 4 * (uintptr_t)p->batch && n0 < l0 + 4 * (uintptr_t)p->batch)
+    // every workgroup of a sequence reads its length, its kept rows and their number
+    auto overlaps = [&](const int32_t *x, int64_t n) {
+        const uintptr_t x0 = reinterpret_cast<uintptr_t>(x), n0 = reinterpret_cast<uintptr_t>(new_lens);
+        return new_lens && x0 < n0 + 4 * (uintptr_t)p->batch && n0 < x0 + 4 * (uintptr_t)n;
+    };
+    if (overlaps(lens, p->batch) || overlaps(kept_lens, p->batch) ||
+        overlaps(kept, p->batch * p->new_tokens))
         return REEF_INVALID_ARGUMENT;
     KeepArgs a = {kept, kept_lens, lens, new_lens, k, v, ks, vs, table, (int32_t)p->kv_heads,
                   (int32_t)p->new_tokens, (int32_t)p->max_context, (int32_t)max_blocks,

@@ -197,6 +197,23 @@ def test_copy_and_keep():
     assert keep_paged(p, pages=0) == INVALID and keep_paged(p, blocks=1 << 26) == INVALID
 
 
+@pytest.mark.parametrize("paged", [False, True])
+def test_keep_writes_no_lengths_over_what_it_reads(paged):
+    """The workgroups of a sequence's other kv heads read its kept rows and their number, too."""
+    lib, p = reef_amd.lib(), KvAppendParams(batch=3, kv_heads=2, head_dim=64, new_tokens=5, max_context=64)
+
+    def keep(new_lens):
+        if paged:
+            return lib.reef_kv_keep_int8_paged(p, at(1), at(2), at(3), at(8), 4, 9, at(4), at(5), at(6),
+                                               at(7), new_lens, None, None)
+        return lib.reef_kv_keep_int8(p, at(1), at(2), at(3), at(4), at(5), at(6), at(7), new_lens, None,
+                                     None)
+
+    for n, rows in ((1, 15), (2, 3), (3, 3)):  # kept [3, 5], kept_lens [3], context_lens [3]
+        for offset in (-8, 0, 4 * (rows - 1)):
+            assert keep(at(n, offset)) == INVALID, (n, offset)
+
+
 # --- norm, product ----------------------------------------------------------------------------
 
 def test_norm():
