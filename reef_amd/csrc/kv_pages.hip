@@ -378,6 +378,7 @@ __global__ __launch_bounds__(256) void apply_moves(CompactArgs a) {
 
 struct CopyArgs {
     const int32_t *src, *dst;
+    int64_t pairs;
     int8_t *pages[2];
     float *scales[2];
     int32_t page_words, scale_words;  // 16-byte words of a page and of its scales
@@ -389,7 +390,9 @@ constexpr int kCopyThreads = 256;
 
 // One workgroup per pair and pool (keys, values).
 __global__ __launch_bounds__(kCopyThreads) void copy_pages(CopyArgs a) {
-    const int s = a.src[blockIdx.x], d = a.dst[blockIdx.x];
+    const int64_t pair = linear_block();
+    if (pair >= a.pairs) return;
+    const int s = a.src[pair], d = a.dst[pair];
     if (s < 0 || d < 0 || s == d) return;
     const int tid = threadIdx.x;
     if (s >= a.num_pages || d >= a.num_pages) {
@@ -669,6 +672,7 @@ extern "C" reef_status reef_kv_copy_pages(const int32_t *src, const int32_t *dst
     CopyArgs a;
     a.src = src;
     a.dst = dst;
+    a.pairs = n;
     a.pages[0] = k_pages;
     a.pages[1] = v_pages;
     a.scales[0] = k_scale_pages;
@@ -677,7 +681,7 @@ extern "C" reef_status reef_kv_copy_pages(const int32_t *src, const int32_t *dst
     a.scale_words = (int32_t)(kv_heads * 4);        // 16 floats a head
     a.num_pages = (int32_t)num_pages;
     a.status = status_word;
-    hipLaunchKernelGGL(copy_pages, dim3((unsigned)n, 2), dim3(kCopyThreads), 0, stream, a);
+    hipLaunchKernelGGL(copy_pages, linear_grid(n, 2), dim3(kCopyThreads), 0, stream, a);
     return launch_status();
 }
 

@@ -130,9 +130,9 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void norm_rows(NormArgs a
     __shared__ uint32_t sBad[WPR];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t row = (int64_t)blockIdx.x * ROWS + wave / WPR;
+    const int64_t row = linear_block() * ROWS + wave / WPR;
     const int part = wave % WPR;
-    if (row >= a.rows) return;  // (only with one wave a row, which meets no barrier)
+    if (row >= a.rows) return;  // (all of a workgroup's waves, or waves that meet no barrier)
     const float *x = a.x + row * a.x_stride;
     f32x4 h[F4], w[F4];
     int col[F4];
@@ -197,7 +197,8 @@ __global__ __launch_bounds__(1024) void norm_long_rows(NormArgs a) {
     __shared__ double sSquares[W], sTop[W];
     __shared__ uint32_t sBad[W];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t row = blockIdx.x;
+    const int64_t row = linear_block();
+    if (row >= a.rows) return;
     const float *x = a.x + row * a.x_stride;
     const float *r = a.residual ? a.residual + row * a.r_stride : nullptr;
     float *o = a.sum ? a.sum + row * a.s_stride : nullptr;
@@ -243,7 +244,7 @@ __global__ __launch_bounds__(1024) void norm_long_rows(NormArgs a) {
 
 template <int WPR, int F4>
 void launch_rows(const NormArgs &a, bool nt, hipStream_t stream) {
-    const dim3 grid((unsigned)(WPR >= 4 ? a.rows : ceil_div(a.rows, 4 / WPR)));
+    const dim3 grid = linear_grid(WPR >= 4 ? a.rows : ceil_div(a.rows, 4 / WPR));
     const dim3 block(WPR > 4 ? 64 * WPR : 256);
     if (nt) hipLaunchKernelGGL((norm_rows<WPR, F4, true>), grid, block, 0, stream, a);
     else hipLaunchKernelGGL((norm_rows<WPR, F4, false>), grid, block, 0, stream, a);
@@ -297,6 +298,6 @@ extern "C" reef_status reef_rmsnorm_quantize_int8(const float *x, int64_t rows, 
     else if (width <= 4096) launch_rows<4, 4>(a, nt, stream);
     else if (width <= 8192) launch_rows<4, 8>(a, nt, stream);
     else if (width <= 16384) launch_rows<8, 8>(a, nt, stream);
-    else hipLaunchKernelGGL(norm_long_rows, dim3((unsigned)rows), dim3(1024), 0, stream, a);
+    else hipLaunchKernelGGL(norm_long_rows, linear_grid(rows), dim3(1024), 0, stream, a);
     return launch_status();
 }

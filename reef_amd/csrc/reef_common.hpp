@@ -184,4 +184,17 @@ inline reef_status launch_status() {
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// A launch of 2^32 threads or more along one dimension starts only their number modulo 2^32,
+// without an error. So n workgroups (of at most 1024 threads) that may be 2^22 or more lie in
+// rows of kGridRow: workgroup linear_block() of them, those from n on have nothing to do.
+constexpr int64_t kGridRow = int64_t(1) << 21;
+
+inline dim3 linear_grid(int64_t n, unsigned y = 1) {
+    return n <= kGridRow ? dim3((unsigned)n, y)
+                         : dim3((unsigned)kGridRow, y, (unsigned)ceil_div(n, kGridRow));
+}
+__device__ __forceinline__ int64_t linear_block() {
+    return (int64_t)blockIdx.z * kGridRow + blockIdx.x;
+}
+
 }  // namespace reef

@@ -188,6 +188,25 @@ def test_copy_pages(reef, heads, D):
     reef.kv_copy_pages(gpu(src[:0]), gpu(dst[:0]), *t)  # nothing
 
 
+def test_copy_of_very_long_lists(reef):
+    """As many workgroups as have 2^32 threads, and some: the pairs at the end are copied too."""
+    print("\n[case] copy pages, 2^24 + 3 pairs", flush=True)
+    rng = np.random.default_rng(24)
+    n = (1 << 24) + 3
+    pools = pool(rng, (8, 1), 64)
+    src = torch.full((n,), -1, dtype=torch.int32, device="cuda")
+    dst = src.clone()
+    for i, (s, d) in enumerate(((0, 1), (2, 3), (4, 5), (6, 7))):
+        at = (0, 1 << 21, (1 << 24) - 1, n - 1)[i]
+        src[at], dst[at] = s, d
+    t = [gpu(x) for x in pools]
+    reef.kv_copy_pages(src, dst, *t)
+    for got, was in zip(t, pools):
+        want = was.copy()
+        want[1::2] = was[::2]
+        assert np.array_equal(host(got), want)
+
+
 def test_copy_on_write_keeps_the_parent(reef):
     """A fork's next token lands in a copy: the parent's bytes stay, also on two layers."""
     print("\n[case] copy on write", flush=True)

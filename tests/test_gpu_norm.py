@@ -174,3 +174,16 @@ def test_norm_feeds_the_product(reef):
     acc = q.double() @ w.double().t()
     ref = acc.float() * (s[:, None] * ws[None, :])
     assert torch.equal(y, ref)
+
+
+def test_more_rows_than_a_launch_has_threads(reef):
+    """Rows past 2^32 / 64 and past the first row of workgroups: each is done."""
+    rows = (1 << 26) + 5
+    print(f"\n[case] norm of {rows} rows of 1", flush=True)
+    x = torch.full((rows, 1), 3.0, device="cuda")
+    x[::2] = -0.5
+    q, s = reef.rmsnorm_quantize(x, eps=0.0)
+    sign = torch.sign(x)
+    assert torch.equal(q, (127 * sign).to(torch.int8))
+    one = float(np.float32(1 / 127))
+    assert bool((s == one).all())
