@@ -619,7 +619,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64, PAGED ? kWgPerCu : 1) void decod
 __global__ void pack_v_pages(const int8_t *__restrict__ v_tokens, int64_t pages, int32_t dim,
                              int8_t *__restrict__ v_pages) {
     // One thread per (page, channel): gathers 16 bytes with stride dim.
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const int64_t i = linear_block() * blockDim.x + threadIdx.x;
     if (i >= pages * dim) return;
     const int64_t page = i / dim;
     const int d = (int)(i % dim);
@@ -860,7 +860,7 @@ extern "C" reef_status reef_kv_pack_v_pages(const int8_t *v_tokens, int64_t page
         !aligned(v_pages, 16))
         return REEF_INVALID_ARGUMENT;
     const int64_t n = pages * head_dim;
-    hipLaunchKernelGGL(pack_v_pages, dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, stream,
+    hipLaunchKernelGGL(pack_v_pages, linear_grid(ceil_div(n, 256)), dim3(256), 0, stream,
                        v_tokens, pages, (int32_t)head_dim, v_pages);
     return launch_status();
 }

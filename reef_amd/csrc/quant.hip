@@ -487,7 +487,7 @@ __global__ __launch_bounds__(kQuantThreads) void token_quantize_regs(
     constexpr int RPW = kWave / LPR;  // rows per wave and group
     constexpr int G = row_groups(PER, NT);
     const int lane = threadIdx.x % kWave, sub = lane / LPR, l = lane % LPR;
-    const int64_t wave_id = (int64_t)blockIdx.x * (kQuantThreads / kWave) + threadIdx.x / kWave;
+    const int64_t wave_id = linear_block() * (kQuantThreads / kWave) + threadIdx.x / kWave;
     float4 v[G][PER];
 #pragma unroll
     for (int g = 0; g < G; ++g) {
@@ -554,10 +554,11 @@ __global__ __launch_bounds__(kQuantThreads) void token_quantize_regs(
 // thread held in registers, the largest magnitude reduced across the block.
 template <int PER, bool NT>
 __global__ __launch_bounds__(kQuantThreads) void token_quantize_wide(
-    const float *__restrict__ x, int32_t w4, int64_t row_stride, int8_t *__restrict__ q,
-    float *__restrict__ scales, uint32_t *status) {
+    const float *__restrict__ x, int64_t rows, int32_t w4, int64_t row_stride,
+    int8_t *__restrict__ q, float *__restrict__ scales, uint32_t *status) {
     __shared__ uint32_t partial[kQuantThreads / kWave];
-    const int64_t row = blockIdx.x;
+    const int64_t row = linear_block();
+    if (row >= rows) return;
     const float4 *r = reinterpret_cast<const float4 *>(x + row * row_stride);
     float4 v[PER];
     uint32_t m = 0;
@@ -608,7 +609,7 @@ __global__ __launch_bounds__(kQuantThreads) void token_quantize(const float *__r
                                                                 float *__restrict__ scales,
                                                                 uint32_t *status) {
     const int lane = threadIdx.x % kWave;
-    const int64_t row = (int64_t)blockIdx.x * (kQuantThreads / kWave) + threadIdx.x / kWave;
+    const int64_t row = linear_block() * (kQuantThreads / kWave) + threadIdx.x / kWave;
     if (row >= rows) return;
     const float *r = x + row * row_stride;
     int8_t *out = q + row * width;
@@ -722,7 +723,7 @@ void launch_rows(const float *x, int64_t rows, int64_t w4, int64_t row_stride, c
         const int per = w4 <= kWave ? 1 : w4 <= 2 * kWave ? 2 : 4;  // float4 per lane
         const int64_t rows_per_block =
             (int64_t)(kWave / lpr) * row_groups(per, NT) * (kQuantThreads / kWave);
-        const dim3 grid((unsigned)ceil_div(rows, rows_per_block));
+        const dim3 grid = linear_grid(ceil_div(rows, rows_per_block));
 #define REEF_TOKEN_LAUNCH(L, P)                                                               \
     hipLaunchKernelGGL((token_quantize_regs<L, P, NT, kHeads>), grid, dim3(kQuantThreads), 0, \
                        stream, x, rows, (int32_t)w4, row_stride, hr, q, scales, status_word)
@@ -740,16 +741,16 @@ void launch_rows(const float *x, int64_t rows, int64_t w4, int64_t row_stride, c
         }
 #undef REEF_TOKEN_LAUNCH
     } else {
-        const dim3 grid((unsigned)rows);
+        const dim3 grid = linear_grid(rows);
         if (w4 <= 2 * kQuantThreads)
             hipLaunchKernelGGL((token_quantize_wide<2, NT>), grid, dim3(kQuantThreads), 0,
-                               stream, x, (int32_t)w4, row_stride, q, scales, status_word);
+                               stream, x, rows, (int32_t)w4, row_stride, q, scales, status_word);
         else if (w4 <= 4 * kQuantThreads)
             hipLaunchKernelGGL((token_quantize_wide<4, NT>), grid, dim3(kQuantThreads), 0,
-                               stream, x, (int32_t)w4, row_stride, q, scales, status_word);
+                               stream, x, rows, (int32_t)w4, row_stride, q, scales, status_word);
         else
             hipLaunchKernelGGL((token_quantize_wide<8, NT>), grid, dim3(kQuantThreads), 0,
-                               stream, x, (int32_t)w4, row_stride, q, scales, status_word);
+                               stream, x, rows, (int32_t)w4, row_stride, q, scales, status_word);
     }
 }
 
@@ -902,7 +903,7 @@ extern "C" reef_status reef_quantize_int8_per_token(const float *x, int64_t rows
             launch_rows<false, false>(x, rows, w4, row_stride, HeadRows{}, q, scales, status_word,
                                       stream);
     } else {
-        const dim3 grid((unsigned)ceil_div(rows, kQuantThreads / kWave));
+        const dim3 grid = linear_grid(ceil_div(rows, kQuantThreads / kWave));
         hipLaunchKernelGGL(token_quantize, grid, dim3(kQuantThreads), 0, stream, x, rows, width,
                            row_stride, q, scales, status_word);
     }

@@ -228,6 +228,16 @@ def test_quantize_rows_bit_exact(reef, rows, width):
     assert np.array_equal(host(q), qo)
 
 
+def test_quantize_rows_past_a_launch_of_2_32_threads(reef):
+    rows = (1 << 26) + 5
+    case(f"quantize_rows {rows}x1")
+    x = torch.full((rows, 1), 3.0, device="cuda")
+    x[::2] = -0.5
+    q, s = reef.quantize_rows(x)
+    assert torch.equal(q, (127 * torch.sign(x)).to(torch.int8))
+    assert torch.equal(s, (x.abs() / torch.tensor(127.0, device="cuda")).view(-1))
+
+
 def test_quantize_rows_with_row_stride(reef):
     case("quantize_rows over a strided [rows, 128] view")
     x = W.lcg_normal(25, 64 * 256).reshape(64, 256)
