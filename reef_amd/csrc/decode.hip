@@ -237,10 +237,10 @@ __device__ __forceinline__ void block_math(const DecodeBlock<D> &cur, int kb, in
     // its share of the row sum (of p itself) exceeds 2^-21.
     if (__any(mt > st.m_run + 6.0f || vmax > st.s_run * 2.0f)) {
         const float m_new = fmaxf(st.m_run, mt);
-        const float s_new = fmaxf(st.s_run, vmax);
+        const float s_new = fmaxf(fmaxf(st.s_run, vmax), kLeastScale);
         const float alpha = st.m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.m_run - m_new);
-        const float alpha_o = s_new > 0.0f ? alpha * (st.s_run / s_new) : alpha;
-        st.inv_s = s_new > 0.0f ? 256.0f / s_new : 0.0f;
+        const float alpha_o = alpha * (st.s_run / s_new);
+        st.inv_s = 256.0f / s_new;
         st.m_run = m_new;
         st.s_run = s_new;
         st.l_run *= alpha;

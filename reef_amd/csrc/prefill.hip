@@ -469,9 +469,9 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs &a, int tile, int
                     // scale so far (within a factor 2), so that p * v_scale * 2^6 / s_run
                     // stays below 2^15 in fp16 and above its subnormals where its weight
                     // counts (the row sum is of p itself).
-                    const float s_new = fmaxf(s_run, svt);
-                    alpha_o = s_new > 0.0f ? alpha * (s_run / s_new) : alpha;
-                    inv_s = s_new > 0.0f ? 64.0f / s_new : 0.0f;
+                    const float s_new = fmaxf(fmaxf(s_run, svt), kLeastScale);
+                    alpha_o = alpha * (s_run / s_new);
+                    inv_s = 64.0f / s_new;
                     s_run = s_new;
                 }
                 m_run = m_new;

@@ -28,6 +28,10 @@ constexpr float kLog2e = 1.44269504088896341f;
 // prefill kernels and decode always split).
 constexpr float kHiOnlyMax = 1.0f;
 
+// The least value scale that weights are normalized by: its inverse, times 2^8 and a weight's 2^6,
+// is in fp32 (value scales from 1e-45 on; the normalizer of a row of zeros does not matter).
+constexpr float kLeastScale = 0x1p-112f;
+
 // --- matrix instructions ---------------------------------------------------------------
 // Output layout of the 32x32 instructions: lane l holds column l % 32 and, in
 // register 4j + i, row 8j + 4(l / 32) + i. Of the 16x16 instructions: lane l

@@ -200,9 +200,8 @@ __device__ __forceinline__ Column column_of(const TreeArgs &a, int kvh, int inde
     return {live, kvh * a.group + i - token * a.group, token};
 }
 
-// Values accumulate in units of 2^-8 of a power of two, so that the unit's inverse is exact and
-// one subtraction. The least of them: its inverse times a weight's 2^6 is in fp32.
-constexpr float kLeastUnit = 0x1p-112f;
+// Values accumulate in units of 2^-8 of a power of two (kLeastScale at least), so that the unit's
+// inverse is exact and one subtraction.
 
 // The power of two at or above x > 0 (2^127 for all above it).
 __device__ __forceinline__ float power_above(float x) {
@@ -516,13 +515,13 @@ __global__ __launch_bounds__(64 * kWaves, kWgPerCu) void tree_kernel(TreeArgs ar
             pg_second = block_pages<PAGED>(a, nxt.b, first_key(nxt) + k_step, nxt.sk, lane);
         }
 
-        float m_run[NC], l_run[NC], s_run[NC], s_least = kLeastUnit;
+        float m_run[NC], l_run[NC], s_run[NC], s_least = kLeastScale;
         f32x4 acc[NC][DB];
 #pragma unroll
         for (int t = 0; t < NC; ++t) {
             m_run[t] = -INFINITY;
             l_run[t] = 0.0f;
-            s_run[t] = kLeastUnit;
+            s_run[t] = kLeastScale;
 #pragma unroll
             for (int d = 0; d < DB; ++d) acc[t][d] = f32x4{};
         }

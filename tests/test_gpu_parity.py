@@ -607,6 +607,44 @@ def test_prefill_many_small_weights_keep_their_precision(reef):
     assert max(errs.values()) <= 1e-4, errs
 
 
+@pytest.mark.parametrize("size", [1e-20, 1e-37])
+def test_value_scales_near_the_bottom_of_fp32(reef, size):
+    """Per-token value scales whose inverse times 2^8 is beyond fp32 (1e-37), in decode and
+    prefill, against the formula in 64 bits. Of the largest value: 4 roundings of an exponent of
+    X log2 units (2.8 X u), 20 u for exp2, the weights' parts and the merges, u = 2^-24, and half
+    a subnormal fp16 step in units of 2^-6 of a value scale (2^-112 at least) a key: 2^-30."""
+    case(f"value scales of {size}")
+    rng = np.random.default_rng(36)
+    B, Hq, H, D, n = 2, 4, 2, 128, 300
+    L = 304
+    q = rng.integers(-127, 128, (B, Hq, n, D)).astype(np.int8)
+    k, v = (rng.integers(-127, 128, (B, H, L, D)).astype(np.int8) for _ in range(2))
+    qs = rng.uniform(0.005, 0.02, (B, Hq, n)).astype(np.float32)
+    ks = rng.uniform(0.005, 0.03, (B, H, L)).astype(np.float32)
+    vs = (rng.uniform(0.5, 1, (B, H, L)) * size).astype(np.float32)
+    scale = np.float32(1 / math.sqrt(D))
+    kk, vv = (np.repeat(x[:, :, :n].astype(np.float64) * s[:, :, :n, None], Hq // H, 1)
+              for x, s in ((k, ks), (v, vs)))
+    s = (q * qs[..., None].astype(np.float64)) @ kk.transpose(0, 1, 3, 2) * float(scale)
+    X = np.abs(s).max() / math.log(2)
+
+    def attend(s):
+        p = np.exp(s - s.max(3, keepdims=True))
+        return p @ vv / p.sum(3, keepdims=True)
+
+    u = 2.0 ** -24
+    tol = np.abs(vv).max() * (2 * 2.8 * X * u + 40 * u) + 127 * max(size, 2.0 ** -112) * n * 2.0 ** -30
+    vp = v.reshape(B, H, L // 16, 16, D).transpose(0, 1, 2, 4, 3)
+    out = reef.attention_decode(gpu(q[:, :, 0]), gpu(qs[:, :, 0]), gpu(k), gpu(vp), gpu(ks), gpu(vs),
+                                gpu(np.full(B, n, np.int32)), softmax_scale=float(scale))
+    assert np.abs(host(out).astype(np.float64) - attend(s[:, :, :1])[:, :, 0]).max() <= tol
+    out = reef.attention_prefill(gpu(q), gpu(k[:, :, :n]), gpu(v[:, :, :n]), gpu(qs), gpu(ks[:, :, :n]),
+                                 gpu(vs[:, :, :n]), softmax_scale=float(scale),
+                                 q_granularity=reef.PER_TOKEN, kv_granularity=reef.PER_TOKEN)
+    s = np.where(np.tril(np.ones((n, n), bool)), s, -np.inf)  # (causal)
+    assert np.abs(host(out).astype(np.float64) - attend(s)).max() <= tol
+
+
 def test_decode_many_small_weights_keep_their_precision(reef):
     """The decode form of the case above: one sequence of 8192 cached keys, per-token
     scales, key 0 carrying the weight and the other 8191 keys each 1.49 2^-24 of it;

@@ -376,7 +376,7 @@ def test_a_drafted_token_with_an_infinite_key_scale(reef, D, Hq, H, T, value):
 def reference_by_row(q, k, v, qs, ks, vs, lens, m, window, scale):
     """(out, tolerance [B, Hq, T, 1]): the tolerance of the file's head from what each row sees
     alone, its exponents and 127 times its largest value scale. (A weight is off by 2^-33 of a
-    power of two that is less than twice that scale; the row sum does not share this.)"""
+    power of two that is less than twice that scale, or 2^-112; the row sum does not share this.)"""
     out, _ = reference(q, k, v, qs, ks, vs, lens, m, window, scale)
     B, Hq, T, D = q.shape
     tol = np.zeros((B, Hq, T, 1))
@@ -393,8 +393,9 @@ def reference_by_row(q, k, v, qs, ks, vs, lens, m, window, scale):
             s = np.abs((q[b, h] * qs[b, h][:, None].astype(np.float64)) @ kk.T) * scale / math.log(2)
             for t in np.flatnonzero(seen.any(1)):
                 X = s[t, seen[t]].max()
-                most = 127.0 * vs[b, h * k.shape[1] // Hq, :n][seen[t]].max()
-                tol[b, h, t] = most * (2 * (2.8 * X * U + 6 * U + n * 2.0 ** -33) + 14 * U)
+                top = vs[b, h * k.shape[1] // Hq, :n][seen[t]].max()
+                tol[b, h, t] = 127.0 * (top * (2 * (2.8 * X * U + 6 * U) + 14 * U)
+                                        + max(top, 2.0 ** -112) * 2 * n * 2.0 ** -33)
     return out, tol
 
 
@@ -424,7 +425,7 @@ def test_large_values_of_a_hidden_token(reef, D, Hq, H, T, large):
         assert (np.abs(out.cpu().numpy() - ref) <= tol).all()
 
 
-@pytest.mark.parametrize("size", [1e-30, 1e-36])
+@pytest.mark.parametrize("size", [1e-30, 1e-36, 1e-37])
 def test_small_values(reef, size):
     """Value scales whose inverse times 2^8 is beyond fp32; beside them drafted tokens of
     ordinary ones, which some rows see."""
