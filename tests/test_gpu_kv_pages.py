@@ -239,6 +239,51 @@ def test_copy_on_write_keeps_the_parent(reef):
     assert one is not None
 
 
+@pytest.mark.parametrize("who", [[0, 2, 3], [2, 3], [0], [3]])
+def test_tokens_after_a_fork_stay_apart(reef, who):
+    """Two forks of a sequence whose last page is partial, then a token for some of the three: each
+    finds the seven tokens from before the fork and its own, and the others' pages stay as they
+    were, byte for byte."""
+    print(f"\n[case] copy on write, tokens of sequences {who}", flush=True)
+    rng = np.random.default_rng(9)
+    B, H, D, P, n = 4, 2, 64, 40, 23
+    m = Model(B, 4, P)
+    table, lens, refs = m.device()
+    reef.kv_reserve(table, lens, refs, n)
+    lens[:2] = n
+    layer = [gpu(x) for x in pool(rng, (P, H), D)]
+    shared = int(table[0, 1])
+    before = [host(x[shared]) for x in layer]
+    reef.kv_fork(gpu(i32([0, 0])), gpu(i32([2, 3])), table, lens, refs)
+    src, dst = reef.kv_reserve(table, lens, refs, 1)
+    reef.kv_copy_pages(src, dst, *layer)
+    tb = host(table)
+    assert len(set(tb[:, 1])) == B and len({tb[0, 0], tb[2, 0], tb[3, 0]}) == 1
+    whole = [host(x) for x in layer]
+    k_new, v_new = (torch.randn(len(who), H, 1, D, generator=torch.Generator().manual_seed(i)).cuda()
+                    for i in range(2))
+    reef.kv_append_paged(k_new, v_new, lens[gpu(i32(who)).long()], table[gpu(i32(who)).long()], *layer)
+    (kq, ks), (vq, vs) = (reef.quantize_rows(x.view(-1, D)) for x in (k_new, v_new))
+    new = [host(x).reshape(len(who), H, -1) for x in (kq, vq, ks, vs)]
+    slot = n % PAGE
+    for i, x in enumerate(layer):
+        got, want = host(x), whole[i].copy()
+        value = i == 1  # [pages, heads, head_dim, 16]: the slot is last
+        for b in (0, 2, 3):
+            page = got[tb[b, 1]]
+            if not value:
+                assert np.array_equal(page[:, :slot], before[i][:, :slot])
+            else:
+                assert np.array_equal(page[..., :slot], before[i][..., :slot])
+        for j, b in enumerate(who):
+            row = new[i][j] if i < 2 else new[i][j][:, 0]
+            if value:
+                want[tb[b, 1]][..., slot] = row
+            else:
+                want[tb[b, 1]][:, slot] = row
+        assert np.array_equal(got, want)
+
+
 @pytest.mark.parametrize("sharers,free,short", [(2, 1, False), (2, 0, True), (5, 4, False), (5, 3, True),
                                                 (2, 2, False), (1300, 1299, False), (1300, 1298, True)])
 def test_the_last_sharer_needs_no_page(reef, sharers, free, short):
