@@ -378,6 +378,14 @@ __device__ void plan_blocks(const DecodeArgs &a, int32_t *sOff, int32_t *sWave) 
     }
 }
 
+// Workgroup g of G owns units [start(g), start(g + 1)) of the T units (64-key
+// blocks of all items, or items), start(g) = g T / G; unit u lies in workgroup
+// ((u + 1) G - 1) / T.
+__device__ __forceinline__ int64_t wg_start(int64_t g, int64_t T, int64_t G) { return g * T / G; }
+__device__ __forceinline__ int wg_of(int64_t u, int64_t T, int64_t G) {
+    return (int)(((u + 1) * G - 1) / T);
+}
+
 // Log-sum-exp merge of the waves' (max, sum, output in absolute value units)
 // through LDS, in wave order; the result is valid in wave 0. The caller places a
 // barrier between this and the next use of sO / sML.

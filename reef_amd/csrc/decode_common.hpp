@@ -1,5 +1,5 @@
-// What the attention kernels over the int8 decode cache share (gfx950): the cache's sizes,
-// operand conversions, and how a launch deals its work out.
+// What the attention kernels over the int8 decode cache share (gfx950): the keys of a step,
+// operand conversions and loads.
 #pragma once
 
 #include "reef_common.hpp"
@@ -7,7 +7,6 @@
 namespace reef {
 
 constexpr int kBlockKeys = 64;  // keys per inner step (4 pages)
-constexpr int kPage = 16;       // tokens per page
 
 // int8 x 16 (one 16-byte word) -> two fp16 x 8 operands, exactly. After the XOR a
 // byte holds u = b + 128; a byte permute puts each u under the exponent byte 0x64,
@@ -45,14 +44,6 @@ __device__ __forceinline__ void row_lanes(float x, float (&out)[16]) {
     out[R] = __int_as_float(
         __builtin_amdgcn_mov_dpp(__float_as_int(x), 0x150 + R, 0xf, 0xf, true));
     if constexpr (R < 15) row_lanes<R + 1>(x, out);
-}
-
-// Workgroup g of G owns units [start(g), start(g + 1)) of the T units (64-key
-// blocks of all items, or items), start(g) = g T / G; unit u lies in workgroup
-// ((u + 1) G - 1) / T.
-__device__ __forceinline__ int64_t wg_start(int64_t g, int64_t T, int64_t G) { return g * T / G; }
-__device__ __forceinline__ int wg_of(int64_t u, int64_t T, int64_t G) {
-    return (int)(((u + 1) * G - 1) / T);
 }
 
 }  // namespace reef

@@ -16,7 +16,6 @@
 namespace reef {
 namespace {
 
-constexpr int kPage = 16;
 constexpr int kAppendThreads = 256;  // 4 waves per (batch, kv head, cache page)
 
 struct AppendArgs {

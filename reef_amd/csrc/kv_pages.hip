@@ -17,8 +17,6 @@
 namespace reef {
 namespace {
 
-constexpr int kPage = 16;
-
 __device__ __forceinline__ bool page_ok(int page, int num_pages) {
     return page >= 0 && page < num_pages;
 }
@@ -419,7 +417,7 @@ __global__ __launch_bounds__(kCopyThreads) void copy_pages(CopyArgs a) {
 
 // ---- keep ------------------------------------------------------------------------------
 
-constexpr int kMaxDrafts = 64, kKeepThreads = 256;
+constexpr int kKeepThreads = 256;
 
 struct KeepArgs {
     const int32_t *kept, *kept_lens, *lens;

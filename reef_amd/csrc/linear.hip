@@ -20,7 +20,6 @@
 namespace reef {
 namespace {
 
-constexpr int kXcds = 8;
 constexpr int kBK = 128;      // bytes of K per step of the tile kernel
 
 struct GemmArgs {

@@ -34,7 +34,6 @@ namespace {
 constexpr int kBM = 128;  // query rows per workgroup
 constexpr int kBN = 64;   // keys per tile
 constexpr int kThreads = 256;
-constexpr int kXcds = 8;  // workgroup i of a launch runs on XCD i % 8
 
 struct PrefillArgs {
     const int8_t *q, *k, *v;

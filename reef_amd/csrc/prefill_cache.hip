@@ -21,7 +21,6 @@ int64_t prefill_balanced_bytes(const reef_attention_params &p);  // prefill.hip
 
 namespace {
 
-constexpr int kPage = 16;
 constexpr int kGatherThreads = 256;
 
 struct GatherArgs {

@@ -19,6 +19,9 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kWave = 64;
+constexpr int kPage = 16;       // tokens per page of the KV cache
+constexpr int kMaxDrafts = 64;  // drafted tokens of a sequence: bits of a mask word
+constexpr int kXcds = 8;        // workgroup i of a launch runs on XCD i % 8
 constexpr float kLog2e = 1.44269504088896341f;
 // P.V precision of the packed prefill: where a head's dequantized values reach above
 // this magnitude, P is split into fp16 hi + lo parts (22 bits). Below it one fp16 P,

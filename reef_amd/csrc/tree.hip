@@ -24,9 +24,7 @@ constexpr int kWaves = 4;      // waves of a workgroup, one per SIMD
 constexpr int kWgPerCu = 2;    // workgroups of a compute unit
 constexpr int kMinBlocks = 2;  // blocks of a wave in a run, at least, while items are whole
 constexpr int kPlan = 2048;    // sequences of a launch (more are launched in slices)
-constexpr int kMaxDrafts = 64; // bits of a mask word
 constexpr int kMaxGroup = 1024;  // query heads of a kv head
-constexpr int kXcds = 8;       // workgroup i of a launch runs on XCD i % 8
 constexpr int kCounters = 2048;
 
 struct TreeArgs {
