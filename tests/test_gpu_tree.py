@@ -393,7 +393,7 @@ def reference_by_row(q, k, v, qs, ks, vs, lens, m, window, scale):
             s = np.abs((q[b, h] * qs[b, h][:, None].astype(np.float64)) @ kk.T) * scale / math.log(2)
             for t in np.flatnonzero(seen.any(1)):
                 X = s[t, seen[t]].max()
-                top = vs[b, h * k.shape[1] // Hq, :n][seen[t]].max()
+                top = float(vs[b, h * k.shape[1] // Hq, :n][seen[t]].max())
                 tol[b, h, t] = 127.0 * (top * (2 * (2.8 * X * U + 6 * U) + 14 * U)
                                         + max(top, 2.0 ** -112) * 2 * n * 2.0 ** -33)
     return out, tol
