@@ -41,10 +41,11 @@ struct GemmArgs {
     int32_t activation;
 };
 
-// The activations, each within a few units in the last place of fp32 (expf, erfcf): the
-// GELUs and SiLU as quotients and complements without a cancellation, so that their small
-// values left of 0 keep their digits. What is not finite stays so (relu makes -inf a NaN), so
-// that the result tells.
+// The activations: the GELUs and SiLU as quotients and complements without a cancellation, each
+// within u (|x| + 4 |y|), with erfc u (|x| + 35 |y|), u = 2^-24. Small values left of 0 keep
+// most of their digits: the rounding of an exponent or of erfc's argument a grows with a and a^2,
+// and where exp(-x) passes fp32 (x below -88) the result is -0. What is not finite stays so (relu
+// makes -inf a NaN), so that the result tells.
 __device__ __forceinline__ float activate(float x, int activation) {
     switch (activation) {  // uniform over the launch
     case REEF_ACT_RELU:
