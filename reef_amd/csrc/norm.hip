@@ -293,6 +293,11 @@ extern "C" reef_status reef_rmsnorm_quantize_int8(const float *x, int64_t rows, 
     // loads in flight fill the memory (65536 x 1024: 147 us against 182 with four waves a row,
     // 4096 x 2048 21.3 against 25.0). With few, four waves share a row's latency (512 x 1024:
     // 4.7 against 5.3, 16 x 2048: 4.4 against 6.5); at 2048 rows of 2048 both take 14.6.
+    // A lane holds as few groups as cover the row (4096 rows of 256 values: 5.0 us with one, 5.5
+    // with two, 10.5 with four waves a row; of 512: 6.6 with two, 8.0 with four, 11.0 with four
+    // waves; of 1024 in four waves: 15.0 with one, 17.0 with two). Four waves or eight, for 512 and
+    // for 4096 rows: of 4096 values 7.0 or 7.3 and 37.5 or 38.6 us, of 8192 12.9 or 12.6 and 77.6 or
+    // 77.0. Eight, sixteen, or the walk of longer rows: of 16384 22.2, 23.7, 24.4 and 146, 151, 179.
     const bool many = rows >= 2048;
     if (width <= 256) launch_rows<1, 1>(a, nt, stream);
     else if (width <= 512) launch_rows<1, 2>(a, nt, stream);
