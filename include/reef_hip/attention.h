@@ -480,6 +480,7 @@ reef_status reef_kv_pack_v_pages(const int8_t *v_tokens, int64_t pages, int64_t 
  *     that row.
  *   - Non-finite values set NON_FINITE (the engine throws before writing; here
  *     the rows of such a call are unspecified).
+ *   - new_tokens of 2^28 - 16 and more are UNSUPPORTED, as is a max_context of 2^30.
  *   - context_lens (optional, may alias start_positions) receives
  *     start_positions[b] + new_tokens for every sequence that was written.
  */
@@ -608,7 +609,7 @@ reef_status reef_kv_keep_int8_paged(const reef_kv_append_params *p, const int32_
  * [B, Hkv, max_context]), paged otherwise (k_cache [P, Hkv, 16, D], v_cache
  * [P, Hkv, D, 16], scales [P, Hkv, 16], block_table [B, max_blocks_per_seq],
  * P = num_pages; max_context is not used). p->kv_len is the number of cached
- * tokens of every sequence (the chunk's included), p->q_len the chunk length,
+ * tokens of every sequence (the chunk's included, below 2^28), p->q_len the chunk length,
  * p->query_start normally kv_len - q_len; p->kv_granularity must be
  * REEF_SCALE_PER_TOKEN (the cache's scales). q, q_scales, out and out_strides are
  * as for reef_attention_prefill_int8. The call gathers the kv_len cached tokens of

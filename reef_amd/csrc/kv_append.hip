@@ -230,7 +230,8 @@ reef_status prepare(const reef_kv_append_params *p, const float *k_new, const re
     if (p->new_tokens > p->max_context) return REEF_CAPACITY;
     if (p->head_dim != 64 && p->head_dim != 128) return REEF_UNSUPPORTED;
     // (grid: pages x kv heads x batch)
-    if (p->max_context >= (int64_t(1) << 30) || p->batch > 65535 || p->kv_heads > 65535)
+    if (p->max_context >= (int64_t(1) << 30) || p->batch > 65535 || p->kv_heads > 65535 ||
+        ceil_div(p->new_tokens, kPage) + 1 > kGridMost256)
         return REEF_UNSUPPORTED;
     const int64_t D = p->head_dim, H = p->kv_heads, T = p->new_tokens;
     const auto strides = [&](const reef_strides *s, int64_t &sb, int64_t &sh, int64_t &st) {

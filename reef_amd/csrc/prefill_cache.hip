@@ -146,7 +146,7 @@ extern "C" reef_status reef_attention_prefill_int8_cache(
         p->query_start + p->q_len > p->kv_len || p->kv_granularity != REEF_SCALE_PER_TOKEN)
         return REEF_INVALID_ARGUMENT;
     if (p->head_dim != 64 && p->head_dim != 128) return REEF_UNSUPPORTED;
-    if (p->kv_len >= (int64_t(1) << 30) || p->batch * p->kv_heads > 65535 ||
+    if (ceil_div(p->kv_len, kPage) > kGridMost256 || p->batch * p->kv_heads > 65535 ||
         p->q_heads > 65535 || p->batch > 65535)
         return REEF_UNSUPPORTED;
     if (!aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(k_scales, 4) ||

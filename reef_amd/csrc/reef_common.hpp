@@ -31,8 +31,8 @@ constexpr float kLog2e = 1.44269504088896341f;
 // prefill kernels and decode always split).
 constexpr float kHiOnlyMax = 1.0f;
 
-// The least value scale that weights are normalized by: its inverse, times 2^8 and a weight's 2^6,
-// is in fp32 (value scales from 1e-45 on; the normalizer of a row of zeros does not matter).
+// The least value scale that weights are normalized by (smaller ones are measured by it): its
+// inverse, times the units' 2^8 and a weight's 2^6, is in fp32.
 constexpr float kLeastScale = 0x1p-112f;
 
 // --- matrix instructions ---------------------------------------------------------------
@@ -195,6 +195,8 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // without an error. So n workgroups (of at most 1024 threads) that may be 2^22 or more lie in
 // rows of kGridRow: workgroup linear_block() of them, those from n on have nothing to do.
 constexpr int64_t kGridRow = int64_t(1) << 21;
+// Workgroups of 256 threads along one dimension that a launch starts in full, at most.
+constexpr int64_t kGridMost256 = (int64_t(1) << 24) - 1;
 
 inline dim3 linear_grid(int64_t n, unsigned y = 1) {
     return n <= kGridRow ? dim3((unsigned)n, y)

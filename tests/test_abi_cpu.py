@@ -125,6 +125,20 @@ def test_prefill_cache_host_validation_and_workspace():
     assert _prefill_cache(p, table=_fake(9), max_blocks=3, pages=0) == reef_amd.INVALID_ARGUMENT
 
 
+def test_caches_longer_than_a_launch_are_refused():
+    """The gather of a prefill over the cache and the append start 256 threads a page: from 2^24
+    pages on a launch would start only some of them."""
+    lib = reef_amd.lib()
+    for n, status in ((1 << 28, reef_amd.UNSUPPORTED), ((1 << 28) - 16, reef_amd.INVALID_ARGUMENT)):
+        p = good_params(kv_granularity=2, q_len=8, kv_len=n, query_start=n - 8)
+        assert _prefill_cache(p, ws_bytes=1000, max_context=1 << 29) == status
+    for n, status in (((1 << 28) - 16, reef_amd.UNSUPPORTED), ((1 << 28) - 32, reef_amd.INVALID_ARGUMENT)):
+        p = reef_amd.KvAppendParams(batch=1, kv_heads=1, head_dim=64, new_tokens=n, max_context=1 << 29)
+        strides = Strides(-1, 0, 0)  # refused after the sizes
+        assert lib.reef_kv_append_int8(p, _fake(1), strides, _fake(2), strides, _fake(3), _fake(4), _fake(5),
+                                       _fake(6), _fake(7), None, None, None) == status
+
+
 def test_decode_host_validation_and_workspace():
     lib = reef_amd.lib()
     p = DecodeParams(batch=64, q_heads=32, kv_heads=8, head_dim=128, max_context=4096,
