@@ -427,7 +427,7 @@ def _own(st):
     if kind == "bounds":
         reef.kv_page_bounds(st["start"], case["tokens"], st["k"], st["ks"], st["bounds"],
                             st["bs"], block_table=table, status=status)
-        return [st["bounds"].float() * st["bs"][..., None, None], st["bs"]]
+        return [reef.dequantize(st["bounds"], st["bs"], 2 * case["head_dim"]), st["bs"]]
     selected = reef.kv_select_pages(st["q"], st["qs"], st["bounds"], st["bs"], st["lens"],
                                     case["budget"], block_table=table, sinks=case["sinks"],
                                     recent=case["recent"], status=status)
