@@ -508,6 +508,148 @@ reef_status reef_kv_append_int8_paged(const reef_kv_append_params *p, const floa
                                       uint32_t *status_word, hipStream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * The cache held in 4 bits: half the bytes of the int8 cache for a decode step to read. The
+ * rule is quantize_rows' (quant.hpp:112-133) with 7 for 127: scale = max|x| / 7 of a token's
+ * row (1 when max is 0), code = clamp(nearbyint(x / scale), -7, 7), IEEE division, ties to
+ * even. A code c is stored as the nibble c + 8. The layouts are the int8 cache's with these
+ * rows and pages:
+ *   keys: a row is D/2 bytes; byte j holds channel j in its low nibble, channel j + D/2 in
+ *   its high one.
+ *   values: a page is [D, 8] bytes, a channel's 16 tokens in 8; token t's code is nibble
+ *   8 (t / 8) + (t % 8) / 2 + 4 (t % 2) of them, low nibbles first (two tokens of an 8-token
+ *   half lie 16 bits apart, so that one mask takes both).
+ *   contiguous: k_cache [B, Hkv, L, D/2]; v_cache [B, Hkv, L/16, D, 8]; scales [B, Hkv, L].
+ *   paged:      k_pages [P, Hkv, 16, D/2]; v_pages [P, Hkv, D, 8]; scales [P, Hkv, 16].
+ * In all calls of this section block_table NULL means the contiguous cache of
+ * p->max_context tokens a sequence (max_blocks_per_seq and num_pages are not used), otherwise
+ * the paged one with max_context <= max_blocks_per_seq * 16. The int8 cache's page calls
+ * (free, fork, reserve, compact) serve either pool.
+ */
+
+/* reef_kv_append_int8 (its limits, status bits and context_lens) into the 4-bit cache. The
+ * codes beside the new ones, in the same bytes too, are left as they were. */
+reef_status reef_kv_append_int4(const reef_kv_append_params *p, const float *k_new,
+                                const reef_strides *k_strides, const float *v_new,
+                                const reef_strides *v_strides, const int32_t *start_positions,
+                                const int32_t *block_table, int64_t max_blocks_per_seq,
+                                int64_t num_pages, uint8_t *k_cache, uint8_t *v_cache,
+                                float *k_scales, float *v_scales, int32_t *context_lens,
+                                uint32_t *status_word, hipStream_t stream);
+
+/* `pages` pages of one head each, in memory order (a contiguous cache has B * Hkv * L / 16, a
+ * pool P * Hkv), as fp32 rows: k and v [pages, 16, D], x = float(code) * scale. k or v NULL:
+ * left out (its codes and scales then are not read). head_dim 64 or 128. */
+reef_status reef_kv_unpack_int4(const uint8_t *k_pages, const uint8_t *v_pages,
+                                const float *k_scales, const float *v_scales, int64_t pages,
+                                int64_t head_dim, float *k, float *v, hipStream_t stream);
+
+/* reef_kv_copy_pages for a pool of the 4-bit cache. */
+reef_status reef_kv_copy_pages_int4(const int32_t *src, const int32_t *dst, int64_t n,
+                                    int64_t kv_heads, int64_t head_dim, uint8_t *k_pages,
+                                    uint8_t *v_pages, float *k_scale_pages, float *v_scale_pages,
+                                    int64_t num_pages, uint32_t *status_word, hipStream_t stream);
+
+/* The pages of 16 tokens that a decode step reads, for every (sequence, kv head): the first
+ * counts[b][h] entries of pages[b][h], numbers of the sequence's pages (page i holds tokens
+ * 16 i .. 16 i + 15), in any order. A negative entry is left out, one at or past the
+ * sequence's ceil(len / 16) sets BAD_PAGE and is left out; a page listed twice counts twice.
+ * A count outside [0, max_pages] sets BAD_LENGTH and yields zeros, as does 0 (without a bit). */
+typedef struct reef_page_selection {
+    const int32_t *pages;  /* [B, Hkv, max_pages], on the device */
+    const int32_t *counts; /* [B, Hkv], on the device */
+    int64_t max_pages;     /* below 2^26 */
+} reef_page_selection;
+
+/* The decode step of reef_attention_decode_int8 over the 4-bit cache, over all keys
+ * (selection NULL) or the listed pages' alone. context_lens may be NULL for the contiguous
+ * cache without a selection. The workspace is the int8 decode's, of the same size. With a
+ * window, tokens before it take no part, whatever is listed. */
+reef_status reef_attention_decode_int4(const reef_decode_params *p, const int8_t *q,
+                                       const float *q_scales, const uint8_t *k_cache,
+                                       const uint8_t *v_cache, const float *k_scales,
+                                       const float *v_scales, const int32_t *block_table,
+                                       int64_t max_blocks_per_seq, int64_t num_pages,
+                                       const int32_t *context_lens,
+                                       const reef_page_selection *selection, float *out,
+                                       void *workspace, size_t workspace_bytes,
+                                       uint32_t *status_word, hipStream_t stream);
+
+/* reef_attention_prefill_int8_cache over the 4-bit cache (max_context as there). The codes
+ * are widened on their way into the workspace, which is that call's, of the same size. */
+reef_status reef_attention_prefill_int4_cache(
+    const reef_attention_params *p, const int8_t *q, const reef_strides *q_strides,
+    const float *q_scales, const uint8_t *k_cache, const uint8_t *v_cache, const float *k_scales,
+    const float *v_scales, int64_t max_context, const int32_t *block_table,
+    int64_t max_blocks_per_seq, int64_t num_pages, float *out, const reef_strides *out_strides,
+    void *workspace, size_t workspace_bytes, uint32_t *status_word, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Attention over the pages that a query selects, for caches too long to be read at every
+ * step. Of every page the largest and the least key of each channel are kept; a query's
+ * products with them bound its score with every key of the page, at 1/16 of the int8 keys'
+ * and values' bytes. block_table NULL: contiguous, as in the section above.
+ *
+ * bounds: int8 codes [B, Hkv, L/16, 2, D] (contiguous) or [P, Hkv, 2, D] (paged), on 16 bytes;
+ * bound_scales: one scale a page and head, [B, Hkv, L/16] or [P, Hkv].
+ */
+
+/* The bounds of the pages that positions start_positions[b] .. start_positions[b] +
+ * new_tokens - 1 fall in, over those pages' tokens before start_positions[b] + new_tokens:
+ * after an append, with its start positions (a page's earlier tokens are read again, so a
+ * page copied by reef_kv_copy_pages needs nothing else); after a compaction, once with start
+ * 0. Of the keys x = float(code) * scale: S = max|x| / 127 (1 where that is 0), [0][d] =
+ * min(127, ceil(max x_d / S)), [1][d] = max(-127, floor(min x_d / S)), IEEE divisions. Key
+ * scales are positive and finite, as the quantizers make them. Sizes and status bits as
+ * for reef_kv_append_int8 (a range past max_context sets CAPACITY and writes nothing). */
+reef_status reef_kv_page_bounds_int8(const reef_kv_append_params *p,
+                                     const int32_t *start_positions, const int8_t *k_cache,
+                                     const float *k_scales, const int32_t *block_table,
+                                     int64_t max_blocks_per_seq, int64_t num_pages, int8_t *bounds,
+                                     float *bound_scales, uint32_t *status_word,
+                                     hipStream_t stream);
+
+reef_status reef_kv_page_bounds_int4(const reef_kv_append_params *p,
+                                     const int32_t *start_positions, const uint8_t *k_cache,
+                                     const float *k_scales, const int32_t *block_table,
+                                     int64_t max_blocks_per_seq, int64_t num_pages, int8_t *bounds,
+                                     float *bound_scales, uint32_t *status_word,
+                                     hipStream_t stream);
+
+/* For every (sequence, kv head) the `budget` pages to read, shared by the group's query
+ * heads, as a reef_page_selection holds them: ascending, -1 behind the last. The first
+ * `sinks` and the last `recent` pages of the sequence are always among them (recent >= 1,
+ * sinks + recent <= budget), then those of the largest score, ties to the lowest page; all
+ * pages where the sequence has no more than `budget`. A page's score is the largest over the
+ * group's query heads of float(sum_d max(q_d, 0) [0][d] + min(q_d, 0) [1][d]) * (s_q * S),
+ * the sum in whole numbers, the two products rounded to fp32 each: the same pages on every
+ * run. q and q_scales as for decode; p->window, softmax_scale and num_splits are not used. A
+ * page number outside [0, num_pages) sets BAD_PAGE, and that page is not selected; a length
+ * outside [1, max_context] sets BAD_LENGTH, its counts are 0. Workspace: 16-byte aligned,
+ * reef_kv_select_pages_workspace_bytes(p) bytes (0: invalid sizes), zero-filled before its
+ * first use; every call leaves it ready for the next of any shape it is large enough for.
+ * Calls that may run at the same time need separate workspaces. At most 65535 (sequence, kv
+ * head) pairs. */
+size_t reef_kv_select_pages_workspace_bytes(const reef_decode_params *p);
+
+reef_status reef_kv_select_pages(const reef_decode_params *p, const int8_t *q,
+                                 const float *q_scales, const int8_t *bounds,
+                                 const float *bound_scales, const int32_t *block_table,
+                                 int64_t max_blocks_per_seq, int64_t num_pages,
+                                 const int32_t *context_lens, int64_t budget, int64_t sinks,
+                                 int64_t recent, int32_t *pages, int32_t *counts, void *workspace,
+                                 size_t workspace_bytes, uint32_t *status_word,
+                                 hipStream_t stream);
+
+/* The decode step of reef_attention_decode_int8 over the listed pages alone
+ * (reef_attention_decode_int4 takes the same list). */
+reef_status reef_attention_decode_int8_selected(
+    const reef_decode_params *p, const int8_t *q, const float *q_scales, const int8_t *k_cache,
+    const int8_t *v_cache, const float *k_scales, const float *v_scales,
+    const int32_t *block_table, int64_t max_blocks_per_seq, int64_t num_pages,
+    const int32_t *context_lens, const reef_page_selection *selection, float *out,
+    void *workspace, size_t workspace_bytes, uint32_t *status_word, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Pages of the paged cache. block_table [batch, max_blocks_per_seq] int32 names the page of
  * every 16-token block of a sequence, -1 where it has none; context_lens [batch] int32 its
  * tokens; page_refs [num_pages] int32 how many table entries name a page: 0 is a free page,

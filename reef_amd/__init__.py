@@ -50,6 +50,10 @@ EXPORTS = [
     "reef_kv_compact", "reef_kv_copy_pages", "reef_kv_keep_int8", "reef_kv_keep_int8_paged",
     "reef_attention_prefill_cache_workspace_bytes",
     "reef_attention_prefill_int8_cache",
+    "reef_kv_append_int4", "reef_kv_unpack_int4", "reef_kv_copy_pages_int4",
+    "reef_attention_decode_int4", "reef_attention_prefill_int4_cache", "reef_kv_page_bounds_int8",
+    "reef_kv_page_bounds_int4", "reef_kv_select_pages_workspace_bytes", "reef_kv_select_pages",
+    "reef_attention_decode_int8_selected",
 ]
 
 
@@ -122,11 +126,16 @@ class Epilogue(C.Structure):
                 ("activation", C.c_int64)]
 
 
+class PageSelection(C.Structure):
+    _fields_ = [("pages", C.c_void_p), ("counts", C.c_void_p), ("max_pages", C.c_int64)]
+
+
 _P = C.c_void_p
 _I64 = C.c_int64
 _ST, _AP = C.POINTER(Strides), C.POINTER(AttentionParams)
 _DP, _KP = C.POINTER(DecodeParams), C.POINTER(KvAppendParams)
 _EP, _TP = C.POINTER(Epilogue), C.POINTER(TreeParams)
+_SP = C.POINTER(PageSelection)
 _SIGS = {
     "reef_quantize_int8_per_tensor": [_P, _I64, _P, _P, _P, _P],
     "reef_quantize_int8_per_head": [_P, _I64, _I64, _I64, _I64, _ST, _P, _P, _P, _P],
@@ -179,6 +188,20 @@ _SIGS = {
     "reef_attention_prefill_cache_workspace_bytes": [_AP],
     "reef_attention_prefill_int8_cache": [_AP, _P, _ST, _P, _P, _P, _P, _P, _I64, _P, _I64, _I64,
                                           _P, _ST, _P, C.c_size_t, _P, _P],
+    "reef_kv_append_int4": [_KP, _P, _ST, _P, _ST, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P],
+    "reef_kv_unpack_int4": [_P, _P, _P, _P, _I64, _I64, _P, _P, _P],
+    "reef_kv_copy_pages_int4": [_P, _P, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P, _P],
+    "reef_attention_decode_int4": [_DP, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _SP, _P, _P,
+                                   C.c_size_t, _P, _P],
+    "reef_attention_prefill_int4_cache": [_AP, _P, _ST, _P, _P, _P, _P, _P, _I64, _P, _I64, _I64,
+                                          _P, _ST, _P, C.c_size_t, _P, _P],
+    "reef_kv_page_bounds_int8": [_KP, _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _P],
+    "reef_kv_page_bounds_int4": [_KP, _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _P],
+    "reef_kv_select_pages_workspace_bytes": [_DP],
+    "reef_kv_select_pages": [_DP, _P, _P, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _P,
+                             C.c_size_t, _P, _P],
+    "reef_attention_decode_int8_selected": [_DP, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _SP,
+                                            _P, _P, C.c_size_t, _P, _P],
 }
 
 _lib_handle = _plain_handle = None
@@ -262,6 +285,7 @@ _DECODE = struct.Struct("=6qf2iI")
 _APPEND = struct.Struct("=5q")
 _EPILOGUE = struct.Struct("=3q")
 _TREE = struct.Struct("=7qfi2I")
+_SELECTION = struct.Struct("=3q")
 
 
 def _require(t, dtype, name):
@@ -662,8 +686,9 @@ def tree_workspace(params: TreeParams, device):
     return torch.zeros(max(n, 256), dtype=torch.uint8, device=device)
 
 
-def _tree_workspace(n, device, stream):
-    """This stream's workspace. A call under graph capture takes one of its own, which lives
+def _step_workspace(n, device, stream):
+    """This stream's workspace of the decode calls over drafted tokens, 4-bit caches and selected
+    pages, whose first 8 KB are counters. A call under graph capture takes one of its own, which lives
     in the graph's memory: graphs that replay at the same time share nothing. Only its
     counters have to be zero, the first 8 KB: not a megabyte of parts at every replay."""
     torch = _torch()
@@ -742,7 +767,7 @@ def attention_decode_tree(q, q_scales, k_cache, v_pages, k_scales, v_scales, con
         D, context_lens, out)
     stream = _stream()
     n = _lib().reef_attention_decode_tree_workspace_bytes(p)
-    ws = _tree_workspace(n, q.device, stream) if workspace is None else _given(workspace)
+    ws = _step_workspace(n, q.device, stream) if workspace is None else _given(workspace)
     own = status or StatusWord(q.device)
     check(_lib().reef_attention_decode_tree_int8(
         p, _ptr(q), _strides4(q), _ptr(q_scales), _ptr(k_cache), _ptr(v_pages), _ptr(k_scales),
@@ -771,7 +796,7 @@ def attention_decode_tree_paged(q, q_scales, k_pages, v_pages, k_scale_pages, v_
         context_lens, out)
     stream = _stream()
     n = _lib().reef_attention_decode_tree_workspace_bytes(p)
-    ws = _tree_workspace(n, q.device, stream) if workspace is None else _given(workspace)
+    ws = _step_workspace(n, q.device, stream) if workspace is None else _given(workspace)
     own = status or StatusWord(q.device)
     check(_lib().reef_attention_decode_tree_int8_paged(
         p, _ptr(q), _strides4(q), _ptr(q_scales), _ptr(k_pages), _ptr(v_pages),
@@ -1045,6 +1070,344 @@ def kv_keep_paged(kept, kept_lens, context_lens, block_table, k_pages, v_pages, 
     if status is None:
         own.check("kv_keep_paged")
     return lens
+
+
+# --- the cache held in 4 bits, and the pages that a query selects ------------------------------
+#
+# One call serves both caches: block_table None is the contiguous one, k_cache [B, Hkv, L, D/2]
+# uint8, v_cache [B, Hkv, L/16, D, 8] uint8, scales [B, Hkv, L]; otherwise block_table is
+# [B, max_blocks] int32 and the cache a pool, [P, Hkv, 16, D/2], [P, Hkv, D, 8] and [P, Hkv, 16].
+# The codes' places in a byte: the C header. An int8 cache (int8 tensors, D for D/2 and 16 for 8)
+# takes the calls that are not named for 4 bits.
+
+def _cache(what, batch, k_cache, v_cache, k_scales, v_scales, block_table, bits):
+    """(heads, tokens a sequence, head_dim, table, blocks, pages) of either cache."""
+    torch = _torch()
+    dtype = torch.int8 if bits == 8 else torch.uint8
+    _expect(what, dtype, (k_cache, "k_cache"))
+    n = k_cache.numel()
+    if k_cache.dim() != 4:
+        raise InvalidArgument(f"{what}: k_cache must have 4 dimensions")
+    lead, heads, tokens, row = k_cache.shape
+    head_dim = row * 8 // bits
+    if v_cache is not None:
+        _expect(what, dtype, (v_cache, "v_cache"))
+        if v_cache.numel() != n:
+            raise InvalidArgument(f"{what}: cache shape mismatch")
+    for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
+        if t is not None:
+            _expect(what, torch.float32, (t, name))
+            if t.numel() * row != n:
+                raise InvalidArgument(f"{what}: scales do not match the cache")
+    if block_table is None:
+        if lead != batch or tokens % PAGE:
+            raise InvalidArgument(f"{what}: cache shape mismatch")
+        return heads, tokens, head_dim, None, 0, 0
+    _expect(what, torch.int32, (block_table, "block_table"))
+    if block_table.dim() != 2 or block_table.shape[0] != batch or tokens != PAGE:
+        raise InvalidArgument(f"{what}: block_table must be [B, max_blocks], pages of 16 tokens")
+    blocks = block_table.shape[1]
+    return heads, blocks * PAGE, head_dim, block_table.data_ptr(), blocks, lead
+
+
+def _lengths(what, t, batch, name="context_lens"):
+    _expect(what, _torch().int32, (t, name))
+    if t.shape != (batch,):
+        raise InvalidArgument(f"{what}: {name} must be [B]")
+
+
+def kv_append_int4(k_new, v_new, start_positions, k_cache, v_cache, k_scales, v_scales,
+                   context_lens=None, *, block_table=None, status: StatusWord | None = None):
+    """kv_append into the 4-bit cache: rows k_new, v_new [B, Hkv, T, D] fp32, one scale
+    max|x| / 7 a row. context_lens, when given, is set to start_positions + T (it may be
+    start_positions itself)."""
+    what = "kv_append_int4"
+    ks, vs = _append_inputs(k_new, v_new)
+    B, H, T, D = k_new.shape
+    heads, tokens, dim, table, blocks, pages = _cache(what, B, k_cache, v_cache, k_scales, v_scales,
+                                                      block_table, 4)
+    if (heads, dim) != (H, D):
+        raise InvalidArgument("KV cache append shape mismatch")
+    _lengths(what, start_positions, B, "start_positions")
+    if context_lens is not None:
+        _lengths(what, context_lens, B)
+    _on_device(what, k_new, v_new)
+    own = status or StatusWord(k_new.device)
+    check(_lib().reef_kv_append_int4(
+        _packed(_APPEND, KvAppendParams, B, H, D, T, tokens), _ptr(k_new), ks, _ptr(v_new), vs,
+        _ptr(start_positions), table, blocks, pages, _ptr(k_cache), _ptr(v_cache), _ptr(k_scales),
+        _ptr(v_scales), _ptr(context_lens), _ptr(own.tensor), _stream()), what)
+    if status is None:
+        own.check(what)
+
+
+def kv_unpack_int4(k_cache, v_cache, k_scales, v_scales):
+    """The 4-bit cache as fp32 rows by pages: keys and values [..., 16, D] each (contiguous:
+    [B, Hkv, L/16, 16, D], a pool: [P, Hkv, 16, D]), float(code) * scale."""
+    what, torch = "kv_unpack_int4", _torch()
+    _expect(what, torch.uint8, (k_cache, "k_cache"), (v_cache, "v_cache"))
+    _expect(what, torch.float32, (k_scales, "k_scales"), (v_scales, "v_scales"))
+    n = k_cache.numel()
+    if v_cache.dim() < 3 or v_cache.shape[-1] != PAGE // 2:
+        raise InvalidArgument(f"{what}: v_cache must be [..., D, 8]")
+    D = v_cache.shape[-2]
+    if v_cache.numel() != n or k_scales.numel() * D != 2 * n or v_scales.numel() * D != 2 * n:
+        raise InvalidArgument(f"{what}: cache shape mismatch")
+    shape = (*v_cache.shape[:-2], PAGE, D)
+    k = torch.empty(shape, dtype=torch.float32, device=k_cache.device)
+    v = torch.empty(shape, dtype=torch.float32, device=k_cache.device)
+    if n:
+        check(_lib().reef_kv_unpack_int4(_ptr(k_cache), _ptr(v_cache), _ptr(k_scales),
+                                         _ptr(v_scales), n // (PAGE // 2 * D), D, _ptr(k), _ptr(v),
+                                         _stream()), what)
+    return k, v
+
+
+def kv_copy_pages_int4(source, place, k_pages, v_pages, k_scale_pages, v_scale_pages,
+                       status: StatusWord | None = None):
+    """kv_copy_pages for one layer's 4-bit pool."""
+    what, torch = "kv_copy_pages_int4", _torch()
+    _expect(what, torch.int32, (source, "source"), (place, "place"))
+    _expect(what, torch.uint8, (k_pages, "k_pages"), (v_pages, "v_pages"))
+    _expect(what, torch.float32, (k_scale_pages, "k_scale_pages"),
+            (v_scale_pages, "v_scale_pages"))
+    if k_pages.dim() != 4 or k_pages.shape[2] != PAGE:
+        raise InvalidArgument(f"{what}: k_pages must be [pages, heads, 16, head_dim / 2]")
+    P, H, _, row = k_pages.shape
+    if (v_pages.numel() != k_pages.numel() or k_scale_pages.numel() != P * H * PAGE
+            or v_scale_pages.numel() != P * H * PAGE):
+        raise InvalidArgument(f"{what}: pages and scale pages do not match")
+    if source.numel() != place.numel():
+        raise InvalidArgument(f"{what}: as many sources as destinations")
+    if source.numel() == 0:
+        return
+    own = status or StatusWord(k_pages.device)
+    check(_lib().reef_kv_copy_pages_int4(
+        _ptr(source), _ptr(place), source.numel(), H, 2 * row, _ptr(k_pages), _ptr(v_pages),
+        _ptr(k_scale_pages), _ptr(v_scale_pages), P, _ptr(own.tensor), _stream()), what)
+    if status is None:
+        own.check(what)
+
+
+def _decode_inputs(what, q, q_scales, q_granularity, head_dim, out):
+    torch = _torch()
+    _expect(what, torch.int8, (q, "q"))
+    _expect(what, torch.float32, (q_scales, "q_scales"))
+    if q.dim() != 3 or q.shape[2] != head_dim:
+        raise InvalidArgument(f"{what}: q must be [B, heads, head_dim of the cache]")
+    B, Hq, _ = q.shape
+    scales = B * Hq if q_granularity == PER_TOKEN else Hq if q_granularity == PER_HEAD else 1
+    if q_scales.numel() != scales:
+        raise InvalidArgument(f"{what}: q_scales do not match q_granularity")
+    if out is None:
+        return torch.empty(q.shape, dtype=torch.float32, device=q.device)
+    _expect(what, torch.float32, (out, "out"))
+    if out.shape != q.shape:
+        raise InvalidArgument(f"{what}: out must have q's shape")
+    return out
+
+
+def _decode_cache(what, function, bits, q, q_scales, k_cache, v_cache, k_scales, v_scales,
+                  context_lens, selected, block_table, window, softmax_scale, q_granularity,
+                  num_splits, workspace, status, out):
+    _require(q, _torch().int8, "q")
+    B = q.shape[0]
+    heads, tokens, dim, table, blocks, pages = _cache(what, B, k_cache, v_cache, k_scales, v_scales,
+                                                      block_table, bits)
+    out = _decode_inputs(what, q, q_scales, q_granularity, dim, out)
+    if context_lens is not None:
+        _lengths(what, context_lens, B)
+    elif block_table is not None or selected is not None:
+        raise InvalidArgument(f"{what}: a paged cache and selected pages need context_lens")
+    listed = None
+    if selected is not None:
+        list_, counts = selected
+        _expect(what, _torch().int32, (list_, "selected pages"), (counts, "selected counts"))
+        if list_.dim() != 3 or list_.shape[:2] != (B, heads) or counts.shape != (B, heads):
+            raise InvalidArgument(f"{what}: selected must be pages [B, heads, n], counts [B, heads]")
+        listed = _SELECTION.pack(list_.data_ptr(), counts.data_ptr(), list_.shape[2])
+    p = _decode_bytes(q, tokens, heads, window, softmax_scale, q_granularity, num_splits)
+    stream = _stream()
+    n = _lib().reef_attention_decode_workspace_bytes(p)
+    ws = _step_workspace(n, q.device, stream) if workspace is None else _given(workspace)
+    own = status or StatusWord(q.device)
+    check(function(p, _ptr(q), _ptr(q_scales), _ptr(k_cache), _ptr(v_cache), _ptr(k_scales),
+                   _ptr(v_scales), table, blocks, pages, _ptr(context_lens), listed, _ptr(out),
+                   _ptr(ws), ws.numel() * ws.element_size(), _ptr(own.tensor), stream), what)
+    if status is None:
+        own.check(what)
+    return out
+
+
+def attention_decode_int4(q, q_scales, k_cache, v_cache, k_scales, v_scales, context_lens=None, *,
+                          block_table=None, selected=None, window=0, softmax_scale=None,
+                          q_granularity=PER_TOKEN, num_splits=0, workspace=None,
+                          status: StatusWord | None = None, out=None):
+    """One decode step over the 4-bit cache: q [B, Hq, D] int8, context_lens [B] int32 (None: a
+    full contiguous cache). selected (pages, counts) from kv_select_pages: over those pages'
+    tokens alone. Returns fp32 [B, Hq, D]."""
+    return _decode_cache("attention_decode_int4", _lib().reef_attention_decode_int4, 4, q, q_scales,
+                         k_cache, v_cache, k_scales, v_scales, context_lens, selected, block_table,
+                         window, softmax_scale, q_granularity, num_splits, workspace, status, out)
+
+
+def attention_decode_selected(q, q_scales, k_cache, v_cache, k_scales, v_scales, context_lens, *,
+                              selected, block_table=None, window=0, softmax_scale=None,
+                              q_granularity=PER_TOKEN, num_splits=0, workspace=None,
+                              status: StatusWord | None = None, out=None):
+    """attention_decode, or (with a block_table) attention_decode_paged, over the tokens of the
+    selected pages alone: selected (pages [B, Hkv, n] int32, counts [B, Hkv] int32) as
+    kv_select_pages returns them. For a 4-bit cache: attention_decode_int4."""
+    if selected is None:
+        raise InvalidArgument("attention_decode_selected: no selected pages")
+    return _decode_cache("attention_decode_selected", _lib().reef_attention_decode_int8_selected, 8,
+                         q, q_scales, k_cache, v_cache, k_scales, v_scales, context_lens, selected,
+                         block_table, window, softmax_scale, q_granularity, num_splits, workspace,
+                         status, out)
+
+
+def attention_prefill_cache_int4(q, q_scales, k_cache, v_cache, k_scales, v_scales, kv_len, *,
+                                 block_table=None, query_start=None, window=0, softmax_scale=None,
+                                 q_granularity=PER_HEAD, status: StatusWord | None = None, out=None):
+    """attention_prefill_cache over the 4-bit cache, which holds the chunk's keys already
+    (kv_append_int4): q [B, Hq, q_len, D] int8, kv_len tokens a sequence. Returns fp32
+    [B, Hq, q_len, D]."""
+    what, torch = "attention_prefill_cache_int4", _torch()
+    _require(q, torch.int8, "q")
+    _expect(what, torch.float32, (q_scales, "q_scales"))
+    qs = _strides4(q)
+    B, Hq, Sq, D = q.shape
+    heads, tokens, dim, table, blocks, pages = _cache(what, B, k_cache, v_cache, k_scales, v_scales,
+                                                      block_table, 4)
+    scales = B * Hq * Sq if q_granularity == PER_TOKEN else Hq if q_granularity == PER_HEAD else 1
+    if dim != D or q_scales.numel() != scales:
+        raise InvalidArgument(f"{what}: q and q_scales do not match the cache and q_granularity")
+    if softmax_scale is None:
+        softmax_scale = 1.0 / math.sqrt(D)
+    start = kv_len - Sq if query_start is None else query_start
+    p = _packed(_ATTENTION, AttentionParams, B, Hq, heads, Sq, kv_len, D, start, window,
+                softmax_scale, q_granularity, PER_TOKEN, 0)
+    if out is None:
+        out = torch.empty((B, Hq, Sq, D), dtype=torch.float32, device=q.device)
+    else:
+        _require(out, torch.float32, "out")
+        if out.shape != q.shape:
+            raise InvalidArgument(f"{what}: out must have q's shape")
+    _on_device(what, q, out)
+    stream = _stream()
+    n = _lib().reef_attention_prefill_cache_workspace_bytes(p)
+    ws = _chunk_workspace(n, q.device, stream)
+    own = status or StatusWord(q.device)
+    check(_lib().reef_attention_prefill_int4_cache(
+        p, _ptr(q), qs, _ptr(q_scales), _ptr(k_cache), _ptr(v_cache), _ptr(k_scales),
+        _ptr(v_scales), tokens, table, blocks, pages, _ptr(out), _strides4(out), _ptr(ws), n,
+        _ptr(own.tensor), stream), what)
+    if status is None:
+        own.check(what)
+    return out
+
+
+def _chunk_workspace(n, device, stream):
+    """attention_prefill_cache's workspace of this stream; under graph capture one of its own, of
+    which the counters alone (65536 words in front) have to be zero."""
+    torch = _torch()
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(max(n, 1 << 18), dtype=torch.uint8, device=device)
+        ws[:1 << 18].zero_()
+        return ws
+    key = ("cache", device.index, stream)
+    ws = _PREFILL_WS.get(key)
+    if ws is None or ws.numel() < n:
+        ws = _PREFILL_WS[key] = torch.zeros(max(n, 256), dtype=torch.uint8, device=device)
+    return ws
+
+
+def _bounds(what, bounds, bound_scales, head_dim, pages):
+    torch = _torch()
+    _expect(what, torch.int8, (bounds, "bounds"))
+    _expect(what, torch.float32, (bound_scales, "bound_scales"))
+    if bounds.shape[-2:] != (2, head_dim) or bounds.numel() != pages * 2 * head_dim or (
+            bound_scales.numel() != pages):
+        raise InvalidArgument(f"{what}: bounds must be [..., pages, 2, head_dim], bound_scales one "
+                              "a page and head")
+
+
+def kv_page_bounds(start_positions, new_tokens: int, k_cache, k_scales, bounds, bound_scales, *,
+                   block_table=None, status: StatusWord | None = None):
+    """The largest and the least key of every channel of the pages that tokens start_positions[b]
+    .. start_positions[b] + new_tokens - 1 fall in, over those pages' tokens up to the last of
+    them: call it after an append, with its start positions. k_cache and k_scales of an int8 or
+    a 4-bit cache; bounds int8 [B, Hkv, L/16, 2, D] and bound_scales [B, Hkv, L/16] (contiguous)
+    or [P, Hkv, 2, D] and [P, Hkv] (a pool) are written in place."""
+    what = "kv_page_bounds"
+    torch = _torch()
+    _expect(what, torch.int32, (start_positions, "start_positions"))
+    if start_positions.dim() != 1:
+        raise InvalidArgument(f"{what}: start_positions must be [B]")
+    B = start_positions.shape[0]
+    bits = 4 if k_cache.dtype is torch.uint8 else 8
+    heads, tokens, dim, table, blocks, pages = _cache(what, B, k_cache, None, k_scales, None,
+                                                      block_table, bits)
+    _bounds(what, bounds, bound_scales, dim, heads * (pages if table else B * tokens // PAGE))
+    own = status or StatusWord(k_cache.device)
+    function = _lib().reef_kv_page_bounds_int4 if bits == 4 else _lib().reef_kv_page_bounds_int8
+    check(function(_packed(_APPEND, KvAppendParams, B, heads, dim, new_tokens, tokens),
+                   _ptr(start_positions), _ptr(k_cache), _ptr(k_scales), table, blocks, pages,
+                   _ptr(bounds), _ptr(bound_scales), _ptr(own.tensor), _stream()), what)
+    if status is None:
+        own.check(what)
+
+
+def kv_select_pages(q, q_scales, bounds, bound_scales, context_lens, budget: int, *,
+                    block_table=None, sinks=0, recent=1, q_granularity=PER_TOKEN,
+                    status: StatusWord | None = None):
+    """The `budget` pages that each sequence's kv heads are to read for the query q [B, Hq, D]
+    int8: its first `sinks` and last `recent` pages and those whose bounds (kv_page_bounds) allow
+    the largest scores for any of the group's query heads, ties to the lowest page. Returns
+    (pages [B, Hkv, budget] int32, ascending, -1 behind the last; counts [B, Hkv] int32), the
+    `selected` of attention_decode_selected and attention_decode_int4."""
+    what, torch = "kv_select_pages", _torch()
+    _require(q, torch.int8, "q")
+    if q.dim() != 3:
+        raise InvalidArgument(f"{what}: q must be [B, heads, head_dim]")
+    B, Hq, D = q.shape
+    if bounds.dim() not in (4, 5):
+        raise InvalidArgument(f"{what}: bounds must be [B, heads, pages, 2, D] or [P, heads, 2, D]")
+    heads = bounds.shape[1]
+    if block_table is None:
+        if bounds.dim() != 5 or bounds.shape[0] != B:
+            raise InvalidArgument(f"{what}: bounds must be [B, heads, pages, 2, D]")
+        tokens, table, blocks, pages = bounds.shape[2] * PAGE, None, 0, 0
+        held = B * heads * bounds.shape[2]
+    else:
+        _expect(what, torch.int32, (block_table, "block_table"))
+        if bounds.dim() != 4 or block_table.dim() != 2 or block_table.shape[0] != B:
+            raise InvalidArgument(f"{what}: bounds must be [P, heads, 2, D], block_table "
+                                  "[B, max_blocks]")
+        blocks, pages = block_table.shape[1], bounds.shape[0]
+        tokens, table, held = blocks * PAGE, block_table.data_ptr(), pages * heads
+    _bounds(what, bounds, bound_scales, D, held)
+    _lengths(what, context_lens, B)
+    _expect(what, torch.int8, (q, "q"))
+    _expect(what, torch.float32, (q_scales, "q_scales"))
+    scales = B * Hq if q_granularity == PER_TOKEN else Hq if q_granularity == PER_HEAD else 1
+    if q_scales.numel() != scales:
+        raise InvalidArgument(f"{what}: q_scales do not match q_granularity")
+    if budget < 1 or heads < 1:
+        raise InvalidArgument(f"{what}: no pages to select")
+    p = _decode_bytes(q, tokens, heads, 0, None, q_granularity, 0)
+    n = _lib().reef_kv_select_pages_workspace_bytes(p)
+    ws = torch.empty(n // 4 + 4, dtype=torch.int32, device=q.device)
+    chosen = torch.empty((B, heads, budget), dtype=torch.int32, device=q.device)
+    counts = torch.empty((B, heads), dtype=torch.int32, device=q.device)
+    own = status or StatusWord(q.device)
+    check(_lib().reef_kv_select_pages(
+        p, _ptr(q), _ptr(q_scales), _ptr(bounds), _ptr(bound_scales), table, blocks, pages,
+        _ptr(context_lens), budget, sinks, recent, _ptr(chosen), _ptr(counts), _ptr(ws), n,
+        _ptr(own.tensor), _stream()), what)
+    if status is None:
+        own.check(what)
+    return chosen, counts
 
 
 # --- integer-only attention (int8.hpp:156-279) -----------------------------------------

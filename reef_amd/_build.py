@@ -15,7 +15,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 SOURCES = ["quant.hip", "prefill.hip", "prefill_packed.hip", "prefill_cache.hip", "decode.hip",
            "kv_append.hip", "int_head.hip", "linear.hip", "norm.hip",
-           "kv_pages.hip", "tree.hip"]
+           "kv_pages.hip", "kv_select.hip", "tree.hip"]
 LIB = os.path.join(PKG, "libreef_hip.so")
 
 FLAGS = [

@@ -28,11 +28,11 @@ __device__ __forceinline__ void int8x16_to_f16(i32x4 w, f16x8 &lo, f16x8 &hi) {
     }
 }
 
-// A 16-byte load of the streamed cache; NT marks it non-temporal (read once: a
+// A vector load of the streamed cache; NT marks it non-temporal (read once: a
 // contiguous cache is not re-read within a step, and keeping it out of the caches
 // measured faster there).
-template <bool NT>
-__device__ __forceinline__ i32x4 load_stream(const i32x4 *p) {
+template <bool NT, typename V>
+__device__ __forceinline__ V load_stream(const V *p) {
     return NT ? __builtin_nontemporal_load(p) : *p;
 }
 

@@ -10,7 +10,10 @@
 // images, and the page then leaves in 16-byte stores, whole pages as they are
 // laid out in the cache (K [16, D], V transposed to [D, 16] on the way out: the
 // layout the decode kernel reads). The capacity check of attention.hpp:321-327 becomes a status
-// bit, since the lengths live on the device.
+// bit, since the lengths live on the device. The 4-bit cache takes the same rule with 7 for
+// 127: the images in LDS hold a code a byte either way, and two of them become a byte on the
+// way out.
+#include "kv_int4.hpp"
 #include "reef_common.hpp"
 
 namespace reef {
@@ -52,6 +55,47 @@ __device__ __forceinline__ uint32_t group_max_u32(uint32_t v) {
     return v;
 }
 
+// Slots [s_lo, s_hi) of the token-major images into a page of the 4-bit cache. A thread owns the
+// bytes that it writes: of a value channel's bytes that hold a new token and an earlier one it
+// keeps the earlier one's nibble.
+template <int D>
+__device__ __forceinline__ void store_int4(const int8_t *sK, const int8_t *sV, int s_lo, int s_hi,
+                                           int8_t *kpage, int8_t *vpage) {
+    constexpr int RB = D / 2;  // bytes of a key row
+    const int tid = threadIdx.x;
+    // Keys: 8 bytes a thread, channels c .. c + 7 and D/2 + c .. D/2 + c + 7 of one row.
+    if (tid < kPage * RB / 8) {
+        const int slot = tid / (RB / 8), c = tid % (RB / 8) * 8;
+        if (slot >= s_lo && slot < s_hi) {
+            const uint2 lo = *reinterpret_cast<const uint2 *>(sK + slot * D + c);
+            const uint2 hi = *reinterpret_cast<const uint2 *>(sK + slot * D + RB + c);
+            auto pack = [](uint32_t l, uint32_t h) {  // c + 8 of every byte: a 4-bit sum
+                return ((l ^ 0x08080808u) & 0x0f0f0f0fu) | ((h ^ 0x08080808u) & 0x0f0f0f0fu) << 4;
+            };
+            *reinterpret_cast<uint2 *>(kpage + slot * RB + c) =
+                make_uint2(pack(lo.x, hi.x), pack(lo.y, hi.y));
+        }
+    }
+    // Values: one channel's half of 8 tokens (4 bytes) a thread.
+    if (tid < 2 * D) {
+        const int ch = tid % D, half = tid / D;
+        uint32_t *dst = reinterpret_cast<uint32_t *>(vpage + ch * 8 + 4 * half);
+        uint32_t w = 0, fresh = 0;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            const int slot = 8 * half + kv_nibble_token(n);
+            if (slot >= s_lo && slot < s_hi) {
+                w |= (uint32_t)((sV[slot * D + ch] + kInt4Zero) & 0xf) << (4 * n);
+                fresh |= 0xfu << (4 * n);
+            }
+        }
+        if (fresh == 0xffffffffu)
+            *dst = w;
+        else if (fresh)
+            *dst = (*dst & ~fresh) | w;
+    }
+}
+
 // Each wave quantizes 8 rows of the page (quantize_rows, quant.hpp:112-133): waves 0
 // and 1 the keys of slots 0-7 and 8-15, waves 2 and 3 the values. A row is spread
 // over LPR = D / 8 lanes holding 8 consecutive channels each, so a wave takes
@@ -64,10 +108,12 @@ __device__ __forceinline__ uint32_t group_max_u32(uint32_t v) {
 // of the IEEE quotient. Unless y is within 2^-14 of a half-integer, rint(y) is the
 // engine's code. When any lane of the wave has such a value (rare: about 1.2e-4
 // per value), or a row is not finite or its scale is tiny, the wave redoes the
-// pass with IEEE divisions.
-template <int D, bool PAGED, bool VEC>
+// pass with IEEE divisions. (In 4 bits |t| is at most 7 (1 + 2^-24), and y nearer to it.)
+template <int D, int BITS, bool PAGED, bool VEC>
 __global__ __launch_bounds__(kAppendThreads) void kv_append(AppendArgs a) {
     constexpr int LPR = D / 8, RPW = kWave / LPR, PASSES = 8 / RPW;
+    constexpr float kMost = BITS == 8 ? 127.0f : kInt4Max;
+    constexpr int kPageBytes = kPage * D * BITS / 8;
     // Both images token-major ([slot][channel]): 8-byte code writes with no bank
     // conflicts. The value page is transposed to [channel][slot] as it is stored.
     __shared__ __attribute__((aligned(16))) int8_t sK[kPage * D];
@@ -143,7 +189,8 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append(AppendArgs a) {
         for (int j = 0; j < 8; ++j) m = m > mag(x[pass][j]) ? m : mag(x[pass][j]);
         m = group_max_u32<LPR>(m);
         const bool row_bad = m >= 0x7f800000u;
-        const float scale = int8_scale(__uint_as_float(m));
+        const float most = __uint_as_float(m);
+        const float scale = most > 0.0f ? most / kMost : 1.0f;
         const float rs = __builtin_amdgcn_rcpf(scale);
         bool near = row_bad || !(scale >= 0x1p-125f);
         float qf[8];
@@ -160,7 +207,7 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append(AppendArgs a) {
         uint32_t c[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float r = qf[j] < -127.0f ? -127.0f : (qf[j] > 127.0f ? 127.0f : qf[j]);
+            const float r = qf[j] < -kMost ? -kMost : (qf[j] > kMost ? kMost : qf[j]);
             c[j] = (uint32_t)(int32_t)r & 0xffu;
         }
         if (valid[pass]) {
@@ -173,8 +220,12 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append(AppendArgs a) {
     }
     if (bad) flag_status(a.status, REEF_STATUS_BIT_NON_FINITE);
     __syncthreads();
-    int8_t *kpage = a.k_dst + page_base * kPage * D;
-    int8_t *vpage = a.v_dst + page_base * D * kPage;
+    int8_t *kpage = a.k_dst + page_base * kPageBytes;
+    int8_t *vpage = a.v_dst + page_base * kPageBytes;
+    if constexpr (BITS == 4) {
+        store_int4<D>(sK, sV, p_lo - page_idx * kPage, p_hi - page_idx * kPage, kpage, vpage);
+        return;
+    }
     if (p_hi - p_lo == kPage) {
         // A whole page: threads [0, D) copy the key image in 16-byte chunks; thread
         // 128 + c gathers channel c's 16 slots of the value image (consecutive lanes
@@ -215,6 +266,53 @@ __global__ void advance_lengths(const int32_t *start, int32_t batch, int32_t new
     if (b >= batch) return;
     const int s = start[b];
     if (s >= 0 && s <= max_context - new_tokens) lens[b] = s + new_tokens;
+}
+
+// --- the 4-bit cache as fp32 rows ----------------------------------------------------------
+
+constexpr int kUnpackThreads = 256;
+constexpr int kUnpackPages = 4;  // pages a workgroup
+
+struct UnpackArgs {
+    const uint8_t *k, *v;
+    const float *ks, *vs;
+    float *k_out, *v_out;
+    int64_t pages;
+};
+
+// A thread turns four channels of a row into one 16-byte store, rows of a page in turn. Keys:
+// four bytes hold two such groups, half a row apart; each is read for its own nibble (the second
+// read hits the cache). Values: the four channels' bytes of the token.
+template <int D>
+__global__ __launch_bounds__(kUnpackThreads) void unpack_int4(UnpackArgs a) {
+    constexpr int CPR = D / 4, RB = D / 2;  // threads a row, bytes of a key row
+    constexpr int RPP = kUnpackThreads / CPR;  // rows at once
+    const int c = threadIdx.x % CPR * 4, r0 = threadIdx.x / CPR;
+    const int64_t row_begin = linear_block() * kUnpackPages * kPage;
+    const int64_t row_end = min(row_begin + kUnpackPages * kPage, a.pages * kPage);
+    for (int64_t row = row_begin + r0; row < row_end; row += RPP) {
+        if (a.k_out) {
+            const uint32_t w = *reinterpret_cast<const uint32_t *>(a.k + row * RB + c % RB);
+            const uint32_t u = c < RB ? low_nibbles(w) : high_nibbles(w);
+            const float s = a.ks[row];
+            f32x4 x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = (float)((int)((u >> (8 * i)) & 0xff) - kInt4Zero) * s;
+            *reinterpret_cast<f32x4 *>(a.k_out + row * D + c) = x;
+        }
+        if (a.v_out) {
+            const int64_t page = row / kPage;
+            const int n = kv_nibble((int)(row % kPage));
+            const float s = a.vs[row];
+            f32x4 x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t w = a.v[(page * D + c + i) * 8 + n / 2];
+                x[i] = (float)((int)((n & 1 ? w >> 4 : w) & 0xf) - kInt4Zero) * s;
+            }
+            *reinterpret_cast<f32x4 *>(a.v_out + row * D + c) = x;
+        }
+    }
 }
 
 reef_status prepare(const reef_kv_append_params *p, const float *k_new, const reef_strides *ks,
@@ -260,7 +358,19 @@ reef_status prepare(const reef_kv_append_params *p, const float *k_new, const re
     return REEF_OK;
 }
 
-template <bool PAGED>
+bool use_table(const reef_kv_append_params *p, const int32_t *block_table,
+               int64_t max_blocks_per_seq, int64_t num_pages, AppendArgs &a) {
+    if (!block_table || max_blocks_per_seq <= 0 || num_pages <= 0 ||
+        max_blocks_per_seq * kPage < p->max_context || num_pages >= (int64_t(1) << 31) ||
+        max_blocks_per_seq >= (int64_t(1) << 26))
+        return false;
+    a.table = block_table;
+    a.max_blocks = (int32_t)max_blocks_per_seq;
+    a.num_pages = (int32_t)num_pages;
+    return true;
+}
+
+template <int BITS, bool PAGED>
 reef_status launch(const reef_kv_append_params *p, AppendArgs &a, int32_t *context_lens,
                    uint32_t *status_word, hipStream_t stream) {
     a.status = status_word;
@@ -276,13 +386,13 @@ reef_status launch(const reef_kv_append_params *p, AppendArgs &a, int32_t *conte
     // 16-byte row loads when every new row starts 16-byte aligned
     const bool vec = aligned(a.k, 16) && aligned(a.v, 16) && a.k_sb % 4 == 0 && a.k_sh % 4 == 0 &&
                      a.k_st % 4 == 0 && a.v_sb % 4 == 0 && a.v_sh % 4 == 0 && a.v_st % 4 == 0;
-    if (p->head_dim == 128) {
-        if (vec) hipLaunchKernelGGL((kv_append<128, PAGED, true>), grid, dim3(kAppendThreads), 0, stream, a);
-        else hipLaunchKernelGGL((kv_append<128, PAGED, false>), grid, dim3(kAppendThreads), 0, stream, a);
-    } else {
-        if (vec) hipLaunchKernelGGL((kv_append<64, PAGED, true>), grid, dim3(kAppendThreads), 0, stream, a);
-        else hipLaunchKernelGGL((kv_append<64, PAGED, false>), grid, dim3(kAppendThreads), 0, stream, a);
-    }
+    const auto run = [&](auto *kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(kAppendThreads), 0, stream, a);
+    };
+    if (p->head_dim == 128)
+        run(vec ? kv_append<128, BITS, PAGED, true> : kv_append<128, BITS, PAGED, false>);
+    else
+        run(vec ? kv_append<64, BITS, PAGED, true> : kv_append<64, BITS, PAGED, false>);
     if (hipGetLastError() != hipSuccess) return REEF_HIP_ERROR;
     if (in_place) {
         hipLaunchKernelGGL(advance_lengths, dim3((unsigned)ceil_div(p->batch, 256)), dim3(256), 0,
@@ -307,7 +417,7 @@ extern "C" reef_status reef_kv_append_int8(const reef_kv_append_params *p, const
     const reef_status s = prepare(p, k_new, k_strides, v_new, v_strides, start_positions, k_cache,
                                   v_cache, k_scales, v_scales, a);
     if (s != REEF_OK) return s;
-    return launch<false>(p, a, context_lens, status_word, stream);
+    return launch<8, false>(p, a, context_lens, status_word, stream);
 }
 
 extern "C" reef_status reef_kv_append_int8_paged(
@@ -320,12 +430,43 @@ extern "C" reef_status reef_kv_append_int8_paged(
     const reef_status s = prepare(p, k_new, k_strides, v_new, v_strides, start_positions, k_pages,
                                   v_pages, k_scale_pages, v_scale_pages, a);
     if (s != REEF_OK) return s;
-    if (!block_table || max_blocks_per_seq <= 0 || num_pages <= 0 ||
-        max_blocks_per_seq * kPage < p->max_context || num_pages >= (int64_t(1) << 31) ||
-        max_blocks_per_seq >= (int64_t(1) << 26))
+    if (!use_table(p, block_table, max_blocks_per_seq, num_pages, a)) return REEF_INVALID_ARGUMENT;
+    return launch<8, true>(p, a, context_lens, status_word, stream);
+}
+
+extern "C" reef_status reef_kv_append_int4(const reef_kv_append_params *p, const float *k_new,
+                                           const reef_strides *k_strides, const float *v_new,
+                                           const reef_strides *v_strides,
+                                           const int32_t *start_positions,
+                                           const int32_t *block_table, int64_t max_blocks_per_seq,
+                                           int64_t num_pages, uint8_t *k_cache, uint8_t *v_cache,
+                                           float *k_scales, float *v_scales,
+                                           int32_t *context_lens, uint32_t *status_word,
+                                           hipStream_t stream) {
+    AppendArgs a;
+    const reef_status s = prepare(p, k_new, k_strides, v_new, v_strides, start_positions, k_cache,
+                                  v_cache, k_scales, v_scales, a);
+    if (s != REEF_OK) return s;
+    if (!aligned(k_cache, 8) || !aligned(v_cache, 8)) return REEF_INVALID_ARGUMENT;
+    if (!block_table) return launch<4, false>(p, a, context_lens, status_word, stream);
+    if (!use_table(p, block_table, max_blocks_per_seq, num_pages, a)) return REEF_INVALID_ARGUMENT;
+    return launch<4, true>(p, a, context_lens, status_word, stream);
+}
+
+extern "C" reef_status reef_kv_unpack_int4(const uint8_t *k_pages, const uint8_t *v_pages,
+                                           const float *k_scales, const float *v_scales,
+                                           int64_t pages, int64_t head_dim, float *k, float *v,
+                                           hipStream_t stream) {
+    if (pages <= 0 || head_dim <= 0 || (!k && !v) || (k && (!k_pages || !k_scales)) ||
+        (v && (!v_pages || !v_scales)) || !aligned(k_pages, 16) || !aligned(v_pages, 16) ||
+        !aligned(k, 16) || !aligned(v, 16) || !aligned(k_scales, 4) || !aligned(v_scales, 4))
         return REEF_INVALID_ARGUMENT;
-    a.table = block_table;
-    a.max_blocks = (int32_t)max_blocks_per_seq;
-    a.num_pages = (int32_t)num_pages;
-    return launch<true>(p, a, context_lens, status_word, stream);
+    if ((head_dim != 64 && head_dim != 128) || pages >= (int64_t(1) << 40)) return REEF_UNSUPPORTED;
+    const UnpackArgs a{k_pages, v_pages, k_scales, v_scales, k, v, pages};
+    const dim3 grid = linear_grid(ceil_div(pages, kUnpackPages));
+    if (head_dim == 128)
+        hipLaunchKernelGGL(unpack_int4<128>, grid, dim3(kUnpackThreads), 0, stream, a);
+    else
+        hipLaunchKernelGGL(unpack_int4<64>, grid, dim3(kUnpackThreads), 0, stream, a);
+    return launch_status();
 }

@@ -655,11 +655,13 @@ extern "C" reef_status reef_kv_compact(int32_t *block_table, int64_t max_blocks_
     return launch_status();
 }
 
-extern "C" reef_status reef_kv_copy_pages(const int32_t *src, const int32_t *dst, int64_t n,
-                                          int64_t kv_heads, int64_t head_dim, int8_t *k_pages,
-                                          int8_t *v_pages, float *k_scale_pages,
-                                          float *v_scale_pages, int64_t num_pages,
-                                          uint32_t *status_word, hipStream_t stream) {
+namespace {
+
+// Pools of `row_bytes` bytes a key row: 16 of them a head's page, and as many value bytes.
+reef_status copy(const int32_t *src, const int32_t *dst, int64_t n, int64_t kv_heads,
+                 int64_t head_dim, int64_t row_bytes, void *k_pages, void *v_pages,
+                 float *k_scale_pages, float *v_scale_pages, int64_t num_pages,
+                 uint32_t *status_word, hipStream_t stream) {
     if (!src || !dst || n <= 0 || kv_heads <= 0 || head_dim <= 0 || num_pages <= 0 || !k_pages ||
         !v_pages || !k_scale_pages || !v_scale_pages || !aligned(k_pages, 16) ||
         !aligned(v_pages, 16) || !aligned(k_scale_pages, 16) || !aligned(v_scale_pages, 16))
@@ -671,16 +673,37 @@ extern "C" reef_status reef_kv_copy_pages(const int32_t *src, const int32_t *dst
     a.src = src;
     a.dst = dst;
     a.pairs = n;
-    a.pages[0] = k_pages;
-    a.pages[1] = v_pages;
+    a.pages[0] = static_cast<int8_t *>(k_pages);
+    a.pages[1] = static_cast<int8_t *>(v_pages);
     a.scales[0] = k_scale_pages;
     a.scales[1] = v_scale_pages;
-    a.page_words = (int32_t)(kv_heads * head_dim);  // 16 rows of head_dim bytes a head
+    a.page_words = (int32_t)(kv_heads * row_bytes);  // 16 rows of row_bytes a head
     a.scale_words = (int32_t)(kv_heads * 4);        // 16 floats a head
     a.num_pages = (int32_t)num_pages;
     a.status = status_word;
     hipLaunchKernelGGL(copy_pages, linear_grid(n, 2), dim3(kCopyThreads), 0, stream, a);
     return launch_status();
+}
+
+}  // namespace
+
+extern "C" reef_status reef_kv_copy_pages(const int32_t *src, const int32_t *dst, int64_t n,
+                                          int64_t kv_heads, int64_t head_dim, int8_t *k_pages,
+                                          int8_t *v_pages, float *k_scale_pages,
+                                          float *v_scale_pages, int64_t num_pages,
+                                          uint32_t *status_word, hipStream_t stream) {
+    return copy(src, dst, n, kv_heads, head_dim, head_dim, k_pages, v_pages, k_scale_pages,
+                v_scale_pages, num_pages, status_word, stream);
+}
+
+extern "C" reef_status reef_kv_copy_pages_int4(const int32_t *src, const int32_t *dst, int64_t n,
+                                               int64_t kv_heads, int64_t head_dim,
+                                               uint8_t *k_pages, uint8_t *v_pages,
+                                               float *k_scale_pages, float *v_scale_pages,
+                                               int64_t num_pages, uint32_t *status_word,
+                                               hipStream_t stream) {
+    return copy(src, dst, n, kv_heads, head_dim, head_dim / 2, k_pages, v_pages, k_scale_pages,
+                v_scale_pages, num_pages, status_word, stream);
 }
 
 extern "C" reef_status reef_kv_keep_int8(const reef_kv_append_params *p, const int32_t *kept,

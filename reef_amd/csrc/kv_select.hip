@@ -1,0 +1,472 @@
+// Pages that a query selects (gfx950): bounds of every page's keys, a query's scores against
+// them, and the best `budget` pages of each (sequence, kv head), for the decode step over a list
+// of pages (decode.hip).
+//
+// A page's bounds are the largest and the least key of each channel, hi and lo, as int8 codes of
+// one scale S a page, rounded outwards. For any key x of the page and a query q,
+//   q . x = sum_d q_d x_d <= S * sum_d (max(q_d, 0) hi_d + min(q_d, 0) lo_d),
+// with codes of q a product of [max(q, 0), min(q, 0)] and [hi, lo], 2 D long: int8 matrix
+// instructions, exact. A page costs 2 D + 4 bytes to score, 1/16 of its int8 keys and values.
+#include <algorithm>
+
+#include "kv_int4.hpp"
+#include "reef_common.hpp"
+
+namespace reef {
+namespace {
+
+// --- bounds --------------------------------------------------------------------------------
+
+constexpr int kBoundWaves = 4;  // waves (one page each) of a workgroup
+
+struct BoundArgs {
+    const uint8_t *k;
+    const float *ks;
+    const int32_t *start;
+    const int32_t *table;  // paged only
+    int8_t *bounds;
+    float *scales;
+    int32_t kv_heads, new_tokens, max_context, max_blocks, num_pages;
+    uint32_t *status;
+};
+
+// One wave takes a page. A lane reads 4 bytes (BITS 8: four channels; 4: four of either half of
+// the row) of every R-th token's row, so that a load covers 256 bytes in order, and keeps their
+// extremes. Lanes that hold the same channels then meet: over 32 lanes one side keeps the
+// largest, the other the least; in 4 bits over 16 lanes either keeps one half of the row; what
+// copies are left combine. Each lane ends with four codes of one bound.
+template <int D, int BITS>
+__global__ __launch_bounds__(kBoundWaves * kWave) void page_bounds(BoundArgs a) {
+    constexpr int RB = D * BITS / 8;      // bytes of a row
+    constexpr int LPR = RB / 4;           // lanes a row
+    constexpr int R = kWave / LPR;        // rows of a load
+    constexpr int C = BITS == 8 ? 4 : 8;  // channels of a lane
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int b = blockIdx.z, kvh = blockIdx.y;
+    const int start = a.start[b];
+    if (start < 0 || start > a.max_context - a.new_tokens) {
+        if (blockIdx.x == 0 && kvh == 0 && threadIdx.x == 0)
+            flag_status(a.status, start < 0 ? REEF_STATUS_BIT_BAD_LENGTH : REEF_STATUS_BIT_CAPACITY);
+        return;
+    }
+    const int end = start + a.new_tokens;
+    const int page_idx = start / kPage + (int)blockIdx.x * kBoundWaves + wave;
+    if (page_idx * kPage >= end) return;
+    int64_t slot;  // index of this (page, kv head)
+    if (a.table) {
+        const int page = a.table[(int64_t)b * a.max_blocks + page_idx];
+        if (page < 0 || page >= a.num_pages) {
+            if (lane == 0) flag_status(a.status, REEF_STATUS_BIT_BAD_PAGE);
+            return;
+        }
+        slot = (int64_t)page * a.kv_heads + kvh;
+    } else {
+        slot = ((int64_t)b * a.kv_heads + kvh) * (a.max_context / kPage) + page_idx;
+    }
+    const int live = min(kPage, end - page_idx * kPage);
+    const int j = lane % LPR, g = lane / LPR;
+    const uint8_t *rows = a.k + slot * (kPage * RB);
+    const float *ks = a.ks + slot * kPage;
+    uint32_t w[kPage / R];
+    float s[kPage / R];
+#pragma unroll
+    for (int i = 0; i < kPage / R; ++i) {
+        w[i] = *reinterpret_cast<const uint32_t *>(rows + (i * R + g) * RB + 4 * j);
+        s[i] = ks[i * R + g];
+    }
+    float hi[C], lo[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        hi[c] = -INFINITY;
+        lo[c] = INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < kPage / R; ++i) {
+        const bool in = i * R + g < live;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int code = BITS == 8 ? (int)(int8_t)(w[i] >> (8 * c))
+                                       : (int)((w[i] >> (8 * (c % 4) + 4 * (c / 4))) & 0xf) - kInt4Zero;
+            const float x = (float)code * s[i];
+            hi[c] = in ? fmaxf(hi[c], x) : hi[c];
+            lo[c] = in ? fminf(lo[c], x) : lo[c];
+        }
+    }
+    // Lanes 0-31 go on with the largest, the others with the least, negated: maxima either way.
+    const bool least = lane >= 32;
+    float m[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const float got = __shfl_xor(least ? hi[c] : -lo[c], 32);
+        m[c] = fmaxf(least ? -lo[c] : hi[c], got);
+    }
+    float n[4];
+    const bool upper = BITS == 4 && (lane & 16);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        if constexpr (BITS == 4) {
+            const float got = __shfl_xor(upper ? m[c] : m[C - 4 + c], 16);
+            n[c] = fmaxf(upper ? m[C - 4 + c] : m[c], got);
+        } else {
+            n[c] = m[c];
+        }
+    }
+    constexpr int kSplit = BITS == 4 ? 16 : 32;  // lanes of one bound (and half)
+#pragma unroll
+    for (int o = LPR; o < kSplit; o <<= 1)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) n[c] = fmaxf(n[c], __shfl_xor(n[c], o));
+    const float top = wave_max(fmaxf(fmaxf(n[0], n[1]), fmaxf(n[2], n[3])));
+    const float scale = int8_scale(top);
+    uint32_t packed = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        // ceil(hi / S), or -floor(lo / S) = ceil(-lo / S), rounded outwards
+        const float code = fminf(__builtin_ceilf(n[c] / scale), 127.0f);
+        packed |= ((uint32_t)(int)(least ? -code : code) & 0xffu) << (8 * c);
+    }
+    if (lane % kSplit < LPR)
+        *reinterpret_cast<uint32_t *>(a.bounds + slot * 2 * D + (least ? D : 0) +
+                                      (upper ? D / 2 : 0) + 4 * j) = packed;
+    if (lane == 0) a.scales[slot] = scale;
+}
+
+template <int BITS>
+reef_status launch_bounds(const reef_kv_append_params *p, const int32_t *start, const void *k,
+                          const float *ks, const int32_t *block_table, int64_t max_blocks_per_seq,
+                          int64_t num_pages, int8_t *bounds, float *bound_scales,
+                          uint32_t *status_word, hipStream_t stream) {
+    if (!p || !start || !k || !ks || !bounds || !bound_scales || p->batch <= 0 ||
+        p->kv_heads <= 0 || p->head_dim <= 0 || p->new_tokens <= 0 || p->max_context <= 0 ||
+        p->max_context % kPage != 0)
+        return REEF_INVALID_ARGUMENT;
+    if (p->new_tokens > p->max_context) return REEF_CAPACITY;
+    const int64_t groups = ceil_div(ceil_div(p->new_tokens, kPage) + 1, kBoundWaves);
+    if ((p->head_dim != 64 && p->head_dim != 128) || p->max_context >= (int64_t(1) << 30) ||
+        p->batch > 65535 || p->kv_heads > 65535 || groups > kGridMost256)
+        return REEF_UNSUPPORTED;
+    if (!aligned(k, 16) || !aligned(ks, 4) || !aligned(bounds, 16) || !aligned(bound_scales, 4))
+        return REEF_INVALID_ARGUMENT;
+    if (block_table && (max_blocks_per_seq <= 0 || num_pages <= 0 ||
+                        max_blocks_per_seq * kPage < p->max_context ||
+                        num_pages >= (int64_t(1) << 31) ||
+                        max_blocks_per_seq >= (int64_t(1) << 26)))
+        return REEF_INVALID_ARGUMENT;
+    BoundArgs a;
+    a.k = static_cast<const uint8_t *>(k);
+    a.ks = ks;
+    a.start = start;
+    a.table = block_table;
+    a.bounds = bounds;
+    a.scales = bound_scales;
+    a.kv_heads = (int32_t)p->kv_heads;
+    a.new_tokens = (int32_t)p->new_tokens;
+    a.max_context = (int32_t)p->max_context;
+    a.max_blocks = (int32_t)(block_table ? max_blocks_per_seq : 0);
+    a.num_pages = (int32_t)(block_table ? num_pages : 0);
+    a.status = status_word;
+    const dim3 grid((unsigned)groups, (unsigned)p->kv_heads, (unsigned)p->batch);
+    if (p->head_dim == 128)
+        hipLaunchKernelGGL((page_bounds<128, BITS>), grid, dim3(kBoundWaves * kWave), 0, stream, a);
+    else
+        hipLaunchKernelGGL((page_bounds<64, BITS>), grid, dim3(kBoundWaves * kWave), 0, stream, a);
+    return launch_status();
+}
+
+// --- selection -------------------------------------------------------------------------------
+
+constexpr int kScoreWaves = 4;     // waves of a scoring workgroup, 64 pages each
+constexpr int kPickThreads = 1024; // of a selecting workgroup
+constexpr int kPickWaves = kPickThreads / kWave;
+// A page's place in the order, larger is better: scores as unsigned words in their order, and
+// beyond them the pages that are always taken and those that cannot be.
+constexpr uint32_t kAlways = 0xffffffffu, kNever = 0;
+
+struct SelectArgs {
+    const int8_t *q;
+    const float *qs;
+    const int8_t *bounds;
+    const float *scales;
+    const int32_t *table;  // paged only
+    const int32_t *lens;
+    uint32_t *keys;  // [items, max_pages]
+    int32_t *pages, *counts;
+    uint32_t *status;
+    int32_t q_heads, kv_heads, group, items;
+    int32_t max_context, max_pages;  // max_pages = max_context / 16
+    int32_t max_blocks, num_pages;
+    int32_t budget, sinks, recent, q_gran;
+};
+
+__device__ __forceinline__ uint32_t score_key(float score) {
+    const uint32_t u = __float_as_uint(score + 0.0f);  // (-0 is 0)
+    const uint32_t k = u & 0x80000000u ? ~u : u | 0x80000000u;
+    return k < 1 ? 1 : k;
+}
+
+// Bytes of a word above and below zero.
+__device__ __forceinline__ void split_signs(uint32_t w, uint32_t &above, uint32_t &below) {
+    const uint32_t negative = ((w >> 7) & 0x01010101u) * 0xffu;
+    above = w & ~negative;
+    below = w & negative;
+}
+
+__device__ __forceinline__ int item_pages(const SelectArgs &a, int b) {
+    const int len = a.lens[b];
+    return len < 1 || len > a.max_context ? 0 : (len + kPage - 1) / kPage;
+}
+
+// Keys of 64 pages a wave: four 16-page x 16-head products. The bounds' rows are the columns of
+// the product (lane % 16), so the group's heads lie in a lane's four registers and over lane
+// groups, and lane group t ends with tile t's pages: one key a lane, in page order.
+template <int D>
+__global__ __launch_bounds__(kScoreWaves * kWave) void score_pages(SelectArgs a) {
+    constexpr int S = 2 * D / 64;  // slices of a row of bounds
+    const int lane = threadIdx.x & (kWave - 1), col = lane & 15, grp = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int item = blockIdx.y, b = item / a.kv_heads, kvh = item - b * a.kv_heads;
+    const int n = item_pages(a, b);
+    const int first = ((int)blockIdx.x * kScoreWaves + wave) * kWave;
+    if (first >= n) return;
+    const int page_idx = min(first + lane, n - 1);
+    int page = page_idx;
+    bool ok = true;
+    int64_t base = (int64_t)item * a.max_pages, step = 1;  // row of bounds of page 0, between pages
+    if (a.table) {
+        page = a.table[(int64_t)b * a.max_blocks + page_idx];
+        ok = page >= 0 && page < a.num_pages;
+        if (!ok) page = 0;
+        base = kvh;
+        step = a.kv_heads;
+    }
+    if (!ok) flag_status(a.status, REEF_STATUS_BIT_BAD_PAGE);
+    uint32_t key = kAlways;
+    if (n > a.budget) {
+        i32x4 x[4][S];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int8_t *row = a.bounds + (base + __shfl(page, 16 * t + col) * step) * (2 * D);
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+                x[t][s] = *reinterpret_cast<const i32x4 *>(row + 64 * s + 16 * grp);
+        }
+        const float scale = a.scales[base + page * step];
+        // The heads' operands: lane % 16 is the head, its slices [above, below].
+        i32x4 q[S];
+        const bool head_ok = col < a.group;
+        const int8_t *qrow = a.q + ((int64_t)b * a.q_heads + kvh * a.group + (head_ok ? col : 0)) * D;
+#pragma unroll
+        for (int s = 0; s < S / 2; ++s) {
+            const i32x4 w = *reinterpret_cast<const i32x4 *>(qrow + 64 * s + 16 * grp);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t above, below;
+                split_signs(head_ok ? (uint32_t)w[i] : 0u, above, below);
+                q[s][i] = (int)above;
+                q[S / 2 + s][i] = (int)below;
+            }
+        }
+        float qs[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int head = kvh * a.group + min(4 * grp + i, a.group - 1);  // (dead ones repeat one)
+            qs[i] = a.q_gran == REEF_SCALE_PER_TENSOR ? a.qs[0]
+                    : a.q_gran == REEF_SCALE_PER_HEAD ? a.qs[head]
+                                                      : a.qs[(int64_t)b * a.q_heads + head];
+        }
+        float best = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            i32x4 sum = {0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < S; ++s) sum = mfma_16x16x64_i8(q[s], x[t][s], sum);
+            const float ps = __shfl(scale, 16 * t + col);
+            float most = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (4 * grp + i < a.group) most = fmaxf(most, (float)sum[i] * (qs[i] * ps));
+            most = fmaxf(most, __shfl_xor(most, 16));
+            most = fmaxf(most, __shfl_xor(most, 32));
+            if (grp == t) best = most;
+        }
+        const bool always = page_idx < a.sinks || page_idx >= n - a.recent;
+        key = always ? kAlways : score_key(best);
+    }
+    if (!ok) key = kNever;
+    if (first + lane < n) a.keys[(int64_t)item * a.max_pages + first + lane] = key;
+}
+
+// Sums of two counts over the workgroup's waves, and over those before this one (through LDS).
+struct PickCounts {
+    int before0, before1, total0, total1;
+};
+__device__ __forceinline__ PickCounts pick_counts(int c0, int c1, int2 *sC, int wave, int lane) {
+    __syncthreads();
+    if (lane == 0) sC[wave] = make_int2(c0, c1);
+    __syncthreads();
+    PickCounts r = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < kPickWaves; ++w) {
+        const int2 x = sC[w];
+        if (w < wave) {
+            r.before0 += x.x;
+            r.before1 += x.y;
+        }
+        r.total0 += x.x;
+        r.total1 += x.y;
+    }
+    return r;
+}
+
+// One workgroup an item: the budget-th largest key bit by bit (the largest T that at least
+// budget keys reach), then the pages above it and the first of those at it, in page order. Wave w
+// holds a run of pages, 64 at a time.
+__global__ __launch_bounds__(kPickThreads) void pick_pages(SelectArgs a) {
+    __shared__ int2 sC[kPickWaves];
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int item = blockIdx.x, b = item / a.kv_heads;
+    const int n = item_pages(a, b);
+    int32_t *list = a.pages + (int64_t)item * a.budget;
+    if (n == 0 && threadIdx.x == 0 && item == b * a.kv_heads)
+        flag_status(a.status, REEF_STATUS_BIT_BAD_LENGTH);
+    const uint32_t *keys = a.keys + (int64_t)item * a.max_pages;
+    const int rounds = (n + kPickThreads - 1) / kPickThreads;
+    const int first = wave * rounds * kWave;
+    auto key_at = [&](int r) {
+        const int i = first + r * kWave + lane;
+        return i < n ? keys[i] : kNever;
+    };
+    // the number of keys at or above t, at most the budget of them needed
+    uint32_t t = kNever;
+    for (int bit = 31; bit >= 0 && n > a.budget; --bit) {
+        const uint32_t trial = t | (1u << bit);
+        int c = 0;
+        for (int r = 0; r < rounds; ++r)
+            c += __popcll(__builtin_amdgcn_ballot_w64(key_at(r) >= trial));
+        if (pick_counts(c, 0, sC, wave, lane).total0 >= a.budget) t = trial;
+    }
+    // above the last key, and at it (a page that cannot be taken never is)
+    int above = 0, at = 0;
+    for (int r = 0; r < rounds; ++r) {
+        const uint32_t key = key_at(r);
+        above += __popcll(__builtin_amdgcn_ballot_w64(key > t));
+        at += __popcll(__builtin_amdgcn_ballot_w64(key == t && key != kNever));
+    }
+    const PickCounts c = pick_counts(above, at, sC, wave, lane);
+    const int need = min(a.budget - c.total0, c.total1);  // of those at it
+    int out = c.before0 + min(c.before1, need), ties = c.before1;
+    const uint64_t below = (uint64_t(1) << lane) - 1;
+    for (int r = 0; r < rounds; ++r) {
+        const uint32_t key = key_at(r);
+        const uint64_t eq = __builtin_amdgcn_ballot_w64(key == t && key != kNever);
+        const bool take = key > t || ((eq >> lane & 1) && ties + __popcll(eq & below) < need);
+        const uint64_t taken = __builtin_amdgcn_ballot_w64(take);
+        if (take) list[out + __popcll(taken & below)] = first + r * kWave + lane;
+        out += __popcll(taken);
+        ties += __popcll(eq);
+    }
+    const int count = c.total0 + need;
+    for (int i = count + threadIdx.x; i < a.budget; i += kPickThreads) list[i] = -1;
+    if (threadIdx.x == 0) a.counts[item] = count;
+}
+
+bool select_sizes(const reef_decode_params *p) {
+    return p && p->batch > 0 && p->q_heads > 0 && p->kv_heads > 0 && p->max_context > 0 &&
+           p->max_context % kPage == 0 && p->q_heads % p->kv_heads == 0;
+}
+
+}  // namespace
+}  // namespace reef
+
+using namespace reef;
+
+extern "C" reef_status reef_kv_page_bounds_int8(const reef_kv_append_params *p,
+                                                const int32_t *start_positions,
+                                                const int8_t *k_cache, const float *k_scales,
+                                                const int32_t *block_table,
+                                                int64_t max_blocks_per_seq, int64_t num_pages,
+                                                int8_t *bounds, float *bound_scales,
+                                                uint32_t *status_word, hipStream_t stream) {
+    return launch_bounds<8>(p, start_positions, k_cache, k_scales, block_table, max_blocks_per_seq,
+                            num_pages, bounds, bound_scales, status_word, stream);
+}
+
+extern "C" reef_status reef_kv_page_bounds_int4(const reef_kv_append_params *p,
+                                                const int32_t *start_positions,
+                                                const uint8_t *k_cache, const float *k_scales,
+                                                const int32_t *block_table,
+                                                int64_t max_blocks_per_seq, int64_t num_pages,
+                                                int8_t *bounds, float *bound_scales,
+                                                uint32_t *status_word, hipStream_t stream) {
+    return launch_bounds<4>(p, start_positions, k_cache, k_scales, block_table, max_blocks_per_seq,
+                            num_pages, bounds, bound_scales, status_word, stream);
+}
+
+extern "C" size_t reef_kv_select_pages_workspace_bytes(const reef_decode_params *p) {
+    if (!select_sizes(p) || p->batch * p->kv_heads > 65535 || p->max_context >= (int64_t(1) << 30))
+        return 0;
+    return (size_t)(p->batch * p->kv_heads * (p->max_context / kPage) * 4);
+}
+
+extern "C" reef_status reef_kv_select_pages(
+    const reef_decode_params *p, const int8_t *q, const float *q_scales, const int8_t *bounds,
+    const float *bound_scales, const int32_t *block_table, int64_t max_blocks_per_seq,
+    int64_t num_pages, const int32_t *context_lens, int64_t budget, int64_t sinks, int64_t recent,
+    int32_t *pages, int32_t *counts, void *workspace, size_t workspace_bytes,
+    uint32_t *status_word, hipStream_t stream) {
+    if (!select_sizes(p) || !q || !q_scales || !bounds || !bound_scales || !context_lens ||
+        !pages || !counts ||
+        (p->q_granularity != REEF_SCALE_PER_TENSOR && p->q_granularity != REEF_SCALE_PER_HEAD &&
+         p->q_granularity != REEF_SCALE_PER_TOKEN))
+        return REEF_INVALID_ARGUMENT;
+    if (sinks < 0 || recent < 1 || budget < 1 || sinks > budget || recent > budget - sinks)
+        return REEF_INVALID_ARGUMENT;
+    if ((p->head_dim != 64 && p->head_dim != 128) || p->q_heads / p->kv_heads > 16 ||
+        p->batch > 65535 || p->kv_heads > 65535 || p->batch * p->kv_heads > 65535 ||
+        p->max_context >= (int64_t(1) << 30) || budget >= (int64_t(1) << 26))
+        return REEF_UNSUPPORTED;
+    if (!aligned(q, 16) || !aligned(q_scales, 4) || !aligned(bounds, 16) ||
+        !aligned(bound_scales, 4) || !aligned(context_lens, 4) || !aligned(pages, 4) ||
+        !aligned(counts, 4))
+        return REEF_INVALID_ARGUMENT;
+    if (block_table && (num_pages <= 0 || num_pages >= (int64_t(1) << 31) ||
+                        max_blocks_per_seq <= 0 || max_blocks_per_seq * kPage < p->max_context ||
+                        max_blocks_per_seq >= (int64_t(1) << 30)))
+        return REEF_INVALID_ARGUMENT;
+    if (!workspace || !aligned(workspace, 16) ||
+        workspace_bytes < reef_kv_select_pages_workspace_bytes(p))
+        return REEF_INVALID_ARGUMENT;
+    SelectArgs a;
+    a.q = q;
+    a.qs = q_scales;
+    a.bounds = bounds;
+    a.scales = bound_scales;
+    a.table = block_table;
+    a.lens = context_lens;
+    a.keys = static_cast<uint32_t *>(workspace);
+    a.pages = pages;
+    a.counts = counts;
+    a.status = status_word;
+    a.q_heads = (int32_t)p->q_heads;
+    a.kv_heads = (int32_t)p->kv_heads;
+    a.group = (int32_t)(p->q_heads / p->kv_heads);
+    a.items = (int32_t)(p->batch * p->kv_heads);
+    a.max_context = (int32_t)p->max_context;
+    a.max_pages = (int32_t)(p->max_context / kPage);
+    a.max_blocks = (int32_t)(block_table ? max_blocks_per_seq : 0);
+    a.num_pages = (int32_t)(block_table ? num_pages : 0);
+    a.budget = (int32_t)budget;
+    a.sinks = (int32_t)sinks;
+    a.recent = (int32_t)recent;
+    a.q_gran = p->q_granularity;
+    const dim3 grid((unsigned)ceil_div(a.max_pages, kScoreWaves * kWave), (unsigned)a.items);
+    if (p->head_dim == 128)
+        hipLaunchKernelGGL(score_pages<128>, grid, dim3(kScoreWaves * kWave), 0, stream, a);
+    else
+        hipLaunchKernelGGL(score_pages<64>, grid, dim3(kScoreWaves * kWave), 0, stream, a);
+    if (hipGetLastError() != hipSuccess) return REEF_HIP_ERROR;
+    hipLaunchKernelGGL(pick_pages, dim3((unsigned)a.items), dim3(kPickThreads), 0, stream, a);
+    return launch_status();
+}

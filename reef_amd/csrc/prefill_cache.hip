@@ -12,7 +12,10 @@
 // runs over them with per-token K/V scales, on the balanced schedule when the
 // chunk has fewer 128-row query tiles than the GPU has compute units (its
 // workspace is the first part of this one). The gather moves 2 (D + 4) bytes per
-// cached token and kv head each way, small beside the chunk's attention.
+// cached token and kv head each way, small beside the chunk's attention. Of a cache held in 4
+// bits it reads D + 8 and widens the codes to the same rows: the prefill's int8 products then
+// see exactly the codes that decode sees.
+#include "kv_int4.hpp"
 #include "reef_common.hpp"
 
 namespace reef {
@@ -36,9 +39,10 @@ struct GatherArgs {
 // One workgroup per (cache page, sequence x kv head): the page's live tokens (the
 // first kv_len of the sequence) move to the token-major rows. A page number
 // outside [0, num_pages) sets BAD_PAGE and yields zero codes and scales.
-template <int D>
+template <int D, int BITS>
 __global__ __launch_bounds__(kGatherThreads) void gather_cache(GatherArgs a) {
     constexpr int CH = D / 16;  // 16-byte chunks per row
+    constexpr int RB = D * BITS / 8;  // bytes of a cached key row
     __shared__ int8_t sT[kPage][D];
     const int pg = blockIdx.x;
     const int item = blockIdx.y;  // b * kv_heads + kvh
@@ -55,14 +59,14 @@ __global__ __launch_bounds__(kGatherThreads) void gather_cache(GatherArgs a) {
         ok = page >= 0 && page < a.num_pages;
         if (!ok) page = 0;
         const int64_t slot = (int64_t)page * a.kv_heads + kvh;
-        kp = a.k + slot * (kPage * D);
-        vp = a.v + slot * (kPage * D);
+        kp = a.k + slot * (kPage * RB);
+        vp = a.v + slot * (kPage * RB);
         ksp = a.ks + slot * kPage;
         vsp = a.vs + slot * kPage;
     } else {
         const int64_t tok = (int64_t)item * a.max_context + t0;
-        kp = a.k + tok * D;
-        vp = a.v + tok * D;  // the [D, 16] pages of a sequence are contiguous in order
+        kp = a.k + tok * RB;
+        vp = a.v + tok * RB;  // the pages of a sequence are contiguous in order
         ksp = a.ks + tok;
         vsp = a.vs + tok;
     }
@@ -73,14 +77,32 @@ __global__ __launch_bounds__(kGatherThreads) void gather_cache(GatherArgs a) {
     if (tid < kPage * CH) {
         const int r = tid / CH, c = tid % CH;
         if (r < n) {
-            const i32x4 w = ok ? *reinterpret_cast<const i32x4 *>(kp + r * D + 16 * c)
-                               : i32x4{0, 0, 0, 0};
+            // (4 bits: chunk c of the lower half is the low nibbles of source chunk c, of the
+            // upper half the high ones of c - CH / 2)
+            const int src = BITS == 8 ? c : c % (CH / 2);
+            i32x4 w = ok ? *reinterpret_cast<const i32x4 *>(kp + r * RB + 16 * src)
+                         : i32x4{0, 0, 0, 0};
+            if (BITS == 4 && ok) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    w[i] = (int)nibbles_to_int8(src == c ? low_nibbles((uint32_t)w[i])
+                                                         : high_nibbles((uint32_t)w[i]));
+            }
             *reinterpret_cast<i32x4 *>(a.k_out + (row0 + r) * D + 16 * c) = w;
         }
     }
-    // Values: channel d's 16 tokens are one 16-byte row of the page; through LDS
-    // to token-major rows.
-    if (tid < D) {
+    // Values: channel d's 16 tokens are one row of the page; through LDS to token-major rows.
+    if constexpr (BITS == 4) {
+        if (tid < D) {
+            const i32x2 w = ok ? *reinterpret_cast<const i32x2 *>(vp + tid * (kPage / 2))
+                               : i32x2{0, 0};
+#pragma unroll
+            for (int t = 0; t < kPage; ++t) {
+                const int nibble = ((uint32_t)w[t / 8] >> (4 * (kv_nibble(t) % 8))) & 0xf;
+                sT[t][tid] = (int8_t)(ok ? nibble - kInt4Zero : 0);
+            }
+        }
+    } else if (tid < D) {
         const i32x4 w = ok ? *reinterpret_cast<const i32x4 *>(vp + tid * kPage)
                            : i32x4{0, 0, 0, 0};
         const int8_t *bytes = reinterpret_cast<const int8_t *>(&w);
@@ -133,12 +155,16 @@ extern "C" size_t reef_attention_prefill_cache_workspace_bytes(const reef_attent
     return (size_t)cache_workspace(p).total;
 }
 
-extern "C" reef_status reef_attention_prefill_int8_cache(
-    const reef_attention_params *p, const int8_t *q, const reef_strides *q_strides,
-    const float *q_scales, const int8_t *k_cache, const int8_t *v_cache, const float *k_scales,
-    const float *v_scales, int64_t max_context, const int32_t *block_table,
-    int64_t max_blocks_per_seq, int64_t num_pages, float *out, const reef_strides *out_strides,
-    void *workspace, size_t workspace_bytes, uint32_t *status_word, hipStream_t stream) {
+namespace {
+
+template <int BITS>
+reef_status prefill_cache(const reef_attention_params *p, const int8_t *q,
+                          const reef_strides *q_strides, const float *q_scales,
+                          const void *k_cache, const void *v_cache, const float *k_scales,
+                          const float *v_scales, int64_t max_context, const int32_t *block_table,
+                          int64_t max_blocks_per_seq, int64_t num_pages, float *out,
+                          const reef_strides *out_strides, void *workspace,
+                          size_t workspace_bytes, uint32_t *status_word, hipStream_t stream) {
     if (!p || !q || !q_scales || !k_cache || !v_cache || !k_scales || !v_scales || !out)
         return REEF_INVALID_ARGUMENT;
     if (p->batch <= 0 || p->q_heads <= 0 || p->kv_heads <= 0 || p->q_len <= 0 ||
@@ -167,8 +193,8 @@ extern "C" reef_status reef_attention_prefill_int8_cache(
 
     char *base = static_cast<char *>(workspace);
     GatherArgs g;
-    g.k = k_cache;
-    g.v = v_cache;
+    g.k = static_cast<const int8_t *>(k_cache);
+    g.v = static_cast<const int8_t *>(v_cache);
     g.ks = k_scales;
     g.vs = v_scales;
     g.table = block_table;
@@ -184,11 +210,35 @@ extern "C" reef_status reef_attention_prefill_int8_cache(
     g.status = status_word;
     const dim3 grid((unsigned)ceil_div(p->kv_len, kPage), (unsigned)(p->batch * p->kv_heads));
     if (p->head_dim == 128)
-        hipLaunchKernelGGL(gather_cache<128>, grid, dim3(kGatherThreads), 0, stream, g);
+        hipLaunchKernelGGL((gather_cache<128, BITS>), grid, dim3(kGatherThreads), 0, stream, g);
     else
-        hipLaunchKernelGGL(gather_cache<64>, grid, dim3(kGatherThreads), 0, stream, g);
+        hipLaunchKernelGGL((gather_cache<64, BITS>), grid, dim3(kGatherThreads), 0, stream, g);
     if (launch_status() != REEF_OK) return REEF_HIP_ERROR;
     return reef_attention_prefill_int8(p, q, q_strides, g.k_out, nullptr, g.v_out, nullptr,
                                        q_scales, g.ks_out, g.vs_out, out, out_strides, workspace,
                                        (size_t)w.balanced, stream);
+}
+
+}  // namespace
+
+extern "C" reef_status reef_attention_prefill_int8_cache(
+    const reef_attention_params *p, const int8_t *q, const reef_strides *q_strides,
+    const float *q_scales, const int8_t *k_cache, const int8_t *v_cache, const float *k_scales,
+    const float *v_scales, int64_t max_context, const int32_t *block_table,
+    int64_t max_blocks_per_seq, int64_t num_pages, float *out, const reef_strides *out_strides,
+    void *workspace, size_t workspace_bytes, uint32_t *status_word, hipStream_t stream) {
+    return prefill_cache<8>(p, q, q_strides, q_scales, k_cache, v_cache, k_scales, v_scales,
+                            max_context, block_table, max_blocks_per_seq, num_pages, out,
+                            out_strides, workspace, workspace_bytes, status_word, stream);
+}
+
+extern "C" reef_status reef_attention_prefill_int4_cache(
+    const reef_attention_params *p, const int8_t *q, const reef_strides *q_strides,
+    const float *q_scales, const uint8_t *k_cache, const uint8_t *v_cache, const float *k_scales,
+    const float *v_scales, int64_t max_context, const int32_t *block_table,
+    int64_t max_blocks_per_seq, int64_t num_pages, float *out, const reef_strides *out_strides,
+    void *workspace, size_t workspace_bytes, uint32_t *status_word, hipStream_t stream) {
+    return prefill_cache<4>(p, q, q_strides, q_scales, k_cache, v_cache, k_scales, v_scales,
+                            max_context, block_table, max_blocks_per_seq, num_pages, out,
+                            out_strides, workspace, workspace_bytes, status_word, stream);
 }
