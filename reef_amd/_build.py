@@ -14,7 +14,7 @@ from concurrent.futures import ThreadPoolExecutor
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 SOURCES = ["quant.hip", "prefill.hip", "prefill_packed.hip", "prefill_cache.hip", "decode.hip",
-           "kv_append.hip", "int_head.hip", "linear.hip", "norm.hip",
+           "decode_entries.hip", "kv_append.hip", "int_head.hip", "linear.hip", "norm.hip",
            "kv_pages.hip", "kv_select.hip", "tree.hip"]
 LIB = os.path.join(PKG, "libreef_hip.so")
 
@@ -39,7 +39,8 @@ FLAGS = [
 # decode over a contiguous cache 0.4 % (64 x 4096, 8 heads of 128: 89.6 us against 89.3). The
 # other kernels of prefill.hip and those of int_head.hip come out the same either way.
 VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
-SOURCE_FLAGS = {s: VGPR_FORM for s in ("linear.hip", "prefill.hip", "decode.hip", "tree.hip")}
+SOURCE_FLAGS = {s: VGPR_FORM for s in ("linear.hip", "prefill.hip", "decode.hip", "decode_entries.hip",
+                                       "tree.hip")}
 
 
 def commands(objdir):

@@ -1,0 +1,538 @@
+// Decode attention over a cache held in 4 bits, and over the pages of either cache that a list
+// names (gfx950). decode.hip's step with two things changed:
+//
+// A block of 64 keys is four pages named by entries: the sequence's pages one after the other, or
+// its list's.
+//
+// Such a block's bytes take less time than decode.hip's arithmetic on the 16 instruction columns,
+// of which G = q_heads / kv_heads are live. Here the scores of a page's 16 keys move into the dead
+// columns, HEADS keys to a column (HEADS: 4, 8 or 16, at least G), so that every lane has live ones
+// and a lane's share is HEADS scores instead of 16. A column's weights are zero for the other
+// columns' keys, each column keeps a softmax of its own, and the columns of a head are merged when
+// a run of keys ends.
+#include "decode_block.hpp"
+
+namespace reef {
+namespace {
+
+constexpr int kEntryThreads = 64 * kDecodeWaves;
+// Blocks a part of an item has at least where workgroups take a part each: two a wave. (With 4 the
+// merges of more parts outweigh them, with 16 the waves wait: 12.5, 12.4, 14.9 us for 8 heads of
+// 256 listed pages.)
+constexpr int kLeastBlocks = 8;
+
+// The block of four pages named by entries (numbers of the sequence's pages, -1: none) that lanes
+// l % 4 hold, with their page numbers from the block table.
+template <int D, int BITS, int HEADS, bool PAGED, bool NT>
+__device__ __forceinline__ void load_entries(const DecodeArgs &a, int b, int kvh, int n_pages,
+                                             int entries, int pages, int col, int grp,
+                                             DecodeBlock<D, BITS, HEADS> &x, bool &bad_page) {
+    const int ke = __shfl(entries, col >> 2), ge = __shfl(entries, grp);
+    // (none is a page past the sequence to page_ref: dead)
+    const PageRef kp = page_ref<D, BITS, PAGED>(a, b, kvh, ke < 0 ? n_pages : ke, n_pages,
+                                                PAGED ? __shfl(pages, col >> 2) : 0);
+    const PageRef gp = page_ref<D, BITS, PAGED>(a, b, kvh, ge < 0 ? n_pages : ge, n_pages,
+                                                PAGED ? __shfl(pages, grp) : 0);
+    x.pos = max(ge, 0) * kPage;
+    load_pages<D, BITS, HEADS, NT>(kp, gp, col, grp, x, bad_page);
+}
+
+// Keys [k_begin, k_end) of (sequence b, kv head kvh) in steps of k_step: the sequence's, or (SEL)
+// the places of its list, 16 to an entry, `count` entries in all. The next block's loads, the
+// page numbers of the one after and the entries of the one after that are issued before the current
+// block is computed, and all of them always, of the last block again where there is none: under a
+// branch the compiler would wait for all loads in flight at the next use of any. (Two blocks in
+// flight instead of one gain nothing.)
+template <int D, int BITS, int HEADS, bool PAGED, bool SEL>
+__device__ __forceinline__ void run_entries(const DecodeArgs &a, int item, int b, int kvh, int lo,
+                                            int len, int count, int k_begin, int k_end, int k_step,
+                                            int n_pages, const Query<D> &q, int lane,
+                                            DecodeRun<D> &st, bool &bad_page) {
+    if (k_begin >= k_end) return;
+    const int col = lane & 15, grp = lane >> 4;
+    const int last = (k_end - k_begin - 1) / k_step;
+    auto entry = [&](int i) {
+        const int at = (k_begin + min(i, last) * k_step) / kPage + (lane & 3);
+        if constexpr (SEL) {
+            const int e = a.sel_pages[(int64_t)item * a.max_sel + min(at, count - 1)];
+            bad_page |= at < count && e >= n_pages;
+            return at < count && e < n_pages ? max(e, -1) : -1;
+        } else {
+            return at < n_pages ? at : -1;
+        }
+    };
+    auto page = [&](int e) {
+        return PAGED ? a.block_table[(int64_t)b * a.max_blocks + max(e, 0)] : 0;
+    };
+    DecodeBlock<D, BITS, HEADS> cur, next;
+    auto load = [&](int e, int p) {
+        load_entries<D, BITS, HEADS, PAGED, !PAGED && !SEL>(a, b, kvh, n_pages, e, p, col, grp, next,
+                                                            bad_page);
+    };
+    auto math = [&](int i) {
+        block_math<D, BITS, HEADS, SEL>(cur, k_begin + i * k_step, lo, SEL ? len : k_end, q, lane, st);
+    };
+    const int e0 = entry(0);
+    int e1 = entry(1), e2 = entry(2);  // of the next block and the one after
+    const int p0 = page(e0);
+    int p1 = page(e1);
+    load(e0, p0);
+    for (int i = 0; i < last; ++i) {
+        const int p2 = page(e2), e3 = entry(i + 3);
+        cur = next;
+        load(e1, p1);
+        math(i);
+        e1 = e2;
+        p1 = p2;
+        e2 = e3;
+    }
+    cur = next;
+    math(last);
+}
+
+// The columns of a head as one: every lane of the row that holds the head has the result.
+template <int ROTATE>
+__device__ __forceinline__ float row_rotated(float x) {
+    return __int_as_float(
+        __builtin_amdgcn_mov_dpp(__float_as_int(x), 0x120 + ROTATE, 0xf, 0xf, true));
+}
+template <int ROTATE>
+__device__ __forceinline__ float row_sum(float x) { return x + row_rotated<ROTATE>(x); }
+
+template <int D, int HEADS>
+__device__ __forceinline__ void merge_columns(float &m, float &l, f32x4 (&o)[D / 16]) {
+    if constexpr (HEADS < 16) {
+        float mt = fmaxf(m, row_rotated<8>(m));
+        if constexpr (HEADS == 4) mt = fmaxf(mt, row_rotated<4>(mt));
+        const float e = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mt);
+        m = mt;
+        auto sum = [&](float x) {
+            x = row_sum<8>(x * e);
+            if constexpr (HEADS == 4) x = row_sum<4>(x);
+            return x;
+        };
+        l = sum(l);
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[d][i] = sum(o[d][i]);
+    }
+}
+
+// Results of the kernels over entries lie by rows: slot s of D HEADS / 4 holds four channels,
+// 4 (s % (D / 4)) .., of head s / (D / 4), with the head's (max, sum) beside. A workgroup's waves
+// leave theirs in LDS, all threads merge a slot each, and a part in the workspace is the slots in
+// order: whole lines, of the live heads alone.
+template <int D, int HEADS>
+struct RowSlots {
+    static constexpr int N = D * HEADS / 4;
+    static constexpr int THREADS = kEntryThreads;
+    static constexpr int PER = N > THREADS ? N / THREADS : 1;     // slots a thread
+    static constexpr int GROUPS = N < THREADS ? THREADS / N : 1;  // parts that threads take at once
+    static_assert((2 * N + HEADS) <= DecodeSlot<D>::ELEMS, "a part's place in the workspace");
+};
+
+struct RowRun {
+    float m, l;
+    f32x4 o;
+};
+__device__ __forceinline__ void merge_rows(RowRun &r, float m, float l, f32x4 o) {
+    const float mn = fmaxf(r.m, m);
+    const float er = r.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(r.m - mn);
+    const float ep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+    r.l = __builtin_fmaf(ep, l, r.l * er);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.o[i] = __builtin_fmaf(ep, o[i], r.o[i] * er);
+    r.m = mn;
+}
+
+// The first `n` runs of slot s in LDS, in order.
+template <int D, int HEADS>
+__device__ __forceinline__ RowRun merge_slot(const f32x4 *sRow, const float2 *sML, int s, int n) {
+    constexpr int N = RowSlots<D, HEADS>::N;
+    const int h = s / (D / 4);
+    RowRun r = {sML[h].x, sML[h].y, sRow[s]};
+    for (int w = 1; w < n; ++w) {
+        const float2 ml = sML[w * 16 + h];
+        merge_rows(r, ml.x, ml.y, sRow[w * N + s]);
+    }
+    return r;
+}
+
+// --- dealing out -----------------------------------------------------------------------------
+
+// A workgroup-wide sum of x (every thread gets it; sWave holds a word a wave).
+__device__ __forceinline__ int workgroup_sum(int x, int32_t *sWave) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sWave[threadIdx.x >> 6] = x;
+    __syncthreads();
+    int s = 0;
+#pragma unroll
+    for (int w = 0; w < kDecodeWaves; ++w) s += sWave[w];
+    return __builtin_amdgcn_readfirstlane(s);
+}
+
+// n units in G runs, the first n % G of them one longer.
+struct Deal {
+    int least, more;  // units of a run, runs with one more
+    __device__ __forceinline__ Deal(int n, int G) : least((uint32_t)n / (uint32_t)G), more(n - least * G) {}
+    __device__ __forceinline__ int start(int g) const { return g * least + min(g, more); }
+    __device__ __forceinline__ int run_of(int u) const {
+        const int cut = more * (least + 1);
+        return u < cut ? (uint32_t)u / (uint32_t)(least + 1) : more + (uint32_t)(u - cut) / (uint32_t)least;
+    }
+};
+
+// The launch's work is the items' (sequence, kv head) 64-key blocks, at least one an item. With
+// at most kPlanItems items every workgroup counts them (from the lengths, in LDS) and finds its own:
+//   single  (no more items than half the workgroups): one part of one item. Parts are of at most c
+//           blocks, c the least that a search from the mean finds to need no more parts than
+//           workgroups; an item's parts are equal to a block. (A run over the end of one item and
+//           the start of the next costs two starts and two merges: 31 us instead of 27 for 128 sequences
+//           of 512 .. 8192 tokens.)
+//   else    an equal run of blocks over the items, whatever the lengths.
+// With more items a workgroup takes an equal run of whole items. Of a part or run the 4 waves take
+// the item's blocks in turn, keep a flash-decoding state each and merge in LDS; an item that lies
+// in one workgroup is stored, the parts of others go to the workspace, and the part that arrives
+// last merges them all.
+template <int D, int BITS, int HEADS, bool PAGED, bool SEL>
+__global__ __launch_bounds__(kEntryThreads, kWgPerCu) void decode_entries(DecodeArgs a, float *out) {
+    using Slots = RowSlots<D, HEADS>;
+    constexpr int DB = D / 16;  // 16-wide output blocks
+    constexpr int N = Slots::N, QD = D / 4;
+    __shared__ int32_t sOff[kPlanItems + 1];
+    __shared__ int32_t sWave[kDecodeWaves];
+    __shared__ f32x4 sRow[kDecodeWaves * N];
+    __shared__ float2 sML[kDecodeWaves * 16];
+    __shared__ int32_t sItem;
+    __shared__ uint32_t sLast;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, grp = lane >> 4;
+    const int g = blockIdx.x;
+
+    int units = a.items;  // parts, blocks or items
+    if (a.flat) {
+        int mine = 0;
+        for (int i = tid; i < a.items; i += kEntryThreads) {
+            const int n = item_keys<SEL>(a, i).blocks;
+            sOff[i + 1] = n;
+            mine += n;
+        }
+        units = workgroup_sum(mine, sWave);
+    }
+    int c = 1;
+    if (a.single) {
+        const int mean = (units + (a.wgs - a.items / 2) - 1) / (a.wgs - a.items / 2);
+        for (c = max(a.single, mean);; c += max(1, c >> 4)) {
+            int mine = 0;
+            for (int i = tid; i < a.items; i += kEntryThreads)
+                mine += (uint32_t)(sOff[i + 1] + c - 1) / (uint32_t)c;
+            units = workgroup_sum(mine, sWave);
+            if (units <= a.wgs) break;
+        }
+    }
+    const Deal deal(units, a.wgs);
+    const int u0 = a.single ? g : deal.start(g), u1 = a.single ? g + 1 : deal.start(g + 1);
+    if (u0 >= min(u1, units)) return;  // nothing for this workgroup (uniform)
+    if (a.flat) {
+        // sOff[i] becomes the units of items 0 .. i - 1, and sItem the item that unit u0 is of.
+        if (tid == 0) sOff[0] = 0;
+        int run = 0;
+        for (int base = 0; base < a.items; base += kEntryThreads) {
+            const int i = base + tid;
+            const int own = i < a.items ? (uint32_t)(sOff[i + 1] + c - 1) / (uint32_t)c : 0;
+            int x = own;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int y = __shfl_up(x, o);
+                if (lane >= o) x += y;
+            }
+            __syncthreads();
+            if (lane == 63) sWave[wave] = x;
+            __syncthreads();
+            int before = run;
+            for (int w = 0; w < kDecodeWaves; ++w) {
+                if (w < wave) before += sWave[w];
+                run += sWave[w];
+            }
+            if (i < a.items) {
+                sOff[i + 1] = before + x;
+                if (u0 < before + x && u0 >= before + x - own) sItem = i;
+            }
+        }
+        __syncthreads();
+    }
+    // Values read from LDS arrive in vector registers; all of these are uniform, and moving them
+    // to scalar registers keeps the loop control and the addresses scalar.
+    auto unit_of = [&](int item) {
+        return a.flat ? __builtin_amdgcn_readfirstlane(sOff[item]) : item;
+    };
+    int item = a.flat ? __builtin_amdgcn_readfirstlane(sItem) : u0;
+
+    for (;;) {
+        const int p_begin = unit_of(item), p_end = unit_of(item + 1);
+        ItemKeys ik = item_keys<SEL>(a, item);
+        ik.len = __builtin_amdgcn_readfirstlane(ik.len);
+        ik.lo = __builtin_amdgcn_readfirstlane(ik.lo);
+        ik.first_block = __builtin_amdgcn_readfirstlane(ik.first_block);
+        ik.blocks = __builtin_amdgcn_readfirstlane(ik.blocks);
+        if constexpr (SEL) ik.count = __builtin_amdgcn_readfirstlane(ik.count);
+        const int b = item / a.kv_heads, kvh = item % a.kv_heads;
+        // This segment's blocks of the item, the workgroups with a part of it (parts from gf on).
+        int s_blk = 0, e_blk = ik.blocks, parts = 1, gf = g;
+        if (a.single) {
+            parts = p_end - p_begin;
+            gf = p_begin;
+            const Deal blocks(ik.blocks, parts);
+            s_blk = blocks.start(g - gf);
+            e_blk = blocks.start(g - gf + 1);
+        } else if (a.flat) {
+            s_blk = max(u0, p_begin) - p_begin;
+            e_blk = min(u1, p_end) - p_begin;
+            if (p_begin < u0 || p_end > u1) {
+                gf = deal.run_of(p_begin);
+                parts = deal.run_of(p_end - 1) - gf + 1;
+            }
+        }
+        if (ik.bad && s_blk == 0 && tid == 0) flag_status(a.status, REEF_STATUS_BIT_BAD_LENGTH);
+
+        const int head = kvh * a.group + col;   // this lane's query head (live if col < group)
+        const int scored = kvh * a.group + col % HEADS;  // the head whose scores it holds
+        const int k_begin = (ik.first_block + s_blk + wave) * kBlockKeys;
+        const int k_end = min(SEL ? ik.count * kPage : ik.len, (ik.first_block + e_blk) * kBlockKeys);
+        const int n_pages = (ik.len + kPage - 1) / kPage;
+        const Query<D> q = load_query<D, BITS>(a, b, head, col < a.group, scored,
+                                               col % HEADS < a.group, grp);
+        DecodeRun<D> st;
+        reset_run<D>(st);
+        bool bad_page = false;
+        run_entries<D, BITS, HEADS, PAGED, SEL>(a, item, b, kvh, ik.lo, ik.len, ik.count, k_begin,
+                                                k_end, kDecodeWaves * kBlockKeys, n_pages, q, lane,
+                                                st, bad_page);
+        if (bad_page) flag_status(a.status, REEF_STATUS_BIT_BAD_PAGE);
+        // Row sums: this lane holds its column's partial over the keys of its lane group.
+        float l = st.l_run;
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        float m = st.m_run;
+        f32x4 o[DB];
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[d] = st.acc[d] * (st.s_run * (1.0f / 256.0f));
+        merge_columns<D, HEADS>(m, l, o);
+        if (col < HEADS) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d) sRow[wave * N + col * QD + 4 * d + grp] = o[d];
+            if (grp == 0) sML[wave * 16 + col] = float2{m, l};
+        }
+        __syncthreads();
+
+        // A sequence with no keys ends with a sum of 0 and stores zeros.
+        auto store = [&](int s, const RowRun &r) {
+            if (s / QD >= a.group) return;
+            const float inv = r.l > 0.0f ? 1.0f / r.l : 0.0f;
+            float *orow = out + ((int64_t)b * a.q_heads + kvh * a.group) * D;
+            *reinterpret_cast<f32x4 *>(orow + 4 * s) = r.o * inv;
+        };
+        if (parts == 1) {  // (uniform)
+#pragma unroll
+            for (int k = 0; k < Slots::PER; ++k) {
+                const int s = tid + k * kEntryThreads;
+                if (s < N) store(s, merge_slot<D, HEADS>(sRow, sML, s, kDecodeWaves));
+            }
+        } else {
+            // A workgroup's part of an item lies in its slot 0 if its run began with it, in slot
+            // 1 if the run ended with it. The slots are written and counted in as in decode.hip.
+            auto part_at = [&](int gg, int slot) {
+                return reinterpret_cast<uint64_t *>(a.slots) +
+                       ((int64_t)gg * 2 + slot) * DecodeSlot<D>::ELEMS;
+            };
+            auto pack = [](float x0, float x1) {
+                return (uint64_t)__float_as_uint(x0) | ((uint64_t)__float_as_uint(x1) << 32);
+            };
+            uint64_t *so = part_at(g, a.single || p_begin <= u0 ? 0 : 1);
+#pragma unroll
+            for (int k = 0; k < Slots::PER; ++k) {
+                const int s = tid + k * kEntryThreads;
+                if (s < N && s / QD < a.group) {
+                    const RowRun r = merge_slot<D, HEADS>(sRow, sML, s, kDecodeWaves);
+                    part_store(so + s, pack(r.o[0], r.o[1]));
+                    part_store(so + N + s, pack(r.o[2], r.o[3]));
+                    if (s % QD == 0) part_store(so + 2 * N + s / QD, pack(r.m, r.l));
+                }
+            }
+            part_stores_done();
+            __syncthreads();
+            if (tid == 0) sLast = part_count(a.counters + item) == (uint32_t)(parts - 1) ? 1u : 0u;
+            __syncthreads();  // publishes sLast
+            if (__builtin_amdgcn_readfirstlane(sLast)) {
+                // Every thread merges its slots of the parts in order (of every GROUPS-th, and the
+                // groups then in LDS): the same result whichever part arrived last. It reads
+                // several parts before it uses the first: a round trip for them all, not one each.
+                constexpr int AHEAD = 16 / Slots::PER;
+                const int gi = tid / N;  // (PER > 1: 0)
+                const int first_slot = !a.single && deal.start(gf) < p_begin ? 1 : 0;
+                auto lo32 = [](uint64_t v) { return __uint_as_float((uint32_t)v); };
+                auto hi32 = [](uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); };
+                RowRun run[Slots::PER];
+                part_claimed();
+#pragma unroll
+                for (int k = 0; k < Slots::PER; ++k) {
+                    const int s = (tid + k * kEntryThreads) % N;
+                    run[k] = {-INFINITY, 0.0f, f32x4{}};
+                    if (s / QD >= a.group) continue;
+                    for (int i0 = gi; i0 < parts; i0 += Slots::GROUPS * AHEAD) {
+                        uint64_t w[AHEAD][3];
+#pragma unroll
+                        for (int i = 0; i < AHEAD; ++i) {
+                            const int part = min(i0 + i * Slots::GROUPS, parts - 1);
+                            const uint64_t *sl = part_at(gf + part, part == 0 ? first_slot : 0);
+                            w[i][0] = part_load(sl + s);
+                            w[i][1] = part_load(sl + N + s);
+                            w[i][2] = part_load(sl + 2 * N + s / QD);
+                        }
+#pragma unroll
+                        for (int i = 0; i < AHEAD; ++i)
+                            if (i0 + i * Slots::GROUPS < parts)
+                                merge_rows(run[k], lo32(w[i][2]), hi32(w[i][2]),
+                                           f32x4{lo32(w[i][0]), hi32(w[i][0]), lo32(w[i][1]),
+                                                 hi32(w[i][1])});
+                    }
+                }
+                if (tid == 0) part_reset(a.counters + item);
+                if constexpr (Slots::GROUPS == 1) {
+#pragma unroll
+                    for (int k = 0; k < Slots::PER; ++k) store(tid + k * kEntryThreads, run[k]);
+                } else {
+                    const int s = tid % N;
+                    sRow[gi * N + s] = run[0].o;
+                    if (s % QD == 0) sML[gi * 16 + s / QD] = float2{run[0].m, run[0].l};
+                    __syncthreads();
+                    if (tid < N) store(s, merge_slot<D, HEADS>(sRow, sML, s, Slots::GROUPS));
+                }
+            }
+        }
+        if (a.single || p_end >= u1) break;
+        ++item;
+        __syncthreads();  // frees sRow, sML and sLast
+    }
+}
+
+template <int BITS, bool PAGED, bool SEL>
+reef_status launch_entries(const reef_decode_params *p, DecodeArgs &a, float *out, void *workspace,
+                           hipStream_t stream) {
+    set_decode_args(p, a);
+    // The tokens that a sequence may read. A list longer than the cache (pages listed twice)
+    // gets no more workgroups than the workspace has slots for.
+    const int64_t tokens = SEL ? (int64_t)a.max_sel * kPage : p->max_context;
+    const int64_t items = a.items, blocks = ceil_div(std::min(tokens, p->max_context), kBlockKeys);
+    // Two workgroups a compute unit, one where items are few: an item's parts are half as many then
+    // and the bytes take no longer (1 x 8 x 131071 tokens: 36 us against 43, 64 parts an item).
+    const int64_t cus = compute_units();
+    const int64_t most = p->num_splits > 0 ? ceil_div(items * p->num_splits, kDecodeWaves)
+                                           : (2 * items <= cus ? 1 : kWgPerCu) * cus;
+    a.flat = decode_flat(p, p->max_context) && decode_flat(p, tokens) ? 1 : 0;
+    const int64_t least = p->num_splits > 0 ? 1 : kLeastBlocks;
+    a.single = a.flat && 2 * items <= most ? (int32_t)least : 0;
+    const int64_t units = a.single ? items * ceil_div(blocks, least) : a.flat ? items * blocks : items;
+    a.wgs = (int32_t)std::max<int64_t>(1, std::min<int64_t>(std::min(most, units), 1 << 20));
+    a.counters = static_cast<uint32_t *>(workspace);
+    a.slots = reinterpret_cast<float *>(static_cast<char *>(workspace) + kDecodeCounterBytes);
+    const auto run = [&](auto *kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)a.wgs), dim3(kEntryThreads), 0, stream, a, out);
+    };
+    if (p->head_dim == 128)
+        run(a.group <= 4   ? decode_entries<128, BITS, 4, PAGED, SEL>
+            : a.group <= 8 ? decode_entries<128, BITS, 8, PAGED, SEL>
+                           : decode_entries<128, BITS, 16, PAGED, SEL>);
+    else
+        run(a.group <= 4   ? decode_entries<64, BITS, 4, PAGED, SEL>
+            : a.group <= 8 ? decode_entries<64, BITS, 8, PAGED, SEL>
+                           : decode_entries<64, BITS, 16, PAGED, SEL>);
+    return launch_status();
+}
+
+// A paged launch's table, or (block_table NULL) a contiguous cache.
+bool use_table(const reef_decode_params *p, const int32_t *block_table,
+               int64_t max_blocks_per_seq, int64_t num_pages, DecodeArgs &a) {
+    if (!a.context_lens || num_pages <= 0 || num_pages >= (int64_t(1) << 31) ||
+        max_blocks_per_seq * kPage < p->max_context || max_blocks_per_seq >= (int64_t(1) << 30))
+        return false;
+    a.block_table = block_table;
+    a.max_blocks = (int32_t)max_blocks_per_seq;
+    a.num_pages = (int32_t)num_pages;
+    return true;
+}
+
+// Decode over a cache of BITS, paged where there is a block table, over a list's pages where
+// there is a list.
+template <int BITS>
+reef_status decode_any(const reef_decode_params *p, const int8_t *q, const float *q_scales,
+                       const void *k, const void *v, const float *k_scales,
+                       const float *v_scales, const int32_t *block_table,
+                       int64_t max_blocks_per_seq, int64_t num_pages,
+                       const int32_t *context_lens, const reef_page_selection *selection,
+                       float *out, void *workspace, size_t workspace_bytes,
+                       uint32_t *status_word, hipStream_t stream) {
+    const reef_status st = decode_validate(p, q, q_scales, out, workspace, workspace_bytes);
+    if (st != REEF_OK) return st;
+    if (!k || !v || !k_scales || !v_scales || !aligned(k, 16) || !aligned(v, 16) ||
+        !aligned(k_scales, 16) || !aligned(v_scales, 16) || !aligned(out, 16))
+        return REEF_INVALID_ARGUMENT;
+    DecodeArgs a = {};
+    a.q = q;
+    a.qs = q_scales;
+    a.k = static_cast<const int8_t *>(k);
+    a.v = static_cast<const int8_t *>(v);
+    a.ks = k_scales;
+    a.vs = v_scales;
+    a.context_lens = context_lens;
+    a.status = status_word;
+    if (block_table && !use_table(p, block_table, max_blocks_per_seq, num_pages, a))
+        return REEF_INVALID_ARGUMENT;
+    if (selection) {
+        if (!selection->pages || !selection->counts || !context_lens || selection->max_pages <= 0 ||
+            !aligned(selection->pages, 4) || !aligned(selection->counts, 4))
+            return REEF_INVALID_ARGUMENT;
+        if (selection->max_pages >= (int64_t(1) << 26)) return REEF_UNSUPPORTED;
+        a.sel_pages = selection->pages;
+        a.sel_counts = selection->counts;
+        a.max_sel = (int32_t)selection->max_pages;
+        return block_table ? launch_entries<BITS, true, true>(p, a, out, workspace, stream)
+                           : launch_entries<BITS, false, true>(p, a, out, workspace, stream);
+    }
+    if constexpr (BITS == 8) return REEF_INVALID_ARGUMENT;  // decode.hip's
+    else
+        return block_table ? launch_entries<BITS, true, false>(p, a, out, workspace, stream)
+                           : launch_entries<BITS, false, false>(p, a, out, workspace, stream);
+}
+
+}  // namespace
+}  // namespace reef
+
+using namespace reef;
+
+extern "C" reef_status reef_attention_decode_int8_selected(
+    const reef_decode_params *p, const int8_t *q, const float *q_scales, const int8_t *k_cache,
+    const int8_t *v_cache, const float *k_scales, const float *v_scales,
+    const int32_t *block_table, int64_t max_blocks_per_seq, int64_t num_pages,
+    const int32_t *context_lens, const reef_page_selection *selection, float *out,
+    void *workspace, size_t workspace_bytes, uint32_t *status_word, hipStream_t stream) {
+    if (!selection) return REEF_INVALID_ARGUMENT;
+    return decode_any<8>(p, q, q_scales, k_cache, v_cache, k_scales, v_scales, block_table,
+                         max_blocks_per_seq, num_pages, context_lens, selection, out, workspace,
+                         workspace_bytes, status_word, stream);
+}
+
+extern "C" reef_status reef_attention_decode_int4(
+    const reef_decode_params *p, const int8_t *q, const float *q_scales, const uint8_t *k_cache,
+    const uint8_t *v_cache, const float *k_scales, const float *v_scales,
+    const int32_t *block_table, int64_t max_blocks_per_seq, int64_t num_pages,
+    const int32_t *context_lens, const reef_page_selection *selection, float *out,
+    void *workspace, size_t workspace_bytes, uint32_t *status_word, hipStream_t stream) {
+    return decode_any<4>(p, q, q_scales, k_cache, v_cache, k_scales, v_scales, block_table,
+                         max_blocks_per_seq, num_pages, context_lens, selection, out, workspace,
+                         workspace_bytes, status_word, stream);
+}

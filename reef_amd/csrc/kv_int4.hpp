@@ -29,14 +29,18 @@ __device__ __forceinline__ uint32_t nibbles_to_int8(uint32_t u) {
 // One half (4 bytes, 8 tokens) of a value channel as fp16 in token order, exactly. Under the
 // exponent of 1024 a nibble in bits 0-3 reads as 1024 + u, one in bits 4-7 as 1024 + 16 u;
 // tokens 2i and 2i + 1 lie 16 bits apart, so one mask takes both. Nine instructions for eight
-// values.
+// values (the empty asm keeps mask and exponent in registers, where one instruction takes both;
+// as literals they cost one each: 64 more of 455 a block of decode at head_dim 128).
 __device__ __forceinline__ f16x8 int4x8_to_f16(uint32_t w) {
     const f16x2 low = {(_Float16)-1032.0f, (_Float16)-1032.0f};
     const f16x2 high = {(_Float16)-72.0f, (_Float16)-72.0f};
     const f16x2 part = {(_Float16)0.0625f, (_Float16)0.0625f};
+    uint32_t lower = 0x000f000fu, upper = 0x00f000f0u, exponent = 0x64006400u;
+    asm("" : "+s"(lower), "+s"(upper));
+    asm("" : "+v"(exponent));
     const uint32_t s = w >> 8;
-    const uint32_t u[4] = {(w & 0x000f000fu) | 0x64006400u, (w & 0x00f000f0u) | 0x64006400u,
-                           (s & 0x000f000fu) | 0x64006400u, (s & 0x00f000f0u) | 0x64006400u};
+    const uint32_t u[4] = {(w & lower) | exponent, (w & upper) | exponent, (s & lower) | exponent,
+                           (s & upper) | exponent};
     f16x8 r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

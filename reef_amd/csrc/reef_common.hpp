@@ -76,7 +76,13 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
     return v;
 }
 
-// max / sum of x over lanes l and l ^ 32, in one VALU op (v_permlane32_swap).
+// max of x over lanes l and l ^ 16, max / sum over l and l ^ 32, in one VALU op each
+// (v_permlane16_swap, v_permlane32_swap).
+__device__ __forceinline__ float xor16_max(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                   false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 __device__ __forceinline__ float xor32_max(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
                                                    false);
@@ -109,17 +115,18 @@ __device__ __forceinline__ int8_t quantize_int8(float x, float scale) {
     return (int8_t)(int)r;
 }
 
-// Eight weights as fp16, and the fp16 of what that leaves of them: 22 bits together. The
+// Weights (eight or four) as fp16, and the fp16 of what that leaves of them: 22 bits together. The
 // empty asm issues nothing; it keeps the rounded weights one value. Without it the compiler
 // converts a weight that is a product twice, for the operand from the rounded product and
 // for the remainder from the unrounded one (v_fma_mixlo_f16, also with contraction off), and
 // where the two round apart, operand and remainder are off by 2^-11 of the weight together.
-__device__ __forceinline__ void split_weights(const float (&w)[8], f16x8 &hi, f16x8 &lo) {
+template <int N, typename V>
+__device__ __forceinline__ void split_weights(const float (&w)[N], V &hi, V &lo) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) hi[e] = (_Float16)w[e];
+    for (int e = 0; e < N; ++e) hi[e] = (_Float16)w[e];
     asm("" : "+v"(hi));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) lo[e] = (_Float16)(w[e] - (float)hi[e]);
+    for (int e = 0; e < N; ++e) lo[e] = (_Float16)(w[e] - (float)hi[e]);
 }
 
 __device__ __forceinline__ void flag_status(uint32_t *word, uint32_t bits) {
