@@ -271,7 +271,7 @@ __global__ void advance_lengths(const int32_t *start, int32_t batch, int32_t new
 // --- the 4-bit cache as fp32 rows ----------------------------------------------------------
 
 constexpr int kUnpackThreads = 256;
-constexpr int kUnpackPages = 4;  // pages a workgroup
+constexpr int kUnpackPages = 8;  // pages a workgroup
 
 struct UnpackArgs {
     const uint8_t *k, *v;
@@ -280,37 +280,67 @@ struct UnpackArgs {
     int64_t pages;
 };
 
-// A thread turns four channels of a row into one 16-byte store, rows of a page in turn. Keys:
-// four bytes hold two such groups, half a row apart; each is read for its own nibble (the second
-// read hits the cache). Values: the four channels' bytes of the token.
+// A wave takes a page, and every store of it writes whole rows or quarters of rows in order. Keys:
+// a lane reads 4 bytes of a row, four channels of either half. Values: a lane reads the 8 bytes of
+// four channels each and writes them for the tokens of its group of lanes.
 template <int D>
 __global__ __launch_bounds__(kUnpackThreads) void unpack_int4(UnpackArgs a) {
-    constexpr int CPR = D / 4, RB = D / 2;  // threads a row, bytes of a key row
-    constexpr int RPP = kUnpackThreads / CPR;  // rows at once
-    const int c = threadIdx.x % CPR * 4, r0 = threadIdx.x / CPR;
-    const int64_t row_begin = linear_block() * kUnpackPages * kPage;
-    const int64_t row_end = min(row_begin + kUnpackPages * kPage, a.pages * kPage);
-    for (int64_t row = row_begin + r0; row < row_end; row += RPP) {
+    constexpr int RB = D / 2;                 // bytes of a key row
+    constexpr int KL = RB / 4, KR = 64 / KL;  // lanes a key row, rows of a load
+    constexpr int VL = D / 4, VG = 64 / VL;   // lanes a value row, groups of lanes
+    constexpr int VT = kPage / VG;            // tokens of a group
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    auto store = [](float *p, f32x4 x) { *reinterpret_cast<f32x4 *>(p) = x; };
+    const int64_t begin = linear_block() * kUnpackPages + wave;
+    const int64_t end = min((linear_block() + 1) * kUnpackPages, a.pages);
+    for (int64_t page = begin; page < end; page += kUnpackThreads / 64) {
         if (a.k_out) {
-            const uint32_t w = *reinterpret_cast<const uint32_t *>(a.k + row * RB + c % RB);
-            const uint32_t u = c < RB ? low_nibbles(w) : high_nibbles(w);
-            const float s = a.ks[row];
-            f32x4 x;
+            const int j = lane % KL, g = lane / KL;
+            const uint8_t *rows = a.k + (page * kPage + g) * RB + 4 * j;
+            float *out = a.k_out + (page * kPage + g) * D + 4 * j;
+            uint32_t w[kPage / KR];
+            float s[kPage / KR];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = (float)((int)((u >> (8 * i)) & 0xff) - kInt4Zero) * s;
-            *reinterpret_cast<f32x4 *>(a.k_out + row * D + c) = x;
+            for (int i = 0; i < kPage / KR; ++i) {
+                w[i] = *reinterpret_cast<const uint32_t *>(rows + i * KR * RB);
+                s[i] = a.ks[page * kPage + i * KR + g];
+            }
+#pragma unroll
+            for (int i = 0; i < kPage / KR; ++i) {
+                f32x4 x, y;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    x[c] = (float)((int)(w[i] >> (8 * c) & 0xf) - kInt4Zero) * s[i];
+                    y[c] = (float)((int)(w[i] >> (8 * c + 4) & 0xf) - kInt4Zero) * s[i];
+                }
+                store(out + i * KR * D, x);
+                store(out + i * KR * D + D / 2, y);
+            }
         }
         if (a.v_out) {
-            const int64_t page = row / kPage;
-            const int n = kv_nibble((int)(row % kPage));
-            const float s = a.vs[row];
-            f32x4 x;
+            const int j = lane % VL, g = lane / VL;
+            // this group's tokens' half of each channel: VT 8 or 4 of 8 nibbles
+            const int half = g * VT / 8;
+            const uint8_t *rows = a.v + (page * D + 4 * j) * 8 + 4 * half;
+            uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t w = a.v[(page * D + c + i) * 8 + n / 2];
-                x[i] = (float)((int)((n & 1 ? w >> 4 : w) & 0xf) - kInt4Zero) * s;
+            for (int c = 0; c < 4; ++c) w[c] = *reinterpret_cast<const uint32_t *>(rows + 8 * c);
+            f32x4 s[VT / 4];
+#pragma unroll
+            for (int i = 0; i < VT / 4; ++i)
+                s[i] = *reinterpret_cast<const f32x4 *>(a.vs + page * kPage + g * VT + 4 * i);
+            float *out = a.v_out + (page * kPage + g * VT) * D + 4 * j;
+            const int base = VT == 8 ? 0 : 8 * (g & 1);  // of the four tokens' low nibbles
+#pragma unroll
+            for (int t = 0; t < VT; ++t) {
+                const int n = 4 * (kv_nibble(t) % 8);
+                f32x4 x;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    x[c] = (float)((int)(w[c] >> (base + n) & 0xf) - kInt4Zero) * s[t / 4][t % 4];
+                store(out + t * D, x);
             }
-            *reinterpret_cast<f32x4 *>(a.v_out + row * D + c) = x;
         }
     }
 }
@@ -459,7 +489,7 @@ extern "C" reef_status reef_kv_unpack_int4(const uint8_t *k_pages, const uint8_t
                                            hipStream_t stream) {
     if (pages <= 0 || head_dim <= 0 || (!k && !v) || (k && (!k_pages || !k_scales)) ||
         (v && (!v_pages || !v_scales)) || !aligned(k_pages, 16) || !aligned(v_pages, 16) ||
-        !aligned(k, 16) || !aligned(v, 16) || !aligned(k_scales, 4) || !aligned(v_scales, 4))
+        !aligned(k, 16) || !aligned(v, 16) || !aligned(k_scales, 4) || !aligned(v_scales, 16))
         return REEF_INVALID_ARGUMENT;
     if ((head_dim != 64 && head_dim != 128) || pages >= (int64_t(1) << 40)) return REEF_UNSUPPORTED;
     const UnpackArgs a{k_pages, v_pages, k_scales, v_scales, k, v, pages};

@@ -17,7 +17,11 @@ namespace {
 
 // --- bounds --------------------------------------------------------------------------------
 
-constexpr int kBoundWaves = 4;  // waves (one page each) of a workgroup
+constexpr int kBoundWaves = 4;  // waves of a workgroup
+// Pages a wave takes in turn, the next one's rows loading while one is reduced, where a launch has
+// pages for more than kBoundFill waves of them; one otherwise (a decode step's).
+constexpr int kBoundPages = 4;
+constexpr int64_t kBoundFill = 8192;
 
 struct BoundArgs {
     const uint8_t *k;
@@ -27,10 +31,11 @@ struct BoundArgs {
     int8_t *bounds;
     float *scales;
     int32_t kv_heads, new_tokens, max_context, max_blocks, num_pages;
+    int32_t turns;  // pages a wave
     uint32_t *status;
 };
 
-// One wave takes a page. A lane reads 4 bytes (BITS 8: four channels; 4: four of either half of
+// A wave takes a page at a time. A lane reads 4 bytes (BITS 8: four channels; 4: four of either half of
 // the row) of every R-th token's row, so that a load covers 256 bytes in order, and keeps their
 // extremes. Lanes that hold the same channels then meet: over 32 lanes one side keeps the
 // largest, the other the least; in 4 bits over 16 lanes either keeps one half of the row; what
@@ -51,85 +56,115 @@ __global__ __launch_bounds__(kBoundWaves * kWave) void page_bounds(BoundArgs a) 
         return;
     }
     const int end = start + a.new_tokens;
-    const int page_idx = start / kPage + (int)blockIdx.x * kBoundWaves + wave;
-    if (page_idx * kPage >= end) return;
-    int64_t slot;  // index of this (page, kv head)
-    if (a.table) {
-        const int page = a.table[(int64_t)b * a.max_blocks + page_idx];
-        if (page < 0 || page >= a.num_pages) {
-            if (lane == 0) flag_status(a.status, REEF_STATUS_BIT_BAD_PAGE);
-            return;
-        }
-        slot = (int64_t)page * a.kv_heads + kvh;
-    } else {
-        slot = ((int64_t)b * a.kv_heads + kvh) * (a.max_context / kPage) + page_idx;
-    }
-    const int live = min(kPage, end - page_idx * kPage);
+    const int stop = (end + kPage - 1) / kPage;
+    int page_idx = start / kPage + (int)blockIdx.x * kBoundWaves * a.turns + wave;
+    const int last = min(stop, start / kPage + ((int)blockIdx.x + 1) * kBoundWaves * a.turns) - 1;
+    if (page_idx > last) return;
     const int j = lane % LPR, g = lane / LPR;
-    const uint8_t *rows = a.k + slot * (kPage * RB);
-    const float *ks = a.ks + slot * kPage;
-    uint32_t w[kPage / R];
-    float s[kPage / R];
+    struct Rows {
+        uint32_t w[kPage / R];
+        float s[kPage / R];
+        int64_t slot;  // index of this (page, kv head); -1: no such page
+    };
+    auto load = [&](int idx) {
+        Rows r;
+        if (a.table) {
+            const int page = a.table[(int64_t)b * a.max_blocks + idx];
+            r.slot = page < 0 || page >= a.num_pages ? -1 : (int64_t)page * a.kv_heads + kvh;
+        } else {
+            r.slot = ((int64_t)b * a.kv_heads + kvh) * (a.max_context / kPage) + idx;
+        }
+        const int64_t at = max(r.slot, (int64_t)0);
+        const uint8_t *rows = a.k + at * (kPage * RB) + g * RB + 4 * j;
+        const float *ks = a.ks + at * kPage + g;
 #pragma unroll
-    for (int i = 0; i < kPage / R; ++i) {
-        w[i] = *reinterpret_cast<const uint32_t *>(rows + (i * R + g) * RB + 4 * j);
-        s[i] = ks[i * R + g];
-    }
-    float hi[C], lo[C];
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-        hi[c] = -INFINITY;
-        lo[c] = INFINITY;
-    }
-#pragma unroll
-    for (int i = 0; i < kPage / R; ++i) {
-        const bool in = i * R + g < live;
+        for (int i = 0; i < kPage / R; ++i) {
+            r.w[i] = *reinterpret_cast<const uint32_t *>(rows + i * R * RB);
+            r.s[i] = ks[i * R];
+        }
+        return r;
+    };
+    Rows next = load(page_idx);
+    for (; page_idx <= last; page_idx += kBoundWaves) {
+        const Rows rows = next;
+        next = load(min(page_idx + kBoundWaves, last));
+        const int64_t slot = rows.slot;
+        if (slot < 0) {
+            if (lane == 0) flag_status(a.status, REEF_STATUS_BIT_BAD_PAGE);
+            continue;
+        }
+        const int live = min(kPage, end - page_idx * kPage);
+        float hi[C], lo[C];
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int code = BITS == 8 ? (int)(int8_t)(w[i] >> (8 * c))
-                                       : (int)((w[i] >> (8 * (c % 4) + 4 * (c / 4))) & 0xf) - kInt4Zero;
-            const float x = (float)code * s[i];
-            hi[c] = in ? fmaxf(hi[c], x) : hi[c];
-            lo[c] = in ? fminf(lo[c], x) : lo[c];
+            hi[c] = -INFINITY;
+            lo[c] = INFINITY;
         }
-    }
-    // Lanes 0-31 go on with the largest, the others with the least, negated: maxima either way.
-    const bool least = lane >= 32;
-    float m[C];
+        auto key = [&](int i, int c) {
+            const int code = BITS == 8 ? (int)(int8_t)(rows.w[i] >> (8 * c))
+                                       : (int)((rows.w[i] >> (8 * (c % 4) + 4 * (c / 4))) & 0xf) - kInt4Zero;
+            return (float)code * rows.s[i];
+        };
+        if (live == kPage) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const float got = __shfl_xor(least ? hi[c] : -lo[c], 32);
-        m[c] = fmaxf(least ? -lo[c] : hi[c], got);
-    }
-    float n[4];
-    const bool upper = BITS == 4 && (lane & 16);
+            for (int i = 0; i < kPage / R; i += 2) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        if constexpr (BITS == 4) {
-            const float got = __shfl_xor(upper ? m[c] : m[C - 4 + c], 16);
-            n[c] = fmaxf(upper ? m[C - 4 + c] : m[c], got);
+                for (int c = 0; c < C; ++c) {
+                    const float x = key(i, c), y = key(i + 1, c);
+                    hi[c] = fmaxf(hi[c], fmaxf(x, y));
+                    lo[c] = fminf(lo[c], fminf(x, y));
+                }
+            }
         } else {
-            n[c] = m[c];
+#pragma unroll
+            for (int i = 0; i < kPage / R; ++i) {
+                const bool in = i * R + g < live;
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const float x = key(i, c);
+                    hi[c] = in ? fmaxf(hi[c], x) : hi[c];
+                    lo[c] = in ? fminf(lo[c], x) : lo[c];
+                }
+            }
         }
+        // Lanes 0-31 go on with the largest, the others with the least, negated: maxima either way.
+        const bool least = lane >= 32;
+        float m[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const float got = __shfl_xor(least ? hi[c] : -lo[c], 32);
+            m[c] = fmaxf(least ? -lo[c] : hi[c], got);
+        }
+        float n[4];
+        const bool upper = BITS == 4 && (lane & 16);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            if constexpr (BITS == 4) {
+                const float got = __shfl_xor(upper ? m[c] : m[C - 4 + c], 16);
+                n[c] = fmaxf(upper ? m[C - 4 + c] : m[c], got);
+            } else {
+                n[c] = m[c];
+            }
+        }
+        constexpr int kSplit = BITS == 4 ? 16 : 32;  // lanes of one bound (and half)
+#pragma unroll
+        for (int o = LPR; o < kSplit; o <<= 1)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) n[c] = fmaxf(n[c], __shfl_xor(n[c], o));
+        const float top = wave_max(fmaxf(fmaxf(n[0], n[1]), fmaxf(n[2], n[3])));
+        const float scale = int8_scale(top);
+        uint32_t packed = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            // ceil(hi / S), or -floor(lo / S) = ceil(-lo / S), rounded outwards
+            const float code = fminf(__builtin_ceilf(n[c] / scale), 127.0f);
+            packed |= ((uint32_t)(int)(least ? -code : code) & 0xffu) << (8 * c);
+        }
+        if (lane % kSplit < LPR)
+            *reinterpret_cast<uint32_t *>(a.bounds + slot * 2 * D + (least ? D : 0) +
+                                          (upper ? D / 2 : 0) + 4 * j) = packed;
+        if (lane == 0) a.scales[slot] = scale;
     }
-    constexpr int kSplit = BITS == 4 ? 16 : 32;  // lanes of one bound (and half)
-#pragma unroll
-    for (int o = LPR; o < kSplit; o <<= 1)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) n[c] = fmaxf(n[c], __shfl_xor(n[c], o));
-    const float top = wave_max(fmaxf(fmaxf(n[0], n[1]), fmaxf(n[2], n[3])));
-    const float scale = int8_scale(top);
-    uint32_t packed = 0;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        // ceil(hi / S), or -floor(lo / S) = ceil(-lo / S), rounded outwards
-        const float code = fminf(__builtin_ceilf(n[c] / scale), 127.0f);
-        packed |= ((uint32_t)(int)(least ? -code : code) & 0xffu) << (8 * c);
-    }
-    if (lane % kSplit < LPR)
-        *reinterpret_cast<uint32_t *>(a.bounds + slot * 2 * D + (least ? D : 0) +
-                                      (upper ? D / 2 : 0) + 4 * j) = packed;
-    if (lane == 0) a.scales[slot] = scale;
 }
 
 template <int BITS>
@@ -142,7 +177,9 @@ reef_status launch_bounds(const reef_kv_append_params *p, const int32_t *start, 
         p->max_context % kPage != 0)
         return REEF_INVALID_ARGUMENT;
     if (p->new_tokens > p->max_context) return REEF_CAPACITY;
-    const int64_t groups = ceil_div(ceil_div(p->new_tokens, kPage) + 1, kBoundWaves);
+    const int64_t pages = ceil_div(p->new_tokens, kPage) + 1;  // that T tokens may fall in
+    const int64_t turns = pages * p->batch * p->kv_heads > kBoundFill * kBoundPages ? kBoundPages : 1;
+    const int64_t groups = ceil_div(pages, kBoundWaves * turns);
     if ((p->head_dim != 64 && p->head_dim != 128) || p->max_context >= (int64_t(1) << 30) ||
         p->batch > 65535 || p->kv_heads > 65535 || groups > kGridMost256)
         return REEF_UNSUPPORTED;
@@ -165,6 +202,7 @@ reef_status launch_bounds(const reef_kv_append_params *p, const int32_t *start, 
     a.max_context = (int32_t)p->max_context;
     a.max_blocks = (int32_t)(block_table ? max_blocks_per_seq : 0);
     a.num_pages = (int32_t)(block_table ? num_pages : 0);
+    a.turns = (int32_t)turns;
     a.status = status_word;
     const dim3 grid((unsigned)groups, (unsigned)p->kv_heads, (unsigned)p->batch);
     if (p->head_dim == 128)
@@ -297,79 +335,206 @@ __global__ __launch_bounds__(kScoreWaves * kWave) void score_pages(SelectArgs a)
     if (first + lane < n) a.keys[(int64_t)item * a.max_pages + first + lane] = key;
 }
 
-// Sums of two counts over the workgroup's waves, and over those before this one (through LDS).
-struct PickCounts {
-    int before0, before1, total0, total1;
+constexpr int kDigit = 8, kBins = 1 << kDigit;
+constexpr int kDigits = (32 + kDigit - 1) / kDigit;
+
+struct PickShared {
+    int bins[kDigits][kBins];  // keys of each value of a digit
+    uint32_t all, any;         // bits of all scores, of any
+    int always;                // pages that are taken whatever the scores
+    uint32_t least;            // the last key so far, and the keys beyond its digit's value
+    int above, done;
+    int2 counts[kPickWaves];
 };
-__device__ __forceinline__ PickCounts pick_counts(int c0, int c1, int2 *sC, int wave, int lane) {
-    __syncthreads();
-    if (lane == 0) sC[wave] = make_int2(c0, c1);
-    __syncthreads();
-    PickCounts r = {0, 0, 0, 0};
+
+// Wave 0, after a count of a digit (`shift` bits below it): the largest value that `rem` keys of
+// the range reach, or exactly so many. Lane l holds the values 4 l .. 4 l + 3 from the top.
+__device__ __forceinline__ void pick_digit(PickShared &sh, const int *bins, uint32_t least, int shift,
+                                           int above, int rem, int lane) {
+    int c[4], sum = 0;
 #pragma unroll
-    for (int w = 0; w < kPickWaves; ++w) {
-        const int2 x = sC[w];
-        if (w < wave) {
-            r.before0 += x.x;
-            r.before1 += x.y;
-        }
-        r.total0 += x.x;
-        r.total1 += x.y;
+    for (int i = 0; i < 4; ++i) {
+        c[i] = bins[kBins - 1 - (4 * lane + i)];
+        sum += c[i];
     }
-    return r;
+    int upto = sum;  // of this lane's values and those above
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(upto, o);
+        if (lane >= o) upto += y;
+    }
+    const uint64_t enough = __builtin_amdgcn_ballot_w64(upto >= rem);
+    if (enough == 0) {  // fewer than that in all: every one of them
+        if (lane == 0) {
+            sh.least = least;
+            sh.done = 1;
+        }
+        return;
+    }
+    if (lane != __builtin_ctzll(enough)) return;
+    int run = upto - sum;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (run + c[i] >= rem) {
+            sh.least = least | (uint32_t)(kBins - 1 - (4 * lane + i)) << shift;
+            sh.above = above + run;
+            sh.done = run + c[i] == rem ? 1 : 0;
+            break;
+        }
+        run += c[i];
+    }
 }
 
-// One workgroup an item: the budget-th largest key bit by bit (the largest T that at least
-// budget keys reach), then the pages above it and the first of those at it, in page order. Wave w
-// holds a run of pages, 64 at a time.
-__global__ __launch_bounds__(kPickThreads) void pick_pages(SelectArgs a) {
-    __shared__ int2 sC[kPickWaves];
+// Keys of the pages that a thread holds: page first + 64 r + lane for r < R. In registers where a
+// sequence has up to 1024 R pages, read again at each use where it has more.
+template <int R>
+struct HeldKeys {
+    uint32_t key[R];
+    __device__ __forceinline__ HeldKeys(const uint32_t *keys, int first, int n, int lane) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int i = first + 64 * r + lane;
+            key[r] = i < n ? keys[i] : kNever;
+        }
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+        for (int r = 0; r < R; ++r) f(r, key[r]);
+    }
+};
+template <>
+struct HeldKeys<0> {
+    const uint32_t *keys;
+    int first, n, lane, rounds;
+    __device__ __forceinline__ HeldKeys(const uint32_t *k, int f, int count, int l)
+        : keys(k), first(f), n(count), lane(l), rounds((count + kPickThreads - 1) / kPickThreads) {}
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+        for (int r = 0; r < rounds; ++r) {
+            const int i = first + 64 * r + lane;
+            f(r, i < n ? keys[i] : kNever);
+        }
+    }
+};
+
+// The budget-th largest of an item's n keys, then the pages above it and the first of those at it,
+// in page order. Wave w holds a run of pages, 64 at a time. The last key taken is found digit by
+// digit from the highest bit in which scores differ (they share sign and most of the exponent): the
+// keys of the range so far are counted by the digit's value in LDS, and the first value that enough
+// of them reach is the next range, until exactly enough do. Two digits mostly: 3 us for 8192 pages
+// (bit by bit 11, with a pass over the keys in memory a bit 62).
+template <int R>
+__device__ __forceinline__ void pick(const SelectArgs &a, int item, int n, const uint32_t *keys,
+                                     PickShared &sh) {
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int item = blockIdx.x, b = item / a.kv_heads;
-    const int n = item_pages(a, b);
-    int32_t *list = a.pages + (int64_t)item * a.budget;
-    if (n == 0 && threadIdx.x == 0 && item == b * a.kv_heads)
-        flag_status(a.status, REEF_STATUS_BIT_BAD_LENGTH);
-    const uint32_t *keys = a.keys + (int64_t)item * a.max_pages;
-    const int rounds = (n + kPickThreads - 1) / kPickThreads;
+    const int rounds = R ? R : (n + kPickThreads - 1) / kPickThreads;
     const int first = wave * rounds * kWave;
-    auto key_at = [&](int r) {
-        const int i = first + r * kWave + lane;
-        return i < n ? keys[i] : kNever;
-    };
-    // the number of keys at or above t, at most the budget of them needed
+    const HeldKeys<R> held(keys, first, n, lane);
     uint32_t t = kNever;
-    for (int bit = 31; bit >= 0 && n > a.budget; --bit) {
-        const uint32_t trial = t | (1u << bit);
-        int c = 0;
-        for (int r = 0; r < rounds; ++r)
-            c += __popcll(__builtin_amdgcn_ballot_w64(key_at(r) >= trial));
-        if (pick_counts(c, 0, sC, wave, lane).total0 >= a.budget) t = trial;
+    if (n > a.budget) {
+        uint32_t all = ~0u, any = 0;
+        int always = 0;
+        held.each([&](int, uint32_t key) {
+            if (key != kNever && key != kAlways) {
+                all &= key;
+                any |= key;
+            }
+            always += __popcll(__builtin_amdgcn_ballot_w64(key == kAlways));
+        });
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            all &= (uint32_t)__shfl_xor((int)all, o);
+            any |= (uint32_t)__shfl_xor((int)any, o);
+        }
+        if (lane == 0) {
+            atomicAnd(&sh.all, all);
+            atomicOr(&sh.any, any);
+            if (always) atomicAdd(&sh.always, always);
+        }
+        __syncthreads();
+        all = __builtin_amdgcn_readfirstlane(sh.all);
+        any = __builtin_amdgcn_readfirstlane(sh.any);
+        int above = __builtin_amdgcn_readfirstlane(sh.always);
+        const uint32_t differ = all ^ any;
+        int left = differ ? 32 - __builtin_clz(differ) : 0;  // bits below those that all share
+        t = left == 32 ? 0 : all & ~0u << left;
+        if (above >= a.budget) {  // no score matters (positive NaNs count as always taken)
+            t = kAlways;
+            left = 0;
+        }
+#pragma unroll
+        for (int digit = 0; digit < kDigits; ++digit) {
+            if (left == 0) break;
+            const int shift = max(left - kDigit, 0);
+            held.each([&](int, uint32_t key) {
+                // (a digit of fewer bits at the end: values below kBins all the same)
+                if (key != kNever && key != kAlways && (left == 32 || (key ^ t) >> left == 0))
+                    atomicAdd(&sh.bins[digit][(key - t) >> shift], 1);
+            });
+            __syncthreads();
+            if (wave == 0) pick_digit(sh, sh.bins[digit], t, shift, above, a.budget - above, lane);
+            __syncthreads();
+            t = (uint32_t)__builtin_amdgcn_readfirstlane((int)sh.least);
+            above = __builtin_amdgcn_readfirstlane(sh.above);
+            if (__builtin_amdgcn_readfirstlane(sh.done)) break;
+            left = shift;
+        }
     }
-    // above the last key, and at it (a page that cannot be taken never is)
+    // the pages above the last key, and those at it (a page that cannot be taken never is)
     int above = 0, at = 0;
-    for (int r = 0; r < rounds; ++r) {
-        const uint32_t key = key_at(r);
+    held.each([&](int, uint32_t key) {
         above += __popcll(__builtin_amdgcn_ballot_w64(key > t));
         at += __popcll(__builtin_amdgcn_ballot_w64(key == t && key != kNever));
+    });
+    if (lane == 0) sh.counts[wave] = make_int2(above, at);
+    __syncthreads();
+    int before0 = 0, before1 = 0, total0 = 0, total1 = 0;
+#pragma unroll
+    for (int w = 0; w < kPickWaves; ++w) {
+        const int2 x = sh.counts[w];
+        before0 += w < wave ? x.x : 0;
+        before1 += w < wave ? x.y : 0;
+        total0 += x.x;
+        total1 += x.y;
     }
-    const PickCounts c = pick_counts(above, at, sC, wave, lane);
-    const int need = min(a.budget - c.total0, c.total1);  // of those at it
-    int out = c.before0 + min(c.before1, need), ties = c.before1;
+    const int need = min(a.budget - total0, total1);  // of those at it
+    int out = before0 + min(before1, need), ties = before1;
+    int32_t *list = a.pages + (int64_t)item * a.budget;
     const uint64_t below = (uint64_t(1) << lane) - 1;
-    for (int r = 0; r < rounds; ++r) {
-        const uint32_t key = key_at(r);
+    held.each([&](int r, uint32_t key) {
         const uint64_t eq = __builtin_amdgcn_ballot_w64(key == t && key != kNever);
         const bool take = key > t || ((eq >> lane & 1) && ties + __popcll(eq & below) < need);
         const uint64_t taken = __builtin_amdgcn_ballot_w64(take);
         if (take) list[out + __popcll(taken & below)] = first + r * kWave + lane;
         out += __popcll(taken);
         ties += __popcll(eq);
-    }
-    const int count = c.total0 + need;
+    });
+    const int count = total0 + need;
     for (int i = count + threadIdx.x; i < a.budget; i += kPickThreads) list[i] = -1;
     if (threadIdx.x == 0) a.counts[item] = count;
+}
+
+// One workgroup an item.
+__global__ __launch_bounds__(kPickThreads) void pick_pages(SelectArgs a) {
+    __shared__ PickShared sh;
+    const int tid = threadIdx.x;
+    for (int i = tid; i < kDigits * kBins; i += kPickThreads) sh.bins[0][i] = 0;
+    if (tid == 0) {
+        sh.all = ~0u;
+        sh.any = 0;
+        sh.always = 0;
+    }
+    const int item = blockIdx.x, b = item / a.kv_heads;
+    const int n = item_pages(a, b);
+    if (n == 0 && tid == 0 && item == b * a.kv_heads)
+        flag_status(a.status, REEF_STATUS_BIT_BAD_LENGTH);
+    const uint32_t *keys = a.keys + (int64_t)item * a.max_pages;
+    __syncthreads();
+    if (n <= 2 * kPickThreads) pick<2>(a, item, n, keys, sh);
+    else if (n <= 8 * kPickThreads) pick<8>(a, item, n, keys, sh);
+    else pick<0>(a, item, n, keys, sh);
 }
 
 bool select_sizes(const reef_decode_params *p) {
