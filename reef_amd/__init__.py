@@ -692,7 +692,7 @@ def _step_workspace(n, device, stream):
     in the graph's memory: graphs that replay at the same time share nothing. Only its
     counters have to be zero, the first 8 KB: not a megabyte of parts at every replay."""
     torch = _torch()
-    if torch.cuda.is_current_stream_capturing():
+    if torch._C._cuda_isCurrentStreamCapturing():
         ws = torch.empty(max(n, 8192), dtype=torch.uint8, device=device)
         ws[:8192].zero_()
         return ws
@@ -1080,40 +1080,50 @@ def kv_keep_paged(kept, kept_lens, context_lens, block_table, k_pages, v_pages, 
 # The codes' places in a byte: the C header. An int8 cache (int8 tensors, D for D/2 and 16 for 8)
 # takes the calls that are not named for 4 bits.
 
-def _cache(what, batch, k_cache, v_cache, k_scales, v_scales, block_table, bits):
-    """(heads, tokens a sequence, head_dim, table, blocks, pages) of either cache."""
-    torch = _torch()
-    dtype = torch.int8 if bits == 8 else torch.uint8
-    _expect(what, dtype, (k_cache, "k_cache"))
-    n = k_cache.numel()
-    if k_cache.dim() != 4:
+def _alike(what, *checks):
+    """(tensor, type, name): contiguous, of its type, on the current device. Tensors that are None
+    are left out."""
+    device = None
+    for t, dtype, name in checks:
+        if t is None:
+            continue
+        try:
+            at = t.get_device()
+            if at >= 0 and t.dtype is dtype and t.is_contiguous():
+                if device is None:
+                    device = _torch_module._C._cuda_getDevice()
+                if at == device:
+                    continue
+        except AttributeError:
+            pass
+        _require(t, dtype, name)
+        raise InvalidArgument(f"{what}: {name} must be contiguous and on the current GPU")
+
+
+def _cache_sizes(what, batch, k_cache, v_cache, k_scales, v_scales, block_table, bits):
+    """(heads, tokens a sequence, head_dim, blocks, pages) of either cache (tensors as _alike
+    leaves them)."""
+    shape = k_cache.shape
+    if len(shape) != 4:
         raise InvalidArgument(f"{what}: k_cache must have 4 dimensions")
-    lead, heads, tokens, row = k_cache.shape
-    head_dim = row * 8 // bits
-    if v_cache is not None:
-        _expect(what, dtype, (v_cache, "v_cache"))
-        if v_cache.numel() != n:
-            raise InvalidArgument(f"{what}: cache shape mismatch")
-    for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
-        if t is not None:
-            _expect(what, torch.float32, (t, name))
-            if t.numel() * row != n:
-                raise InvalidArgument(f"{what}: scales do not match the cache")
+    lead, heads, tokens, row = shape
+    rows = lead * heads * tokens
+    if v_cache is not None and v_cache.numel() != rows * row:
+        raise InvalidArgument(f"{what}: cache shape mismatch")
+    if k_scales.numel() != rows or (v_scales is not None and v_scales.numel() != rows):
+        raise InvalidArgument(f"{what}: scales do not match the cache")
     if block_table is None:
         if lead != batch or tokens % PAGE:
             raise InvalidArgument(f"{what}: cache shape mismatch")
-        return heads, tokens, head_dim, None, 0, 0
-    _expect(what, torch.int32, (block_table, "block_table"))
-    if block_table.dim() != 2 or block_table.shape[0] != batch or tokens != PAGE:
+        return heads, tokens, row * 8 // bits, 0, 0
+    table = block_table.shape
+    if len(table) != 2 or table[0] != batch or tokens != PAGE or not table[1]:
         raise InvalidArgument(f"{what}: block_table must be [B, max_blocks], pages of 16 tokens")
-    blocks = block_table.shape[1]
-    return heads, blocks * PAGE, head_dim, block_table.data_ptr(), blocks, lead
+    return heads, table[1] * PAGE, row * 8 // bits, table[1], lead
 
 
-def _lengths(what, t, batch, name="context_lens"):
-    _expect(what, _torch().int32, (t, name))
-    if t.shape != (batch,):
-        raise InvalidArgument(f"{what}: {name} must be [B]")
+def _scale_count(q_granularity, q_heads, rows):
+    return (rows if q_granularity == PER_TOKEN else q_heads if q_granularity == PER_HEAD else 1)
 
 
 def kv_append_int4(k_new, v_new, start_positions, k_cache, v_cache, k_scales, v_scales,
@@ -1121,22 +1131,26 @@ def kv_append_int4(k_new, v_new, start_positions, k_cache, v_cache, k_scales, v_
     """kv_append into the 4-bit cache: rows k_new, v_new [B, Hkv, T, D] fp32, one scale
     max|x| / 7 a row. context_lens, when given, is set to start_positions + T (it may be
     start_positions itself)."""
-    what = "kv_append_int4"
+    what, torch = "kv_append_int4", _torch()
     ks, vs = _append_inputs(k_new, v_new)
-    B, H, T, D = k_new.shape
-    heads, tokens, dim, table, blocks, pages = _cache(what, B, k_cache, v_cache, k_scales, v_scales,
-                                                      block_table, 4)
-    if (heads, dim) != (H, D):
-        raise InvalidArgument("KV cache append shape mismatch")
-    _lengths(what, start_positions, B, "start_positions")
-    if context_lens is not None:
-        _lengths(what, context_lens, B)
+    byte, f32, i32 = torch.uint8, torch.float32, torch.int32
+    _alike(what, (k_cache, byte, "k_cache"), (v_cache, byte, "v_cache"),
+           (k_scales, f32, "k_scales"), (v_scales, f32, "v_scales"),
+           (start_positions, i32, "start_positions"), (context_lens, i32, "context_lens"),
+           (block_table, i32, "block_table"))
     _on_device(what, k_new, v_new)
+    B, H, T, D = k_new.shape
+    heads, tokens, dim, blocks, pages = _cache_sizes(what, B, k_cache, v_cache, k_scales, v_scales,
+                                                     block_table, 4)
+    if heads != H or dim != D or start_positions.shape != (B,) or (
+            context_lens is not None and context_lens.shape != (B,)):
+        raise InvalidArgument("KV cache append shape mismatch")
     own = status or StatusWord(k_new.device)
     check(_lib().reef_kv_append_int4(
-        _packed(_APPEND, KvAppendParams, B, H, D, T, tokens), _ptr(k_new), ks, _ptr(v_new), vs,
-        _ptr(start_positions), table, blocks, pages, _ptr(k_cache), _ptr(v_cache), _ptr(k_scales),
-        _ptr(v_scales), _ptr(context_lens), _ptr(own.tensor), _stream()), what)
+        _packed(_APPEND, KvAppendParams, B, H, D, T, tokens), k_new.data_ptr(), ks,
+        v_new.data_ptr(), vs, start_positions.data_ptr(), _ptr(block_table), blocks, pages,
+        k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+        _ptr(context_lens), own.tensor.data_ptr(), _stream()), what)
     if status is None:
         own.check(what)
 
@@ -1145,21 +1159,22 @@ def kv_unpack_int4(k_cache, v_cache, k_scales, v_scales):
     """The 4-bit cache as fp32 rows by pages: keys and values [..., 16, D] each (contiguous:
     [B, Hkv, L/16, 16, D], a pool: [P, Hkv, 16, D]), float(code) * scale."""
     what, torch = "kv_unpack_int4", _torch()
-    _expect(what, torch.uint8, (k_cache, "k_cache"), (v_cache, "v_cache"))
-    _expect(what, torch.float32, (k_scales, "k_scales"), (v_scales, "v_scales"))
-    n = k_cache.numel()
-    if v_cache.dim() < 3 or v_cache.shape[-1] != PAGE // 2:
+    byte, f32 = torch.uint8, torch.float32
+    _alike(what, (k_cache, byte, "k_cache"), (v_cache, byte, "v_cache"),
+           (k_scales, f32, "k_scales"), (v_scales, f32, "v_scales"))
+    n, shape = k_cache.numel(), v_cache.shape
+    if len(shape) < 3 or shape[-1] != PAGE // 2:
         raise InvalidArgument(f"{what}: v_cache must be [..., D, 8]")
-    D = v_cache.shape[-2]
+    D = shape[-2]
     if v_cache.numel() != n or k_scales.numel() * D != 2 * n or v_scales.numel() * D != 2 * n:
         raise InvalidArgument(f"{what}: cache shape mismatch")
-    shape = (*v_cache.shape[:-2], PAGE, D)
-    k = torch.empty(shape, dtype=torch.float32, device=k_cache.device)
-    v = torch.empty(shape, dtype=torch.float32, device=k_cache.device)
+    shape = (*shape[:-2], PAGE, D)
+    k = torch.empty(shape, dtype=f32, device=k_cache.device)
+    v = torch.empty(shape, dtype=f32, device=k_cache.device)
     if n:
-        check(_lib().reef_kv_unpack_int4(_ptr(k_cache), _ptr(v_cache), _ptr(k_scales),
-                                         _ptr(v_scales), n // (PAGE // 2 * D), D, _ptr(k), _ptr(v),
-                                         _stream()), what)
+        check(_lib().reef_kv_unpack_int4(
+            k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+            n // (PAGE // 2 * D), D, k.data_ptr(), v.data_ptr(), _stream()), what)
     return k, v
 
 
@@ -1167,10 +1182,10 @@ def kv_copy_pages_int4(source, place, k_pages, v_pages, k_scale_pages, v_scale_p
                        status: StatusWord | None = None):
     """kv_copy_pages for one layer's 4-bit pool."""
     what, torch = "kv_copy_pages_int4", _torch()
-    _expect(what, torch.int32, (source, "source"), (place, "place"))
-    _expect(what, torch.uint8, (k_pages, "k_pages"), (v_pages, "v_pages"))
-    _expect(what, torch.float32, (k_scale_pages, "k_scale_pages"),
-            (v_scale_pages, "v_scale_pages"))
+    byte, f32, i32 = torch.uint8, torch.float32, torch.int32
+    _alike(what, (source, i32, "source"), (place, i32, "place"), (k_pages, byte, "k_pages"),
+           (v_pages, byte, "v_pages"), (k_scale_pages, f32, "k_scale_pages"),
+           (v_scale_pages, f32, "v_scale_pages"))
     if k_pages.dim() != 4 or k_pages.shape[2] != PAGE:
         raise InvalidArgument(f"{what}: k_pages must be [pages, heads, 16, head_dim / 2]")
     P, H, _, row = k_pages.shape
@@ -1189,51 +1204,64 @@ def kv_copy_pages_int4(source, place, k_pages, v_pages, k_scale_pages, v_scale_p
         own.check(what)
 
 
-def _decode_inputs(what, q, q_scales, q_granularity, head_dim, out):
-    torch = _torch()
-    _expect(what, torch.int8, (q, "q"))
-    _expect(what, torch.float32, (q_scales, "q_scales"))
-    if q.dim() != 3 or q.shape[2] != head_dim:
-        raise InvalidArgument(f"{what}: q must be [B, heads, head_dim of the cache]")
-    B, Hq, _ = q.shape
-    scales = B * Hq if q_granularity == PER_TOKEN else Hq if q_granularity == PER_HEAD else 1
-    if q_scales.numel() != scales:
-        raise InvalidArgument(f"{what}: q_scales do not match q_granularity")
-    if out is None:
-        return torch.empty(q.shape, dtype=torch.float32, device=q.device)
-    _expect(what, torch.float32, (out, "out"))
-    if out.shape != q.shape:
-        raise InvalidArgument(f"{what}: out must have q's shape")
-    return out
+_DECODE_BYTES = {}
+
+
+def _decode_workspace_bytes(p):
+    """Workspace bytes of a decode call of these (packed) sizes."""
+    n = _DECODE_BYTES.get(p)
+    if n is None:
+        n = _lib().reef_attention_decode_workspace_bytes(p)
+        if isinstance(p, bytes) and len(_DECODE_BYTES) < 4096:
+            _DECODE_BYTES[p] = n
+    return n
 
 
 def _decode_cache(what, function, bits, q, q_scales, k_cache, v_cache, k_scales, v_scales,
                   context_lens, selected, block_table, window, softmax_scale, q_granularity,
                   num_splits, workspace, status, out):
-    _require(q, _torch().int8, "q")
-    B = q.shape[0]
-    heads, tokens, dim, table, blocks, pages = _cache(what, B, k_cache, v_cache, k_scales, v_scales,
-                                                      block_table, bits)
-    out = _decode_inputs(what, q, q_scales, q_granularity, dim, out)
-    if context_lens is not None:
-        _lengths(what, context_lens, B)
-    elif block_table is not None or selected is not None:
-        raise InvalidArgument(f"{what}: a paged cache and selected pages need context_lens")
-    listed = None
+    torch = _torch()
+    code, f32, i32 = torch.int8 if bits == 8 else torch.uint8, torch.float32, torch.int32
+    chosen = counts = listed = None
     if selected is not None:
-        list_, counts = selected
-        _expect(what, _torch().int32, (list_, "selected pages"), (counts, "selected counts"))
-        if list_.dim() != 3 or list_.shape[:2] != (B, heads) or counts.shape != (B, heads):
+        chosen, counts = selected
+    _alike(what, (q, torch.int8, "q"), (q_scales, f32, "q_scales"), (k_cache, code, "k_cache"),
+           (v_cache, code, "v_cache"), (k_scales, f32, "k_scales"), (v_scales, f32, "v_scales"),
+           (context_lens, i32, "context_lens"), (block_table, i32, "block_table"),
+           (chosen, i32, "selected pages"), (counts, i32, "selected counts"), (out, f32, "out"))
+    shape = q.shape
+    if len(shape) != 3:
+        raise InvalidArgument(f"{what}: q must be [B, heads, head_dim]")
+    B, Hq, D = shape
+    heads, tokens, dim, blocks, pages = _cache_sizes(what, B, k_cache, v_cache, k_scales, v_scales,
+                                                     block_table, bits)
+    if dim != D:
+        raise InvalidArgument(f"{what}: q must have the cache's head_dim")
+    if q_scales.numel() != _scale_count(q_granularity, Hq, B * Hq):
+        raise InvalidArgument(f"{what}: q_scales do not match q_granularity")
+    if context_lens is not None:
+        if context_lens.shape != (B,):
+            raise InvalidArgument(f"{what}: context_lens must be [B]")
+    elif block_table is not None or chosen is not None:
+        raise InvalidArgument(f"{what}: a paged cache and selected pages need context_lens")
+    if chosen is not None:
+        n = chosen.shape
+        if len(n) != 3 or n[:2] != (B, heads) or counts.shape != (B, heads):
             raise InvalidArgument(f"{what}: selected must be pages [B, heads, n], counts [B, heads]")
-        listed = _SELECTION.pack(list_.data_ptr(), counts.data_ptr(), list_.shape[2])
+        listed = _SELECTION.pack(chosen.data_ptr(), counts.data_ptr(), n[2])
+    if out is None:
+        out = torch.empty(shape, dtype=f32, device=q.device)
+    elif out.shape != shape:
+        raise InvalidArgument(f"{what}: out must have q's shape")
     p = _decode_bytes(q, tokens, heads, window, softmax_scale, q_granularity, num_splits)
     stream = _stream()
-    n = _lib().reef_attention_decode_workspace_bytes(p)
-    ws = _step_workspace(n, q.device, stream) if workspace is None else _given(workspace)
+    ws = (_step_workspace(_decode_workspace_bytes(p), q.device, stream) if workspace is None
+          else _given(workspace))
     own = status or StatusWord(q.device)
-    check(function(p, _ptr(q), _ptr(q_scales), _ptr(k_cache), _ptr(v_cache), _ptr(k_scales),
-                   _ptr(v_scales), table, blocks, pages, _ptr(context_lens), listed, _ptr(out),
-                   _ptr(ws), ws.numel() * ws.element_size(), _ptr(own.tensor), stream), what)
+    check(function(p, q.data_ptr(), q_scales.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                   k_scales.data_ptr(), v_scales.data_ptr(), _ptr(block_table), blocks, pages,
+                   _ptr(context_lens), listed, out.data_ptr(), ws.data_ptr(),
+                   ws.numel() * ws.element_size(), own.tensor.data_ptr(), stream), what)
     if status is None:
         own.check(what)
     return out
@@ -1273,14 +1301,16 @@ def attention_prefill_cache_int4(q, q_scales, k_cache, v_cache, k_scales, v_scal
     (kv_append_int4): q [B, Hq, q_len, D] int8, kv_len tokens a sequence. Returns fp32
     [B, Hq, q_len, D]."""
     what, torch = "attention_prefill_cache_int4", _torch()
+    byte, f32 = torch.uint8, torch.float32
     _require(q, torch.int8, "q")
-    _expect(what, torch.float32, (q_scales, "q_scales"))
+    _alike(what, (q_scales, f32, "q_scales"), (k_cache, byte, "k_cache"),
+           (v_cache, byte, "v_cache"), (k_scales, f32, "k_scales"), (v_scales, f32, "v_scales"),
+           (block_table, torch.int32, "block_table"))
     qs = _strides4(q)
-    B, Hq, Sq, D = q.shape
-    heads, tokens, dim, table, blocks, pages = _cache(what, B, k_cache, v_cache, k_scales, v_scales,
-                                                      block_table, 4)
-    scales = B * Hq * Sq if q_granularity == PER_TOKEN else Hq if q_granularity == PER_HEAD else 1
-    if dim != D or q_scales.numel() != scales:
+    shape = B, Hq, Sq, D = q.shape
+    heads, tokens, dim, blocks, pages = _cache_sizes(what, B, k_cache, v_cache, k_scales, v_scales,
+                                                     block_table, 4)
+    if dim != D or q_scales.numel() != _scale_count(q_granularity, Hq, B * Hq * Sq):
         raise InvalidArgument(f"{what}: q and q_scales do not match the cache and q_granularity")
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(D)
@@ -1288,10 +1318,10 @@ def attention_prefill_cache_int4(q, q_scales, k_cache, v_cache, k_scales, v_scal
     p = _packed(_ATTENTION, AttentionParams, B, Hq, heads, Sq, kv_len, D, start, window,
                 softmax_scale, q_granularity, PER_TOKEN, 0)
     if out is None:
-        out = torch.empty((B, Hq, Sq, D), dtype=torch.float32, device=q.device)
+        out = torch.empty(shape, dtype=f32, device=q.device)
     else:
-        _require(out, torch.float32, "out")
-        if out.shape != q.shape:
+        _require(out, f32, "out")
+        if out.shape != shape:
             raise InvalidArgument(f"{what}: out must have q's shape")
     _on_device(what, q, out)
     stream = _stream()
@@ -1299,9 +1329,9 @@ def attention_prefill_cache_int4(q, q_scales, k_cache, v_cache, k_scales, v_scal
     ws = _chunk_workspace(n, q.device, stream)
     own = status or StatusWord(q.device)
     check(_lib().reef_attention_prefill_int4_cache(
-        p, _ptr(q), qs, _ptr(q_scales), _ptr(k_cache), _ptr(v_cache), _ptr(k_scales),
-        _ptr(v_scales), tokens, table, blocks, pages, _ptr(out), _strides4(out), _ptr(ws), n,
-        _ptr(own.tensor), stream), what)
+        p, q.data_ptr(), qs, q_scales.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+        k_scales.data_ptr(), v_scales.data_ptr(), tokens, _ptr(block_table), blocks, pages,
+        out.data_ptr(), _strides4(out), ws.data_ptr(), n, own.tensor.data_ptr(), stream), what)
     if status is None:
         own.check(what)
     return out
@@ -1311,7 +1341,7 @@ def _chunk_workspace(n, device, stream):
     """attention_prefill_cache's workspace of this stream; under graph capture one of its own, of
     which the counters alone (65536 words in front) have to be zero."""
     torch = _torch()
-    if torch.cuda.is_current_stream_capturing():
+    if torch._C._cuda_isCurrentStreamCapturing():
         ws = torch.empty(max(n, 1 << 18), dtype=torch.uint8, device=device)
         ws[:1 << 18].zero_()
         return ws
@@ -1322,16 +1352,6 @@ def _chunk_workspace(n, device, stream):
     return ws
 
 
-def _bounds(what, bounds, bound_scales, head_dim, pages):
-    torch = _torch()
-    _expect(what, torch.int8, (bounds, "bounds"))
-    _expect(what, torch.float32, (bound_scales, "bound_scales"))
-    if bounds.shape[-2:] != (2, head_dim) or bounds.numel() != pages * 2 * head_dim or (
-            bound_scales.numel() != pages):
-        raise InvalidArgument(f"{what}: bounds must be [..., pages, 2, head_dim], bound_scales one "
-                              "a page and head")
-
-
 def kv_page_bounds(start_positions, new_tokens: int, k_cache, k_scales, bounds, bound_scales, *,
                    block_table=None, status: StatusWord | None = None):
     """The largest and the least key of every channel of the pages that tokens start_positions[b]
@@ -1339,21 +1359,29 @@ def kv_page_bounds(start_positions, new_tokens: int, k_cache, k_scales, bounds, 
     them: call it after an append, with its start positions. k_cache and k_scales of an int8 or
     a 4-bit cache; bounds int8 [B, Hkv, L/16, 2, D] and bound_scales [B, Hkv, L/16] (contiguous)
     or [P, Hkv, 2, D] and [P, Hkv] (a pool) are written in place."""
-    what = "kv_page_bounds"
-    torch = _torch()
-    _expect(what, torch.int32, (start_positions, "start_positions"))
-    if start_positions.dim() != 1:
+    what, torch = "kv_page_bounds", _torch()
+    int4 = getattr(k_cache, "dtype", None) is torch.uint8
+    f32, i32 = torch.float32, torch.int32
+    _alike(what, (start_positions, i32, "start_positions"),
+           (k_cache, torch.uint8 if int4 else torch.int8, "k_cache"), (k_scales, f32, "k_scales"),
+           (bounds, torch.int8, "bounds"), (bound_scales, f32, "bound_scales"),
+           (block_table, i32, "block_table"))
+    shape = start_positions.shape
+    if len(shape) != 1:
         raise InvalidArgument(f"{what}: start_positions must be [B]")
-    B = start_positions.shape[0]
-    bits = 4 if k_cache.dtype is torch.uint8 else 8
-    heads, tokens, dim, table, blocks, pages = _cache(what, B, k_cache, None, k_scales, None,
-                                                      block_table, bits)
-    _bounds(what, bounds, bound_scales, dim, heads * (pages if table else B * tokens // PAGE))
+    B = shape[0]
+    heads, tokens, dim, blocks, pages = _cache_sizes(what, B, k_cache, None, k_scales, None,
+                                                     block_table, 4 if int4 else 8)
+    held = heads * (B * tokens // PAGE if block_table is None else pages)
+    if bounds.numel() != held * 2 * dim or bound_scales.numel() != held:
+        raise InvalidArgument(f"{what}: bounds must hold 2 rows, bound_scales one scale a page and "
+                              "head")
     own = status or StatusWord(k_cache.device)
-    function = _lib().reef_kv_page_bounds_int4 if bits == 4 else _lib().reef_kv_page_bounds_int8
+    function = _lib().reef_kv_page_bounds_int4 if int4 else _lib().reef_kv_page_bounds_int8
     check(function(_packed(_APPEND, KvAppendParams, B, heads, dim, new_tokens, tokens),
-                   _ptr(start_positions), _ptr(k_cache), _ptr(k_scales), table, blocks, pages,
-                   _ptr(bounds), _ptr(bound_scales), _ptr(own.tensor), _stream()), what)
+                   start_positions.data_ptr(), k_cache.data_ptr(), k_scales.data_ptr(),
+                   _ptr(block_table), blocks, pages, bounds.data_ptr(), bound_scales.data_ptr(),
+                   own.tensor.data_ptr(), _stream()), what)
     if status is None:
         own.check(what)
 
@@ -1367,44 +1395,46 @@ def kv_select_pages(q, q_scales, bounds, bound_scales, context_lens, budget: int
     (pages [B, Hkv, budget] int32, ascending, -1 behind the last; counts [B, Hkv] int32), the
     `selected` of attention_decode_selected and attention_decode_int4."""
     what, torch = "kv_select_pages", _torch()
-    _require(q, torch.int8, "q")
-    if q.dim() != 3:
+    f32, i32 = torch.float32, torch.int32
+    _alike(what, (q, torch.int8, "q"), (q_scales, f32, "q_scales"), (bounds, torch.int8, "bounds"),
+           (bound_scales, f32, "bound_scales"), (context_lens, i32, "context_lens"),
+           (block_table, i32, "block_table"))
+    shape, form = q.shape, bounds.shape
+    if len(shape) != 3:
         raise InvalidArgument(f"{what}: q must be [B, heads, head_dim]")
-    B, Hq, D = q.shape
-    if bounds.dim() not in (4, 5):
-        raise InvalidArgument(f"{what}: bounds must be [B, heads, pages, 2, D] or [P, heads, 2, D]")
-    heads = bounds.shape[1]
+    B, Hq, D = shape
     if block_table is None:
-        if bounds.dim() != 5 or bounds.shape[0] != B:
-            raise InvalidArgument(f"{what}: bounds must be [B, heads, pages, 2, D]")
-        tokens, table, blocks, pages = bounds.shape[2] * PAGE, None, 0, 0
-        held = B * heads * bounds.shape[2]
+        if len(form) != 5 or form[0] != B or form[3:] != (2, D):
+            raise InvalidArgument(f"{what}: bounds must be [B, heads, pages, 2, head_dim]")
+        heads, tokens, blocks, pages = form[1], form[2] * PAGE, 0, 0
+        held = B * heads * form[2]
     else:
-        _expect(what, torch.int32, (block_table, "block_table"))
-        if bounds.dim() != 4 or block_table.dim() != 2 or block_table.shape[0] != B:
-            raise InvalidArgument(f"{what}: bounds must be [P, heads, 2, D], block_table "
+        table = block_table.shape
+        if len(form) != 4 or form[2:] != (2, D) or len(table) != 2 or table[0] != B or not table[1]:
+            raise InvalidArgument(f"{what}: bounds must be [P, heads, 2, head_dim], block_table "
                                   "[B, max_blocks]")
-        blocks, pages = block_table.shape[1], bounds.shape[0]
-        tokens, table, held = blocks * PAGE, block_table.data_ptr(), pages * heads
-    _bounds(what, bounds, bound_scales, D, held)
-    _lengths(what, context_lens, B)
-    _expect(what, torch.int8, (q, "q"))
-    _expect(what, torch.float32, (q_scales, "q_scales"))
-    scales = B * Hq if q_granularity == PER_TOKEN else Hq if q_granularity == PER_HEAD else 1
-    if q_scales.numel() != scales:
+        pages, heads, blocks = form[0], form[1], table[1]
+        tokens, held = blocks * PAGE, pages * heads
+    if bound_scales.numel() != held:
+        raise InvalidArgument(f"{what}: bound_scales must hold one scale a page and head")
+    if context_lens.shape != (B,):
+        raise InvalidArgument(f"{what}: context_lens must be [B]")
+    if q_scales.numel() != _scale_count(q_granularity, Hq, B * Hq):
         raise InvalidArgument(f"{what}: q_scales do not match q_granularity")
     if budget < 1 or heads < 1:
         raise InvalidArgument(f"{what}: no pages to select")
-    p = _decode_bytes(q, tokens, heads, 0, None, q_granularity, 0)
+    p = _decode_bytes(q, tokens, heads, 0, 1.0, q_granularity, 0)
     n = _lib().reef_kv_select_pages_workspace_bytes(p)
-    ws = torch.empty(n // 4 + 4, dtype=torch.int32, device=q.device)
-    chosen = torch.empty((B, heads, budget), dtype=torch.int32, device=q.device)
-    counts = torch.empty((B, heads), dtype=torch.int32, device=q.device)
-    own = status or StatusWord(q.device)
+    device = q.device
+    ws = torch.empty(n // 4, dtype=i32, device=device)
+    chosen = torch.empty((B, heads, budget), dtype=i32, device=device)
+    counts = torch.empty((B, heads), dtype=i32, device=device)
+    own = status or StatusWord(device)
     check(_lib().reef_kv_select_pages(
-        p, _ptr(q), _ptr(q_scales), _ptr(bounds), _ptr(bound_scales), table, blocks, pages,
-        _ptr(context_lens), budget, sinks, recent, _ptr(chosen), _ptr(counts), _ptr(ws), n,
-        _ptr(own.tensor), _stream()), what)
+        p, q.data_ptr(), q_scales.data_ptr(), bounds.data_ptr(), bound_scales.data_ptr(),
+        _ptr(block_table), blocks, pages, context_lens.data_ptr(), budget, sinks, recent,
+        chosen.data_ptr(), counts.data_ptr(), ws.data_ptr(), n, own.tensor.data_ptr(), _stream()),
+        what)
     if status is None:
         own.check(what)
     return chosen, counts

@@ -111,8 +111,8 @@ __global__ __launch_bounds__(kBoundWaves * kWave) void page_bounds(BoundArgs a) 
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
                     const float x = key(i, c), y = key(i + 1, c);
-                    hi[c] = fmaxf(hi[c], fmaxf(x, y));
-                    lo[c] = fminf(lo[c], fminf(x, y));
+                    hi[c] = i ? fmaxf(fmaxf(hi[c], x), y) : fmaxf(x, y);
+                    lo[c] = i ? fminf(fminf(lo[c], x), y) : fminf(x, y);
                 }
             }
         } else {
@@ -128,30 +128,32 @@ __global__ __launch_bounds__(kBoundWaves * kWave) void page_bounds(BoundArgs a) 
             }
         }
         // Lanes 0-31 go on with the largest, the others with the least, negated: maxima either way.
+        // A swap of halves leaves a lane its own and its partner's of what it goes on with.
+        auto meet = [](auto r) { return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])); };
         const bool least = lane >= 32;
         float m[C];
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const float got = __shfl_xor(least ? hi[c] : -lo[c], 32);
-            m[c] = fmaxf(least ? -lo[c] : hi[c], got);
-        }
+        for (int c = 0; c < C; ++c)
+            m[c] = meet(__builtin_amdgcn_permlane32_swap(__float_as_uint(hi[c]), __float_as_uint(-lo[c]),
+                                                         false, false));
         float n[4];
         const bool upper = BITS == 4 && (lane & 16);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            if constexpr (BITS == 4) {
-                const float got = __shfl_xor(upper ? m[c] : m[C - 4 + c], 16);
-                n[c] = fmaxf(upper ? m[C - 4 + c] : m[c], got);
-            } else {
-                n[c] = m[c];
-            }
+            if constexpr (BITS == 4)
+                n[c] = meet(__builtin_amdgcn_permlane16_swap(
+                    __float_as_uint(m[c]), __float_as_uint(m[C - 4 + c]), false, false));
+            else
+                n[c] = D == 64 ? xor16_max(m[c]) : m[c];
+            if constexpr (BITS == 4 && D == 64)
+                n[c] = fmaxf(n[c], __int_as_float(__builtin_amdgcn_mov_dpp(
+                                       __float_as_int(n[c]), 0x128, 0xf, 0xf, true)));  // row_ror 8
         }
         constexpr int kSplit = BITS == 4 ? 16 : 32;  // lanes of one bound (and half)
-#pragma unroll
-        for (int o = LPR; o < kSplit; o <<= 1)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) n[c] = fmaxf(n[c], __shfl_xor(n[c], o));
-        const float top = wave_max(fmaxf(fmaxf(n[0], n[1]), fmaxf(n[2], n[3])));
+        const float top = __uint_as_float(wave_reduce(
+            __float_as_uint(fmaxf(fmaxf(n[0], n[1]), fmaxf(n[2], n[3]))), [](uint32_t x, uint32_t y) {
+                return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y)));
+            }));
         const float scale = int8_scale(top);
         uint32_t packed = 0;
 #pragma unroll
@@ -443,11 +445,8 @@ __device__ __forceinline__ void pick(const SelectArgs &a, int item, int n, const
             }
             always += __popcll(__builtin_amdgcn_ballot_w64(key == kAlways));
         });
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            all &= (uint32_t)__shfl_xor((int)all, o);
-            any |= (uint32_t)__shfl_xor((int)any, o);
-        }
+        all = wave_reduce(all, [](uint32_t x, uint32_t y) { return x & y; });
+        any = wave_reduce(any, [](uint32_t x, uint32_t y) { return x | y; });
         if (lane == 0) {
             atomicAnd(&sh.all, all);
             atomicOr(&sh.any, any);

@@ -94,6 +94,20 @@ __device__ __forceinline__ float xor32_sum(float x) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// f over all 64 lanes of an associative and commutative f on 32-bit words, in every lane, in VALU
+// ops: four rotations within a row of 16 and two swaps of halves.
+template <typename F>
+__device__ __forceinline__ uint32_t wave_reduce(uint32_t x, F f) {
+    x = f(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x128, 0xf, 0xf, true));  // row_ror 8
+    x = f(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x124, 0xf, 0xf, true));
+    x = f(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x122, 0xf, 0xf, true));
+    x = f(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x121, 0xf, 0xf, true));
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = f(r[0], r[1]);
+    const auto s = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return f(s[0], s[1]);
+}
+
 // A raw buffer resource over [base, base + bytes): loads through it take a
 // per-lane VGPR offset and a uniform SGPR offset, and read zeros past the end.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_rsrc(const void *base, uint32_t bytes) {
