@@ -538,7 +538,8 @@ reef_status reef_kv_append_int4(const reef_kv_append_params *p, const float *k_n
 
 /* `pages` pages of one head each, in memory order (a contiguous cache has B * Hkv * L / 16, a
  * pool P * Hkv), as fp32 rows: k and v [pages, 16, D], x = float(code) * scale. k or v NULL:
- * left out (its codes and scales then are not read). head_dim 64 or 128. */
+ * left out (its codes and scales then are not read). head_dim 64 or 128; pointers 16-byte
+ * aligned, k_scales 4. */
 reef_status reef_kv_unpack_int4(const uint8_t *k_pages, const uint8_t *v_pages,
                                 const float *k_scales, const float *v_scales, int64_t pages,
                                 int64_t head_dim, float *k, float *v, hipStream_t stream);
@@ -596,8 +597,9 @@ reef_status reef_attention_prefill_int4_cache(
 /* The bounds of the pages that positions start_positions[b] .. start_positions[b] +
  * new_tokens - 1 fall in, over those pages' tokens before start_positions[b] + new_tokens:
  * after an append, with its start positions (a page's earlier tokens are read again, so a
- * page copied by reef_kv_copy_pages needs nothing else); after a compaction, once with start
- * 0. Of the keys x = float(code) * scale: S = max|x| / 127 (1 where that is 0), [0][d] =
+ * page copied by reef_kv_copy_pages needs nothing else); after reef_kv_keep_int8, with the
+ * drafted tokens' start positions and number (rows that were not kept only loosen their page's
+ * bounds); after a compaction, once with start 0. Of the keys x = float(code) * scale: S = max|x| / 127 (1 where that is 0), [0][d] =
  * min(127, ceil(max x_d / S)), [1][d] = max(-127, floor(min x_d / S)), IEEE divisions. Key
  * scales are positive and finite, as the quantizers make them. Sizes and status bits as
  * for reef_kv_append_int8 (a range past max_context sets CAPACITY and writes nothing). */
@@ -624,11 +626,10 @@ reef_status reef_kv_page_bounds_int4(const reef_kv_append_params *p,
  * the sum in whole numbers, the two products rounded to fp32 each: the same pages on every
  * run. q and q_scales as for decode; p->window, softmax_scale and num_splits are not used. A
  * page number outside [0, num_pages) sets BAD_PAGE, and that page is not selected; a length
- * outside [1, max_context] sets BAD_LENGTH, its counts are 0. Workspace: 16-byte aligned,
- * reef_kv_select_pages_workspace_bytes(p) bytes (0: invalid sizes), zero-filled before its
- * first use; every call leaves it ready for the next of any shape it is large enough for.
- * Calls that may run at the same time need separate workspaces. At most 65535 (sequence, kv
- * head) pairs. */
+ * outside [1, max_context] sets BAD_LENGTH, its counts are 0. Scales are finite. Workspace:
+ * 16-byte aligned, reef_kv_select_pages_workspace_bytes(p) bytes (0: invalid sizes); nothing in
+ * it is kept, calls that may run at the same time need separate ones. At most 65535 (sequence,
+ * kv head) pairs. */
 size_t reef_kv_select_pages_workspace_bytes(const reef_decode_params *p);
 
 reef_status reef_kv_select_pages(const reef_decode_params *p, const int8_t *q,

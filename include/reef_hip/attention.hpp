@@ -308,6 +308,126 @@ inline void kv_copy_pages(const int32_t *src, const int32_t *dst, int64_t n, int
           "kv_copy_pages");
 }
 
+// --- the cache held in 4 bits, and the pages that a query selects ------------------------------
+
+// block_table nullptr: the contiguous cache; otherwise the paged one (attention.h).
+inline void append_kv_cache_int4(const reef_kv_append_params &p, const float *k_new,
+                                 const reef_strides *k_strides, const float *v_new,
+                                 const reef_strides *v_strides, const int32_t *start_positions,
+                                 const int32_t *block_table, int64_t max_blocks_per_seq,
+                                 int64_t num_pages, uint8_t *k_cache, uint8_t *v_cache,
+                                 float *k_scales, float *v_scales, int32_t *context_lens,
+                                 uint32_t *status_word, hipStream_t stream) {
+    check(reef_kv_append_int4(&p, k_new, k_strides, v_new, v_strides, start_positions, block_table,
+                              max_blocks_per_seq, num_pages, k_cache, v_cache, k_scales, v_scales,
+                              context_lens, status_word, stream),
+          "append_kv_cache");
+}
+
+inline void kv_unpack_int4(const uint8_t *k_pages, const uint8_t *v_pages, const float *k_scales,
+                           const float *v_scales, int64_t pages, int64_t head_dim, float *k,
+                           float *v, hipStream_t stream) {
+    check(reef_kv_unpack_int4(k_pages, v_pages, k_scales, v_scales, pages, head_dim, k, v, stream),
+          "kv_unpack");
+}
+
+inline void kv_copy_pages(const int32_t *src, const int32_t *dst, int64_t n, int64_t kv_heads,
+                          int64_t head_dim, uint8_t *k_pages, uint8_t *v_pages,
+                          float *k_scale_pages, float *v_scale_pages, int64_t num_pages,
+                          uint32_t *status_word, hipStream_t stream) {
+    check(reef_kv_copy_pages_int4(src, dst, n, kv_heads, head_dim, k_pages, v_pages,
+                                  k_scale_pages, v_scale_pages, num_pages, status_word, stream),
+          "kv_copy_pages");
+}
+
+// One decode step over the 4-bit cache (the workspace: decode_workspace_bytes), over all keys or
+// (selection) the listed pages' alone.
+inline void decode_int4(const reef_decode_params &p, const int8_t *q, const float *q_scales,
+                        const uint8_t *k_cache, const uint8_t *v_cache, const float *k_scales,
+                        const float *v_scales, const int32_t *block_table,
+                        int64_t max_blocks_per_seq, int64_t num_pages,
+                        const int32_t *context_lens, const reef_page_selection *selection,
+                        float *out, void *workspace, size_t workspace_bytes,
+                        uint32_t *status_word, hipStream_t stream) {
+    check(reef_attention_decode_int4(&p, q, q_scales, k_cache, v_cache, k_scales, v_scales,
+                                     block_table, max_blocks_per_seq, num_pages, context_lens,
+                                     selection, out, workspace, workspace_bytes, status_word,
+                                     stream),
+          "attention decode");
+}
+
+// The same over the listed pages of the int8 cache.
+inline void decode_selected(const reef_decode_params &p, const int8_t *q, const float *q_scales,
+                            const int8_t *k_cache, const int8_t *v_cache, const float *k_scales,
+                            const float *v_scales, const int32_t *block_table,
+                            int64_t max_blocks_per_seq, int64_t num_pages,
+                            const int32_t *context_lens, const reef_page_selection &selection,
+                            float *out, void *workspace, size_t workspace_bytes,
+                            uint32_t *status_word, hipStream_t stream) {
+    check(reef_attention_decode_int8_selected(&p, q, q_scales, k_cache, v_cache, k_scales, v_scales,
+                                              block_table, max_blocks_per_seq, num_pages,
+                                              context_lens, &selection, out, workspace,
+                                              workspace_bytes, status_word, stream),
+          "attention decode");
+}
+
+// context_cache over the 4-bit cache; its workspace is context_cache's.
+inline void context_cache(const reef_attention_params &p, const int8_t *q,
+                          const reef_strides *q_strides, const float *q_scales,
+                          const uint8_t *k_cache, const uint8_t *v_cache, const float *k_scales,
+                          const float *v_scales, int64_t max_context, const int32_t *block_table,
+                          int64_t max_blocks_per_seq, int64_t num_pages, float *out,
+                          const reef_strides *out_strides, void *workspace,
+                          size_t workspace_bytes, uint32_t *status_word, hipStream_t stream) {
+    check(reef_attention_prefill_int4_cache(&p, q, q_strides, q_scales, k_cache, v_cache,
+                                            k_scales, v_scales, max_context, block_table,
+                                            max_blocks_per_seq, num_pages, out, out_strides,
+                                            workspace, workspace_bytes, status_word, stream),
+          "attention context over the cache");
+}
+
+// The bounds of the pages that an append wrote to, of either cache.
+inline void kv_page_bounds(const reef_kv_append_params &p, const int32_t *start_positions,
+                           const int8_t *k_cache, const float *k_scales,
+                           const int32_t *block_table, int64_t max_blocks_per_seq,
+                           int64_t num_pages, int8_t *bounds, float *bound_scales,
+                           uint32_t *status_word, hipStream_t stream) {
+    check(reef_kv_page_bounds_int8(&p, start_positions, k_cache, k_scales, block_table,
+                                   max_blocks_per_seq, num_pages, bounds, bound_scales,
+                                   status_word, stream),
+          "kv_page_bounds");
+}
+
+inline void kv_page_bounds(const reef_kv_append_params &p, const int32_t *start_positions,
+                           const uint8_t *k_cache, const float *k_scales,
+                           const int32_t *block_table, int64_t max_blocks_per_seq,
+                           int64_t num_pages, int8_t *bounds, float *bound_scales,
+                           uint32_t *status_word, hipStream_t stream) {
+    check(reef_kv_page_bounds_int4(&p, start_positions, k_cache, k_scales, block_table,
+                                   max_blocks_per_seq, num_pages, bounds, bound_scales,
+                                   status_word, stream),
+          "kv_page_bounds");
+}
+
+// The pages to read for a query, ascending in pages [B, Hkv, budget] with their number in counts
+// [B, Hkv]: a reef_page_selection of max_pages = budget.
+inline size_t select_workspace_bytes(const reef_decode_params &p) {
+    return reef_kv_select_pages_workspace_bytes(&p);
+}
+
+inline void kv_select_pages(const reef_decode_params &p, const int8_t *q, const float *q_scales,
+                            const int8_t *bounds, const float *bound_scales,
+                            const int32_t *block_table, int64_t max_blocks_per_seq,
+                            int64_t num_pages, const int32_t *context_lens, int64_t budget,
+                            int64_t sinks, int64_t recent, int32_t *pages, int32_t *counts,
+                            void *workspace, size_t workspace_bytes, uint32_t *status_word,
+                            hipStream_t stream) {
+    check(reef_kv_select_pages(&p, q, q_scales, bounds, bound_scales, block_table,
+                               max_blocks_per_seq, num_pages, context_lens, budget, sinks, recent,
+                               pages, counts, workspace, workspace_bytes, status_word, stream),
+          "kv_select_pages");
+}
+
 // A block table with its lengths and page counts, all on the device, and the calls that
 // change it (attention.h, "Pages of the paged cache"). A full pool throws std::length_error
 // once the status word is checked.

@@ -266,20 +266,18 @@ __global__ __launch_bounds__(kScoreWaves * kWave) void score_pages(SelectArgs a)
     const int lane = threadIdx.x & (kWave - 1), col = lane & 15, grp = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int item = blockIdx.y, b = item / a.kv_heads, kvh = item - b * a.kv_heads;
-    const int n = item_pages(a, b);
     const int first = ((int)blockIdx.x * kScoreWaves + wave) * kWave;
+    if (first >= a.max_pages) return;
+    const int page_idx = first + lane;
+    // (read beside the length, not after it; past the sequence's pages it is not used)
+    int page = a.table ? a.table[(int64_t)b * a.max_blocks + min(page_idx, a.max_pages - 1)] : page_idx;
+    const int n = item_pages(a, b);
     if (first >= n) return;
-    const int page_idx = min(first + lane, n - 1);
-    int page = page_idx;
-    bool ok = true;
-    int64_t base = (int64_t)item * a.max_pages, step = 1;  // row of bounds of page 0, between pages
-    if (a.table) {
-        page = a.table[(int64_t)b * a.max_blocks + page_idx];
-        ok = page >= 0 && page < a.num_pages;
-        if (!ok) page = 0;
-        base = kvh;
-        step = a.kv_heads;
-    }
+    const bool here = page_idx < n;
+    const bool ok = !here || !a.table || (page >= 0 && page < a.num_pages);
+    if (!here || !ok) page = 0;
+    // row of bounds of page 0, between pages
+    const int64_t base = a.table ? kvh : (int64_t)item * a.max_pages, step = a.table ? a.kv_heads : 1;
     if (!ok) flag_status(a.status, REEF_STATUS_BIT_BAD_PAGE);
     uint32_t key = kAlways;
     if (n > a.budget) {
@@ -334,7 +332,7 @@ __global__ __launch_bounds__(kScoreWaves * kWave) void score_pages(SelectArgs a)
         key = always ? kAlways : score_key(best);
     }
     if (!ok) key = kNever;
-    if (first + lane < n) a.keys[(int64_t)item * a.max_pages + first + lane] = key;
+    if (here) a.keys[(int64_t)item * a.max_pages + page_idx] = key;
 }
 
 constexpr int kDigit = 8, kBins = 1 << kDigit;
@@ -388,16 +386,20 @@ __device__ __forceinline__ void pick_digit(PickShared &sh, const int *bins, uint
 }
 
 // Keys of the pages that a thread holds: page first + 64 r + lane for r < R. In registers where a
-// sequence has up to 1024 R pages, read again at each use where it has more.
+// cache has up to 1024 R pages (read beside the sequence's length), read again at each use where
+// it has more.
 template <int R>
 struct HeldKeys {
     uint32_t key[R];
-    __device__ __forceinline__ HeldKeys(const uint32_t *keys, int first, int n, int lane) {
+    __device__ __forceinline__ HeldKeys(const SelectArgs &a, const uint32_t *keys, int wave, int lane,
+                                        int b, int &n) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int i = first + 64 * r + lane;
-            key[r] = i < n ? keys[i] : kNever;
-        }
+        for (int r = 0; r < R; ++r)
+            key[r] = keys[min((wave * R + r) * kWave + lane, a.max_pages - 1)];
+        n = item_pages(a, b);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if ((wave * R + r) * kWave + lane >= n) key[r] = kNever;
     }
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
@@ -409,8 +411,13 @@ template <>
 struct HeldKeys<0> {
     const uint32_t *keys;
     int first, n, lane, rounds;
-    __device__ __forceinline__ HeldKeys(const uint32_t *k, int f, int count, int l)
-        : keys(k), first(f), n(count), lane(l), rounds((count + kPickThreads - 1) / kPickThreads) {}
+    __device__ __forceinline__ HeldKeys(const SelectArgs &a, const uint32_t *k, int wave, int l, int b,
+                                        int &count)
+        : keys(k), lane(l) {
+        count = n = item_pages(a, b);
+        rounds = (n + kPickThreads - 1) / kPickThreads;
+        first = wave * rounds * kWave;
+    }
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
         for (int r = 0; r < rounds; ++r) {
@@ -420,20 +427,30 @@ struct HeldKeys<0> {
     }
 };
 
-// The budget-th largest of an item's n keys, then the pages above it and the first of those at it,
+// One workgroup an item: the budget-th largest of its n keys, then the pages above it and the first of those at it,
 // in page order. Wave w holds a run of pages, 64 at a time. The last key taken is found digit by
 // digit from the highest bit in which scores differ (they share sign and most of the exponent): the
 // keys of the range so far are counted by the digit's value in LDS, and the first value that enough
 // of them reach is the next range, until exactly enough do. Two digits mostly: 3 us for 8192 pages
 // (bit by bit 11, with a pass over the keys in memory a bit 62).
 template <int R>
-__device__ __forceinline__ void pick(const SelectArgs &a, int item, int n, const uint32_t *keys,
-                                     PickShared &sh) {
-    const int lane = threadIdx.x & (kWave - 1);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__global__ __launch_bounds__(kPickThreads) void pick_pages(SelectArgs a) {
+    __shared__ PickShared sh;
+    const int tid = threadIdx.x, lane = tid & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int item = blockIdx.x, b = item / a.kv_heads;
+    int n;
+    const HeldKeys<R> held(a, a.keys + (int64_t)item * a.max_pages, wave, lane, b, n);
+    for (int i = tid; i < kDigits * kBins; i += kPickThreads) sh.bins[0][i] = 0;
+    if (tid == 0) {
+        sh.all = ~0u;
+        sh.any = 0;
+        sh.always = 0;
+        if (n == 0 && item == b * a.kv_heads) flag_status(a.status, REEF_STATUS_BIT_BAD_LENGTH);
+    }
+    __syncthreads();
     const int rounds = R ? R : (n + kPickThreads - 1) / kPickThreads;
     const int first = wave * rounds * kWave;
-    const HeldKeys<R> held(keys, first, n, lane);
     uint32_t t = kNever;
     if (n > a.budget) {
         uint32_t all = ~0u, any = 0;
@@ -513,27 +530,6 @@ __device__ __forceinline__ void pick(const SelectArgs &a, int item, int n, const
     const int count = total0 + need;
     for (int i = count + threadIdx.x; i < a.budget; i += kPickThreads) list[i] = -1;
     if (threadIdx.x == 0) a.counts[item] = count;
-}
-
-// One workgroup an item.
-__global__ __launch_bounds__(kPickThreads) void pick_pages(SelectArgs a) {
-    __shared__ PickShared sh;
-    const int tid = threadIdx.x;
-    for (int i = tid; i < kDigits * kBins; i += kPickThreads) sh.bins[0][i] = 0;
-    if (tid == 0) {
-        sh.all = ~0u;
-        sh.any = 0;
-        sh.always = 0;
-    }
-    const int item = blockIdx.x, b = item / a.kv_heads;
-    const int n = item_pages(a, b);
-    if (n == 0 && tid == 0 && item == b * a.kv_heads)
-        flag_status(a.status, REEF_STATUS_BIT_BAD_LENGTH);
-    const uint32_t *keys = a.keys + (int64_t)item * a.max_pages;
-    __syncthreads();
-    if (n <= 2 * kPickThreads) pick<2>(a, item, n, keys, sh);
-    else if (n <= 8 * kPickThreads) pick<8>(a, item, n, keys, sh);
-    else pick<0>(a, item, n, keys, sh);
 }
 
 bool select_sizes(const reef_decode_params *p) {
@@ -631,6 +627,11 @@ extern "C" reef_status reef_kv_select_pages(
     else
         hipLaunchKernelGGL(score_pages<64>, grid, dim3(kScoreWaves * kWave), 0, stream, a);
     if (hipGetLastError() != hipSuccess) return REEF_HIP_ERROR;
-    hipLaunchKernelGGL(pick_pages, dim3((unsigned)a.items), dim3(kPickThreads), 0, stream, a);
+    const auto pick = [&](auto *kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)a.items), dim3(kPickThreads), 0, stream, a);
+    };
+    pick(a.max_pages <= 2 * kPickThreads   ? pick_pages<2>
+         : a.max_pages <= 8 * kPickThreads ? pick_pages<8>
+                                           : pick_pages<0>);
     return launch_status();
 }
