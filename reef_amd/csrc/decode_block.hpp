@@ -111,7 +111,8 @@ struct DecodeBlock : BlockRows<D, BITS> {
     static constexpr int S = HEADS == 16 ? 1 : HEADS;  // scales a lane loads
     float ks[S], vs[S];
     bool live;
-    int pos;  // SEL: position of the first token of this lane group's page
+    int pos;  // entries: position of the first token of this lane group's page
+    bool ok;  // a chunk's entries: whether that page is there
 };
 
 // A wave's running state over its keys: max (log2 units), row sum, the value
@@ -403,23 +404,20 @@ __device__ __forceinline__ void block_math(const DecodeBlock<D, BITS, HEADS> &cu
     }
 }
 
-// The q^T operand of query head `head` of sequence b (zeros for dead heads) and the log2-domain
-// score factor of head `scored` (the one whose scores the lane holds; zero for a dead one).
+// The q^T operand of a query row (zeros for a dead column), with the score factor c.
 template <int D, int BITS>
-__device__ __forceinline__ Query<D> load_query(const DecodeArgs &a, int b, int head, bool head_ok,
-                                               int scored, bool scored_ok, int grp) {
+__device__ __forceinline__ Query<D> query_of(const int8_t *qrow, bool live, float c, int grp) {
     Query<D> q;
     q.zero = 0;
-    const int8_t *qrow = a.q + ((int64_t)b * a.q_heads + (head_ok ? head : 0)) * D;
     if constexpr (BITS == 4 && D == 64) {
         const i32x2 lo = *reinterpret_cast<const i32x2 *>(qrow + 8 * grp);
         const i32x2 hi = *reinterpret_cast<const i32x2 *>(qrow + 32 + 8 * grp);
-        q.op[0] = head_ok ? i32x4{lo[0], lo[1], hi[0], hi[1]} : i32x4{0, 0, 0, 0};
+        q.op[0] = live ? i32x4{lo[0], lo[1], hi[0], hi[1]} : i32x4{0, 0, 0, 0};
     } else {
 #pragma unroll
         for (int s = 0; s < D / 64; ++s)
-            q.op[s] = head_ok ? *reinterpret_cast<const i32x4 *>(qrow + 64 * s + 16 * grp)
-                              : i32x4{0, 0, 0, 0};
+            q.op[s] = live ? *reinterpret_cast<const i32x4 *>(qrow + 64 * s + 16 * grp)
+                           : i32x4{0, 0, 0, 0};
     }
     if constexpr (BITS == 4) {
         int sum = 0;
@@ -431,14 +429,23 @@ __device__ __forceinline__ Query<D> load_query(const DecodeArgs &a, int b, int h
         sum += __shfl_xor(sum, 32);
         q.zero = -kInt4Zero * sum;
     }
+    q.c = c;
+    return q;
+}
+
+// The q^T operand of query head `head` of sequence b (zeros for dead heads) and the log2-domain
+// score factor of head `scored` (the one whose scores the lane holds; zero for a dead one).
+template <int D, int BITS>
+__device__ __forceinline__ Query<D> load_query(const DecodeArgs &a, int b, int head, bool head_ok,
+                                               int scored, bool scored_ok, int grp) {
+    const int8_t *qrow = a.q + ((int64_t)b * a.q_heads + (head_ok ? head : 0)) * D;
     float cq = 0.0f;
     if (scored_ok) {
         cq = a.q_gran == REEF_SCALE_PER_TENSOR ? a.qs[0]
              : a.q_gran == REEF_SCALE_PER_HEAD ? a.qs[scored]
                                                 : a.qs[(int64_t)b * a.q_heads + scored];
     }
-    q.c = cq * a.score_scale;
-    return q;
+    return query_of<D, BITS>(qrow, head_ok, cq * a.score_scale, grp);
 }
 
 // Keys of one item (sequence b = item / kv_heads): its length (0 if the length is
@@ -488,6 +495,17 @@ bool decode_flat(const reef_decode_params *p, int64_t tokens);
 
 // The workspace's counters, one per (sequence, kv head), ahead of the part slots.
 constexpr int64_t kDecodeCounterBytes = kPlanItems * 4;
+
+// A chunk's attention over the 4-bit cache in decode_entries.hip: whether it is small enough to be
+// the faster way, and the launch (arguments as prefill_cache.hip has checked them; counters zero
+// and left so, slots for two parts a workgroup, two workgroups a compute unit).
+bool chunk_entries_fit(const reef_attention_params *p);
+reef_status launch_chunk_int4(const reef_attention_params *p, const int8_t *q, const int64_t (&qst)[3],
+                              const float *q_scales, const uint8_t *k_cache, const uint8_t *v_cache,
+                              const float *k_scales, const float *v_scales, int64_t max_context,
+                              const int32_t *block_table, int64_t max_blocks_per_seq,
+                              int64_t num_pages, float *out, const int64_t (&ost)[3], char *counters,
+                              char *slots, uint32_t *status_word, hipStream_t stream);
 
 inline void set_decode_args(const reef_decode_params *p, DecodeArgs &a) {
     a.batch = (int32_t)p->batch;

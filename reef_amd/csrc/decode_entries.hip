@@ -10,6 +10,10 @@
 // and a lane's share is HEADS scores instead of 16. A column's weights are zero for the other
 // columns' keys, each column keeps a softmax of its own, and the columns of a head are merged when
 // a run of keys ends.
+//
+// A short chunk of a prompt over the 4-bit cache runs here too (its rows and the group's heads are
+// the columns, 16 or fewer to an item, with an end of their own each): a launch without the copy of
+// the cache that prefill_cache.hip makes for a long one.
 #include "decode_block.hpp"
 
 namespace reef {
@@ -23,7 +27,8 @@ constexpr int kLeastBlocks = 8;
 
 // The block of four pages named by entries (numbers of the sequence's pages, -1: none) that lanes
 // l % 4 hold, with their page numbers from the block table.
-template <int D, int BITS, int HEADS, bool PAGED, bool NT>
+// (Of a chunk's sequence a page that is not there reads as zero codes, elsewhere it takes no part.)
+template <int D, int BITS, int HEADS, bool PAGED, bool NT, bool CHUNK>
 __device__ __forceinline__ void load_entries(const DecodeArgs &a, int b, int kvh, int n_pages,
                                              int entries, int pages, int col, int grp,
                                              DecodeBlock<D, BITS, HEADS> &x, bool &bad_page) {
@@ -35,16 +40,51 @@ __device__ __forceinline__ void load_entries(const DecodeArgs &a, int b, int kvh
                                                 PAGED ? __shfl(pages, grp) : 0);
     x.pos = max(ge, 0) * kPage;
     load_pages<D, BITS, HEADS, NT>(kp, gp, col, grp, x, bad_page);
+    if constexpr (CHUNK && PAGED) x.ok = gp.ok;
 }
 
-// Keys [k_begin, k_end) of (sequence b, kv head kvh) in steps of k_step: the sequence's, or (SEL)
-// the places of its list, 16 to an entry, `count` entries in all. The next block's loads, the
+// What an item reads: a sequence's pages, a list's, or a sequence's for a chunk's rows.
+enum Form { kAll, kListed, kChunk };
+
+struct EntryArgs : DecodeArgs {
+    // kChunk: an item is (sequence, kv head, tile) of HEADS columns of q_len rows x group heads
+    int64_t q_sb, q_sh, q_st, o_sb, o_sh, o_st;
+    int32_t tiles, q_len, query_start;
+};
+
+// Rows of the chunk that columns c and c' of tile t are of (past the last: the last).
+template <int HEADS>
+__device__ __forceinline__ int chunk_row(const EntryArgs &a, int tile, int c) {
+    return min((tile * HEADS + c) / a.group, a.q_len - 1);
+}
+
+template <int HEADS, Form FORM>
+__device__ __forceinline__ ItemKeys entry_keys(const EntryArgs &a, int item) {
+    if constexpr (FORM != kChunk) {
+        return item_keys<FORM == kListed>(a, item);
+    } else {
+        const int tile = item % a.tiles;
+        const int first = a.query_start + chunk_row<HEADS>(a, tile, 0);
+        ItemKeys r;
+        r.bad = false;
+        r.count = 0;
+        r.len = a.query_start + chunk_row<HEADS>(a, tile, HEADS - 1) + 1;
+        r.lo = a.window > 0 ? max(0, first + 1 - a.window) : 0;
+        r.first_block = r.lo / kBlockKeys;
+        r.blocks = (r.len + kBlockKeys - 1) / kBlockKeys - r.first_block;
+        return r;
+    }
+}
+
+// Keys [k_begin, k_end) of (sequence b, kv head kvh) in steps of k_step: the sequence's, or (listed)
+// the places of its list, 16 to an entry, `count` entries in all; this lane's column sees those in
+// [lo, len). The next block's loads, the
 // page numbers of the one after and the entries of the one after that are issued before the current
 // block is computed, and all of them always, of the last block again where there is none: under a
 // branch the compiler would wait for all loads in flight at the next use of any. (Two blocks in
 // flight instead of one gain nothing.)
-template <int D, int BITS, int HEADS, bool PAGED, bool SEL>
-__device__ __forceinline__ void run_entries(const DecodeArgs &a, int item, int b, int kvh, int lo,
+template <int D, int BITS, int HEADS, bool PAGED, Form FORM>
+__device__ __forceinline__ void run_entries(const EntryArgs &a, int item, int b, int kvh, int lo,
                                             int len, int count, int k_begin, int k_end, int k_step,
                                             int n_pages, const Query<D> &q, int lane,
                                             DecodeRun<D> &st, bool &bad_page) {
@@ -53,7 +93,7 @@ __device__ __forceinline__ void run_entries(const DecodeArgs &a, int item, int b
     const int last = (k_end - k_begin - 1) / k_step;
     auto entry = [&](int i) {
         const int at = (k_begin + min(i, last) * k_step) / kPage + (lane & 3);
-        if constexpr (SEL) {
+        if constexpr (FORM == kListed) {
             const int e = a.sel_pages[(int64_t)item * a.max_sel + min(at, count - 1)];
             bad_page |= at < count && e >= n_pages;
             return at < count && e < n_pages ? max(e, -1) : -1;
@@ -66,11 +106,22 @@ __device__ __forceinline__ void run_entries(const DecodeArgs &a, int item, int b
     };
     DecodeBlock<D, BITS, HEADS> cur, next;
     auto load = [&](int e, int p) {
-        load_entries<D, BITS, HEADS, PAGED, !PAGED && !SEL>(a, b, kvh, n_pages, e, p, col, grp, next,
-                                                            bad_page);
+        load_entries<D, BITS, HEADS, PAGED, !PAGED && FORM == kAll, FORM == kChunk>(
+            a, b, kvh, n_pages, e, p, col, grp, next, bad_page);
     };
     auto math = [&](int i) {
-        block_math<D, BITS, HEADS, SEL>(cur, k_begin + i * k_step, lo, SEL ? len : k_end, q, lane, st);
+        if constexpr (FORM == kChunk && PAGED) {
+            if (__any(!cur.ok)) {  // (zero codes: scores and values of zero, which take part)
+#pragma unroll
+                for (int j = 0; j < DecodeBlock<D, BITS, HEADS>::S; ++j) {
+                    cur.ks[j] = cur.ok ? cur.ks[j] : 0.0f;
+                    cur.vs[j] = cur.ok ? cur.vs[j] : 0.0f;
+                }
+                cur.live |= !cur.ok;
+            }
+        }
+        block_math<D, BITS, HEADS, FORM != kAll>(cur, k_begin + i * k_step, lo,
+                                                 FORM == kAll ? k_end : len, q, lane, st);
     };
     const int e0 = entry(0);
     int e1 = entry(1), e2 = entry(2);  // of the next block and the one after
@@ -197,8 +248,8 @@ struct Deal {
 // the item's blocks in turn, keep a flash-decoding state each and merge in LDS; an item that lies
 // in one workgroup is stored, the parts of others go to the workspace, and the part that arrives
 // last merges them all.
-template <int D, int BITS, int HEADS, bool PAGED, bool SEL>
-__global__ __launch_bounds__(kEntryThreads, kWgPerCu) void decode_entries(DecodeArgs a, float *out) {
+template <int D, int BITS, int HEADS, bool PAGED, Form FORM>
+__global__ __launch_bounds__(kEntryThreads, kWgPerCu) void decode_entries(EntryArgs a, float *out) {
     using Slots = RowSlots<D, HEADS>;
     constexpr int DB = D / 16;  // 16-wide output blocks
     constexpr int N = Slots::N, QD = D / 4;
@@ -217,7 +268,7 @@ __global__ __launch_bounds__(kEntryThreads, kWgPerCu) void decode_entries(Decode
     if (a.flat) {
         int mine = 0;
         for (int i = tid; i < a.items; i += kEntryThreads) {
-            const int n = item_keys<SEL>(a, i).blocks;
+            const int n = entry_keys<HEADS, FORM>(a, i).blocks;
             sOff[i + 1] = n;
             mine += n;
         }
@@ -274,13 +325,17 @@ __global__ __launch_bounds__(kEntryThreads, kWgPerCu) void decode_entries(Decode
 
     for (;;) {
         const int p_begin = unit_of(item), p_end = unit_of(item + 1);
-        ItemKeys ik = item_keys<SEL>(a, item);
+        ItemKeys ik = entry_keys<HEADS, FORM>(a, item);
         ik.len = __builtin_amdgcn_readfirstlane(ik.len);
         ik.lo = __builtin_amdgcn_readfirstlane(ik.lo);
         ik.first_block = __builtin_amdgcn_readfirstlane(ik.first_block);
         ik.blocks = __builtin_amdgcn_readfirstlane(ik.blocks);
-        if constexpr (SEL) ik.count = __builtin_amdgcn_readfirstlane(ik.count);
-        const int b = item / a.kv_heads, kvh = item % a.kv_heads;
+        if constexpr (FORM == kListed) ik.count = __builtin_amdgcn_readfirstlane(ik.count);
+        const int tile = FORM == kChunk ? item % a.tiles : 0;
+        const int pair = FORM == kChunk ? item / a.tiles : item;
+        const int b = pair / a.kv_heads, kvh = pair % a.kv_heads;
+        // columns of the item, HEADS at most
+        const int cols = FORM == kChunk ? min(HEADS, a.q_len * a.group - tile * HEADS) : a.group;
         // This segment's blocks of the item, the workgroups with a part of it (parts from gf on).
         int s_blk = 0, e_blk = ik.blocks, parts = 1, gf = g;
         if (a.single) {
@@ -299,19 +354,40 @@ __global__ __launch_bounds__(kEntryThreads, kWgPerCu) void decode_entries(Decode
         }
         if (ik.bad && s_blk == 0 && tid == 0) flag_status(a.status, REEF_STATUS_BIT_BAD_LENGTH);
 
-        const int head = kvh * a.group + col;   // this lane's query head (live if col < group)
-        const int scored = kvh * a.group + col % HEADS;  // the head whose scores it holds
         const int k_begin = (ik.first_block + s_blk + wave) * kBlockKeys;
-        const int k_end = min(SEL ? ik.count * kPage : ik.len, (ik.first_block + e_blk) * kBlockKeys);
+        const int k_end = min(FORM == kListed ? ik.count * kPage : ik.len,
+                              (ik.first_block + e_blk) * kBlockKeys);
         const int n_pages = (ik.len + kPage - 1) / kPage;
-        const Query<D> q = load_query<D, BITS>(a, b, head, col < a.group, scored,
-                                               col % HEADS < a.group, grp);
+        // the column whose operand this lane holds, and the one whose scores
+        const int scored = col % HEADS;
+        int lo = ik.lo, len = ik.len;
+        Query<D> q;
+        if constexpr (FORM == kChunk) {
+            const int t = chunk_row<HEADS>(a, tile, scored);
+            len = a.query_start + t + 1;
+            lo = a.window > 0 ? max(0, len - a.window) : 0;
+            const auto head = [&](int c) { return kvh * a.group + (tile * HEADS + c) % a.group; };
+            const bool live = col < cols, scores = scored < cols;
+            const int8_t *qrow = a.q + b * a.q_sb + (live ? head(col) : 0) * a.q_sh +
+                                 (live ? chunk_row<HEADS>(a, tile, col) : 0) * a.q_st;
+            float scale = 0.0f;
+            if (scores) {
+                const int h = head(scored);
+                scale = a.q_gran == REEF_SCALE_PER_TENSOR ? a.qs[0]
+                        : a.q_gran == REEF_SCALE_PER_HEAD ? a.qs[h]
+                                                          : a.qs[((int64_t)b * a.q_heads + h) * a.q_len + t];
+            }
+            q = query_of<D, BITS>(qrow, live, scale * a.score_scale, grp);
+        } else {
+            const int head = kvh * a.group + col;
+            q = load_query<D, BITS>(a, b, head, col < cols, kvh * a.group + scored, scored < cols, grp);
+        }
         DecodeRun<D> st;
         reset_run<D>(st);
         bool bad_page = false;
-        run_entries<D, BITS, HEADS, PAGED, SEL>(a, item, b, kvh, ik.lo, ik.len, ik.count, k_begin,
-                                                k_end, kDecodeWaves * kBlockKeys, n_pages, q, lane,
-                                                st, bad_page);
+        run_entries<D, BITS, HEADS, PAGED, FORM>(a, item, b, kvh, lo, len, ik.count, k_begin, k_end,
+                                                 kDecodeWaves * kBlockKeys, n_pages, q, lane, st,
+                                                 bad_page);
         if (bad_page) flag_status(a.status, REEF_STATUS_BIT_BAD_PAGE);
         // Row sums: this lane holds its column's partial over the keys of its lane group.
         float l = st.l_run;
@@ -331,10 +407,17 @@ __global__ __launch_bounds__(kEntryThreads, kWgPerCu) void decode_entries(Decode
 
         // A sequence with no keys ends with a sum of 0 and stores zeros.
         auto store = [&](int s, const RowRun &r) {
-            if (s / QD >= a.group) return;
+            if (s / QD >= cols) return;
             const float inv = r.l > 0.0f ? 1.0f / r.l : 0.0f;
-            float *orow = out + ((int64_t)b * a.q_heads + kvh * a.group) * D;
-            *reinterpret_cast<f32x4 *>(orow + 4 * s) = r.o * inv;
+            if constexpr (FORM == kChunk) {
+                const int c = tile * HEADS + s / QD;
+                float *orow = out + b * a.o_sb + (int64_t)(kvh * a.group + c % a.group) * a.o_sh +
+                              (int64_t)(c / a.group) * a.o_st;
+                *reinterpret_cast<f32x4 *>(orow + 4 * (s % QD)) = r.o * inv;
+            } else {
+                float *orow = out + ((int64_t)b * a.q_heads + kvh * a.group) * D;
+                *reinterpret_cast<f32x4 *>(orow + 4 * s) = r.o * inv;
+            }
         };
         if (parts == 1) {  // (uniform)
 #pragma unroll
@@ -356,7 +439,7 @@ __global__ __launch_bounds__(kEntryThreads, kWgPerCu) void decode_entries(Decode
 #pragma unroll
             for (int k = 0; k < Slots::PER; ++k) {
                 const int s = tid + k * kEntryThreads;
-                if (s < N && s / QD < a.group) {
+                if (s < N && s / QD < cols) {
                     const RowRun r = merge_slot<D, HEADS>(sRow, sML, s, kDecodeWaves);
                     part_store(so + s, pack(r.o[0], r.o[1]));
                     part_store(so + N + s, pack(r.o[2], r.o[3]));
@@ -382,7 +465,7 @@ __global__ __launch_bounds__(kEntryThreads, kWgPerCu) void decode_entries(Decode
                 for (int k = 0; k < Slots::PER; ++k) {
                     const int s = (tid + k * kEntryThreads) % N;
                     run[k] = {-INFINITY, 0.0f, f32x4{}};
-                    if (s / QD >= a.group) continue;
+                    if (s / QD >= cols) continue;
                     for (int i0 = gi; i0 < parts; i0 += Slots::GROUPS * AHEAD) {
                         uint64_t w[AHEAD][3];
 #pragma unroll
@@ -420,43 +503,58 @@ __global__ __launch_bounds__(kEntryThreads, kWgPerCu) void decode_entries(Decode
     }
 }
 
-template <int BITS, bool PAGED, bool SEL>
-reef_status launch_entries(const reef_decode_params *p, DecodeArgs &a, float *out, void *workspace,
+// Launches `a`, whose sequences have `blocks` 64-key blocks at most, of (batch, kv head) pairs that
+// read up to `tokens` tokens (a list's may be longer than the cache); num_splits as for decode.
+template <int BITS, bool PAGED, Form FORM>
+reef_status launch_entries(EntryArgs &a, int64_t head_dim, int64_t columns, int64_t blocks, bool flat,
+                           int64_t num_splits, float *out, char *counters, char *slots,
                            hipStream_t stream) {
+    const int64_t items = a.items;
+    flat = flat && items <= kPlanItems;  // (the plan's words in LDS)
+    // Two workgroups a compute unit, one where items are few: an item's parts are half as many then
+    // and the bytes take no longer (1 x 8 x 131071 tokens: 36 us against 43, 64 parts an item).
+    const int64_t cus = compute_units();
+    const int64_t most = num_splits > 0 ? ceil_div(items * num_splits, kDecodeWaves)
+                                        : (2 * items <= cus ? 1 : kWgPerCu) * cus;
+    a.flat = flat ? 1 : 0;
+    const int64_t least = num_splits > 0 ? 1 : kLeastBlocks;
+    a.single = flat && 2 * items <= most ? (int32_t)least : 0;
+    const int64_t units = a.single ? items * ceil_div(blocks, least) : flat ? items * blocks : items;
+    a.wgs = (int32_t)std::max<int64_t>(1, std::min<int64_t>(std::min(most, units), 1 << 20));
+    a.counters = reinterpret_cast<uint32_t *>(counters);
+    a.slots = reinterpret_cast<float *>(slots);
+    const auto run = [&](auto *kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)a.wgs), dim3(kEntryThreads), 0, stream, a, out);
+    };
+    if (head_dim == 128)
+        run(columns <= 4   ? decode_entries<128, BITS, 4, PAGED, FORM>
+            : columns <= 8 ? decode_entries<128, BITS, 8, PAGED, FORM>
+                           : decode_entries<128, BITS, 16, PAGED, FORM>);
+    else
+        run(columns <= 4   ? decode_entries<64, BITS, 4, PAGED, FORM>
+            : columns <= 8 ? decode_entries<64, BITS, 8, PAGED, FORM>
+                           : decode_entries<64, BITS, 16, PAGED, FORM>);
+    return launch_status();
+}
+
+// A decode step's.
+template <int BITS, bool PAGED, bool SEL>
+reef_status launch_decode(const reef_decode_params *p, EntryArgs &a, float *out, void *workspace,
+                          hipStream_t stream) {
     set_decode_args(p, a);
     // The tokens that a sequence may read. A list longer than the cache (pages listed twice)
     // gets no more workgroups than the workspace has slots for.
     const int64_t tokens = SEL ? (int64_t)a.max_sel * kPage : p->max_context;
-    const int64_t items = a.items, blocks = ceil_div(std::min(tokens, p->max_context), kBlockKeys);
-    // Two workgroups a compute unit, one where items are few: an item's parts are half as many then
-    // and the bytes take no longer (1 x 8 x 131071 tokens: 36 us against 43, 64 parts an item).
-    const int64_t cus = compute_units();
-    const int64_t most = p->num_splits > 0 ? ceil_div(items * p->num_splits, kDecodeWaves)
-                                           : (2 * items <= cus ? 1 : kWgPerCu) * cus;
-    a.flat = decode_flat(p, p->max_context) && decode_flat(p, tokens) ? 1 : 0;
-    const int64_t least = p->num_splits > 0 ? 1 : kLeastBlocks;
-    a.single = a.flat && 2 * items <= most ? (int32_t)least : 0;
-    const int64_t units = a.single ? items * ceil_div(blocks, least) : a.flat ? items * blocks : items;
-    a.wgs = (int32_t)std::max<int64_t>(1, std::min<int64_t>(std::min(most, units), 1 << 20));
-    a.counters = static_cast<uint32_t *>(workspace);
-    a.slots = reinterpret_cast<float *>(static_cast<char *>(workspace) + kDecodeCounterBytes);
-    const auto run = [&](auto *kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)a.wgs), dim3(kEntryThreads), 0, stream, a, out);
-    };
-    if (p->head_dim == 128)
-        run(a.group <= 4   ? decode_entries<128, BITS, 4, PAGED, SEL>
-            : a.group <= 8 ? decode_entries<128, BITS, 8, PAGED, SEL>
-                           : decode_entries<128, BITS, 16, PAGED, SEL>);
-    else
-        run(a.group <= 4   ? decode_entries<64, BITS, 4, PAGED, SEL>
-            : a.group <= 8 ? decode_entries<64, BITS, 8, PAGED, SEL>
-                           : decode_entries<64, BITS, 16, PAGED, SEL>);
-    return launch_status();
+    char *base = static_cast<char *>(workspace);
+    return launch_entries<BITS, PAGED, SEL ? kListed : kAll>(
+        a, p->head_dim, a.group, ceil_div(std::min(tokens, p->max_context), kBlockKeys),
+        decode_flat(p, p->max_context) && decode_flat(p, tokens), p->num_splits, out, base,
+        base + kDecodeCounterBytes, stream);
 }
 
 // A paged launch's table, or (block_table NULL) a contiguous cache.
 bool use_table(const reef_decode_params *p, const int32_t *block_table,
-               int64_t max_blocks_per_seq, int64_t num_pages, DecodeArgs &a) {
+               int64_t max_blocks_per_seq, int64_t num_pages, EntryArgs &a) {
     if (!a.context_lens || num_pages <= 0 || num_pages >= (int64_t(1) << 31) ||
         max_blocks_per_seq * kPage < p->max_context || max_blocks_per_seq >= (int64_t(1) << 30))
         return false;
@@ -481,7 +579,7 @@ reef_status decode_any(const reef_decode_params *p, const int8_t *q, const float
     if (!k || !v || !k_scales || !v_scales || !aligned(k, 16) || !aligned(v, 16) ||
         !aligned(k_scales, 16) || !aligned(v_scales, 16) || !aligned(out, 16))
         return REEF_INVALID_ARGUMENT;
-    DecodeArgs a = {};
+    EntryArgs a = {};
     a.q = q;
     a.qs = q_scales;
     a.k = static_cast<const int8_t *>(k);
@@ -500,16 +598,73 @@ reef_status decode_any(const reef_decode_params *p, const int8_t *q, const float
         a.sel_pages = selection->pages;
         a.sel_counts = selection->counts;
         a.max_sel = (int32_t)selection->max_pages;
-        return block_table ? launch_entries<BITS, true, true>(p, a, out, workspace, stream)
-                           : launch_entries<BITS, false, true>(p, a, out, workspace, stream);
+        return block_table ? launch_decode<BITS, true, true>(p, a, out, workspace, stream)
+                           : launch_decode<BITS, false, true>(p, a, out, workspace, stream);
     }
     if constexpr (BITS == 8) return REEF_INVALID_ARGUMENT;  // decode.hip's
     else
-        return block_table ? launch_entries<BITS, true, false>(p, a, out, workspace, stream)
-                           : launch_entries<BITS, false, false>(p, a, out, workspace, stream);
+        return block_table ? launch_decode<BITS, true, false>(p, a, out, workspace, stream)
+                           : launch_decode<BITS, false, false>(p, a, out, workspace, stream);
 }
 
 }  // namespace
+
+// A 64-key block of 16 columns costs about 1.4 ns of the whole GPU's time here, one of a 128-row
+// tile 9 ns there, behind a copy of the cache and a schedule's start of 25 us. So a chunk runs here
+// if it has few blocks (2 x 12 heads x 77 rows over 1021 keys: 13.8 us against 29.8; 32 heads x
+// 64 rows over 4096 24.9 against 47.6) or if its tiles of 128 rows stay part empty (100 rows over
+// 8000 keys, 2 x 32 heads: 81 against 107; 16 rows over 6000, 8 x 16: 25 against 153). With full
+// tiles and many blocks it does not (512 rows over 4608, 4 x 32: 388 against 248).
+bool chunk_entries_fit(const reef_attention_params *p) {
+    constexpr int64_t kFew = 8192, kRows = 128;
+    const int64_t group = p->q_heads / p->kv_heads;
+    if (p->q_len > (1 << 20) || p->q_len * group > (1 << 20)) return false;
+    const int64_t items = p->batch * p->kv_heads * ceil_div(p->q_len * group, 16);
+    const int64_t tiles = p->batch * p->q_heads * ceil_div(p->q_len, kRows);
+    const int64_t end = p->query_start + p->q_len;
+    const int64_t blocks = ceil_div(p->window > 0 ? std::min(end, p->window + p->q_len) : end, kBlockKeys);
+    return items <= kPlanItems && (items * blocks <= kFew || 2 * items <= 13 * tiles);
+}
+
+reef_status launch_chunk_int4(const reef_attention_params *p, const int8_t *q, const int64_t (&qst)[3],
+                              const float *q_scales, const uint8_t *k_cache, const uint8_t *v_cache,
+                              const float *k_scales, const float *v_scales, int64_t max_context,
+                              const int32_t *block_table, int64_t max_blocks_per_seq,
+                              int64_t num_pages, float *out, const int64_t (&ost)[3], char *counters,
+                              char *slots, uint32_t *status_word, hipStream_t stream) {
+    EntryArgs a = {};
+    a.q = q;
+    a.qs = q_scales;
+    a.k = reinterpret_cast<const int8_t *>(k_cache);
+    a.v = reinterpret_cast<const int8_t *>(v_cache);
+    a.ks = k_scales;
+    a.vs = v_scales;
+    a.status = status_word;
+    a.block_table = block_table;
+    a.max_blocks = (int32_t)(block_table ? max_blocks_per_seq : 0);
+    a.num_pages = (int32_t)(block_table ? num_pages : 0);
+    a.batch = (int32_t)p->batch;
+    a.q_heads = (int32_t)p->q_heads;
+    a.kv_heads = (int32_t)p->kv_heads;
+    a.group = (int32_t)(p->q_heads / p->kv_heads);
+    a.max_context = (int32_t)(block_table ? 0 : max_context);
+    a.window = (int32_t)std::min<int64_t>(p->window, INT32_MAX);
+    a.q_gran = p->q_granularity;
+    a.score_scale = p->softmax_scale * kLog2e;
+    a.q_sb = qst[0], a.q_sh = qst[1], a.q_st = qst[2];
+    a.o_sb = ost[0], a.o_sh = ost[1], a.o_st = ost[2];
+    a.q_len = (int32_t)p->q_len;
+    a.query_start = (int32_t)p->query_start;
+    const int64_t columns = p->q_len * a.group, width = columns <= 4 ? 4 : columns <= 8 ? 8 : 16;
+    a.tiles = (int32_t)ceil_div(columns, width);
+    a.items = (int32_t)(p->batch * p->kv_heads * a.tiles);
+    const int64_t blocks = ceil_div(p->query_start + p->q_len, kBlockKeys);
+    return block_table ? launch_entries<4, true, kChunk>(a, p->head_dim, columns, blocks, true, 0, out,
+                                                         counters, slots, stream)
+                       : launch_entries<4, false, kChunk>(a, p->head_dim, columns, blocks, true, 0,
+                                                          out, counters, slots, stream);
+}
+
 }  // namespace reef
 
 using namespace reef;

@@ -14,9 +14,11 @@
 // workspace is the first part of this one). The gather moves 2 (D + 4) bytes per
 // cached token and kv head each way, small beside the chunk's attention. Of a cache held in 4
 // bits it reads D + 8 and widens the codes to the same rows: the prefill's int8 products then
-// see exactly the codes that decode sees.
-#include "kv_int4.hpp"
-#include "reef_common.hpp"
+// see exactly the codes that decode sees. A short chunk over it takes no copy: its rows run as the
+// columns of decode_entries.hip.
+#include <cmath>
+
+#include "decode_block.hpp"
 
 namespace reef {
 
@@ -122,6 +124,9 @@ __global__ __launch_bounds__(kGatherThreads) void gather_cache(GatherArgs a) {
     }
 }
 
+// The prefill's counters, ahead of its part slots: a short chunk's are the first of either.
+constexpr int64_t kChunkCounterBytes = 65536 * 4;
+
 int64_t round256(int64_t n) { return ceil_div(n, 256) * 256; }
 
 // Workspace layout: the prefill's balanced-schedule workspace (item counters, zero
@@ -192,6 +197,32 @@ reef_status prefill_cache(const reef_attention_params *p, const int8_t *q,
         return REEF_INVALID_ARGUMENT;
 
     char *base = static_cast<char *>(workspace);
+    if constexpr (BITS == 4) {
+        if ((p->flags & REEF_ATTN_SCHED_MASK) == REEF_ATTN_SCHED_AUTO && chunk_entries_fit(p)) {
+            const int64_t D = p->head_dim;
+            const auto strides = [&](const reef_strides *s, int64_t unit, int64_t (&to)[3]) {
+                to[0] = s ? s->batch : p->q_heads * p->q_len * D;
+                to[1] = s ? s->head : p->q_len * D;
+                to[2] = s ? s->token : D;
+                return to[0] >= 0 && to[1] >= 0 && to[2] >= 0 && to[0] % unit == 0 &&
+                       to[1] % unit == 0 && to[2] % unit == 0;
+            };
+            // (what the prefill entry point refuses of the others)
+            int64_t qst[3], ost[3];
+            if (p->window < 0 || p->softmax_scale <= 0.0f || !std::isfinite(p->softmax_scale) ||
+                (p->q_granularity != REEF_SCALE_PER_TENSOR && p->q_granularity != REEF_SCALE_PER_HEAD &&
+                 p->q_granularity != REEF_SCALE_PER_TOKEN) ||
+                !strides(q_strides, 16, qst) || !strides(out_strides, 4, ost) || !aligned(q, 16) ||
+                !aligned(out, 16))
+                return REEF_INVALID_ARGUMENT;
+            if (p->window >= (int64_t(1) << 30)) return REEF_UNSUPPORTED;
+            if (aligned(k_scales, 16) && aligned(v_scales, 16))
+                return launch_chunk_int4(p, q, qst, q_scales, static_cast<const uint8_t *>(k_cache),
+                                         static_cast<const uint8_t *>(v_cache), k_scales, v_scales,
+                                         max_context, block_table, max_blocks_per_seq, num_pages, out,
+                                         ost, base, base + kChunkCounterBytes, status_word, stream);
+        }
+    }
     GatherArgs g;
     g.k = static_cast<const int8_t *>(k_cache);
     g.v = static_cast<const int8_t *>(v_cache);

@@ -195,8 +195,7 @@ def test_decode_bad_lengths_and_pages(reef):
     (2, 1, 8, 128, 77, 333, 0), (1, 2, 1, 64, 130, 1021, 0), (2, 1, 2, 128, 40, 200, 64),
 ])
 def test_chunk(reef, paged, B, H, G, D, T, n, window):
-    """As attention() of tests' kv_reads, row by row. Its rows' products run in units of one
-    fp16 part (2^-11 of a weight) where values stay below 1, two otherwise: the operator's 1e-3."""
+    """Row by row, whichever way the chunk runs: the prefill's own tolerance is 1e-3."""
     rng = np.random.default_rng(T + n + paged)
     L = -(-n // PAGE) * PAGE
     cache = Cache(rng, 4, B, H, D, L, [n] * B, paged)
@@ -212,16 +211,65 @@ def test_chunk(reef, paged, B, H, G, D, T, n, window):
         assert np.abs(got[:, :, i] - want).max() <= max(tol, 1e-3), i
 
 
-def test_chunk_is_the_int8_prefill_on_the_same_codes(reef):
-    """The widened codes are the int8 cache's: the same results, bit for bit."""
+def test_long_chunk_is_the_int8_prefill_on_the_same_codes(reef):
+    """Where the codes are widened they are the int8 cache's: the same results, bit for bit."""
     rng = np.random.default_rng(15)
-    cache = Cache(rng, 4, 2, 2, 128, 96, [90, 90], True)
+    cache = Cache(rng, 4, 2, 2, 128, 2064, [2060, 2060], True)
     k, v, ks, vs = cache.tensors
     wide_k = torch.from_numpy(unpack_keys(k.cpu().numpy()).astype(np.int8)).cuda()
     wide_v = torch.from_numpy(np.ascontiguousarray(
         np.swapaxes(unpack_values(v.cpu().numpy()), -1, -2)).astype(np.int8)).cuda()
-    q = torch.from_numpy(rng.integers(-127, 128, (2, 4, 50, 128)).astype(np.int8)).cuda()
-    qs = torch.rand(4, device="cuda") * 0.01 + 0.01
-    a = reef.attention_prefill_cache_int4(q, qs, *cache.tensors, 90, block_table=cache.block_table)
-    b = reef.attention_prefill_cache(q, qs, wide_k, wide_v, ks, vs, 90, block_table=cache.block_table)
+    q = torch.from_numpy(rng.integers(-127, 128, (2, 16, 128, 128)).astype(np.int8)).cuda()
+    qs = torch.rand(16, device="cuda") * 0.01 + 0.01
+    a = reef.attention_prefill_cache_int4(q, qs, *cache.tensors, 2060, block_table=cache.block_table)
+    b = reef.attention_prefill_cache(q, qs, wide_k, wide_v, ks, vs, 2060, block_table=cache.block_table)
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("paged", [False, True])
+@pytest.mark.parametrize("B,H,G,D,T,n,window,form", [
+    (1, 1, 1, 64, 3, 3, 0, 2), (2, 1, 3, 128, 1, 130, 0, 2), (1, 2, 4, 128, 2, 700, 100, 1),
+    (3, 2, 1, 64, 17, 65, 0, 0), (1, 1, 7, 64, 9, 1500, 0, 2), (2, 3, 5, 128, 10, 64, 20, 1),
+    (1, 1, 40, 64, 2, 300, 0, 2), (2, 2, 2, 64, 300, 300, 0, 1), (1, 1, 2, 128, 64, 5000, 0, 2),
+])
+def test_short_chunk(reef, paged, B, H, G, D, T, n, window, form):
+    """Rows as columns: groups that end inside a tile of them, strided rows, every form of scales,
+    a query of its own place (query_start). Tolerance: kv_reads.attention's."""
+    rng = np.random.default_rng(T + n + paged)
+    L = -(-n // PAGE) * PAGE + 16
+    cache = Cache(rng, 4, B, H, D, L, [n] * B, paged)
+    q = rng.integers(-127, 128, (B, T, H * G, D)).astype(np.int8)  # as a projection lays them out
+    shape = {0: (1,), 1: (H * G,), 2: (B, H * G, T)}[form]
+    qs = rng.uniform(0.005, 0.02, shape).astype(np.float32)
+    full = np.broadcast_to(qs.reshape({0: (1, 1, 1), 1: (1, H * G, 1), 2: shape}[form]), (B, H * G, T))
+    tq = torch.from_numpy(q).cuda().transpose(1, 2)
+    out = torch.full((B, T, H * G, D), 9.0, device="cuda").transpose(1, 2)
+    for start in (n - T, (n - T) // 2):
+        reef.attention_prefill_cache_int4(tq, torch.from_numpy(qs).cuda(), *cache.tensors, n,
+                                          block_table=cache.block_table, window=window,
+                                          query_start=start, q_granularity=form, out=out)
+        got = out.double().cpu().numpy()
+        for i in range(T):
+            end = start + i + 1
+            want, tol = attention(cache, q[:, i], full[:, :, i],
+                                  lambda b, h: range(max(0, end - window) if window else 0, end))
+            assert np.abs(got[:, :, i] - want).max() <= tol, (start, i)
+
+
+def test_short_chunk_bad_pages_read_as_zero_codes(reef):
+    rng = np.random.default_rng(17)
+    cache = Cache(rng, 4, 2, 2, 64, 96, [90, 90], True)
+    q = rng.integers(-127, 128, (2, 4, 5, 64)).astype(np.int8)
+    qs = rng.uniform(0.005, 0.02, 4).astype(np.float32)
+    table = cache.block_table.clone()
+    table[0, 1], table[1, 3] = -1, 1 << 20
+    cache.k[0, :, 16:32] = cache.v[0, :, 16:32] = 0
+    cache.k[1, :, 48:64] = cache.v[1, :, 48:64] = 0
+    status = reef.StatusWord("cuda")
+    got = reef.attention_prefill_cache_int4(torch.from_numpy(q).cuda(), torch.from_numpy(qs).cuda(),
+                                            *cache.tensors, 90, block_table=table, status=status)
+    with pytest.raises(reef.InvalidArgument):
+        status.check("chunk")
+    for i in range(5):
+        want, tol = attention(cache, q[:, :, i], np.broadcast_to(qs, (2, 4)), lambda b, h: range(86 + i))
+        assert np.abs(got[:, :, i].double().cpu().numpy() - want).max() <= tol

@@ -118,19 +118,27 @@ def test_decode(bits):
 def test_prefill_over_the_cache():
     lib = reef_amd.lib()
 
-    def chunk(ws_bytes=1 << 40, tokens=64, table=None, blocks=0, pages=0, k=at(3), **kw):
+    def chunk(ws_bytes=1 << 40, tokens=64, table=None, blocks=0, pages=0, k=at(3), q=at(1), out=at(7),
+              q_strides=None, out_strides=None, **kw):
         d = dict(batch=2, q_heads=8, kv_heads=2, q_len=8, kv_len=40, head_dim=128, query_start=32,
                  window=0, softmax_scale=0.1, q_granularity=1, kv_granularity=2, flags=0)
         d.update(kw)
         return lib.reef_attention_prefill_int4_cache(
-            AttentionParams(**d), at(1), None, at(2), k, at(4), at(5), at(6), tokens, table, blocks, pages,
-            at(7), None, at(8), ws_bytes, None, None)
+            AttentionParams(**d), q, q_strides, at(2), k, at(4), at(5), at(6), tokens, table, blocks, pages,
+            out, out_strides, at(8), ws_bytes, None, None)
 
     for bad in (dict(kv_granularity=1), dict(query_start=33), dict(tokens=32), dict(tokens=72),
                 dict(ws_bytes=1000), dict(k=None), dict(k=at(3, 8)), dict(q_heads=3),
-                dict(table=at(9), blocks=2, pages=9), dict(table=at(9), blocks=3, pages=0)):
+                dict(table=at(9), blocks=2, pages=9), dict(table=at(9), blocks=3, pages=0),
+                dict(window=-1), dict(softmax_scale=0.0), dict(softmax_scale=float("nan")),
+                dict(q_granularity=3), dict(q=at(1, 8)), dict(out=at(7, 4)),
+                dict(q_strides=Strides(0, 120, 128)), dict(q_strides=Strides(0, -128, 128)),
+                dict(out_strides=Strides(0, 130, 128)), dict(out_strides=Strides(0, 128, -4))):
         assert chunk(**bad) == INVALID, bad
-    assert chunk(head_dim=96) == UNSUPPORTED
+        long = dict(q_len=2000, kv_len=2048, query_start=48, tokens=2048, **bad)  # (run the other way)
+        if not set(bad) & {"query_start", "tokens", "table"}:
+            assert chunk(**long) == INVALID, bad
+    assert chunk(head_dim=96) == UNSUPPORTED and chunk(window=1 << 30) == UNSUPPORTED
 
 
 @pytest.mark.parametrize("bits", [4, 8])
