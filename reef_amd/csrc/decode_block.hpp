@@ -35,7 +35,6 @@ struct DecodeArgs {
     const int32_t *sel_pages;   // SEL only: [items, max_sel] page numbers of the sequence
     const int32_t *sel_counts;  // [items]
     int32_t max_sel;
-    int32_t single;  // entries: blocks a part has at least, where a workgroup takes one part; or 0
     int32_t q_gran;
     float score_scale;  // softmax_scale * log2(e)
 };

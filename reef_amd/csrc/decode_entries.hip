@@ -50,6 +50,9 @@ struct EntryArgs : DecodeArgs {
     // kChunk: an item is (sequence, kv head, tile) of HEADS columns of q_len rows x group heads
     int64_t q_sb, q_sh, q_st, o_sb, o_sh, o_st;
     int32_t tiles, q_len, query_start;
+    // dealing out: whether by blocks, whether of few items, the blocks a part has at least where
+    // there is room, the workgroups that run at once
+    int32_t planned, few, least, round;
 };
 
 // Rows of the chunk that columns c and c' of tile t are of (past the last: the last).
@@ -225,106 +228,108 @@ __device__ __forceinline__ int workgroup_sum(int x, int32_t *sWave) {
     return __builtin_amdgcn_readfirstlane(s);
 }
 
-// n units in G runs, the first n % G of them one longer.
-struct Deal {
-    int least, more;  // units of a run, runs with one more
-    __device__ __forceinline__ Deal(int n, int G) : least((uint32_t)n / (uint32_t)G), more(n - least * G) {}
-    __device__ __forceinline__ int start(int g) const { return g * least + min(g, more); }
-    __device__ __forceinline__ int run_of(int u) const {
-        const int cut = more * (least + 1);
-        return u < cut ? (uint32_t)u / (uint32_t)(least + 1) : more + (uint32_t)(u - cut) / (uint32_t)least;
-    }
-};
-
-// The launch's work is the items' (sequence, kv head) 64-key blocks, at least one an item. With
-// at most kPlanItems items every workgroup counts them (from the lengths, in LDS) and finds its own:
-//   single  (no more items than half the workgroups): one part of one item. Parts are of at most c
-//           blocks, c the least that a search from the mean finds to need no more parts than
-//           workgroups; an item's parts are equal to a block. (A run over the end of one item and
-//           the start of the next costs two starts and two merges: 31 us instead of 27 for 128 sequences
-//           of 512 .. 8192 tokens.)
-//   else    an equal run of blocks over the items, whatever the lengths.
-// With more items a workgroup takes an equal run of whole items. Of a part or run the 4 waves take
-// the item's blocks in turn, keep a flash-decoding state each and merge in LDS; an item that lies
-// in one workgroup is stored, the parts of others go to the workspace, and the part that arrives
-// last merges them all.
+// The launch's work is the items' (sequence, kv head) 64-key blocks, at least one an item. A
+// workgroup takes one part of an item. With at most kPlanItems items every workgroup counts the
+// blocks (from the lengths, in LDS) and finds its own; parts are of at most c blocks, an item's
+// equal to a block:
+//   few items (half the workgroups that run at once at most): c is the least, within a sixteenth,
+//             that needs no more parts than those. (Equal runs of blocks over the items' borders
+//             cost two starts and two merges each: 31 us instead of 27 for 128 sequences of 512 ..
+//             8192 tokens.)
+//   more:     c is a workgroup's share of all blocks: an item no longer than that is one part, and
+//             a workgroup takes several parts in turn. (Equal runs of blocks: 94 us instead of 48
+//             for 128 x 16 heads of 16 .. 1024 tokens.)
+// With more items, or none of more than kLeastBlocks blocks, a part is an item. The 4 waves take a
+// part's blocks in turn, keep a flash-decoding state each and merge in LDS; an item in one part is
+// stored, the parts of others go to the workspace, and the part that arrives last merges them all.
 template <int D, int BITS, int HEADS, bool PAGED, Form FORM>
 __global__ __launch_bounds__(kEntryThreads, kWgPerCu) void decode_entries(EntryArgs a, float *out) {
     using Slots = RowSlots<D, HEADS>;
     constexpr int DB = D / 16;  // 16-wide output blocks
     constexpr int N = Slots::N, QD = D / 4;
-    __shared__ int32_t sOff[kPlanItems + 1];
+    __shared__ int32_t sPlan[kPlanItems + 1];  // blocks of the items, then prefixes
     __shared__ int32_t sWave[kDecodeWaves];
     __shared__ f32x4 sRow[kDecodeWaves * N];
     __shared__ float2 sML[kDecodeWaves * 16];
-    __shared__ int32_t sItem;
+    __shared__ int32_t sItem, sPart, sParts, sSlot;
     __shared__ uint32_t sLast;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, grp = lane >> 4;
     const int g = blockIdx.x;
 
-    int units = a.items;  // parts, blocks or items
-    if (a.flat) {
+    const int per = (a.items + kEntryThreads - 1) / kEntryThreads;  // items of a thread's plan
+    const int from = min(tid * per, a.items), to = min(from + per, a.items);
+    int units = a.items;  // parts
+    if (a.planned) {
         int mine = 0;
-        for (int i = tid; i < a.items; i += kEntryThreads) {
+        for (int i = from; i < to; ++i) {
             const int n = entry_keys<HEADS, FORM>(a, i).blocks;
-            sOff[i + 1] = n;
+            sPlan[i] = n;
             mine += n;
         }
-        units = workgroup_sum(mine, sWave);
-    }
-    int c = 1;
-    if (a.single) {
-        const int mean = (units + (a.wgs - a.items / 2) - 1) / (a.wgs - a.items / 2);
-        for (c = max(a.single, mean);; c += max(1, c >> 4)) {
-            int mine = 0;
-            for (int i = tid; i < a.items; i += kEntryThreads)
-                mine += (uint32_t)(sOff[i + 1] + c - 1) / (uint32_t)c;
-            units = workgroup_sum(mine, sWave);
-            if (units <= a.wgs) break;
+        const int total = workgroup_sum(mine, sWave);
+        int c = max(a.least, (total + a.round - 1) / a.round);
+        auto parts_of = [&](int i) { return (int)((uint32_t)(sPlan[i] + c - 1) / (uint32_t)c); };
+        if (a.few) {
+            const int spare = a.round - a.items / 2;  // (parts are rounded up by half of one)
+            for (c = max(a.least, (total + spare - 1) / spare);; c += max(1, c >> 4)) {
+                mine = 0;
+                for (int i = from; i < to; ++i) mine += parts_of(i);
+                if (workgroup_sum(mine, sWave) <= a.round) break;
+            }
         }
-    }
-    const Deal deal(units, a.wgs);
-    const int u0 = a.single ? g : deal.start(g), u1 = a.single ? g + 1 : deal.start(g + 1);
-    if (u0 >= min(u1, units)) return;  // nothing for this workgroup (uniform)
-    if (a.flat) {
-        // sOff[i] becomes the units of items 0 .. i - 1, and sItem the item that unit u0 is of.
-        if (tid == 0) sOff[0] = 0;
-        int run = 0;
-        for (int base = 0; base < a.items; base += kEntryThreads) {
-            const int i = base + tid;
-            const int own = i < a.items ? (uint32_t)(sOff[i + 1] + c - 1) / (uint32_t)c : 0;
-            int x = own;
+        // Prefixes of the parts, which are the workgroups, and of those of items with several,
+        // which are the slots: in the upper half of a word (few items: the slots are the parts).
+        auto words = [&](int n) { return a.few || n == 1 ? n : n | n << 16; };
+        int own = 0;
+        for (int i = from; i < to; ++i) own += words(parts_of(i));
+        int x = own;
 #pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int y = __shfl_up(x, o);
-                if (lane >= o) x += y;
-            }
-            __syncthreads();
-            if (lane == 63) sWave[wave] = x;
-            __syncthreads();
-            int before = run;
-            for (int w = 0; w < kDecodeWaves; ++w) {
-                if (w < wave) before += sWave[w];
-                run += sWave[w];
-            }
-            if (i < a.items) {
-                sOff[i + 1] = before + x;
-                if (u0 < before + x && u0 >= before + x - own) sItem = i;
-            }
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(x, o);
+            if (lane >= o) x += y;
         }
         __syncthreads();
+        if (lane == 63) sWave[wave] = x;
+        __syncthreads();
+        int before = x - own, all = 0;
+        for (int w = 0; w < kDecodeWaves; ++w) {
+            before += w < wave ? sWave[w] : 0;
+            all += sWave[w];
+        }
+        for (int i = from; i < to; ++i) {
+            const int n = words(parts_of(i));
+            sPlan[i] = before;
+            before += n;
+        }
+        if (tid == 0) sPlan[a.items] = all;
+        units = __builtin_amdgcn_readfirstlane(a.few ? all : all & 0xffff);
+        __syncthreads();
     }
-    // Values read from LDS arrive in vector registers; all of these are uniform, and moving them
-    // to scalar registers keeps the loop control and the addresses scalar.
-    auto unit_of = [&](int item) {
-        return a.flat ? __builtin_amdgcn_readfirstlane(sOff[item]) : item;
-    };
-    int item = a.flat ? __builtin_amdgcn_readfirstlane(sItem) : u0;
 
-    for (;;) {
-        const int p_begin = unit_of(item), p_end = unit_of(item + 1);
+    for (int unit = g; unit < units; unit += a.wgs) {
+        // The item, this part of it, the item's parts and the first one's slot.
+        int item = unit, part = 0, parts = 1, slot = 0;
+        if (a.planned) {
+            for (int i = from; i < to; ++i) {
+                const int here = sPlan[i], next = sPlan[i + 1];
+                const int first = a.few ? here : here & 0xffff, end = a.few ? next : next & 0xffff;
+                if (unit >= first && unit < end) {
+                    sItem = i;
+                    sPart = unit - first;
+                    sParts = end - first;
+                    sSlot = a.few ? here : here >> 16;
+                }
+            }
+            __syncthreads();
+            // Values read from LDS arrive in vector registers; all of these are uniform, and
+            // moving them to scalar registers keeps the loop control and the addresses scalar.
+            item = __builtin_amdgcn_readfirstlane(sItem);
+            part = __builtin_amdgcn_readfirstlane(sPart);
+            parts = __builtin_amdgcn_readfirstlane(sParts);
+            slot = __builtin_amdgcn_readfirstlane(sSlot);
+        }
         ItemKeys ik = entry_keys<HEADS, FORM>(a, item);
         ik.len = __builtin_amdgcn_readfirstlane(ik.len);
         ik.lo = __builtin_amdgcn_readfirstlane(ik.lo);
@@ -336,22 +341,10 @@ __global__ __launch_bounds__(kEntryThreads, kWgPerCu) void decode_entries(EntryA
         const int b = pair / a.kv_heads, kvh = pair % a.kv_heads;
         // columns of the item, HEADS at most
         const int cols = FORM == kChunk ? min(HEADS, a.q_len * a.group - tile * HEADS) : a.group;
-        // This segment's blocks of the item, the workgroups with a part of it (parts from gf on).
-        int s_blk = 0, e_blk = ik.blocks, parts = 1, gf = g;
-        if (a.single) {
-            parts = p_end - p_begin;
-            gf = p_begin;
-            const Deal blocks(ik.blocks, parts);
-            s_blk = blocks.start(g - gf);
-            e_blk = blocks.start(g - gf + 1);
-        } else if (a.flat) {
-            s_blk = max(u0, p_begin) - p_begin;
-            e_blk = min(u1, p_end) - p_begin;
-            if (p_begin < u0 || p_end > u1) {
-                gf = deal.run_of(p_begin);
-                parts = deal.run_of(p_end - 1) - gf + 1;
-            }
-        }
+        // The part's blocks of the item: the first `more` parts have one more than the others.
+        const int least = (uint32_t)ik.blocks / (uint32_t)parts, more = ik.blocks - least * parts;
+        const int s_blk = part * least + min(part, more);
+        const int e_blk = s_blk + least + (part < more ? 1 : 0);
         if (ik.bad && s_blk == 0 && tid == 0) flag_status(a.status, REEF_STATUS_BIT_BAD_LENGTH);
 
         const int k_begin = (ik.first_block + s_blk + wave) * kBlockKeys;
@@ -426,16 +419,15 @@ __global__ __launch_bounds__(kEntryThreads, kWgPerCu) void decode_entries(EntryA
                 if (s < N) store(s, merge_slot<D, HEADS>(sRow, sML, s, kDecodeWaves));
             }
         } else {
-            // A workgroup's part of an item lies in its slot 0 if its run began with it, in slot
-            // 1 if the run ended with it. The slots are written and counted in as in decode.hip.
-            auto part_at = [&](int gg, int slot) {
+            // (written and counted in as in decode.hip)
+            auto part_at = [&](int i) {
                 return reinterpret_cast<uint64_t *>(a.slots) +
-                       ((int64_t)gg * 2 + slot) * DecodeSlot<D>::ELEMS;
+                       (int64_t)(slot + i) * DecodeSlot<D>::ELEMS;
             };
             auto pack = [](float x0, float x1) {
                 return (uint64_t)__float_as_uint(x0) | ((uint64_t)__float_as_uint(x1) << 32);
             };
-            uint64_t *so = part_at(g, a.single || p_begin <= u0 ? 0 : 1);
+            uint64_t *so = part_at(part);
 #pragma unroll
             for (int k = 0; k < Slots::PER; ++k) {
                 const int s = tid + k * kEntryThreads;
@@ -456,7 +448,6 @@ __global__ __launch_bounds__(kEntryThreads, kWgPerCu) void decode_entries(EntryA
                 // several parts before it uses the first: a round trip for them all, not one each.
                 constexpr int AHEAD = 16 / Slots::PER;
                 const int gi = tid / N;  // (PER > 1: 0)
-                const int first_slot = !a.single && deal.start(gf) < p_begin ? 1 : 0;
                 auto lo32 = [](uint64_t v) { return __uint_as_float((uint32_t)v); };
                 auto hi32 = [](uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); };
                 RowRun run[Slots::PER];
@@ -470,8 +461,7 @@ __global__ __launch_bounds__(kEntryThreads, kWgPerCu) void decode_entries(EntryA
                         uint64_t w[AHEAD][3];
 #pragma unroll
                         for (int i = 0; i < AHEAD; ++i) {
-                            const int part = min(i0 + i * Slots::GROUPS, parts - 1);
-                            const uint64_t *sl = part_at(gf + part, part == 0 ? first_slot : 0);
+                            const uint64_t *sl = part_at(min(i0 + i * Slots::GROUPS, parts - 1));
                             w[i][0] = part_load(sl + s);
                             w[i][1] = part_load(sl + N + s);
                             w[i][2] = part_load(sl + 2 * N + s / QD);
@@ -497,30 +487,33 @@ __global__ __launch_bounds__(kEntryThreads, kWgPerCu) void decode_entries(EntryA
                 }
             }
         }
-        if (a.single || p_end >= u1) break;
-        ++item;
-        __syncthreads();  // frees sRow, sML and sLast
+        __syncthreads();  // frees what this part had in LDS
     }
 }
 
-// Launches `a`, whose sequences have `blocks` 64-key blocks at most, of (batch, kv head) pairs that
-// read up to `tokens` tokens (a list's may be longer than the cache); num_splits as for decode.
+// Launches `a`, whose items have `blocks` 64-key blocks at most (lists that name pages of the cache
+// twice may have more); flat: the blocks of all fit 31 bits; num_splits as for decode.
 template <int BITS, bool PAGED, Form FORM>
 reef_status launch_entries(EntryArgs &a, int64_t head_dim, int64_t columns, int64_t blocks, bool flat,
                            int64_t num_splits, float *out, char *counters, char *slots,
                            hipStream_t stream) {
     const int64_t items = a.items;
-    flat = flat && items <= kPlanItems;  // (the plan's words in LDS)
     // Two workgroups a compute unit, one where items are few: an item's parts are half as many then
     // and the bytes take no longer (1 x 8 x 131071 tokens: 36 us against 43, 64 parts an item).
     const int64_t cus = compute_units();
-    const int64_t most = num_splits > 0 ? ceil_div(items * num_splits, kDecodeWaves)
-                                        : (2 * items <= cus ? 1 : kWgPerCu) * cus;
-    a.flat = flat ? 1 : 0;
+    const int64_t round = num_splits > 0 ? ceil_div(items * num_splits, kDecodeWaves)
+                                         : (2 * items <= cus ? 1 : kWgPerCu) * cus;
     const int64_t least = num_splits > 0 ? 1 : kLeastBlocks;
-    a.single = flat && 2 * items <= most ? (int32_t)least : 0;
-    const int64_t units = a.single ? items * ceil_div(blocks, least) : flat ? items * blocks : items;
-    a.wgs = (int32_t)std::max<int64_t>(1, std::min<int64_t>(std::min(most, units), 1 << 20));
+    a.few = (num_splits > 0 ? items : 2 * items) <= round;
+    // (the plan has words for kPlanItems items; asked for fewer waves than items: items)
+    a.planned = flat && items <= kPlanItems && blocks > least && (a.few || num_splits == 0);
+    a.least = (int32_t)least;
+    // (of few items as many workgroups as parts: the search keeps to them; of more, slots for 2 round
+    // parts are more than the items of several parts have)
+    const int64_t wgs = !a.planned ? std::min(items, num_splits > 0 ? items : round)
+                        : a.few    ? std::min(round, items * ceil_div(blocks, least)) : round;
+    a.wgs = (int32_t)std::max<int64_t>(1, std::min<int64_t>(wgs, 1 << 20));
+    a.round = a.wgs;
     a.counters = reinterpret_cast<uint32_t *>(counters);
     a.slots = reinterpret_cast<float *>(slots);
     const auto run = [&](auto *kernel) {

@@ -152,6 +152,24 @@ def test_decode_scale_forms_and_a_full_cache(reef):
         assert np.abs(got.double().cpu().numpy() - want).max() <= tol
 
 
+@pytest.mark.parametrize("B,H,L", [(20, 8, 1040), (48, 8, 1040), (256, 8, 704), (2, 1, 6000)])
+def test_decode_lengths_far_apart(reef, B, H, L):
+    """One or a few long sequences among short ones: items of several parts and of one, few and many
+    of them, the same bits on every run."""
+    rng = np.random.default_rng(B)
+    lens = [int(n) for n in rng.integers(1, 200, B)]
+    for i in rng.choice(B, max(1, B // 16), replace=False):
+        lens[i] = L - int(rng.integers(0, 100))
+    cache = Cache(rng, 4, B, H, 64, L, lens, True)
+    q, qs = queries(rng, B, 2 * H, 64)
+    tq, tqs = torch.from_numpy(q).cuda(), torch.from_numpy(qs).cuda()
+    want, tol = attention(cache, q, qs, lambda b, h: range(lens[b]))
+    runs = [reef.attention_decode_int4(tq, tqs, *cache.tensors, cache.context_lens,
+                                       block_table=cache.block_table) for _ in range(4)]
+    assert np.abs(runs[0].double().cpu().numpy() - want).max() <= tol
+    assert all(torch.equal(r, runs[0]) for r in runs)
+
+
 def test_decode_more_sequences_than_a_plan(reef):
     """Beyond 2048 (sequence, kv head) pairs a launch deals out whole sequences."""
     rng = np.random.default_rng(12)

@@ -219,6 +219,29 @@ def test_decode_listed_more_sequences_than_a_plan(reef, bits):
     assert np.abs(got.double().cpu().numpy() - want).max() <= tol
 
 
+@pytest.mark.parametrize("B,H", [(1, 3), (40, 8), (130, 8)])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_decode_lists_longer_than_the_cache(reef, bits, B, H):
+    """A few pages named many times, by some sequences: parts of long lists next to short ones."""
+    rng = np.random.default_rng(bits + B)
+    L = 592  # 10 blocks of 64 keys: more than a part has at least
+    lens = [L if i % 2 else 16 for i in range(B)]
+    cache = Cache(rng, bits, B, H, 64, L, lens, False)
+    q, qs = queries(rng, B, H, 64)
+    listed = np.stack([rng.integers(0, -(-lens[i // H] // PAGE), 300) for i in range(B * H)])
+    listed = listed.reshape(B, H, 300).astype(np.int32)
+    counts = np.where(rng.random((B, H)) < 0.2, 300, rng.integers(0, 20, (B, H))).astype(np.int32)
+    counts[0, 0] = 300
+    call = reef.attention_decode_int4 if bits == 4 else reef.attention_decode_selected
+    want, tol = attention(cache, q, qs, lambda b, h: [
+        t for p in listed[b, h, :counts[b, h]] for t in range(PAGE * p, min(PAGE * p + PAGE, lens[b]))])
+    for _ in range(2):
+        got = call(torch.from_numpy(q).cuda(), torch.from_numpy(qs).cuda(), *cache.tensors,
+                   cache.context_lens,
+                   selected=(torch.from_numpy(listed).cuda(), torch.from_numpy(counts).cuda()))
+        assert np.abs(got.double().cpu().numpy() - want).max() <= tol
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 def test_decode_listed_bad_entries(reef, bits):
     rng = np.random.default_rng(bits)
