@@ -604,19 +604,22 @@ reef_status decode_any(const reef_decode_params *p, const int8_t *q, const float
 
 // A 64-key block of 16 columns costs about 1.4 ns of the whole GPU's time here, one of a 128-row
 // tile 9 ns there, behind a copy of the cache and a schedule's start of 25 us. So a chunk runs here
-// if it has few blocks (2 x 12 heads x 77 rows over 1021 keys: 13.8 us against 29.8; 32 heads x
-// 64 rows over 4096 24.9 against 47.6) or if its tiles of 128 rows stay part empty (100 rows over
-// 8000 keys, 2 x 32 heads: 81 against 107; 16 rows over 6000, 8 x 16: 25 against 153). With full
-// tiles and many blocks it does not (512 rows over 4608, 4 x 32: 388 against 248).
+// if it has few blocks (2 x 12 heads of 64, 77 rows over 1021 keys: 13.6 us against 30; 32 heads, 8
+// of keys, of 128, 64 rows over 4096 24.5 against 46; 12 heads of 64, 1024 rows over 1024 24 against
+// 32) or if its tiles of 128 rows stay part empty (8 x 16 heads of 64, 16 rows over 6000: 25 against
+// 155; 2 x 32 heads of 128, 100 rows over 8000 95 against 105). With full tiles and many blocks it
+// does not (32 heads of 128, 1024 rows over 1024: 65 against 46; 4 x 32, 512 over 4608 382 against
+// 261; 8 x 12 of 64, 512 over 1024 61 against 51).
 bool chunk_entries_fit(const reef_attention_params *p) {
-    constexpr int64_t kFew = 8192, kRows = 128;
+    constexpr int64_t kRows = 128;
+    const int64_t few = p->head_dim == 64 ? 32768 : 16384;
     const int64_t group = p->q_heads / p->kv_heads;
     if (p->q_len > (1 << 20) || p->q_len * group > (1 << 20)) return false;
     const int64_t items = p->batch * p->kv_heads * ceil_div(p->q_len * group, 16);
     const int64_t tiles = p->batch * p->q_heads * ceil_div(p->q_len, kRows);
     const int64_t end = p->query_start + p->q_len;
     const int64_t blocks = ceil_div(p->window > 0 ? std::min(end, p->window + p->q_len) : end, kBlockKeys);
-    return items <= kPlanItems && (items * blocks <= kFew || 2 * items <= 13 * tiles);
+    return items <= kPlanItems && (items * blocks <= few || 2 * items <= 13 * tiles);
 }
 
 reef_status launch_chunk_int4(const reef_attention_params *p, const int8_t *q, const int64_t (&qst)[3],

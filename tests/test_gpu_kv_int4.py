@@ -232,15 +232,15 @@ def test_chunk(reef, paged, B, H, G, D, T, n, window):
 def test_long_chunk_is_the_int8_prefill_on_the_same_codes(reef):
     """Where the codes are widened they are the int8 cache's: the same results, bit for bit."""
     rng = np.random.default_rng(15)
-    cache = Cache(rng, 4, 2, 2, 128, 2064, [2060, 2060], True)
+    cache = Cache(rng, 4, 2, 2, 128, 4112, [4100, 4100], True)
     k, v, ks, vs = cache.tensors
     wide_k = torch.from_numpy(unpack_keys(k.cpu().numpy()).astype(np.int8)).cuda()
     wide_v = torch.from_numpy(np.ascontiguousarray(
         np.swapaxes(unpack_values(v.cpu().numpy()), -1, -2)).astype(np.int8)).cuda()
     q = torch.from_numpy(rng.integers(-127, 128, (2, 16, 128, 128)).astype(np.int8)).cuda()
     qs = torch.rand(16, device="cuda") * 0.01 + 0.01
-    a = reef.attention_prefill_cache_int4(q, qs, *cache.tensors, 2060, block_table=cache.block_table)
-    b = reef.attention_prefill_cache(q, qs, wide_k, wide_v, ks, vs, 2060, block_table=cache.block_table)
+    a = reef.attention_prefill_cache_int4(q, qs, *cache.tensors, 4100, block_table=cache.block_table)
+    b = reef.attention_prefill_cache(q, qs, wide_k, wide_v, ks, vs, 4100, block_table=cache.block_table)
     assert torch.equal(a, b)
 
 
