@@ -523,7 +523,8 @@ reef_status reef_kv_append_int8_paged(const reef_kv_append_params *p, const floa
  * In all calls of this section block_table NULL means the contiguous cache of
  * p->max_context tokens a sequence (max_blocks_per_seq and num_pages are not used), otherwise
  * the paged one with max_context <= max_blocks_per_seq * 16. The int8 cache's page calls
- * (free, fork, reserve, compact) serve either pool.
+ * (free, fork, reserve, compact) serve either pool. Decode and unpack take their scales on 16
+ * bytes (unpack's keys': 4), as any allocation is.
  */
 
 /* reef_kv_append_int8 (its limits, status bits and context_lens) into the 4-bit cache. The
@@ -575,8 +576,13 @@ reef_status reef_attention_decode_int4(const reef_decode_params *p, const int8_t
                                        void *workspace, size_t workspace_bytes,
                                        uint32_t *status_word, hipStream_t stream);
 
-/* reef_attention_prefill_int8_cache over the 4-bit cache (max_context as there). The codes
- * are widened on their way into the workspace, which is that call's, of the same size. */
+/* reef_attention_prefill_int8_cache over the 4-bit cache (max_context as there; the workspace
+ * is that call's, of the same size, zero-filled once). A long chunk's codes are widened on
+ * their way into the workspace: the results of that call on an int8 cache of the same codes. A
+ * short one, with REEF_ATTN_SCHED_AUTO and scales on 16 bytes, reads the cache in place as
+ * decode does: the same sums in another order, with P in two fp16 parts. Either way a page number
+ * outside [0, num_pages) sets BAD_PAGE and its page reads as zero codes; a short chunk looks at
+ * the pages that its rows see. */
 reef_status reef_attention_prefill_int4_cache(
     const reef_attention_params *p, const int8_t *q, const reef_strides *q_strides,
     const float *q_scales, const uint8_t *k_cache, const uint8_t *v_cache, const float *k_scales,

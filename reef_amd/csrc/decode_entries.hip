@@ -55,7 +55,7 @@ struct EntryArgs : DecodeArgs {
     int32_t planned, few, least, round;
 };
 
-// Rows of the chunk that columns c and c' of tile t are of (past the last: the last).
+// The chunk's row that column c of a tile is of (past the last: the last).
 template <int HEADS>
 __device__ __forceinline__ int chunk_row(const EntryArgs &a, int tile, int c) {
     return min((tile * HEADS + c) / a.group, a.q_len - 1);
@@ -618,7 +618,8 @@ bool chunk_entries_fit(const reef_attention_params *p) {
     const int64_t items = p->batch * p->kv_heads * ceil_div(p->q_len * group, 16);
     const int64_t tiles = p->batch * p->q_heads * ceil_div(p->q_len, kRows);
     const int64_t end = p->query_start + p->q_len;
-    const int64_t blocks = ceil_div(p->window > 0 ? std::min(end, p->window + p->q_len) : end, kBlockKeys);
+    const int64_t blocks = ceil_div(p->window > 0 ? std::min(end, std::min(end, p->window) + p->q_len) : end,
+                                    kBlockKeys);
     return items <= kPlanItems && (items * blocks <= few || 2 * items <= 13 * tiles);
 }
 

@@ -1,6 +1,6 @@
 // Pages that a query selects (gfx950): bounds of every page's keys, a query's scores against
 // them, and the best `budget` pages of each (sequence, kv head), for the decode step over a list
-// of pages (decode.hip).
+// of pages (decode_entries.hip).
 //
 // A page's bounds are the largest and the least key of each channel, hi and lo, as int8 codes of
 // one scale S a page, rounded outwards. For any key x of the page and a query q,
@@ -427,12 +427,13 @@ struct HeldKeys<0> {
     }
 };
 
-// One workgroup an item: the budget-th largest of its n keys, then the pages above it and the first of those at it,
-// in page order. Wave w holds a run of pages, 64 at a time. The last key taken is found digit by
+// One workgroup an item: the budget-th largest of its n keys, then the pages above it and the first
+// of those at it, in page order. Wave w holds a run of pages, 64 at a time. The last key taken is found digit by
 // digit from the highest bit in which scores differ (they share sign and most of the exponent): the
 // keys of the range so far are counted by the digit's value in LDS, and the first value that enough
-// of them reach is the next range, until exactly enough do. Two digits mostly: 3 us for 8192 pages
-// (bit by bit 11, with a pass over the keys in memory a bit 62).
+// of them reach is the next range, until exactly enough do. Two digits mostly: 8.8 us of a launch of
+// 8 items of 8192 pages (bit by bit 12, with a pass over the keys in memory a bit 63), 5.6 of one of
+// 128 items of up to 512.
 template <int R>
 __global__ __launch_bounds__(kPickThreads) void pick_pages(SelectArgs a) {
     __shared__ PickShared sh;

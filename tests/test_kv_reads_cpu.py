@@ -138,6 +138,17 @@ def test_prefill_over_the_cache():
     assert chunk(head_dim=96) == UNSUPPORTED and chunk(window=1 << 30) == UNSUPPORTED
 
 
+def test_the_widest_window():
+    """The widest 64-bit window is refused like others past 2^30, on the way of a short chunk too."""
+    for q_len in (1, 8):
+        p = AttentionParams(batch=2, q_heads=8, kv_heads=2, q_len=q_len, kv_len=4096, head_dim=128,
+                            query_start=4096 - q_len, window=(1 << 63) - 1, softmax_scale=0.1,
+                            q_granularity=1, kv_granularity=2, flags=0)
+        assert reef_amd.lib().reef_attention_prefill_int4_cache(
+            p, at(1), None, at(2), at(3), at(4), at(5), at(6), 4096, None, 0, 0, at(7), None, at(8),
+            1 << 40, None, None) == UNSUPPORTED
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 def test_bounds(bits):
     for change, status in ((dict(batch=0), INVALID), (dict(new_tokens=0), INVALID),
