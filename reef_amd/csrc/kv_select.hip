@@ -150,10 +150,10 @@ __global__ __launch_bounds__(kBoundWaves * kWave) void page_bounds(BoundArgs a) 
                                        __float_as_int(n[c]), 0x128, 0xf, 0xf, true)));  // row_ror 8
         }
         constexpr int kSplit = BITS == 4 ? 16 : 32;  // lanes of one bound (and half)
-        const float top = __uint_as_float(wave_reduce(
-            __float_as_uint(fmaxf(fmaxf(n[0], n[1]), fmaxf(n[2], n[3]))), [](uint32_t x, uint32_t y) {
-                return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y)));
-            }));
+        // (the largest magnitude: not below zero, so the order of the words is the values')
+        const float lane_top = fmaxf(fmaxf(fmaxf(n[0], n[1]), fmaxf(n[2], n[3])), 0.0f);
+        const float top = __uint_as_float(
+            wave_reduce(__float_as_uint(lane_top), [](uint32_t x, uint32_t y) { return max(x, y); }));
         const float scale = int8_scale(top);
         uint32_t packed = 0;
 #pragma unroll
@@ -357,12 +357,7 @@ __device__ __forceinline__ void pick_digit(PickShared &sh, const int *bins, uint
         c[i] = bins[kBins - 1 - (4 * lane + i)];
         sum += c[i];
     }
-    int upto = sum;  // of this lane's values and those above
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(upto, o);
-        if (lane >= o) upto += y;
-    }
+    const int upto = wave_scan(sum);  // of this lane's values and those above
     const uint64_t enough = __builtin_amdgcn_ballot_w64(upto >= rem);
     if (enough == 0) {  // fewer than that in all: every one of them
         if (lane == 0) {

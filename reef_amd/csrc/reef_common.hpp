@@ -108,6 +108,17 @@ __device__ __forceinline__ uint32_t wave_reduce(uint32_t x, F f) {
     return f(s[0], s[1]);
 }
 
+// Inclusive sums over the 64 lanes, in VALU ops.
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 to rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to the upper half
+    return x;
+}
+
 // A raw buffer resource over [base, base + bytes): loads through it take a
 // per-lane VGPR offset and a uniform SGPR offset, and read zeros past the end.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_rsrc(const void *base, uint32_t bytes) {
