@@ -574,8 +574,10 @@ reef_status launch_entries(EntryArgs &a, int64_t head_dim, int64_t columns, int6
                                          : (2 * items <= cus ? 1 : kWgPerCu) * cus;
     const int64_t least = num_splits > 0 ? 1 : kLeastBlocks;
     a.few = (num_splits > 0 ? items : 2 * items) <= round;
-    // (the plan has words for kPlanItems items; asked for fewer waves than items: items)
-    a.planned = flat && items <= kPlanItems && blocks > least && (a.few || num_splits == 0);
+    // (the plan has words for kPlanItems items and counts blocks in 31 bits; asked for fewer waves
+    // than items: items)
+    a.planned = flat && items <= kPlanItems && items * blocks < (int64_t(1) << 31) && blocks > least &&
+                (a.few || num_splits == 0);
     a.least = (int32_t)least;
     // (of few items as many workgroups as parts: the search keeps to them; of more, slots for 2 round
     // parts are more than the items of several parts have)
