@@ -166,3 +166,28 @@ def test_window_that_leaves_a_list_nothing(reef, bits):
     want, tol = attention(cache, q, qs, lambda b, h: range(624, 630) if b else [])
     assert np.abs(got.double().cpu().numpy() - want).max() <= tol
     assert not got[0].any()
+
+
+@pytest.mark.parametrize("B,H,splits", [(40, 8, 9), (33, 8, 4), (33, 8, 1), (70, 1, 30), (300, 8, 7)])
+def test_asked_for_splits_of_many_sequences(reef, B, H, splits):
+    """num_splits with more items than a wave's plan holds, and than a workgroup's."""
+    rng = np.random.default_rng(B + splits)
+    lens = [int(n) for n in rng.integers(1, 641, B)]
+    cache = Cache(rng, 4, B, H, 64, 640, lens, True)
+    q, qs = queries(rng, B, H, 64)
+    want, tol = attention(cache, q, qs, lambda b, h: range(lens[b]))
+    tq, tqs = torch.from_numpy(q).cuda(), torch.from_numpy(qs).cuda()
+    for _ in range(2):
+        got = reef.attention_decode_int4(tq, tqs, *cache.tensors, cache.context_lens,
+                                         block_table=cache.block_table, num_splits=splits)
+        assert np.abs(got.double().cpu().numpy() - want).max() <= tol
+    listed = torch.arange(39, -1, -1, dtype=torch.int32).cuda().expand(B, H, 40).contiguous()
+    counts = torch.full((B, H), 40, dtype=torch.int32)
+    for b in range(B):
+        counts[b] = -(-lens[b] // PAGE)
+    # (a list in descending order holds the pages at its end: the rest is left out by a negative entry)
+    listed = torch.where(listed < counts.cuda()[..., None], listed, -1).contiguous()
+    got = reef.attention_decode_int4(tq, tqs, *cache.tensors, cache.context_lens, num_splits=splits,
+                                     selected=(listed, torch.full((B, H), 40, dtype=torch.int32).cuda()),
+                                     block_table=cache.block_table)
+    assert np.abs(got.double().cpu().numpy() - want).max() <= tol
