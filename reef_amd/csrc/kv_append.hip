@@ -275,9 +275,6 @@ __global__ void advance_lengths(const int32_t *start, int32_t batch, int32_t new
 
 // --- the 4-bit cache as fp32 rows ----------------------------------------------------------
 
-constexpr int kUnpackThreads = 256;
-constexpr int kUnpackPages = 8;  // pages a workgroup
-
 struct UnpackArgs {
     const uint8_t *k, *v;
     const float *ks, *vs;
@@ -285,67 +282,66 @@ struct UnpackArgs {
     int64_t pages;
 };
 
-// A wave takes a page, and every store of it writes whole rows or quarters of rows in order. Keys:
-// a lane reads 4 bytes of a row, four channels of either half. Values: a lane reads the 8 bytes of
-// four channels each and writes them for the tokens of its group of lanes.
+// A wave takes a page and is a workgroup (two pages a wave, four waves a workgroup: 11.0 us instead of
+// 9.8 for 2560 pages of 128 channels, 35.6 instead of 33.8 for 8192), and every store of it writes
+// whole rows or quarters of rows in order. Keys: a lane reads 4 bytes of a row, four channels of
+// either half. Values: a lane reads the 8 bytes of four channels each and writes them for the tokens
+// of its group of lanes.
 template <int D>
-__global__ __launch_bounds__(kUnpackThreads) void unpack_int4(UnpackArgs a) {
+__global__ __launch_bounds__(kWave) void unpack_int4(UnpackArgs a) {
     constexpr int RB = D / 2;                 // bytes of a key row
     constexpr int KL = RB / 4, KR = 64 / KL;  // lanes a key row, rows of a load
     constexpr int VL = D / 4, VG = 64 / VL;   // lanes a value row, groups of lanes
     constexpr int VT = kPage / VG;            // tokens of a group
-    const int lane = threadIdx.x & (kWave - 1);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x;
+    const int64_t page = linear_block();
+    if (page >= a.pages) return;
     auto store = [](float *p, f32x4 x) { *reinterpret_cast<f32x4 *>(p) = x; };
-    const int64_t begin = linear_block() * kUnpackPages + wave;
-    const int64_t end = min((linear_block() + 1) * kUnpackPages, a.pages);
-    for (int64_t page = begin; page < end; page += kUnpackThreads / 64) {
-        if (a.k_out) {
-            const int j = lane % KL, g = lane / KL;
-            const uint8_t *rows = a.k + (page * kPage + g) * RB + 4 * j;
-            float *out = a.k_out + (page * kPage + g) * D + 4 * j;
-            uint32_t w[kPage / KR];
-            float s[kPage / KR];
+    if (a.k_out) {
+        const int j = lane % KL, g = lane / KL;
+        const uint8_t *rows = a.k + (page * kPage + g) * RB + 4 * j;
+        float *out = a.k_out + (page * kPage + g) * D + 4 * j;
+        uint32_t w[kPage / KR];
+        float s[kPage / KR];
 #pragma unroll
-            for (int i = 0; i < kPage / KR; ++i) {
-                w[i] = *reinterpret_cast<const uint32_t *>(rows + i * KR * RB);
-                s[i] = a.ks[page * kPage + i * KR + g];
-            }
-#pragma unroll
-            for (int i = 0; i < kPage / KR; ++i) {
-                f32x4 x, y;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    x[c] = (float)((int)(w[i] >> (8 * c) & 0xf) - kInt4Zero) * s[i];
-                    y[c] = (float)((int)(w[i] >> (8 * c + 4) & 0xf) - kInt4Zero) * s[i];
-                }
-                store(out + i * KR * D, x);
-                store(out + i * KR * D + D / 2, y);
-            }
+        for (int i = 0; i < kPage / KR; ++i) {
+            w[i] = *reinterpret_cast<const uint32_t *>(rows + i * KR * RB);
+            s[i] = a.ks[page * kPage + i * KR + g];
         }
-        if (a.v_out) {
-            const int j = lane % VL, g = lane / VL;
-            // this group's tokens' half of each channel: VT 8 or 4 of 8 nibbles
-            const int half = g * VT / 8;
-            const uint8_t *rows = a.v + (page * D + 4 * j) * 8 + 4 * half;
-            uint32_t w[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) w[c] = *reinterpret_cast<const uint32_t *>(rows + 8 * c);
-            f32x4 s[VT / 4];
+        for (int i = 0; i < kPage / KR; ++i) {
+            f32x4 x, y;
 #pragma unroll
-            for (int i = 0; i < VT / 4; ++i)
-                s[i] = *reinterpret_cast<const f32x4 *>(a.vs + page * kPage + g * VT + 4 * i);
-            float *out = a.v_out + (page * kPage + g * VT) * D + 4 * j;
-            const int base = VT == 8 ? 0 : 8 * (g & 1);  // of the four tokens' low nibbles
-#pragma unroll
-            for (int t = 0; t < VT; ++t) {
-                const int n = 4 * (kv_nibble(t) % 8);
-                f32x4 x;
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    x[c] = (float)((int)(w[c] >> (base + n) & 0xf) - kInt4Zero) * s[t / 4][t % 4];
-                store(out + t * D, x);
+            for (int c = 0; c < 4; ++c) {
+                x[c] = (float)((int)(w[i] >> (8 * c) & 0xf) - kInt4Zero) * s[i];
+                y[c] = (float)((int)(w[i] >> (8 * c + 4) & 0xf) - kInt4Zero) * s[i];
             }
+            store(out + i * KR * D, x);
+            store(out + i * KR * D + D / 2, y);
+        }
+    }
+    if (a.v_out) {
+        const int j = lane % VL, g = lane / VL;
+        // this group's tokens' half of each channel: VT 8 or 4 of 8 nibbles
+        const int half = g * VT / 8;
+        const uint8_t *rows = a.v + (page * D + 4 * j) * 8 + 4 * half;
+        uint32_t w[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) w[c] = *reinterpret_cast<const uint32_t *>(rows + 8 * c);
+        f32x4 s[VT / 4];
+#pragma unroll
+        for (int i = 0; i < VT / 4; ++i)
+            s[i] = *reinterpret_cast<const f32x4 *>(a.vs + page * kPage + g * VT + 4 * i);
+        float *out = a.v_out + (page * kPage + g * VT) * D + 4 * j;
+        const int base = VT == 8 ? 0 : 8 * (g & 1);  // of the four tokens' low nibbles
+#pragma unroll
+        for (int t = 0; t < VT; ++t) {
+            const int n = 4 * (kv_nibble(t) % 8);
+            f32x4 x;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                x[c] = (float)((int)(w[c] >> (base + n) & 0xf) - kInt4Zero) * s[t / 4][t % 4];
+            store(out + t * D, x);
         }
     }
 }
@@ -498,12 +494,12 @@ extern "C" reef_status reef_kv_unpack_int4(const uint8_t *k_pages, const uint8_t
         (v && (!v_pages || !v_scales)) || !aligned(k_pages, 16) || !aligned(v_pages, 16) ||
         !aligned(k, 16) || !aligned(v, 16) || !aligned(k_scales, 4) || !aligned(v_scales, 16))
         return REEF_INVALID_ARGUMENT;
-    if ((head_dim != 64 && head_dim != 128) || pages >= (int64_t(1) << 40)) return REEF_UNSUPPORTED;
+    if ((head_dim != 64 && head_dim != 128) || pages >= (int64_t(1) << 36)) return REEF_UNSUPPORTED;
     const UnpackArgs a{k_pages, v_pages, k_scales, v_scales, k, v, pages};
-    const dim3 grid = linear_grid(ceil_div(pages, kUnpackPages));
+    const dim3 grid = linear_grid(pages);
     if (head_dim == 128)
-        hipLaunchKernelGGL(unpack_int4<128>, grid, dim3(kUnpackThreads), 0, stream, a);
+        hipLaunchKernelGGL(unpack_int4<128>, grid, dim3(kWave), 0, stream, a);
     else
-        hipLaunchKernelGGL(unpack_int4<64>, grid, dim3(kUnpackThreads), 0, stream, a);
+        hipLaunchKernelGGL(unpack_int4<64>, grid, dim3(kWave), 0, stream, a);
     return launch_status();
 }
