@@ -1080,12 +1080,12 @@ def kv_keep_paged(kept, kept_lens, context_lens, block_table, k_pages, v_pages, 
 # The codes' places in a byte: the C header. An int8 cache (int8 tensors, D for D/2 and 16 for 8)
 # takes the calls that are not named for 4 bits.
 
-def _alike(what, *checks):
-    """(tensor, type, name): contiguous, of its type, on the current device. Tensors that are None
-    are left out."""
+def _alike(what, *checks, optional=("block_table",)):
+    """(tensor, type, name): contiguous, of its type, on the current device. Those of the optional
+    names may be None."""
     device = None
     for t, dtype, name in checks:
-        if t is None:
+        if t is None and name in optional:
             continue
         try:
             at = t.get_device()
@@ -1137,7 +1137,7 @@ def kv_append_int4(k_new, v_new, start_positions, k_cache, v_cache, k_scales, v_
     _alike(what, (k_cache, byte, "k_cache"), (v_cache, byte, "v_cache"),
            (k_scales, f32, "k_scales"), (v_scales, f32, "v_scales"),
            (start_positions, i32, "start_positions"), (context_lens, i32, "context_lens"),
-           (block_table, i32, "block_table"))
+           (block_table, i32, "block_table"), optional=("context_lens", "block_table"))
     _on_device(what, k_new, v_new)
     B, H, T, D = k_new.shape
     heads, tokens, dim, blocks, pages = _cache_sizes(what, B, k_cache, v_cache, k_scales, v_scales,
@@ -1223,12 +1223,14 @@ def _decode_cache(what, function, bits, q, q_scales, k_cache, v_cache, k_scales,
     torch = _torch()
     code, f32, i32 = torch.int8 if bits == 8 else torch.uint8, torch.float32, torch.int32
     chosen = counts = listed = None
+    picked = ()
     if selected is not None:
         chosen, counts = selected
+        picked = (chosen, i32, "selected pages"), (counts, i32, "selected counts")
     _alike(what, (q, torch.int8, "q"), (q_scales, f32, "q_scales"), (k_cache, code, "k_cache"),
            (v_cache, code, "v_cache"), (k_scales, f32, "k_scales"), (v_scales, f32, "v_scales"),
-           (context_lens, i32, "context_lens"), (block_table, i32, "block_table"),
-           (chosen, i32, "selected pages"), (counts, i32, "selected counts"), (out, f32, "out"))
+           (context_lens, i32, "context_lens"), (block_table, i32, "block_table"), *picked,
+           (out, f32, "out"), optional=("context_lens", "block_table", "out"))
     shape = q.shape
     if len(shape) != 3:
         raise InvalidArgument(f"{what}: q must be [B, heads, head_dim]")

@@ -1,0 +1,62 @@
+"""Arguments of the 4-bit cache's and the page selection's wrappers that are missing: refused by
+name, as every other call of the library refuses them."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import reef_amd as r
+
+
+def calls(device):
+    """(name, call, required tensors, other arguments) of every wrapper."""
+    def ints(*shape):
+        return torch.zeros(shape, dtype=torch.int32, device=device)
+
+    f32 = dict(device=device)
+    new = torch.zeros(2, 2, 1, 64, **f32)
+    four = [torch.zeros(2, 2, 16, 32, dtype=torch.uint8, **f32),
+            torch.zeros(2, 2, 1, 64, 8, dtype=torch.uint8, **f32)]
+    eight = [torch.zeros(2, 2, 16, 64, dtype=torch.int8, **f32),
+             torch.zeros(2, 2, 1, 64, 16, dtype=torch.int8, **f32)]
+    scales = [torch.ones(2, 2, 16, **f32), torch.ones(2, 2, 16, **f32)]
+    q, qs = torch.zeros(2, 4, 64, dtype=torch.int8, **f32), torch.ones(2, 4, **f32)
+    bounds = [torch.zeros(2, 2, 1, 2, 64, dtype=torch.int8, **f32), torch.ones(2, 2, 1, **f32)]
+
+    def selected(call):
+        return lambda *t: call(*t[:-2], selected=t[-2:])
+
+    return [
+        ("append", r.kv_append_int4, [new, new, ints(2), *four, *scales]),
+        ("unpack", r.kv_unpack_int4, [*four, *scales]),
+        ("copy", r.kv_copy_pages_int4, [ints(1), ints(1), *four, *scales]),
+        ("decode", r.attention_decode_int4, [q, qs, *four, *scales]),
+        ("decode listed", selected(r.attention_decode_int4),
+         [q, qs, *four, *scales, ints(2), ints(2, 2, 1), ints(2, 2)]),
+        ("decode selected", selected(r.attention_decode_selected),
+         [q, qs, *eight, *scales, ints(2), ints(2, 2, 1), ints(2, 2)]),
+        ("chunk", lambda *t: r.attention_prefill_cache_int4(*t, 16, q_granularity=r.PER_TENSOR),
+         [q[:, :, None], torch.ones(1, **f32), *four, *scales]),
+        ("bounds", lambda start, *t: r.kv_page_bounds(start, 1, *t),
+         [ints(2), eight[0], scales[0], *bounds]),
+        ("bounds of 4 bits", lambda start, *t: r.kv_page_bounds(start, 1, *t),
+         [ints(2), four[0], scales[0], *bounds]),
+        ("select", lambda *t: r.kv_select_pages(*t, 1), [q, qs, *bounds, ints(2)]),
+    ]
+
+
+@pytest.mark.parametrize("i", range(10))
+def test_nothing_but_none(i):
+    name, call, tensors = calls("cpu")[i]
+    with pytest.raises(r.InvalidArgument):
+        call(*[None] * len(tensors))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("i", range(10))
+def test_each_tensor_missing(i):
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    name, call, tensors = calls("cuda")[i]
+    for at in range(len(tensors)):
+        with pytest.raises(r.InvalidArgument):
+            call(*tensors[:at], None, *tensors[at + 1:])
