@@ -1207,13 +1207,15 @@ def kv_copy_pages_int4(source, place, k_pages, v_pages, k_scale_pages, v_scale_p
 _DECODE_BYTES = {}
 
 
-def _decode_workspace_bytes(p):
-    """Workspace bytes of a decode call of these (packed) sizes."""
-    n = _DECODE_BYTES.get(p)
+def _decode_workspace_bytes(p, device):
+    """Workspace bytes of a decode call of these (packed) sizes on the current device (its index):
+    they go by its compute units."""
+    key = p, device
+    n = _DECODE_BYTES.get(key)
     if n is None:
         n = _lib().reef_attention_decode_workspace_bytes(p)
         if isinstance(p, bytes) and len(_DECODE_BYTES) < 4096:
-            _DECODE_BYTES[p] = n
+            _DECODE_BYTES[key] = n
     return n
 
 
@@ -1257,8 +1259,11 @@ def _decode_cache(what, function, bits, q, q_scales, k_cache, v_cache, k_scales,
         raise InvalidArgument(f"{what}: out must have q's shape")
     p = _decode_bytes(q, tokens, heads, window, softmax_scale, q_granularity, num_splits)
     stream = _stream()
-    ws = (_step_workspace(_decode_workspace_bytes(p), q.device, stream) if workspace is None
-          else _given(workspace))
+    if workspace is None:
+        device = q.device
+        ws = _step_workspace(_decode_workspace_bytes(p, device.index), device, stream)
+    else:
+        ws = _given(workspace)
     own = status or StatusWord(q.device)
     check(function(p, q.data_ptr(), q_scales.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                    k_scales.data_ptr(), v_scales.data_ptr(), _ptr(block_table), blocks, pages,

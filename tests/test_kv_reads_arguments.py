@@ -1,5 +1,6 @@
-"""Arguments of the 4-bit cache's and the page selection's wrappers that are missing: refused by
-name, as every other call of the library refuses them."""
+"""What the 4-bit cache's and the page selection's wrappers make of their arguments: missing ones are
+refused by name, as every other call of the library refuses them, and sizes that are kept are those of
+the device."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -60,3 +61,20 @@ def test_each_tensor_missing(i):
     for at in range(len(tensors)):
         with pytest.raises(r.InvalidArgument):
             call(*tensors[:at], None, *tensors[at + 1:])
+
+
+def test_workspace_bytes_are_the_devices(monkeypatch):
+    """A size that is kept from one device is not another's, which may have more compute units."""
+    class Library:
+        current = 0
+
+        def reef_attention_decode_workspace_bytes(self, p):
+            return (1000, 4000)[self.current]
+
+    lib = Library()
+    monkeypatch.setattr(r, "_lib", lambda: lib)
+    monkeypatch.setattr(r, "_DECODE_BYTES", {})
+    sizes = b"the packed sizes of a call"
+    for _ in range(2):
+        for lib.current in (0, 1):
+            assert r._decode_workspace_bytes(sizes, lib.current) == (1000, 4000)[lib.current]
