@@ -602,13 +602,15 @@ reef_status reef_attention_prefill_int4_cache(
 
 /* The bounds of the pages that positions start_positions[b] .. start_positions[b] +
  * new_tokens - 1 fall in, over those pages' tokens before start_positions[b] + new_tokens:
- * after an append, with its start positions (a page's earlier tokens are read again, so a
- * page copied by reef_kv_copy_pages needs nothing else); after reef_kv_keep_int8, with the
- * drafted tokens' start positions and number (rows that were not kept only loosen their page's
- * bounds); after a compaction, once with start 0. Of the keys x = float(code) * scale: S = max|x| / 127 (1 where that is 0), [0][d] =
- * min(127, ceil(max x_d / S)), [1][d] = max(-127, floor(min x_d / S)), IEEE divisions. Key
- * scales are positive and finite, as the quantizers make them. Sizes and status bits as
- * for reef_kv_append_int8 (a range past max_context sets CAPACITY and writes nothing). */
+ * after an append, with its start positions (a page's earlier tokens are read again: the page
+ * that reef_kv_reserve gave instead of a shared one, its tokens copied, needs nothing else);
+ * after reef_kv_keep_int8, with the drafted tokens' start positions and number (rows that were
+ * not kept only loosen their page's bounds). Pages that move take no bounds with them: after a
+ * compaction and its copies, the _ragged call below. Of the keys x = float(code) * scale:
+ * S = max|x| / 127 (1 where that is 0), [0][d] = min(127, ceil(max x_d / S)), [1][d] =
+ * max(-127, floor(min x_d / S)), IEEE divisions. Key scales are positive and finite, as the
+ * quantizers make them. Sizes and status bits as for reef_kv_append_int8 (a range past
+ * max_context sets CAPACITY and writes nothing). */
 reef_status reef_kv_page_bounds_int8(const reef_kv_append_params *p,
                                      const int32_t *start_positions, const int8_t *k_cache,
                                      const float *k_scales, const int32_t *block_table,
@@ -622,6 +624,23 @@ reef_status reef_kv_page_bounds_int4(const reef_kv_append_params *p,
                                      int64_t max_blocks_per_seq, int64_t num_pages, int8_t *bounds,
                                      float *bound_scales, uint32_t *status_word,
                                      hipStream_t stream);
+
+/* The same with an end for each sequence: the positions start_positions[b] ..
+ * min(start_positions[b] + new_tokens, context_lens[b]) - 1, over those pages' tokens before
+ * that end (context_lens [B] on the device; a sequence that ends at its start or before has
+ * none, a length outside [0, max_context] sets BAD_LENGTH and writes nothing for it). Starts
+ * of 0 and max_context tokens are every page that the sequences have tokens in. */
+reef_status reef_kv_page_bounds_int8_ragged(
+    const reef_kv_append_params *p, const int32_t *start_positions, const int32_t *context_lens,
+    const int8_t *k_cache, const float *k_scales, const int32_t *block_table,
+    int64_t max_blocks_per_seq, int64_t num_pages, int8_t *bounds, float *bound_scales,
+    uint32_t *status_word, hipStream_t stream);
+
+reef_status reef_kv_page_bounds_int4_ragged(
+    const reef_kv_append_params *p, const int32_t *start_positions, const int32_t *context_lens,
+    const uint8_t *k_cache, const float *k_scales, const int32_t *block_table,
+    int64_t max_blocks_per_seq, int64_t num_pages, int8_t *bounds, float *bound_scales,
+    uint32_t *status_word, hipStream_t stream);
 
 /* For every (sequence, kv head) the `budget` pages to read, shared by the group's query
  * heads, as a reef_page_selection holds them: ascending, -1 behind the last. The first

@@ -409,6 +409,30 @@ inline void kv_page_bounds(const reef_kv_append_params &p, const int32_t *start_
           "kv_page_bounds");
 }
 
+// The same up to each sequence's length: with starts of 0 and max_context tokens the bounds of every
+// page that holds tokens, as after a compaction.
+inline void kv_page_bounds(const reef_kv_append_params &p, const int32_t *start_positions,
+                           const int32_t *context_lens, const int8_t *k_cache,
+                           const float *k_scales, const int32_t *block_table,
+                           int64_t max_blocks_per_seq, int64_t num_pages, int8_t *bounds,
+                           float *bound_scales, uint32_t *status_word, hipStream_t stream) {
+    check(reef_kv_page_bounds_int8_ragged(&p, start_positions, context_lens, k_cache, k_scales,
+                                          block_table, max_blocks_per_seq, num_pages, bounds,
+                                          bound_scales, status_word, stream),
+          "kv_page_bounds");
+}
+
+inline void kv_page_bounds(const reef_kv_append_params &p, const int32_t *start_positions,
+                           const int32_t *context_lens, const uint8_t *k_cache,
+                           const float *k_scales, const int32_t *block_table,
+                           int64_t max_blocks_per_seq, int64_t num_pages, int8_t *bounds,
+                           float *bound_scales, uint32_t *status_word, hipStream_t stream) {
+    check(reef_kv_page_bounds_int4_ragged(&p, start_positions, context_lens, k_cache, k_scales,
+                                          block_table, max_blocks_per_seq, num_pages, bounds,
+                                          bound_scales, status_word, stream),
+          "kv_page_bounds");
+}
+
 // The pages to read for a query, ascending in pages [B, Hkv, budget] with their number in counts
 // [B, Hkv]: a reef_page_selection of max_pages = budget.
 inline size_t select_workspace_bytes(const reef_decode_params &p) {

@@ -52,7 +52,8 @@ EXPORTS = [
     "reef_attention_prefill_int8_cache",
     "reef_kv_append_int4", "reef_kv_unpack_int4", "reef_kv_copy_pages_int4",
     "reef_attention_decode_int4", "reef_attention_prefill_int4_cache", "reef_kv_page_bounds_int8",
-    "reef_kv_page_bounds_int4", "reef_kv_select_pages_workspace_bytes", "reef_kv_select_pages",
+    "reef_kv_page_bounds_int4", "reef_kv_page_bounds_int8_ragged",
+    "reef_kv_page_bounds_int4_ragged", "reef_kv_select_pages_workspace_bytes", "reef_kv_select_pages",
     "reef_attention_decode_int8_selected",
 ]
 
@@ -197,6 +198,8 @@ _SIGS = {
                                           _P, _ST, _P, C.c_size_t, _P, _P],
     "reef_kv_page_bounds_int8": [_KP, _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _P],
     "reef_kv_page_bounds_int4": [_KP, _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _P],
+    "reef_kv_page_bounds_int8_ragged": [_KP, _P, _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _P],
+    "reef_kv_page_bounds_int4_ragged": [_KP, _P, _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _P],
     "reef_kv_select_pages_workspace_bytes": [_DP],
     "reef_kv_select_pages": [_DP, _P, _P, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _P,
                              C.c_size_t, _P, _P],
@@ -1361,10 +1364,12 @@ def _chunk_workspace(n, device, stream):
 
 
 def kv_page_bounds(start_positions, new_tokens: int, k_cache, k_scales, bounds, bound_scales, *,
-                   block_table=None, status: StatusWord | None = None):
+                   block_table=None, context_lens=None, status: StatusWord | None = None):
     """The largest and the least key of every channel of the pages that tokens start_positions[b]
     .. start_positions[b] + new_tokens - 1 fall in, over those pages' tokens up to the last of
-    them: call it after an append, with its start positions. k_cache and k_scales of an int8 or
+    them: call it after an append, with its start positions. context_lens [B] ends a sequence's
+    tokens there where that is sooner: after a compaction and its copies, starts of 0 and
+    new_tokens of the whole table (max_blocks * 16) with the lengths are every page's. k_cache and k_scales of an int8 or
     a 4-bit cache; bounds int8 [B, Hkv, L/16, 2, D] and bound_scales [B, Hkv, L/16] (contiguous)
     or [P, Hkv, 2, D] and [P, Hkv] (a pool) are written in place."""
     what, torch = "kv_page_bounds", _torch()
@@ -1373,10 +1378,13 @@ def kv_page_bounds(start_positions, new_tokens: int, k_cache, k_scales, bounds, 
     _alike(what, (start_positions, i32, "start_positions"),
            (k_cache, torch.uint8 if int4 else torch.int8, "k_cache"), (k_scales, f32, "k_scales"),
            (bounds, torch.int8, "bounds"), (bound_scales, f32, "bound_scales"),
-           (block_table, i32, "block_table"))
+           (context_lens, i32, "context_lens"), (block_table, i32, "block_table"),
+           optional=("context_lens", "block_table"))
     shape = start_positions.shape
     if len(shape) != 1:
         raise InvalidArgument(f"{what}: start_positions must be [B]")
+    if context_lens is not None and context_lens.shape != shape:
+        raise InvalidArgument(f"{what}: context_lens must be [B]")
     B = shape[0]
     heads, tokens, dim, blocks, pages = _cache_sizes(what, B, k_cache, None, k_scales, None,
                                                      block_table, 4 if int4 else 8)
@@ -1385,9 +1393,15 @@ def kv_page_bounds(start_positions, new_tokens: int, k_cache, k_scales, bounds, 
         raise InvalidArgument(f"{what}: bounds must hold 2 rows, bound_scales one scale a page and "
                               "head")
     own = status or StatusWord(k_cache.device)
-    function = _lib().reef_kv_page_bounds_int4 if int4 else _lib().reef_kv_page_bounds_int8
+    lib, ends = _lib(), ()
+    if context_lens is None:
+        function = lib.reef_kv_page_bounds_int4 if int4 else lib.reef_kv_page_bounds_int8
+    else:
+        function = (lib.reef_kv_page_bounds_int4_ragged if int4
+                    else lib.reef_kv_page_bounds_int8_ragged)
+        ends = (context_lens.data_ptr(),)
     check(function(_packed(_APPEND, KvAppendParams, B, heads, dim, new_tokens, tokens),
-                   start_positions.data_ptr(), k_cache.data_ptr(), k_scales.data_ptr(),
+                   start_positions.data_ptr(), *ends, k_cache.data_ptr(), k_scales.data_ptr(),
                    _ptr(block_table), blocks, pages, bounds.data_ptr(), bound_scales.data_ptr(),
                    own.tensor.data_ptr(), _stream()), what)
     if status is None:

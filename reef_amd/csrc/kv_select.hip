@@ -27,6 +27,7 @@ struct BoundArgs {
     const uint8_t *k;
     const float *ks;
     const int32_t *start;
+    const int32_t *lens;   // may be null
     const int32_t *table;  // paged only
     int8_t *bounds;
     float *scales;
@@ -55,7 +56,17 @@ __global__ __launch_bounds__(kBoundWaves * kWave) void page_bounds(BoundArgs a) 
             flag_status(a.status, start < 0 ? REEF_STATUS_BIT_BAD_LENGTH : REEF_STATUS_BIT_CAPACITY);
         return;
     }
-    const int end = start + a.new_tokens;
+    int end = start + a.new_tokens;
+    if (a.lens) {
+        const int len = a.lens[b];
+        if (len < 0 || len > a.max_context) {
+            if (blockIdx.x == 0 && kvh == 0 && threadIdx.x == 0)
+                flag_status(a.status, REEF_STATUS_BIT_BAD_LENGTH);
+            return;
+        }
+        end = min(end, len);
+        if (end <= start) return;
+    }
     const int stop = (end + kPage - 1) / kPage;
     int page_idx = start / kPage + (int)blockIdx.x * kBoundWaves * a.turns + wave;
     const int last = min(stop, start / kPage + ((int)blockIdx.x + 1) * kBoundWaves * a.turns) - 1;
@@ -170,10 +181,10 @@ __global__ __launch_bounds__(kBoundWaves * kWave) void page_bounds(BoundArgs a) 
 }
 
 template <int BITS>
-reef_status launch_bounds(const reef_kv_append_params *p, const int32_t *start, const void *k,
-                          const float *ks, const int32_t *block_table, int64_t max_blocks_per_seq,
-                          int64_t num_pages, int8_t *bounds, float *bound_scales,
-                          uint32_t *status_word, hipStream_t stream) {
+reef_status launch_bounds(const reef_kv_append_params *p, const int32_t *start, const int32_t *lens,
+                          const void *k, const float *ks, const int32_t *block_table,
+                          int64_t max_blocks_per_seq, int64_t num_pages, int8_t *bounds,
+                          float *bound_scales, uint32_t *status_word, hipStream_t stream) {
     if (!p || !start || !k || !ks || !bounds || !bound_scales || p->batch <= 0 ||
         p->kv_heads <= 0 || p->head_dim <= 0 || p->new_tokens <= 0 || p->max_context <= 0 ||
         p->max_context % kPage != 0)
@@ -196,6 +207,7 @@ reef_status launch_bounds(const reef_kv_append_params *p, const int32_t *start, 
     a.k = static_cast<const uint8_t *>(k);
     a.ks = ks;
     a.start = start;
+    a.lens = lens;
     a.table = block_table;
     a.bounds = bounds;
     a.scales = bound_scales;
@@ -545,8 +557,8 @@ extern "C" reef_status reef_kv_page_bounds_int8(const reef_kv_append_params *p,
                                                 int64_t max_blocks_per_seq, int64_t num_pages,
                                                 int8_t *bounds, float *bound_scales,
                                                 uint32_t *status_word, hipStream_t stream) {
-    return launch_bounds<8>(p, start_positions, k_cache, k_scales, block_table, max_blocks_per_seq,
-                            num_pages, bounds, bound_scales, status_word, stream);
+    return launch_bounds<8>(p, start_positions, nullptr, k_cache, k_scales, block_table,
+                            max_blocks_per_seq, num_pages, bounds, bound_scales, status_word, stream);
 }
 
 extern "C" reef_status reef_kv_page_bounds_int4(const reef_kv_append_params *p,
@@ -556,8 +568,28 @@ extern "C" reef_status reef_kv_page_bounds_int4(const reef_kv_append_params *p,
                                                 int64_t max_blocks_per_seq, int64_t num_pages,
                                                 int8_t *bounds, float *bound_scales,
                                                 uint32_t *status_word, hipStream_t stream) {
-    return launch_bounds<4>(p, start_positions, k_cache, k_scales, block_table, max_blocks_per_seq,
-                            num_pages, bounds, bound_scales, status_word, stream);
+    return launch_bounds<4>(p, start_positions, nullptr, k_cache, k_scales, block_table,
+                            max_blocks_per_seq, num_pages, bounds, bound_scales, status_word, stream);
+}
+
+extern "C" reef_status reef_kv_page_bounds_int8_ragged(
+    const reef_kv_append_params *p, const int32_t *start_positions, const int32_t *context_lens,
+    const int8_t *k_cache, const float *k_scales, const int32_t *block_table,
+    int64_t max_blocks_per_seq, int64_t num_pages, int8_t *bounds, float *bound_scales,
+    uint32_t *status_word, hipStream_t stream) {
+    if (!context_lens) return REEF_INVALID_ARGUMENT;
+    return launch_bounds<8>(p, start_positions, context_lens, k_cache, k_scales, block_table,
+                            max_blocks_per_seq, num_pages, bounds, bound_scales, status_word, stream);
+}
+
+extern "C" reef_status reef_kv_page_bounds_int4_ragged(
+    const reef_kv_append_params *p, const int32_t *start_positions, const int32_t *context_lens,
+    const uint8_t *k_cache, const float *k_scales, const int32_t *block_table,
+    int64_t max_blocks_per_seq, int64_t num_pages, int8_t *bounds, float *bound_scales,
+    uint32_t *status_word, hipStream_t stream) {
+    if (!context_lens) return REEF_INVALID_ARGUMENT;
+    return launch_bounds<4>(p, start_positions, context_lens, k_cache, k_scales, block_table,
+                            max_blocks_per_seq, num_pages, bounds, bound_scales, status_word, stream);
 }
 
 extern "C" size_t reef_kv_select_pages_workspace_bytes(const reef_decode_params *p) {

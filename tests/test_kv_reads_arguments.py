@@ -78,3 +78,25 @@ def test_workspace_bytes_are_the_devices(monkeypatch):
     for _ in range(2):
         for lib.current in (0, 1):
             assert r._decode_workspace_bytes(sizes, lib.current) == (1000, 4000)[lib.current]
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_bounds_up_to_lengths_refuses(bits):
+    """The refusals of the call without lengths, and of lengths that are not there."""
+    def at(n, offset=0):  # host addresses: validation never dereferences them
+        return 0x10000 * n + offset
+
+    lib = r.lib()
+    f = lib.reef_kv_page_bounds_int4_ragged if bits == 4 else lib.reef_kv_page_bounds_int8_ragged
+
+    def call(lens=at(2), k=at(3), out=at(5), table=None, blocks=0, pages=0, **kw):
+        sizes = dict(batch=2, kv_heads=2, head_dim=128, new_tokens=5, max_context=64)
+        return f(r.KvAppendParams(**{**sizes, **kw}), at(1), lens, k, at(4), table, blocks, pages, out,
+                 at(6), None, None)
+
+    for bad in (dict(lens=None), dict(k=None), dict(k=at(3, 8)), dict(out=None), dict(batch=0),
+                dict(new_tokens=0), dict(max_context=40), dict(table=at(7), blocks=3, pages=9),
+                dict(table=at(7), blocks=4, pages=0)):
+        assert call(**bad) == r.INVALID_ARGUMENT, bad
+    assert call(new_tokens=65) == r.CAPACITY
+    assert call(head_dim=96) == r.UNSUPPORTED and call(batch=65536) == r.UNSUPPORTED
