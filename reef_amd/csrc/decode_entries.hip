@@ -238,6 +238,14 @@ __device__ __forceinline__ int wave_sum(int x) {
         (int)wave_reduce((uint32_t)x, [](uint32_t y, uint32_t z) { return y + z; }));
 }
 
+// A share of `total` blocks (below 2^31) among n, rounded up: their sum with n may pass 31 bits (300
+// lists that name a few pages 28 million times each).
+__host__ __device__ constexpr int share_of(int total, int n) {
+    return (int)(((uint32_t)total + (uint32_t)n - 1) / (uint32_t)n);
+}
+static_assert(share_of(INT32_MAX, 512) == 1 << 22 && share_of(INT32_MAX, 1 << 20) == 1 << 11 &&
+              share_of(1, 512) == 1 && share_of(1025, 512) == 3, "rounded up, without overflow");
+
 // A workgroup's part: item, number of it, the item's parts and the first one's slot.
 struct Part {
     int item, part, parts, slot;
@@ -261,7 +269,7 @@ __device__ __forceinline__ Part wave_plan(const EntryArgs &a, int g, int lane) {
     }
     const int total = wave_sum(mine);
     const int spare = a.round - a.items / 2;  // (parts are rounded up by half of one)
-    int p[K], c = max(a.least, (total + spare - 1) / spare);
+    int p[K], c = max(a.least, share_of(total, spare));
     for (;; c += max(1, c >> 4)) {
         mine = 0;
 #pragma unroll
@@ -337,11 +345,11 @@ __global__ __launch_bounds__(kEntryThreads, kWgPerCu) void decode_entries(EntryA
             mine += n;
         }
         const int total = workgroup_sum(mine, sWave);
-        int c = max(a.least, (total + a.round - 1) / a.round);
+        int c = max(a.least, share_of(total, a.round));
         auto parts_of = [&](int i) { return (int)((uint32_t)(sPlan[i] + c - 1) / (uint32_t)c); };
         if (a.few) {
             const int spare = a.round - a.items / 2;  // (parts are rounded up by half of one)
-            for (c = max(a.least, (total + spare - 1) / spare);; c += max(1, c >> 4)) {
+            for (c = max(a.least, share_of(total, spare));; c += max(1, c >> 4)) {
                 mine = 0;
                 for (int i = from; i < to; ++i) mine += parts_of(i);
                 if (workgroup_sum(mine, sWave) <= a.round) break;
