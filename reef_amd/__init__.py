@@ -528,12 +528,8 @@ def attention_prefill_cache(q, q_scales, k_cache, v_cache, k_scales, v_scales, k
         max_context, table = 0, block_table.contiguous()
         max_blocks, pages = table.shape[1], k_cache.shape[0]
     n = _lib().reef_attention_prefill_cache_workspace_bytes(p)
-    device, stream = q.device, _stream()
-    key = ("cache", device.index, stream)
-    ws = _PREFILL_WS.get(key)
-    if ws is None or ws.numel() < n:  # zero-filled once; every call leaves it so
-        ws = torch.zeros(max(n, 256), dtype=torch.uint8, device=device)
-        _PREFILL_WS[key] = ws
+    stream = _stream()
+    ws = _chunk_workspace(n, q.device, stream)
     if out is None:
         out = torch.empty((B, Hq, Sq, D), dtype=torch.float32, device=q.device)
     qs, os_ = _strides4(q), _strides4(out)
@@ -1349,8 +1345,10 @@ def attention_prefill_cache_int4(q, q_scales, k_cache, v_cache, k_scales, v_scal
 
 
 def _chunk_workspace(n, device, stream):
-    """attention_prefill_cache's workspace of this stream; under graph capture one of its own, of
-    which the counters alone (65536 words in front) have to be zero."""
+    """The workspace of this stream's chunks over either cache, zero-filled once (every call leaves it
+    so); under graph capture one of its own, of which the counters alone (65536 words in front) have to
+    be zero. (A graph that held the stream's would read freed memory once a longer chunk of either
+    cache has replaced it.)"""
     torch = _torch()
     if torch._C._cuda_isCurrentStreamCapturing():
         ws = torch.empty(max(n, 1 << 18), dtype=torch.uint8, device=device)
