@@ -1411,7 +1411,9 @@ def kv_select_pages(q, q_scales, bounds, bound_scales, context_lens, budget: int
                     status: StatusWord | None = None):
     """The `budget` pages that each sequence's kv heads are to read for the query q [B, Hq, D]
     int8: its first `sinks` and last `recent` pages and those whose bounds (kv_page_bounds) allow
-    the largest scores for any of the group's query heads, ties to the lowest page. Returns
+    the largest scores for any of the group's query heads, ties to the lowest page. (A window is
+    not looked at: pages before it are selected too, and decode with a window leaves their tokens
+    out.) Returns
     (pages [B, Hkv, budget] int32, ascending, -1 behind the last; counts [B, Hkv] int32), the
     `selected` of attention_decode_selected and attention_decode_int4."""
     what, torch = "kv_select_pages", _torch()

@@ -24,7 +24,8 @@ struct DecodeArgs {
     const int32_t *block_table;  // paged only
     const int32_t *context_lens; // may be null
     uint32_t *counters;     // one per (sequence, kv head); zero between launches
-    float *slots;           // [B * Hkv, groups] parts (DecodeSlot), with groups > 1
+    float *slots;           // DecodeSlot each: two a workgroup (decode.hip: the first and the last of
+                            // its run), or one a part, in the plan's order (decode_entries.hip)
     uint32_t *status;
     int32_t batch, q_heads, kv_heads, group;
     int32_t max_context, window;

@@ -311,6 +311,9 @@ __device__ __forceinline__ Part wave_plan(const EntryArgs &a, int g, int lane) {
 // With more items, or none of more than kLeastBlocks blocks, a part is an item. The 4 waves take a
 // part's blocks in turn, keep a flash-decoding state each and merge in LDS; an item in one part is
 // stored, the parts of others go to the workspace, and the part that arrives last merges them all.
+// (Registers: lists of the int8 cache at head_dim 128 take all 256, and for 8 or 16 heads spill 20 to
+// 64 bytes a lane outside the loop over blocks, at a part's start and its merge: 22.0 us with 8 heads
+// to a kv head, 21.0 with 4, for 16 x 8 kv heads of 128 pages.)
 template <int D, int BITS, int HEADS, bool PAGED, Form FORM>
 __global__ __launch_bounds__(kEntryThreads, kWgPerCu) void decode_entries(EntryArgs a, float *out) {
     using Slots = RowSlots<D, HEADS>;
@@ -683,12 +686,13 @@ reef_status decode_any(const reef_decode_params *p, const int8_t *q, const float
 
 // A 64-key block of 16 columns costs about 1.4 ns of the whole GPU's time here, one of a 128-row
 // tile 9 ns there, behind a copy of the cache and a schedule's start of 25 us. So a chunk runs here
-// if it has few blocks (2 x 12 heads of 64, 77 rows over 1021 keys: 13.6 us against 30; 32 heads, 8
-// of keys, of 128, 64 rows over 4096 24.5 against 46; 12 heads of 64, 1024 rows over 1024 24 against
-// 32) or if its tiles of 128 rows stay part empty (8 x 16 heads of 64, 16 rows over 6000: 25 against
-// 155; 2 x 32 heads of 128, 100 rows over 8000 95 against 105). With full tiles and many blocks it
-// does not (32 heads of 128, 1024 rows over 1024: 65 against 46; 4 x 32, 512 over 4608 382 against
-// 261; 8 x 12 of 64, 512 over 1024 61 against 51).
+// if it has few blocks (us a call, here against there: 2 x 12 heads of 64, 77 rows over 1021 keys 12
+// against 29; 32 heads, 8 of keys, of 128, 64 rows over 4096 23 against 45; 12 heads of 64, 1024 rows
+// over 1024 23 against 31) or if its tiles of 128 rows stay part empty (8 x 16 heads of 64, 16 rows
+// over 6000 24 against 138; 2 x 32 heads, 4 of keys, of 128, 100 rows over 8000 95 against 98). With
+// full tiles and many blocks it does not (32 heads of 128, 1024 rows over 1024: 66 against 44; 2 x 32,
+// 512 over 2048 102 against 91); of few full tiles over many keys that gives some away (32 heads, 8 of
+// keys, of 128, 128 rows over 8192: 51 against 67, 512 over 4608 99 against 103).
 bool chunk_entries_fit(const reef_attention_params *p) {
     constexpr int64_t kRows = 128;
     const int64_t few = p->head_dim == 64 ? 32768 : 16384;

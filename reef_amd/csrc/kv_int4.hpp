@@ -30,7 +30,7 @@ __device__ __forceinline__ uint32_t nibbles_to_int8(uint32_t u) {
 // exponent of 1024 a nibble in bits 0-3 reads as 1024 + u, one in bits 4-7 as 1024 + 16 u;
 // tokens 2i and 2i + 1 lie 16 bits apart, so one mask takes both. Nine instructions for eight
 // values (the empty asm keeps mask and exponent in registers, where one instruction takes both;
-// as literals they cost one each: 64 more of 455 a block of decode at head_dim 128).
+// as literals they cost one each: 64 more a block of decode at head_dim 128, which has about 440).
 __device__ __forceinline__ f16x8 int4x8_to_f16(uint32_t w) {
     const f16x2 low = {(_Float16)-1032.0f, (_Float16)-1032.0f};
     const f16x2 high = {(_Float16)-72.0f, (_Float16)-72.0f};

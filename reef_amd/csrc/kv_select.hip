@@ -5,8 +5,10 @@
 // A page's bounds are the largest and the least key of each channel, hi and lo, as int8 codes of
 // one scale S a page, rounded outwards. For any key x of the page and a query q,
 //   q . x = sum_d q_d x_d <= S * sum_d (max(q_d, 0) hi_d + min(q_d, 0) lo_d),
-// with codes of q a product of [max(q, 0), min(q, 0)] and [hi, lo], 2 D long: int8 matrix
-// instructions, exact. A page costs 2 D + 4 bytes to score, 1/16 of its int8 keys and values.
+// up to fp32's rounding: S and the quotients are rounded before the codes are, and a code past 127
+// is cut to it. With codes of q the sum is a product of [max(q, 0), min(q, 0)] and [hi, lo], 2 D
+// long: int8 matrix instructions, exact. A page costs 2 D + 4 bytes to score, 1/16 of its int8 keys
+// and values.
 #include <algorithm>
 
 #include "kv_int4.hpp"
@@ -438,9 +440,9 @@ struct HeldKeys<0> {
 // of those at it, in page order. Wave w holds a run of pages, 64 at a time. The last key taken is found digit by
 // digit from the highest bit in which scores differ (they share sign and most of the exponent): the
 // keys of the range so far are counted by the digit's value in LDS, and the first value that enough
-// of them reach is the next range, until exactly enough do. Two digits mostly: 8.8 us of a launch of
-// 8 items of 8192 pages (bit by bit 12, with a pass over the keys in memory a bit 63), 5.6 of one of
-// 128 items of up to 512.
+// of them reach is the next range, until exactly enough do. Two digits mostly: 8.1 us of a launch of
+// 8 items of 8192 pages (bit by bit 12, with a pass over the keys in memory a bit 63), 5.2 of one of
+// 128 items of up to 2048.
 template <int R>
 __global__ __launch_bounds__(kPickThreads) void pick_pages(SelectArgs a) {
     __shared__ PickShared sh;
@@ -484,7 +486,7 @@ __global__ __launch_bounds__(kPickThreads) void pick_pages(SelectArgs a) {
         const uint32_t differ = all ^ any;
         int left = differ ? 32 - __builtin_clz(differ) : 0;  // bits below those that all share
         t = left == 32 ? 0 : all & ~0u << left;
-        if (above >= a.budget) {  // no score matters (positive NaNs count as always taken)
+        if (above >= a.budget) {  // sinks and recent pages are the budget: no score matters
             t = kAlways;
             left = 0;
         }
