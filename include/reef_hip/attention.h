@@ -628,8 +628,9 @@ reef_status reef_kv_page_bounds_int4(const reef_kv_append_params *p,
 /* The same with an end for each sequence: the positions start_positions[b] ..
  * min(start_positions[b] + new_tokens, context_lens[b]) - 1, over those pages' tokens before
  * that end (context_lens [B] on the device; a sequence that ends at its start or before has
- * none, a length outside [0, max_context] sets BAD_LENGTH and writes nothing for it). Starts
- * of 0 and max_context tokens are every page that the sequences have tokens in. */
+ * none, a length outside [0, max_context] sets BAD_LENGTH and writes nothing for it; a page
+ * that several sequences name holds as many tokens of each, as forks' pages do). Starts of 0
+ * and max_context tokens are every page that the sequences have tokens in. */
 reef_status reef_kv_page_bounds_int8_ragged(
     const reef_kv_append_params *p, const int32_t *start_positions, const int32_t *context_lens,
     const int8_t *k_cache, const float *k_scales, const int32_t *block_table,

@@ -1,6 +1,10 @@
 """What the 4-bit cache's and the page selection's wrappers make of their arguments: missing ones are
 refused by name, as every other call of the library refuses them, and sizes that are kept are those of
 the device."""
+import os
+import shutil
+import subprocess
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -100,3 +104,16 @@ def test_bounds_up_to_lengths_refuses(bits):
         assert call(**bad) == r.INVALID_ARGUMENT, bad
     assert call(new_tokens=65) == r.CAPACITY
     assert call(head_dim=96) == r.UNSUPPORTED and call(batch=65536) == r.UNSUPPORTED
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_bounds_up_to_lengths_in_cxx(tmp_path):
+    r.lib()  # the library must be built
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe, libdir = tmp_path / "kv_bounds_check", os.path.dirname(r.LIB_PATH)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Wextra", "-Werror", "-D__HIP_PLATFORM_AMD__",
+                    "-I", os.path.join(root, "include"), "-isystem", "/opt/rocm/include",
+                    os.path.join(root, "tests", "cxx", "kv_bounds_check.cpp"), "-L", libdir, "-lreef_hip",
+                    f"-Wl,-rpath,{libdir}", "-o", str(exe)], check=True, capture_output=True, text=True)
+    done = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert done.returncode == 0, done.stdout + done.stderr
